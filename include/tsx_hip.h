@@ -207,6 +207,74 @@ int tsx_gemm_i8(int32_t m, int32_t n, int32_t k, const int8_t *a_dev, const void
                 const tsx_epilogue *ep, float *out_f32_dev, int8_t *out_i8_dev, int32_t *out_acc_dev,
                 void *workspace_dev, size_t workspace_bytes, void *stream);
 
+/* ---------------------------------------------------------------- tokens: rows with scales of their own
+ * No counterpart in the reference, whose quantized operators take scales fixed beforehand and whose tensors here are fp32.
+ * A token is a row of values with one scale; rows lie at any stride of at least their length (strides count elements), at any
+ * address that is a multiple of their elements' size.  Values are fp32, fp16 or bf16; arithmetic is fp32 (sums of int8
+ * products int32) and a result is rounded once, to nearest even, to the output's type. */
+#define TSX_TYPE_F32  0
+#define TSX_TYPE_F16  1
+#define TSX_TYPE_BF16 2
+#define TSX_TYPE_I8   3   /* where a call says so */
+/* x / (1 + exp(-x)), on the hardware's exponential and reciprocal; only in the calls on tokens and in the group norm, which take
+ * TSX_ACT_NONE, _RELU, _LEAKY_RELU, _MISH_FAST and this (the exact Mish is the host's bits for a given fp32 number: there is
+ * none to match here).  A negative zero and a NaN become 0 under ReLU, as in the activations' SIMD body. */
+#define TSX_ACT_SILU 5
+
+/* Each row to int8 by its own largest magnitude a:  scale = fp32(a / 127),  q = x * fp32(127 / a) rounded to nearest even (the
+ * product exact), so q * scale stands for x.  A row of zeros has the scale 0.  A row with an infinity or a NaN has q = 0 and
+ * the scale NaN.  rows may be 0; cols is at most 2^30. */
+int tsx_quantize_tokens(int64_t rows, int32_t cols, const void *x_dev, int32_t x_type, int64_t x_stride, int8_t *q_dev,
+                        int64_t q_stride, float *scales_dev, void *stream);
+
+/* int8 product with a scale for each token and each channel:
+ *   out[i][j] = act(float(sum_k q[i][k] w[k][j]) * w_scales[j] * x_scales[i] + bias[j])
+ * x_type TSX_TYPE_I8: x holds q, x_scales its scales, as tsx_quantize_tokens or tsx_group_norm_tokens_nhwc write them.  Another type:
+ * the rows are quantized by the call, with the values of tsx_quantize_tokens (x_scales is not read).  Weights as
+ * tsx_gemm_i8_pack_weights packs them; k is below 2^17, m may be 0.  The workspace (16-byte aligned, its contents written and read by
+ * each call: calls that share one must not overlap) may be asked for as 0 bytes. */
+typedef struct tsx_token_gemm {
+    int32_t m, n, k;
+    int32_t x_type, out_type;
+    int32_t act;                 /* TSX_ACT_* as above */
+    float slope;                 /* leaky_relu */
+    const void *x_dev;
+    int64_t x_stride;
+    const float *x_scales_dev;   /* [m], int8 rows only */
+    const void *packed_w_dev;
+    const float *w_scales_dev;   /* [n] */
+    const float *bias_dev;       /* [n] or NULL */
+    void *out_dev;
+    int64_t out_stride;
+} tsx_token_gemm;
+size_t tsx_gemm_i8_tokens_workspace_bytes(const tsx_token_gemm *g);
+int tsx_gemm_i8_tokens(const tsx_token_gemm *g, void *workspace_dev, size_t workspace_bytes, void *stream);
+
+/* Group norm with an activation on channels-last tensors x[n][pixels][c], in groups of c / groups consecutive channels:
+ *   y = act((x - mean) / sqrt(variance + epsilon) * weight[c] + bias[c]),  mean and variance over a group's channels of all pixels of
+ * an image (the variance divides by their count).  Images and pixels lie at any stride (pixels at one of at least c); c is at
+ * most 8192, n below 65536; n or pixels may be 0.
+ *   nhwc         the result in x's type, dense [n][pixels][c] (may be x itself where that is dense)
+ *   tokens_nhwc  the result (as fp32, before any rounding) as int8 tokens, a pixel a token: q dense [n][pixels][c],
+ *                scales [n][pixels], with the rule of tsx_quantize_tokens
+ * The workspace (8-byte aligned) is written and read by each call: calls that share one must not overlap. */
+typedef struct tsx_group_norm {
+    int32_t n, c, groups;
+    int32_t type;
+    int64_t pixels;
+    int64_t image_stride, pixel_stride;
+    const void *x_dev;
+    const float *weight_dev;     /* [c] or NULL */
+    const float *bias_dev;       /* [c] or NULL */
+    float epsilon;
+    int32_t act;
+    float slope;
+} tsx_group_norm;
+size_t tsx_group_norm_workspace_bytes(const tsx_group_norm *g);
+int tsx_group_norm_nhwc(const tsx_group_norm *g, void *out_dev, void *workspace_dev, size_t workspace_bytes, void *stream);
+int tsx_group_norm_tokens_nhwc(const tsx_group_norm *g, int8_t *q_dev, float *scales_dev, void *workspace_dev,
+                               size_t workspace_bytes, void *stream);
+
 /* ---------------------------------------------------------------- fp32 conv2d / inner_prod
  * cpu::Conv2DCore::conv2d (src/kernels/cpu/conv2d_core.cpp:101-119, interface
  * include/backend/base/base_conv2d_core.h:14-32): im2col + GEMM, here one implicit-GEMM kernel on

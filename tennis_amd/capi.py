@@ -28,6 +28,9 @@ _sz = ctypes.c_size_t
 ACT_NONE, ACT_RELU, ACT_LEAKY_RELU = 0, 1, 2
 _ACT = {None: ACT_NONE, "none": ACT_NONE, "relu": ACT_RELU, "leaky_relu": ACT_LEAKY_RELU, "mish": 3, "mish_fast": 4}
 
+# of the calls on tokens and of the group norm: with SiLU, without the exact Mish, whose bits are the host's for a given fp32 number
+_TOKEN_ACT = {None: ACT_NONE, "none": ACT_NONE, "relu": ACT_RELU, "leaky_relu": ACT_LEAKY_RELU, "mish_fast": 4, "silu": 5}
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3}
 
 _POOL = {"max": 0, "avg": 1}
 
@@ -44,6 +47,20 @@ class Epilogue(ctypes.Structure):
                 ("q_scales_dev", _vp), ("n_qscales", _i32), ("residual_dev", _vp), ("staged_out_dev", _vp),
                 ("staged_hs", _i32), ("staged_ws", _i32), ("staged_cp", _i32), ("staged_pad_top", _i32),
                 ("staged_pad_left", _i32), ("residual_after_act", _i32), ("staged_upsample", _i32)]
+
+
+class TokenGemm(ctypes.Structure):
+    """tsx_token_gemm."""
+    _fields_ = [("m", _i32), ("n", _i32), ("k", _i32), ("x_type", _i32), ("out_type", _i32), ("act", _i32), ("slope", _f32),
+                ("x_dev", _vp), ("x_stride", _i64), ("x_scales_dev", _vp), ("packed_w_dev", _vp), ("w_scales_dev", _vp),
+                ("bias_dev", _vp), ("out_dev", _vp), ("out_stride", _i64)]
+
+
+class GroupNorm(ctypes.Structure):
+    """tsx_group_norm."""
+    _fields_ = [("n", _i32), ("c", _i32), ("groups", _i32), ("type", _i32), ("pixels", _i64), ("image_stride", _i64),
+                ("pixel_stride", _i64), ("x_dev", _vp), ("weight_dev", _vp), ("bias_dev", _vp), ("epsilon", _f32), ("act", _i32),
+                ("slope", _f32)]
 
 
 class TsxError(RuntimeError):
@@ -107,6 +124,12 @@ SIGNATURES = {
     "tsx_depthwise_conv2d_f32": (ctypes.c_int, [ctypes.POINTER(ConvGeom), _vp, _vp, _f32, _vp, _i32, _f32, _vp, _vp]),
     "tsx_pooling2d_out_size": (ctypes.c_int, [_i32] * 10 + [ctypes.POINTER(_i32), ctypes.POINTER(_i32)]),
     "tsx_pooling2d_f32": (ctypes.c_int, [_vp, _i64] + [_i32] * 10 + [_vp, _i32, _i32, _vp]),
+    "tsx_quantize_tokens": (ctypes.c_int, [_i64, _i32, _vp, _i32, _i64, _vp, _i64, _vp, _vp]),
+    "tsx_gemm_i8_tokens_workspace_bytes": (_sz, [ctypes.POINTER(TokenGemm)]),
+    "tsx_gemm_i8_tokens": (ctypes.c_int, [ctypes.POINTER(TokenGemm), _vp, _sz, _vp]),
+    "tsx_group_norm_workspace_bytes": (_sz, [ctypes.POINTER(GroupNorm)]),
+    "tsx_group_norm_nhwc": (ctypes.c_int, [ctypes.POINTER(GroupNorm), _vp, _vp, _sz, _vp]),
+    "tsx_group_norm_tokens_nhwc": (ctypes.c_int, [ctypes.POINTER(GroupNorm), _vp, _vp, _vp, _sz, _vp]),
     "tsx_winograd_f63_kernel_bytes": (_sz, [_i32, _i32]),
     "tsx_winograd_f63_transform_kernel": (ctypes.c_int, [_i32, _i32, _vp, _vp, _vp]),
     "tsx_winograd_f63_workspace_bytes": (_sz, [ctypes.POINTER(ConvGeom)]),
@@ -573,6 +596,179 @@ class GemmI8:
         check(lib().tsx_gemm_i8(m, self.n, k, _ptr(a), _ptr(self.packed), ctypes.byref(ep.c) if ep else None,
                                 _ptr(out_f32), _ptr(out_i8), _ptr(acc), _ptr(self._workspace), ws_bytes, _stream()))
         return out_f32, out_i8, acc
+
+
+# ---------------------------------------------------------------- tokens and channels-last tensors
+# Tensors of fp32, fp16 or bf16 values on one device, taken at their strides; the calls run on the current stream of that device.
+# They allocate their workspace for the call, so calls on several streams or in several captured graphs share none.  Results carry
+# no gradient.
+
+def _token_act(act):
+    if act not in _TOKEN_ACT:
+        raise TsxError("activation %r (one of %s)" % (act, ", ".join(repr(a) for a in _TOKEN_ACT)))
+    return _TOKEN_ACT[act]
+
+
+def _token_operand(what, x, types):
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise TsxError("%s: expected a device tensor" % what)
+    if x.dtype not in types:
+        raise TsxError("%s: %s (one of %s)" % (what, x.dtype, ", ".join(str(t) for t in types)))
+    return x
+
+
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _vector(what, t, count, x):
+    """An fp32 vector of `count` values on the device of x, or None."""
+    if t is None:
+        return None
+    t = _dev(t, torch.float32)
+    if t.device != x.device:
+        raise TsxError("%s is on %s, the tensor on %s" % (what, t.device, x.device))
+    if t.numel() != count:
+        raise TsxError("%s: %d values for %d" % (what, t.numel(), count))
+    return t
+
+
+def _axis(x, first, last):
+    """Axes [first, last) of x as one: (count, stride between neighbours), or None where they are none."""
+    count, stride = 1, 0
+    for d in range(last - 1, first - 1, -1):
+        if x.shape[d] != 1:
+            if count > 1 and x.stride(d) != stride * count:
+                return None
+            if count == 1:
+                stride = x.stride(d)
+        count *= x.shape[d]
+    return count, stride
+
+
+def _rows(x):
+    """x as rows of its last axis at a stride of at least their length: (x or a dense copy, rows, stride)."""
+    k = x.shape[-1]
+    lead = _axis(x, 0, x.dim() - 1)
+    if lead is None or (k > 1 and x.stride(-1) != 1) or (lead[0] > 1 and lead[1] < k):
+        x = x.contiguous()
+        lead = _axis(x, 0, x.dim() - 1)
+    return x, lead[0], lead[1] if lead[0] > 1 else k
+
+
+def quantize_tokens(x):
+    """tsx_quantize_tokens: (q, scales) of x [..., k] in fp32, fp16 or bf16; q int8 of x's shape, scales fp32 [...], so that
+    q * scales[..., None] stands for x with each row's largest magnitude at 127."""
+    out = _native().quantize_tokens(x)
+    if out is not NotImplemented:
+        return out
+    _token_operand("quantize_tokens", x, _FLOATS)
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise TsxError("quantize_tokens: rows without values, %s" % (tuple(x.shape),))
+    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    if x.numel():
+        with torch.cuda.device(x.device):
+            x, rows, stride = _rows(x)
+            check(lib().tsx_quantize_tokens(rows, x.shape[-1], _ptr(x), _TYPES[x.dtype], stride, _ptr(q), x.shape[-1], _ptr(scales), _stream()))
+    return q, scales
+
+
+class TokenGemmI8:
+    """int8 product with a scale for each token and each channel, with packed weights: w_i8 is [n][k], or [k][n] where
+    transpose is false, w_scales [n] what one step of a channel stands for; bias [n]."""
+
+    def __init__(self, w_i8, w_scales, bias=None, transpose=True):
+        self.w = _dev(_token_operand("weights", w_i8, (torch.int8,)), torch.int8)
+        if self.w.dim() != 2 or 0 in self.w.shape:
+            raise TsxError("weights of shape %s" % (tuple(self.w.shape),))
+        self.transpose = bool(transpose)
+        self.n, self.k = (self.w.shape if self.transpose else self.w.shape[::-1])
+        if w_scales is None:
+            raise TsxError("weights need a scale for each channel")
+        self.w_scales = _vector("w_scales", w_scales, self.n, self.w)
+        self.bias = _vector("bias", bias, self.n, self.w)
+        with torch.cuda.device(self.w.device):
+            self.packed = torch.empty(lib().tsx_gemm_i8_packed_weight_bytes(self.k, self.n), dtype=torch.uint8, device=self.w.device)
+            check(lib().tsx_gemm_i8_pack_weights(self.k, self.n, int(self.transpose), _ptr(self.w), _ptr(self.packed), _stream()))
+
+    @classmethod
+    def from_float(cls, w, bias=None):
+        """Weights [n][k] in fp32, fp16 or bf16, each channel quantized by its own largest magnitude."""
+        q, scales = quantize_tokens(w)
+        return cls(q, scales, bias)
+
+    def __call__(self, x, x_scales=None, act=None, slope=0.0, out_dtype=None):
+        """x [..., k] in fp32, fp16 or bf16, quantized token by token in the call; or int8 with x_scales [...], as
+        quantize_tokens and group_norm_tokens give them.  Returns [..., n] in out_dtype, by default x's type (int8: fp32)."""
+        act = _token_act(act)
+        if out_dtype is None and x_scales is not None:
+            out_dtype = torch.float32
+        out = _native_module.token_gemm(self.packed, self.k, self.n, self.w_scales, self.bias, x, x_scales, act, slope,
+                                        -1 if out_dtype is None else _TYPES.get(out_dtype, 3))
+        if out is not NotImplemented:
+            return out
+        _token_operand("token product", x, _FLOATS + (torch.int8,))
+        if x.device != self.w.device:
+            raise TsxError("tokens on %s, weights on %s" % (x.device, self.w.device))
+        if x.dim() < 1 or x.shape[-1] != self.k:
+            raise TsxError("tokens of shape %s, weights of %d rows" % (tuple(x.shape), self.k))
+        if (x.dtype == torch.int8) != (x_scales is not None):
+            raise TsxError("int8 tokens come with their scales, others without")
+        out_dtype = out_dtype or x.dtype
+        if out_dtype not in _FLOATS:
+            raise TsxError("token product: output type %s" % out_dtype)
+        out = torch.empty(x.shape[:-1] + (self.n,), dtype=out_dtype, device=x.device)
+        x_scales = _vector("x_scales", x_scales, x.numel() // self.k, x)
+        if x.numel() == 0:
+            return out
+        with torch.cuda.device(x.device):
+            x, rows, stride = _rows(x)
+            g = TokenGemm(rows, self.n, self.k, _TYPES[x.dtype], _TYPES[out_dtype], act, float(slope), _ptr(x), stride, _ptr(x_scales),
+                          _ptr(self.packed), _ptr(self.w_scales), _ptr(self.bias), _ptr(out), self.n)
+            nbytes = lib().tsx_gemm_i8_tokens_workspace_bytes(ctypes.byref(g))
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+            check(lib().tsx_gemm_i8_tokens(ctypes.byref(g), _ptr(workspace), nbytes, _stream()))
+        return out
+
+
+def _group_norm(x, groups, weight, bias, epsilon, act, slope, tokens):
+    act = _token_act(act)
+    out = _native().group_norm(x, groups, weight, bias, epsilon, act, slope, tokens)
+    if out is not NotImplemented:
+        return out
+    _token_operand("group_norm", x, _FLOATS)
+    if x.dim() < 2 or x.shape[-1] == 0:
+        raise TsxError("group_norm: shape %s ([n, ..., c] expected)" % (tuple(x.shape),))
+    n, c = x.shape[0], x.shape[-1]
+    weight, bias = _vector("weight", weight, c, x), _vector("bias", bias, c, x)
+    out = torch.empty(x.shape, dtype=torch.int8 if tokens else x.dtype, device=x.device)
+    scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if tokens else None
+    with torch.cuda.device(x.device):
+        pixels = _axis(x, 1, x.dim() - 1)
+        if pixels is None or (c > 1 and x.stride(-1) != 1) or (pixels[0] > 1 and pixels[1] < c) or x.stride(0) < 0:
+            x = x.contiguous()
+            pixels = _axis(x, 1, x.dim() - 1)
+        g = GroupNorm(n, c, int(groups), _TYPES[x.dtype], pixels[0], x.stride(0), pixels[1] if pixels[0] > 1 else c, _ptr(x), _ptr(weight),
+                      _ptr(bias), float(epsilon), act, float(slope))
+        nbytes = lib().tsx_group_norm_workspace_bytes(ctypes.byref(g))
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+        if tokens:
+            check(lib().tsx_group_norm_tokens_nhwc(ctypes.byref(g), _ptr(out), _ptr(scales), _ptr(workspace), nbytes, _stream()))
+        else:
+            check(lib().tsx_group_norm_nhwc(ctypes.byref(g), _ptr(out), _ptr(workspace), nbytes, _stream()))
+    return (out, scales) if tokens else out
+
+
+def group_norm(x, groups, weight=None, bias=None, epsilon=1e-5, act=None, slope=0.0):
+    """tsx_group_norm_nhwc: group norm and an activation on channels-last x [n, ..., c] in fp32, fp16 or bf16 (a tensor of torch's
+    channels_last format is one as x.permute(0, 2, 3, 1)); weight and bias [c].  Returns a dense tensor of x's shape and type."""
+    return _group_norm(x, groups, weight, bias, epsilon, act, slope, False)
+
+
+def group_norm_tokens(x, groups, weight=None, bias=None, epsilon=1e-5, act=None, slope=0.0):
+    """tsx_group_norm_tokens_nhwc: the same as int8 tokens, a pixel a token: (q of x's shape, scales of x.shape[:-1]), what
+    TokenGemmI8 takes."""
+    return _group_norm(x, groups, weight, bias, epsilon, act, slope, True)
 
 
 def conv2d_f32(x, w, pads=(0, 0, 0, 0), strides=(1, 1), dilations=(1, 1), padding_value=0.0, bias=None, act=None,

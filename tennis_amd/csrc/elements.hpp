@@ -1,0 +1,160 @@
+// Tensors of fp32, fp16 and bf16 values: runs of them to and from registers, their magnitudes, and their rows as int8 tokens.
+// All arithmetic on them is in fp32; a result is rounded once, to nearest even, when it is stored.
+#pragma once
+#include "tsx_common.hpp"
+
+namespace tsx {
+
+inline size_t element_bytes(int type) { return type == TSX_TYPE_F32 ? 4 : type == TSX_TYPE_I8 ? 1 : 2; }
+inline bool is_float_type(int type) { return type == TSX_TYPE_F32 || type == TSX_TYPE_F16 || type == TSX_TYPE_BF16; }
+inline bool is_token_act(int act) {      // the exact Mish is the host's bits for a given fp32 number, which no sum here has
+    return act == TSX_ACT_NONE || act == TSX_ACT_RELU || act == TSX_ACT_LEAKY_RELU || act == TSX_ACT_MISH_FAST || act == TSX_ACT_SILU;
+}
+
+#ifdef __HIPCC__
+
+typedef unsigned v2u __attribute__((ext_vector_type(2)));
+typedef unsigned v4u __attribute__((ext_vector_type(4)));
+// at any address: global memory takes 16 bytes wherever they begin
+typedef unsigned v2u_any __attribute__((ext_vector_type(2), aligned(1)));
+typedef unsigned v4u_any __attribute__((ext_vector_type(4), aligned(1)));
+
+// N consecutive values as they lie in memory
+template <int TYPE, int N>
+struct Run {
+    static constexpr int BYTES = N * (TYPE == TSX_TYPE_F32 ? 4 : 2), WORDS = BYTES / 4, PER_WORD = TYPE == TSX_TYPE_F32 ? 1 : 2;
+    static_assert(BYTES % 8 == 0, "whole pairs of words");
+    unsigned word[WORDS];
+
+    __device__ __forceinline__ void clear() {
+        static_for<0, WORDS>([&](auto wc) { word[decltype(wc)::value] = 0; });
+    }
+    __device__ __forceinline__ void load(const void *at) {
+        if constexpr (BYTES % 16 == 0)
+            static_for<0, BYTES / 16>([&](auto wc) {
+                constexpr int w = decltype(wc)::value;
+                const v4u v = reinterpret_cast<const v4u_any *>(at)[w];
+                static_for<0, 4>([&](auto jc) { word[4 * w + decltype(jc)::value] = v[decltype(jc)::value]; });
+            });
+        else
+            static_for<0, BYTES / 8>([&](auto wc) {
+                constexpr int w = decltype(wc)::value;
+                const v2u v = reinterpret_cast<const v2u_any *>(at)[w];
+                static_for<0, 2>([&](auto jc) { word[2 * w + decltype(jc)::value] = v[decltype(jc)::value]; });
+            });
+    }
+    // the first `left` values, behind them zeros
+    __device__ __forceinline__ void load_some(const void *at, int left) {
+        static_for<0, WORDS>([&](auto wc) {
+            constexpr int w = decltype(wc)::value;
+            if constexpr (TYPE == TSX_TYPE_F32) {
+                word[w] = w < left ? reinterpret_cast<const unsigned *>(at)[w] : 0u;
+            } else {
+                const unsigned short *h = reinterpret_cast<const unsigned short *>(at);
+                const unsigned lo = 2 * w < left ? h[2 * w] : 0, hi = 2 * w + 1 < left ? h[2 * w + 1] : 0;
+                word[w] = lo | hi << 16;
+            }
+        });
+    }
+    __device__ __forceinline__ void store(void *at) const {
+        if constexpr (BYTES % 16 == 0)
+            static_for<0, BYTES / 16>([&](auto wc) {
+                constexpr int w = decltype(wc)::value;
+                reinterpret_cast<v4u_any *>(at)[w] = v4u{word[4 * w], word[4 * w + 1], word[4 * w + 2], word[4 * w + 3]};
+            });
+        else
+            static_for<0, BYTES / 8>([&](auto wc) {
+                constexpr int w = decltype(wc)::value;
+                reinterpret_cast<v2u_any *>(at)[w] = v2u{word[2 * w], word[2 * w + 1]};
+            });
+    }
+    __device__ __forceinline__ void store_some(void *at, int left) const {
+        static_for<0, N>([&](auto ec) {
+            constexpr int e = decltype(ec)::value;
+            if (e < left) {
+                if constexpr (TYPE == TSX_TYPE_F32) reinterpret_cast<unsigned *>(at)[e] = word[e];
+                else reinterpret_cast<unsigned short *>(at)[e] = (unsigned short)(word[e / 2] >> (16 * (e % 2)));
+            }
+        });
+    }
+    template <int E>
+    __device__ __forceinline__ float get() const {
+        if constexpr (TYPE == TSX_TYPE_F32) return __builtin_bit_cast(float, word[E]);
+        else if constexpr (TYPE == TSX_TYPE_BF16) return __builtin_bit_cast(float, E % 2 ? word[E / 2] & 0xffff0000u : word[E / 2] << 16);
+        else return float(__builtin_bit_cast(_Float16, (unsigned short)(word[E / 2] >> (16 * (E % 2)))));
+    }
+    __device__ __forceinline__ void set(const float (&v)[N]) {
+        static_for<0, WORDS>([&](auto wc) {
+            constexpr int w = decltype(wc)::value;
+            if constexpr (TYPE == TSX_TYPE_F32) {
+                word[w] = __builtin_bit_cast(unsigned, v[w]);
+            } else if constexpr (TYPE == TSX_TYPE_BF16) {
+                typedef __bf16 pair __attribute__((ext_vector_type(2)));
+                typedef float two __attribute__((ext_vector_type(2)));
+                word[w] = __builtin_bit_cast(unsigned, __builtin_convertvector((two{v[2 * w], v[2 * w + 1]}), pair));
+            } else {
+                typedef _Float16 pair __attribute__((ext_vector_type(2)));
+                word[w] = __builtin_bit_cast(unsigned, pair{_Float16(v[2 * w]), _Float16(v[2 * w + 1])});
+            }
+        });
+    }
+    // The largest magnitude as the bits of that magnitude, which sort as whole numbers do: two 16-bit ones a word, or one of 32.
+    // Infinities and NaN are the largest.
+    __device__ __forceinline__ unsigned top(unsigned so_far) const {
+        static_for<0, WORDS>([&](auto wc) { so_far = larger<TYPE>(so_far, word[decltype(wc)::value] & (PER_WORD == 1 ? 0x7fffffffu : 0x7fff7fffu)); });
+        return so_far;
+    }
+    template <int KIND>
+    static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) {
+        if constexpr (KIND == TSX_TYPE_F32) return a > b ? a : b;
+        typedef unsigned short pair __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(pair, a), __builtin_bit_cast(pair, b)));
+    }
+};
+
+// the magnitude that Run::top found, as an fp32 number
+template <int TYPE>
+__device__ __forceinline__ float top_value(unsigned top) {
+    if constexpr (TYPE == TSX_TYPE_F32) return __builtin_bit_cast(float, top);
+    const unsigned lo = top & 0xffffu, hi = top >> 16, most = lo > hi ? lo : hi;
+    if constexpr (TYPE == TSX_TYPE_BF16) return __builtin_bit_cast(float, most << 16);
+    return float(__builtin_bit_cast(_Float16, (unsigned short)most));
+}
+
+// A token's way to int8: the largest magnitude a of a row becomes 127.
+//   scale = fp32(a / 127),  q = round to nearest even of x * fp32(127 / a), the product exact.
+// Rows below 2^-64, where 127 / a would leave fp32, are lifted by 2^64 first; a row with an infinity or NaN has zeros and the scale NaN.
+struct TokenScale {
+    float lift, reciprocal, scale;
+    __device__ __forceinline__ explicit TokenScale(float top) {
+        const bool finite = top < __builtin_inff();      // false for NaN
+        lift = top < 0x1p-64f ? 0x1p64f : 1.f;
+        reciprocal = finite && top > 0.f ? __fdiv_rn(127.f, __fmul_rn(top, lift)) : 0.f;
+        scale = finite ? __fdiv_rn(top, 127.f) : __builtin_nanf("");
+    }
+    // One fused multiply-add: behind 1.5 * 2^23 the sum's last bit is 1, so its rounding, half to even, is that of the exact
+    // product, and its low byte is the product in two's complement.  0 * infinity never gets here: then `reciprocal` is 0 and
+    // the caller takes zeros (an infinity in the row), or x is finite.
+    __device__ __forceinline__ unsigned bits(float x) const { return __builtin_bit_cast(unsigned, __builtin_fmaf(x, reciprocal, 0x1.8p23f)); }
+};
+__device__ __forceinline__ unsigned low_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
+    return __builtin_amdgcn_perm(b, a, 0x0c0c0400u) | __builtin_amdgcn_perm(d, c, 0x04000c0cu);
+}
+
+// silu and the activations of the epilogues on results of fp32 arithmetic
+__device__ __forceinline__ float silu(float x) {
+    return __fmul_rn(x, __builtin_amdgcn_rcpf(__fadd_rn(1.f, __builtin_amdgcn_exp2f(__fmul_rn(x, -1.4426950216293335f)))));
+}
+template <int N>
+__device__ __forceinline__ void activate_tokens(float (&v)[N], int act, float slope) {
+    if (act == TSX_ACT_SILU) {
+        asm volatile("; silu");
+        static_for<0, N>([&](auto rc) { constexpr int r = decltype(rc)::value; v[r] = silu(v[r]); });
+    } else {
+        activate_results(v, act, slope);
+    }
+}
+
+#endif  // __HIPCC__
+
+}  // namespace tsx

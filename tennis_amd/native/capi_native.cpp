@@ -11,6 +11,7 @@
 
 #include <ATen/core/TensorBase.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -32,7 +33,9 @@ namespace {
     X(tsx_batch_norm_f32) X(tsx_batch_scale_f32) X(tsx_fused_batch_norm_f32) X(tsx_depthwise_conv2d_f32)                    \
     X(tsx_pooling2d_out_size) X(tsx_pooling2d_f32) X(tsx_max_pooling2d_i8_staged) X(tsx_winograd_f63_workspace_bytes)       \
     X(tsx_winograd_f63_fast_workspace_bytes) X(tsx_winograd_f23_workspace_bytes) X(tsx_conv2d_winograd_f63_nchw)            \
-    X(tsx_conv2d_winograd_f63_fast_nchw) X(tsx_conv2d_winograd_f23_nchw)
+    X(tsx_conv2d_winograd_f63_fast_nchw) X(tsx_conv2d_winograd_f23_nchw) X(tsx_quantize_tokens)                             \
+    X(tsx_gemm_i8_tokens_workspace_bytes) X(tsx_gemm_i8_tokens) X(tsx_group_norm_workspace_bytes) X(tsx_group_norm_nhwc)    \
+    X(tsx_group_norm_tokens_nhwc)
 
 struct Library {
 #define X(name) decltype(&::name) name;
@@ -674,6 +677,147 @@ PyObject *conv_i8_staged(PyObject *const *a, Py_ssize_t) {
     return results(out_f32, out_i8);
 }
 
+// ---- tokens and channels-last tensors
+
+int32_t type_code(c10::ScalarType t) {
+    switch (t) {
+        case c10::kFloat: return TSX_TYPE_F32;
+        case c10::kHalf: return TSX_TYPE_F16;
+        case c10::kBFloat16: return TSX_TYPE_BF16;
+        case c10::kChar: return TSX_TYPE_I8;
+        default: throw Decline{};
+    }
+}
+
+// a tensor of the current device, at any strides
+const at::Tensor &strided(PyObject *o) {
+    if (!THPVariable_Check(o)) throw Decline{};
+    const at::Tensor &t = THPVariable_Unpack(o);
+    if (!t.is_cuda() || t.get_device() != c10::hip::current_device() || t.is_conj() || t.is_neg()) throw Decline{};
+    return t;
+}
+const float *f32_of(PyObject *o, int64_t count) {      // fp32 values, or None
+    if (o == Py_None) return nullptr;
+    const at::Tensor &t = f32(o);
+    if (t.numel() != count || t.get_device() != c10::hip::current_device()) throw Decline{};
+    return t.const_data_ptr<float>();
+}
+
+// Axes [first, last) of a tensor as one: their count, and the stride between neighbours (0: there are no two)
+struct Axis {
+    int64_t count = 1, stride = 0;
+    Axis(const at::Tensor &t, int64_t first, int64_t last) {
+        for (int64_t d = last - 1; d >= first; --d) {
+            const int64_t size = t.size(d);
+            if (size != 1) {
+                if (count > 1 && t.stride(d) != stride * count) throw Decline{};
+                if (count == 1) stride = t.stride(d);
+            }
+            count *= size;
+        }
+    }
+};
+
+struct Rows {                                          // x as rows of its last axis
+    int64_t rows, stride;
+    int32_t cols;
+    explicit Rows(const at::Tensor &x) {
+        if (x.dim() < 1 || x.numel() == 0) throw Decline{};
+        const int64_t k = x.size(-1);
+        if ((k > 1 && x.stride(-1) != 1) || k > 1 << 30) throw Decline{};
+        const Axis lead(x, 0, x.dim() - 1);
+        rows = lead.count;
+        stride = rows > 1 ? lead.stride : k;
+        cols = int32_t(k);
+        if (stride < k) throw Decline{};
+    }
+};
+
+PyObject *quantize_tokens(PyObject *const *a, Py_ssize_t) {           // x
+    const at::Tensor &x = strided(a[0]);
+    const int32_t type = type_code(x.scalar_type());
+    if (type == TSX_TYPE_I8) throw Decline{};
+    const Rows r(x);
+    at::TensorBase q, scales;
+    launch([&] {
+        q = empty(x.sizes(), c10::kChar, x);
+        scales = empty(x.sizes().slice(0, x.dim() - 1), c10::kFloat, x);
+        return L.tsx_quantize_tokens(r.rows, r.cols, x.const_data_ptr(), type, r.stride, data<int8_t>(q), r.cols, data<float>(scales), stream());
+    });
+    return results(q, scales);
+}
+
+PyObject *token_gemm(PyObject *const *a, Py_ssize_t) {                // packed, k, n, w_scales, bias, x, x_scales, act, slope, out_type
+    const at::Tensor &packed = tensor(a[0], c10::kByte), &x = strided(a[5]);
+    tsx_token_gemm g{};
+    g.k = int32_t(integer(a[1]));
+    g.n = int32_t(integer(a[2]));
+    const Rows r(x);
+    if (r.cols != g.k || r.rows >= 1 << 30 || packed.get_device() != x.get_device()) throw Decline{};
+    g.m = int32_t(r.rows);
+    g.x_type = type_code(x.scalar_type());
+    g.x_stride = r.stride;
+    g.x_dev = x.const_data_ptr();
+    g.w_scales_dev = f32_of(a[3], g.n);
+    g.bias_dev = f32_of(a[4], g.n);
+    g.x_scales_dev = f32_of(a[6], r.rows);
+    if (!g.w_scales_dev || (g.x_type == TSX_TYPE_I8) != (g.x_scales_dev != nullptr)) throw Decline{};
+    g.act = int32_t(integer(a[7]));
+    g.slope = float(number(a[8]));
+    const long out_type = integer(a[9]);
+    if (out_type > TSX_TYPE_BF16 || (out_type < 0 && g.x_type == TSX_TYPE_I8)) throw Decline{};
+    g.out_type = out_type < 0 ? g.x_type : int32_t(out_type);
+    g.out_stride = g.n;
+    g.packed_w_dev = packed.const_data_ptr();
+    at::TensorBase out;
+    launch([&] {
+        c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
+        shape.back() = g.n;
+        out = empty(shape, g.out_type == TSX_TYPE_F32 ? c10::kFloat : g.out_type == TSX_TYPE_F16 ? c10::kHalf : c10::kBFloat16, x);
+        g.out_dev = out.mutable_data_ptr();
+        const size_t bytes = L.tsx_gemm_i8_tokens_workspace_bytes(&g);
+        at::TensorBase workspace;     // the allocator's again when the call is enqueued, for what follows on this stream
+        if (bytes) workspace = empty({int64_t(bytes)}, c10::kByte, x);
+        return L.tsx_gemm_i8_tokens(&g, data<void>(workspace), bytes, stream());
+    });
+    return wrap(out);
+}
+
+PyObject *group_norm(PyObject *const *a, Py_ssize_t) {                // x, groups, weight, bias, epsilon, act, slope, tokens
+    const at::Tensor &x = strided(a[0]);
+    if (x.dim() < 2 || x.numel() == 0) throw Decline{};
+    tsx_group_norm g{};
+    g.type = type_code(x.scalar_type());
+    const int64_t c = x.size(-1);
+    if (g.type == TSX_TYPE_I8 || (c > 1 && x.stride(-1) != 1) || c > 1 << 20 || x.size(0) >= 65536) throw Decline{};
+    const Axis pixels(x, 1, x.dim() - 1);
+    g.n = int32_t(x.size(0));
+    g.c = int32_t(c);
+    g.groups = int32_t(integer(a[1]));
+    g.pixels = pixels.count;
+    g.pixel_stride = pixels.count > 1 ? pixels.stride : c;
+    g.image_stride = x.stride(0);
+    if (g.pixel_stride < c) throw Decline{};
+    g.x_dev = x.const_data_ptr();
+    g.weight_dev = f32_of(a[2], c);
+    g.bias_dev = f32_of(a[3], c);
+    g.epsilon = float(number(a[4]));
+    g.act = int32_t(integer(a[5]));
+    g.slope = float(number(a[6]));
+    const bool tokens = truth(a[7]);
+    at::TensorBase out, scales;
+    launch([&] {
+        const size_t bytes = L.tsx_group_norm_workspace_bytes(&g);
+        at::TensorBase workspace;
+        if (bytes) workspace = empty({int64_t(bytes)}, c10::kByte, x);
+        out = empty(x.sizes(), tokens ? c10::kChar : x.scalar_type(), x);
+        if (!tokens) return L.tsx_group_norm_nhwc(&g, out.mutable_data_ptr(), data<void>(workspace), bytes, stream());
+        scales = empty(x.sizes().slice(0, x.dim() - 1), c10::kFloat, x);
+        return L.tsx_group_norm_tokens_nhwc(&g, data<int8_t>(out), data<float>(scales), data<void>(workspace), bytes, stream());
+    });
+    return tokens ? results(out, scales) : wrap(out);
+}
+
 // ---- module
 
 PyObject *bind(PyObject *, PyObject *args) {           // {entry point: address}, TsxError
@@ -704,6 +848,7 @@ PyMethodDef methods[] = {
     TSX_METHOD(unary, 3), TSX_METHOD(add, 5), TSX_METHOD(mul, 2), TSX_METHOD(quantize, 2), TSX_METHOD(add_bias, 3), TSX_METHOD(batch_norm, 7),
     TSX_METHOD(pooling2d, 6), TSX_METHOD(max_pooling2d_staged, 5), TSX_METHOD(conv2d_f32, 9), TSX_METHOD(depthwise_conv2d, 9),
     TSX_METHOD(inner_prod_f32, 3), TSX_METHOD(winograd, 10), TSX_METHOD(gemm_i8, 13), TSX_METHOD(conv_i8, 14), TSX_METHOD(conv_i8_staged, 12),
+    TSX_METHOD(quantize_tokens, 1), TSX_METHOD(token_gemm, 10), TSX_METHOD(group_norm, 8),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tsx_native", "The host work of tennis_amd.capi's calls.", -1, methods, nullptr, nullptr, nullptr, nullptr};
