@@ -11,6 +11,18 @@ inline bool is_token_act(int act) {      // the exact Mish is the host's bits fo
     return act == TSX_ACT_NONE || act == TSX_ACT_RELU || act == TSX_ACT_LEAKY_RELU || act == TSX_ACT_MISH_FAST || act == TSX_ACT_SILU;
 }
 
+// f(the activation as a constant)
+template <class F>
+auto with_act(int act, F &&f) {
+    switch (act) {
+        case TSX_ACT_RELU: return f(std::integral_constant<int, TSX_ACT_RELU>{});
+        case TSX_ACT_LEAKY_RELU: return f(std::integral_constant<int, TSX_ACT_LEAKY_RELU>{});
+        case TSX_ACT_MISH_FAST: return f(std::integral_constant<int, TSX_ACT_MISH_FAST>{});
+        case TSX_ACT_SILU: return f(std::integral_constant<int, TSX_ACT_SILU>{});
+        default: return f(std::integral_constant<int, TSX_ACT_NONE>{});
+    }
+}
+
 #ifdef __HIPCC__
 
 typedef unsigned v2u __attribute__((ext_vector_type(2)));
@@ -19,6 +31,9 @@ typedef unsigned v4u __attribute__((ext_vector_type(4)));
 typedef unsigned v2u_any __attribute__((ext_vector_type(2), aligned(1)));
 typedef unsigned v4u_any __attribute__((ext_vector_type(4), aligned(1)));
 
+// a value the compiler knows nothing of: not what it was computed from, nor that it is the same one later
+__device__ __forceinline__ void renew(unsigned &word) { asm volatile("" : "+v"(word)); }
+
 // N consecutive values as they lie in memory
 template <int TYPE, int N>
 struct Run {
@@ -26,6 +41,9 @@ struct Run {
     static_assert(BYTES % 8 == 0, "whole pairs of words");
     unsigned word[WORDS];
 
+    __device__ __forceinline__ void renew_words() {
+        static_for<0, WORDS>([&](auto wc) { renew(word[decltype(wc)::value]); });
+    }
     __device__ __forceinline__ void clear() {
         static_for<0, WORDS>([&](auto wc) { word[decltype(wc)::value] = 0; });
     }
@@ -144,6 +162,18 @@ __device__ __forceinline__ unsigned low_bytes(unsigned a, unsigned b, unsigned c
 // silu and the activations of the epilogues on results of fp32 arithmetic
 __device__ __forceinline__ float silu(float x) {
     return __fmul_rn(x, __builtin_amdgcn_rcpf(__fadd_rn(1.f, __builtin_amdgcn_exp2f(__fmul_rn(x, -1.4426950216293335f)))));
+}
+// The activation as a constant of the code: kernels bound by their arithmetic have a path for each, since five of them in turn
+// behind each other's branches put every one an instruction-cache miss apart.
+template <int ACT, int N>
+__device__ __forceinline__ void activate_as(float (&v)[N], float slope) {
+    static_for<0, N>([&](auto rc) {
+        constexpr int r = decltype(rc)::value;
+        if constexpr (ACT == TSX_ACT_RELU) v[r] = max_zero(v[r]);
+        if constexpr (ACT == TSX_ACT_LEAKY_RELU) v[r] = __builtin_fmaf(slope, min_zero(v[r]), max_zero(v[r]));
+        if constexpr (ACT == TSX_ACT_MISH_FAST) v[r] = mish_short(v[r]);
+        if constexpr (ACT == TSX_ACT_SILU) v[r] = silu(v[r]);
+    });
 }
 template <int N>
 __device__ __forceinline__ void activate_tokens(float (&v)[N], int act, float slope) {

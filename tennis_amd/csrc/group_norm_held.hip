@@ -1,0 +1,226 @@
+// Group norm in one launch, where the pixels of a few groups are what one workgroup's registers hold.
+//
+// A workgroup takes B groups of one image, B * d channels of every pixel: whole pieces of V values.  Its threads hold them from the one
+// read to the one write; in between the mean, as the sum over all of them, and then the sums of x - mean and of its square, whose first
+// corrects the mean's rounding.  Two kernels read the tensor twice and wait for each other: 8 x 8 x 1280 on 2 images 21 us there.
+#include <algorithm>
+
+#include "group_norm.hpp"
+
+namespace tsx {
+namespace {
+
+struct HeldParams : NormParams {
+    int B, pieces_a_pixel, held_lanes, bundles, per_xcd;
+    int TG, TL;                        // threads that sum one group's entries, of them on lanes of their own
+};
+
+template <int TYPE, int V, int NP, int ACT>
+__global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_held_kernel(HeldParams p) {
+    extern __shared__ float entries[];                       // [2][lanes][pitch]
+    __shared__ float2 group[NORM_MOST_THREADS];
+    __shared__ float2 waves[NORM_MOST_THREADS / 64];
+    constexpr int SIZE = Kind<TYPE>::SIZE;
+    const int t = threadIdx.x, lanes = p.held_lanes, channels = p.B * p.d, row_entries = channels / p.run, pitch = row_entries | 1;
+    // consecutive bundles of an image on one XCD: they share cache lines
+    const int id = int(blockIdx.x % 8) * p.per_xcd + int(blockIdx.x / 8);
+    if (int(blockIdx.x / 8) >= p.per_xcd || id >= p.bundles) return;       // uniform
+    const int a_image = p.groups / p.B, image = id / a_image, ch0 = (id - image * a_image) * channels, pixels = int(p.pixels);
+    const int lane = t / p.pieces_a_pixel, j = t - lane * p.pieces_a_pixel;
+    const bool mine = lane < lanes;
+    const char *const x = static_cast<const char *>(p.x) + (int64_t(image) * p.image_stride + ch0 + j * V) * SIZE;
+    Run<TYPE, V> v[NP];
+    static_for<0, NP>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        v[i].clear();
+        if (mine && lane + i * lanes < pixels) v[i].load(x + int64_t(lane + i * lanes) * p.pixel_stride * SIZE);
+    });
+    // The packed words anew for each pass over them: unpacked once for all three they would be twice as many registers.
+    auto again = [&] { static_for<0, NP>([&](auto ic) { v[decltype(ic)::value].renew_words(); }); };
+    // `leave`: a thread's V sums into LDS, neighbours of one group added up
+    auto leave = [&](float *to, float (&s)[V]) __attribute__((always_inline)) {
+        join_runs<V>(p.run, [&](auto ac, auto fc) { constexpr int a = decltype(ac)::value; s[a] += s[a + decltype(fc)::value]; });
+        if (!mine) return;
+        int at = lane * pitch + j * V / p.run;
+        static_for<0, V>([&](auto ec) { if ((decltype(ec)::value & (p.run - 1)) == 0) to[at++] = s[decltype(ec)::value]; });
+    };
+    // The sums of both arrays over a group's entries, for the TG threads of that group
+    const int g = t / p.TG, tg = t % p.TG, tl = tg % p.TL, te = tg / p.TL, TE = p.TG / p.TL, group_entries = p.d / p.run;
+    const float *const second = entries + lanes * pitch;
+    auto gather = [&](bool both) __attribute__((always_inline)) {
+        float2 s = {0.f, 0.f};
+        if (g < p.B)
+            for (int l = tl; l < lanes; l += p.TL)
+                for (int k = te; k < group_entries; k += TE) {
+                    const int at = l * pitch + g * group_entries + k;
+                    s.x += entries[at];
+                    if (both) s.y += second[at];
+                }
+        const int width = min(p.TG, 64);
+        s.x = sum_of(s.x, width);
+        if (both) s.y = sum_of(s.y, width);
+        if (p.TG > 64) {                                     // uniform
+            if (t % 64 == 0) waves[t / 64] = s;
+            __syncthreads();
+            s = float2{0.f, 0.f};
+            for (int w = 0; w < p.TG / 64; ++w) {
+                const float2 part = waves[g * (p.TG / 64) + w];
+                s.x += part.x;
+                s.y += part.y;
+            }
+        }
+        return s;
+    };
+    const float of_count = 1.f / (float(pixels) * float(p.d));
+    float sum[V];
+    static_for<0, V>([&](auto ec) { sum[decltype(ec)::value] = 0.f; });
+    static_for<0, NP>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        static_for<0, V>([&](auto ec) { constexpr int e = decltype(ec)::value; sum[e] += v[i].template get<e>(); });
+    });
+    leave(entries, sum);
+    __syncthreads();
+    const float rough = gather(false).x * of_count;
+    if (tg == 0 && g < p.B) group[g] = float2{rough, 0.f};
+    __syncthreads();
+    again();
+    float square[V], mean[V];
+    {
+        int gi = mine ? j * V / p.d : 0, left = (gi + 1) * p.d - j * V;
+        static_for<0, V>([&](auto ec) {
+            constexpr int e = decltype(ec)::value;
+            mean[e] = group[gi].x;
+            if (--left == 0) left = p.d, gi = min(gi + 1, p.B - 1);
+            sum[e] = square[e] = 0.f;
+        });
+    }
+    static_for<0, NP>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        if (lane + i * lanes < pixels)
+            static_for<0, V>([&](auto ec) {
+                constexpr int e = decltype(ec)::value;
+                const float d = v[i].template get<e>() - mean[e];
+                sum[e] += d;
+                square[e] = __builtin_fmaf(d, d, square[e]);
+            });
+    });
+    leave(entries, sum);
+    leave(entries + lanes * pitch, square);
+    __syncthreads();
+    const float2 total = gather(true);
+    if (tg == 0 && g < p.B) {
+        const float shift = total.x * of_count, squares = __builtin_fmaf(-shift, total.x, total.y);
+        // a NaN stays one (fmaxf drops it)
+        group[g] = float2{rough + shift, 1.f / sqrtf((squares == squares ? fmaxf(squares, 0.f) * of_count : squares) + p.epsilon)};
+    }
+    __syncthreads();
+    if (!mine) return;
+    again();
+    const Affine<V> affine(p, group, j * V, channels, p.weight ? p.weight + ch0 : nullptr, p.bias ? p.bias + ch0 : nullptr);
+    char *const out = static_cast<char *>(p.out) + (int64_t(image) * pixels * p.c + ch0 + j * V) * SIZE;
+    static_for<0, NP>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        if (lane + i * lanes < pixels) {
+            Piece<TYPE, V> a;
+            static_for<0, V>([&](auto ec) { a.v[decltype(ec)::value] = v[i].template get<decltype(ec)::value>(); });
+            affine.template apply<ACT>(p.act, p.slope, a);
+            a.store(out, int64_t(lane + i * lanes) * p.c, V);
+        }
+    });
+}
+
+int power_of_two(int v) {      // the next one up
+    int p = 1;
+    while (p < v) p *= 2;
+    return p;
+}
+
+// Whether the one-launch kernel takes the call, on which pieces and threads: V = 0, it does not.
+struct HeldPlan {
+    HeldParams p;
+    int V, NP, threads;
+};
+
+HeldPlan held_plan(const tsx_group_norm *g, const NormParams &rows) {
+    HeldPlan best{};
+    float best_cost = 0.f;
+    if (g->pixels > 16384) return best;
+    const int pixels = int(g->pixels), d = g->c / g->groups, whole = g->type == TSX_TYPE_F32 ? 4 : 8;
+    for (int V = whole; V >= 4; V -= 4)
+        for (int B = 1; B <= g->groups; ++B) {
+            if (g->groups % B || B * d % V) continue;
+            const int a_pixel = B * d / V;
+            if (a_pixel > NORM_MOST_THREADS) break;
+            const int most = V == 8 ? 12 : g->type == TSX_TYPE_F32 ? 16 : 24;      // what 128 registers hold beside the rest
+            int threads = 256;
+            while (threads < NORM_MOST_THREADS && (threads < a_pixel || ceil_div(pixels, threads / a_pixel) > 4)) threads *= 2;
+            const int lanes = threads / a_pixel, need = int(ceil_div(pixels, lanes));
+            if (need > most) break;
+            if (power_of_two(B) > threads) continue;
+            const int64_t bundles = int64_t(g->n) * (g->groups / B);
+            if (bundles > 1 << 24) continue;
+            const float cost = float(ceil_div(bundles, 256)) * float(pixels) * float(B * d) / 8000.f;
+            if (best.V && cost >= best_cost) continue;
+            best_cost = cost;
+            best.V = V;
+            best.NP = need;
+            best.threads = threads;
+            HeldParams &p = best.p;
+            static_cast<NormParams &>(p) = rows;
+            p.run = gcd(d, V);
+            p.B = B;
+            p.pieces_a_pixel = a_pixel;
+            p.held_lanes = lanes;
+            p.bundles = int(bundles);
+            p.per_xcd = int(ceil_div(bundles, 8));
+            p.TG = threads / power_of_two(B);
+            p.TL = std::min(p.TG, power_of_two(lanes));
+        }
+    return best;
+}
+
+template <int TYPE, int V, int NP>
+int launch_held(const HeldPlan &h, hipStream_t stream) {
+    const HeldParams &p = h.p;
+    const size_t lds = size_t(p.held_lanes) * ((p.B * p.d / p.run) | 1) * 2 * sizeof(float);
+    const auto kernel = p.act == TSX_ACT_SILU ? group_norm_held_kernel<TYPE, V, NP, TSX_ACT_SILU> : group_norm_held_kernel<TYPE, V, NP, ANY_ACT>;
+    if (lds > 48 * 1024)
+        TSX_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024));
+    hipLaunchKernelGGL(kernel, dim3(unsigned(8 * p.per_xcd)), dim3(h.threads), lds, stream, p);
+    TSX_LAUNCH_CHECK("group_norm_held_kernel");
+    return 0;
+}
+
+template <int TYPE, int V>
+int held(const HeldPlan &h, hipStream_t stream) {
+    if (h.NP <= 2) return launch_held<TYPE, V, 2>(h, stream);
+    if (h.NP <= 4) return launch_held<TYPE, V, 4>(h, stream);
+    if (h.NP <= 8) return launch_held<TYPE, V, 8>(h, stream);
+    if constexpr (V == 8) {
+        if (h.NP <= 12) return launch_held<TYPE, V, 12>(h, stream);
+    } else {
+        if (h.NP <= 16) return launch_held<TYPE, V, 16>(h, stream);
+        if constexpr (TYPE != TSX_TYPE_F32) return launch_held<TYPE, V, 24>(h, stream);
+    }
+    return fail(TSX_E_INVALID, "group_norm: %d pieces a thread", h.NP);
+}
+
+template <int TYPE>
+int run_held(const HeldPlan &h, hipStream_t stream) {
+    if constexpr (TYPE != TSX_TYPE_F32) {
+        if (h.V == 8) return held<TYPE, 8>(h, stream);
+    }
+    return held<TYPE, 4>(h, stream);
+}
+
+}  // namespace
+
+int group_norm_held(const tsx_group_norm *g, const NormParams &p, hipStream_t stream, bool *taken) {
+    const HeldPlan h = held_plan(g, p);
+    *taken = h.V != 0;
+    if (!*taken) return 0;
+    return g->type == TSX_TYPE_F32 ? run_held<TSX_TYPE_F32>(h, stream) : g->type == TSX_TYPE_F16 ? run_held<TSX_TYPE_F16>(h, stream)
+                                                                                                : run_held<TSX_TYPE_BF16>(h, stream);
+}
+
+}  // namespace tsx

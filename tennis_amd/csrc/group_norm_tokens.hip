@@ -1,0 +1,126 @@
+// The group norm's values as int8 tokens: a pixel's largest value decides its scale, so a pixel stays with one wavefront.
+//
+// L lanes of a wavefront share a pixel, each with P pieces of eight of its channels, which they hold from the load to the store.
+// Mean, scale and bias of the channels lie in LDS: 12 bytes a value read from there at HBM's pace are a third of what LDS gives.
+#include <algorithm>
+
+#include "group_norm.hpp"
+
+namespace tsx {
+namespace {
+
+template <int TYPE, int L, int P, int ACT>
+__global__ __launch_bounds__(256) void group_norm_tokens_kernel(NormParams p) {
+    extern __shared__ float2 group[];                        // [groups], behind them [3][channels in whole pieces]
+    constexpr int V = 8, SIZE = Kind<TYPE>::SIZE;
+    const int pieces = (p.c + V - 1) / V, width = pieces * V;
+    float *const means = reinterpret_cast<float *>(group + (p.groups + 1) / 2 * 2), *const scales = means + width, *const shifts = scales + width;
+    const int at = blockIdx.x % p.places, part = blockIdx.x / p.places;
+    const Place place(p, p.places % 8 == 0 ? p.places - 8 - at / 8 * 8 + at % 8 : at);
+    merge_chunks(p, place.image, group);
+    __syncthreads();
+    for (int ch = threadIdx.x; ch < width; ch += 256) {
+        const float2 g = ch < p.c ? group[ch / p.d] : float2{0.f, 0.f};
+        means[ch] = g.x;
+        scales[ch] = ch < p.c && p.weight ? g.y * p.weight[ch] : g.y;
+        shifts[ch] = ch < p.c && p.bias ? p.bias[ch] : 0.f;
+    }
+    __syncthreads();
+    const int64_t chunk_pixels = p.chunk_rows * p.S, chunk_end = place.chunk == p.chunks - 1 ? p.pixels : (place.chunk + 1) * chunk_pixels;
+    const int64_t first = place.chunk * chunk_pixels + part * p.part_pixels, end = part == p.parts - 1 ? chunk_end : min(first + p.part_pixels, chunk_end);
+    const int l = threadIdx.x % L;
+    const char *const x = static_cast<const char *>(p.x) + place.image * p.image_stride * SIZE;
+    for (int64_t base = first; base < end; base += 256 / L) {
+        const int64_t pixel = base + threadIdx.x / L;
+        const bool there = pixel < end;                      // a pixel's lanes agree
+        const char *const from = x + (there ? pixel : end - 1) * p.pixel_stride * SIZE;
+        Run<TYPE, V> in[P];
+        static_for<0, P>([&](auto ic) {
+            constexpr int i = decltype(ic)::value;
+            const int j = l + i * L;
+            in[i].clear();
+            if ((j + 1) * V <= p.c) in[i].load(from + j * (V * SIZE));
+            else if (j < pieces) in[i].load_some(from + j * (V * SIZE), p.c - j * V);
+        });
+        float y[P][V];
+        unsigned top = 0;
+        static_for<0, P>([&](auto ic) {
+            constexpr int i = decltype(ic)::value;
+            const int j = min(l + i * L, pieces - 1);
+            static_for<0, 2>([&](auto hc) {
+                constexpr int h = 4 * decltype(hc)::value;
+                typedef float v4f __attribute__((ext_vector_type(4)));
+                const v4f m = *reinterpret_cast<const v4f *>(means + j * V + h), a = *reinterpret_cast<const v4f *>(scales + j * V + h),
+                          b = *reinterpret_cast<const v4f *>(shifts + j * V + h);
+                static_for<0, 4>([&](auto ec) { constexpr int e = decltype(ec)::value; y[i][h + e] = __builtin_fmaf(in[i].template get<h + e>() - m[e], a[e], b[e]); });
+            });
+            if constexpr (ACT == ANY_ACT) activate_tokens(y[i], p.act, p.slope);
+            else activate_as<ACT>(y[i], p.slope);
+            if (l + i * L < pieces - 1 || (l + i * L == pieces - 1 && width == p.c))
+                static_for<0, V>([&](auto ec) { top = max(top, __builtin_bit_cast(unsigned, y[i][decltype(ec)::value]) & 0x7fffffffu); });
+            else if (l + i * L < pieces)
+                static_for<0, V>([&](auto ec) {
+                    constexpr int e = decltype(ec)::value;
+                    if ((pieces - 1) * V + e < p.c) top = max(top, __builtin_bit_cast(unsigned, y[i][e]) & 0x7fffffffu);
+                });
+        });
+#pragma unroll
+        for (int far = 1; far < L; far *= 2) top = max(top, unsigned(__shfl_xor(int(top), far)));
+        const TokenScale s(__builtin_bit_cast(float, top));
+        const int64_t token = place.image * p.pixels + pixel;
+        if (there && l == 0) p.scales[token] = s.scale;
+        if (there)
+            static_for<0, P>([&](auto ic) {
+                constexpr int i = decltype(ic)::value;
+                const int j = l + i * L;
+                if (j >= pieces) return;
+                unsigned b[V];
+                static_for<0, V>([&](auto ec) { constexpr int e = decltype(ec)::value; b[e] = s.bits(__fmul_rn(y[i][e], s.lift)); });
+                v2u word = {low_bytes(b[0], b[1], b[2], b[3]), low_bytes(b[4], b[5], b[6], b[7])};
+                if (s.reciprocal == 0.f) word = v2u{0, 0};
+                int8_t *const to = p.q + token * p.c + j * V;
+                if ((j + 1) * V <= p.c) *reinterpret_cast<v2u_any *>(to) = word;
+                else static_for<0, V>([&](auto ec) { constexpr int e = decltype(ec)::value; if (j * V + e < p.c) to[e] = int8_t(word[e / 4] >> (8 * (e % 4))); });
+            });
+    }
+}
+
+template <int TYPE, int L, int P>
+int launch_tokens(NormParams p, hipStream_t stream) {
+    // four workgroups a CU, of two turns at least
+    const int64_t chunk_pixels = p.chunk_rows * p.S, parts = std::max<int64_t>(1, std::min<int64_t>(ceil_div(1024, p.places), chunk_pixels / (2 * 256 / L)));
+    p.part_pixels = ceil_div(chunk_pixels, parts);
+    p.parts = int(ceil_div(chunk_pixels, p.part_pixels));
+    const size_t lds = size_t(round_up(p.groups, 2)) * sizeof(float2) + size_t(round_up(p.c, 8)) * 3 * sizeof(float);
+    const auto kernel = p.act == TSX_ACT_SILU ? group_norm_tokens_kernel<TYPE, L, P, TSX_ACT_SILU> : group_norm_tokens_kernel<TYPE, L, P, ANY_ACT>;
+    if (lds > 64 * 1024)
+        TSX_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+    hipLaunchKernelGGL(kernel, dim3(unsigned(p.places) * unsigned(p.parts)), dim3(256), lds, stream, p);
+    TSX_LAUNCH_CHECK("group_norm_tokens_kernel");
+    return 0;
+}
+
+template <int TYPE>
+int launch(const NormParams &p, hipStream_t stream) {
+    // the fewest lanes that hold a pixel in at most five pieces each
+    const int pieces = int(ceil_div(p.c, 8));
+    if (pieces <= 8) return launch_tokens<TYPE, 4, 2>(p, stream);
+    if (pieces <= 16) return launch_tokens<TYPE, 8, 2>(p, stream);
+    if (pieces <= 24) return launch_tokens<TYPE, 8, 3>(p, stream);
+    if (pieces <= 32) return launch_tokens<TYPE, 8, 4>(p, stream);
+    if (pieces <= 40) return launch_tokens<TYPE, 8, 5>(p, stream);
+    if (pieces <= 64) return launch_tokens<TYPE, 16, 4>(p, stream);
+    if (pieces <= 80) return launch_tokens<TYPE, 16, 5>(p, stream);
+    if (pieces <= 128) return launch_tokens<TYPE, 32, 4>(p, stream);
+    if (pieces <= 160) return launch_tokens<TYPE, 32, 5>(p, stream);
+    if (pieces <= 320) return launch_tokens<TYPE, 64, 5>(p, stream);
+    return launch_tokens<TYPE, 64, 16>(p, stream);
+}
+
+}  // namespace
+
+int group_norm_tokens(const NormParams &p, int type, hipStream_t stream) {
+    return type == TSX_TYPE_F32 ? launch<TSX_TYPE_F32>(p, stream) : type == TSX_TYPE_F16 ? launch<TSX_TYPE_F16>(p, stream) : launch<TSX_TYPE_BF16>(p, stream);
+}
+
+}  // namespace tsx
