@@ -28,8 +28,38 @@ auto with_act(int act, F &&f) {
 typedef unsigned v2u __attribute__((ext_vector_type(2)));
 typedef unsigned v4u __attribute__((ext_vector_type(4)));
 // at any address: global memory takes 16 bytes wherever they begin
+typedef unsigned u_any __attribute__((aligned(1)));
 typedef unsigned v2u_any __attribute__((ext_vector_type(2), aligned(1)));
 typedef unsigned v4u_any __attribute__((ext_vector_type(4), aligned(1)));
+
+// A value from the lane that is 2^K away (K < 6), for sums and maxima: up to there lanes hold one value, so a mirrored lane does for
+// an exchanged one.  Vector instructions all the way: a shuffle through LDS takes some hundred cycles, and six of them a reduction.
+template <int K>
+__device__ __forceinline__ unsigned partner(unsigned v) {
+    if constexpr (K < 4) {
+        constexpr int CTRL = K == 0 ? 0xb1 : K == 1 ? 0x4e : K == 2 ? 0x141 : 0x140;      // quads [1,0,3,2] and [2,3,0,1], mirrors of 8 and of 16
+        return unsigned(__builtin_amdgcn_update_dpp(0, int(v), CTRL, 0xf, 0xf, true));
+    } else {
+        // both results together hold a lane's own value and its partner's
+        const auto s = K == 4 ? __builtin_amdgcn_permlane16_swap(v, v, false, false) : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return (threadIdx.x >> K) & 1 ? s[0] : s[1];
+    }
+}
+// f over 2^lg consecutive lanes (lg uniform), in every one of them
+template <class F>
+__device__ __forceinline__ unsigned over_lanes(unsigned v, int lg, F &&f) {
+    static_for<0, 6>([&](auto kc) {
+        constexpr int K = decltype(kc)::value;
+        if (lg > K) v = f(v, partner<K>(v));
+    });
+    return v;
+}
+__device__ __forceinline__ float sum_over_lanes(float v, int lg) {
+    return __builtin_bit_cast(float, over_lanes(__builtin_bit_cast(unsigned, v), lg, [](unsigned a, unsigned b) {
+        return __builtin_bit_cast(unsigned, __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b));
+    }));
+}
+constexpr int lg_of(int power) { return power <= 1 ? 0 : 1 + lg_of(power / 2); }
 
 // a value the compiler knows nothing of: not what it was computed from, nor that it is the same one later
 __device__ __forceinline__ void renew(unsigned &word) { asm volatile("" : "+v"(word)); }
@@ -38,7 +68,7 @@ __device__ __forceinline__ void renew(unsigned &word) { asm volatile("" : "+v"(w
 template <int TYPE, int N>
 struct Run {
     static constexpr int BYTES = N * (TYPE == TSX_TYPE_F32 ? 4 : 2), WORDS = BYTES / 4, PER_WORD = TYPE == TSX_TYPE_F32 ? 1 : 2;
-    static_assert(BYTES % 8 == 0, "whole pairs of words");
+    static_assert(BYTES == 4 || BYTES % 8 == 0, "a word or whole pairs of words");
     unsigned word[WORDS];
 
     __device__ __forceinline__ void renew_words() {
@@ -48,7 +78,9 @@ struct Run {
         static_for<0, WORDS>([&](auto wc) { word[decltype(wc)::value] = 0; });
     }
     __device__ __forceinline__ void load(const void *at) {
-        if constexpr (BYTES % 16 == 0)
+        if constexpr (BYTES == 4)
+            word[0] = *reinterpret_cast<const u_any *>(at);
+        else if constexpr (BYTES % 16 == 0)
             static_for<0, BYTES / 16>([&](auto wc) {
                 constexpr int w = decltype(wc)::value;
                 const v4u v = reinterpret_cast<const v4u_any *>(at)[w];
@@ -75,7 +107,9 @@ struct Run {
         });
     }
     __device__ __forceinline__ void store(void *at) const {
-        if constexpr (BYTES % 16 == 0)
+        if constexpr (BYTES == 4)
+            *reinterpret_cast<u_any *>(at) = word[0];
+        else if constexpr (BYTES % 16 == 0)
             static_for<0, BYTES / 16>([&](auto wc) {
                 constexpr int w = decltype(wc)::value;
                 reinterpret_cast<v4u_any *>(at)[w] = v4u{word[4 * w], word[4 * w + 1], word[4 * w + 2], word[4 * w + 3]};

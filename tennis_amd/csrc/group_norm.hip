@@ -21,7 +21,7 @@ template <int TYPE, int V>
 __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_statistics_kernel(NormParams p) {
     extern __shared__ float entries[];                       // [lanes + 1][pitch] means, then squares
     const int threads = blockDim.x, t = threadIdx.x;
-    const int lanes = p.lanes ? p.lanes : 1, row_values = p.S * p.c, pixel_entries = p.c / p.run;
+    const int lanes = p.lanes ? p.lanes : 1, row_values = p.S * p.c, pixel_entries = p.c >> p.lg_run;
     const int pitch = (p.S * pixel_entries) | 1;             // odd: the lanes of one place lie in different banks
     float *const means = entries, *const squares = means + (lanes + 1) * pitch;
     const Place place(p, blockIdx.x);
@@ -32,7 +32,7 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_statistics_kerne
     // the incomplete row, with the last chunk: entries of its own behind the lanes'
     const int tail = place.chunk == p.chunks - 1 ? int(p.pixels - p.rows * p.S) * p.c : 0;
     auto leave = [&](int lane, int j, const float (&mean)[V], const float (&square)[V]) __attribute__((always_inline)) {
-        const int at = lane * pitch + j * V / p.run;
+        const int at = lane * pitch + (j * V >> p.lg_run);
         int k = 0;
         static_for<0, V>([&](auto ec) {
             constexpr int e = decltype(ec)::value;
@@ -53,7 +53,7 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_statistics_kerne
         });
     };
     for (int j0 = 0; j0 < p.pieces; j0 += threads) {         // one turn where the threads cover a row
-        const int lane = p.lanes ? t / p.pieces : 0, j = p.lanes ? t - lane * p.pieces : j0 + t;
+        const int lane = p.lanes ? udiv(t, p.pieces, p.pieces_magic) : 0, j = p.lanes ? t - lane * p.pieces : j0 + t;
         if (lane < lanes && j < p.pieces) {
             float base[V], sum[V], square[V];
             static_for<0, V>([&](auto ec) { base[decltype(ec)::value] = sum[decltype(ec)::value] = square[decltype(ec)::value] = 0.f; });
@@ -107,9 +107,9 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_statistics_kerne
     }
     __syncthreads();
     // T threads a group, TL of them on lanes of their own, which share the lane's entries of the group
-    const int group_entries = p.d / p.run, sides = lanes + (tail ? 1 : 0);
-    const int T = threads_a_group(threads, p.groups, sides * p.S * group_entries), TL = threads_a_group(T, 1, sides), TE = T / TL;
-    const int tl = t % T % TL, te = t % T / TL, tail_pixels = tail / p.c;
+    const int group_entries = p.d >> p.lg_run, sides = lanes + (tail ? 1 : 0);
+    const int T = 1 << p.lg_T, TL = 1 << p.lg_TL, TE = T >> p.lg_TL;
+    const int tl = t & (TL - 1), te = (t & (T - 1)) >> p.lg_TL, tail_pixels = int(p.pixels - p.rows * p.S);
     auto each = [&](int g, auto &&body) __attribute__((always_inline)) {
         for (int lane = tl; lane < sides; lane += TL) {
             const float n = float(p.run * (lane == lanes ? 1 : lane < rows ? (rows - lane - 1) / lanes + 1 : 0));
@@ -118,8 +118,8 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_statistics_kerne
                 for (int k = te; k < group_entries; k += TE) body(lane * pitch + pixel * pixel_entries + g * group_entries + k, n);
         }
     };
-    for (int g0 = 0; g0 < p.groups; g0 += threads / T) {
-        const int g = g0 + t / T;
+    for (int g0 = 0; g0 < p.groups; g0 += threads >> p.lg_T) {
+        const int g = g0 + (t >> p.lg_T);
         if (g >= p.groups) continue;                         // T threads agree
         float n = 0.f, s = 0.f, m2 = 0.f;
         const float about = means[(rows ? 0 : lanes * pitch) + g * group_entries];
@@ -127,15 +127,15 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_statistics_kerne
             n += ni;
             s = __builtin_fmaf(ni, means[at] - about, s);
         });
-        n = sum_of(n, T);
-        s = sum_of(s, T);
+        n = sum_over_lanes(n, p.lg_T);
+        s = sum_over_lanes(s, p.lg_T);
         const float mean = about + (n > 0.f ? s / n : 0.f);
         each(g, [&](int at, float ni) __attribute__((always_inline)) {
             const float d = means[at] - mean;
             m2 += __builtin_fmaf(ni * d, d, squares[at]);
         });
-        m2 = sum_of(m2, T);
-        if (t % T == 0) p.partial[int64_t(blockIdx.x) * p.groups + g] = float2{mean, m2};
+        m2 = sum_over_lanes(m2, p.lg_T);
+        if ((t & (T - 1)) == 0) p.partial[int64_t(blockIdx.x) * p.groups + g] = float2{mean, m2};
     }
 }
 
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_apply_kernel(Nor
     extern __shared__ float2 group[];
     const int threads = blockDim.x, t = threadIdx.x;
     const int lanes = p.lanes ? p.lanes : 1, row_values = p.S * p.c;
-    const int at = blockIdx.x % p.places, part = blockIdx.x / p.places;
+    const int part = udiv(blockIdx.x, p.places, p.places_magic), at = blockIdx.x - part * p.places;
     // The last chunks first, since the statistics ended with them: what they read is still in the caches.  Each on the XCD that
     // read it.
     const Place place(p, p.places % 8 == 0 ? p.places - 8 - at / 8 * 8 + at % 8 : at);
@@ -160,9 +160,11 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_apply_kernel(Nor
     const int rows = int(max(min(p.part_rows, chunk_end - first), int64_t(0)));
     const int tail = place.chunk == p.chunks - 1 && part == 0 ? int(p.pixels - p.rows * p.S) * p.c : 0;
     for (int j0 = 0; j0 < p.pieces; j0 += threads) {
-        const int lane = p.lanes ? t / p.pieces : 0, j = p.lanes ? t - lane * p.pieces : j0 + t;
+        const int lane = p.lanes ? udiv(t, p.pieces, p.pieces_magic) : 0, j = p.lanes ? t - lane * p.pieces : j0 + t;
         if (lane < lanes && j < p.pieces) {
-            const Affine<V> affine(p, group, p.S > 1 ? j * V % p.c : j * V, p.c, p.weight, p.bias);
+            const int ch = p.S > 1 ? j * V % p.c : j * V;
+            Affine<V> affine(ch, p.c, p.weight, p.bias);
+            affine.take(group, ch, p.c, p.d, p.d_magic);
             const char *from = x + ((first + lane) * row_stride + j * V) * Kind<TYPE>::SIZE;
             char *to = out + ((first + lane) * row_values + j * V) * Kind<TYPE>::SIZE;
             const int64_t in_step = lanes * row_stride * Kind<TYPE>::SIZE, out_step = int64_t(lanes) * row_values * Kind<TYPE>::SIZE;
@@ -244,6 +246,14 @@ NormPlan plan_of(const tsx_group_norm *g) {
     const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(ceil_div(512, p.places), p.chunk_rows / (4 * side)));
     p.part_rows = std::max<int64_t>(1, ceil_div(p.chunk_rows, parts));
     p.parts = int(std::max<int64_t>(1, ceil_div(p.chunk_rows, p.part_rows)));
+    p.lg_run = lg_of(p.run);
+    p.pieces_magic = div_magic(p.pieces, NORM_MOST_THREADS);
+    p.chunks_magic = div_magic(p.chunks, p.places);
+    p.places_magic = div_magic(p.places, int64_t(p.places) * p.parts);
+    p.d_magic = div_magic(p.d, NORM_MOST_CHANNELS);
+    p.lg_T = lg_threads(pl.threads, p.groups, (side + 1) * p.S * (p.d / p.run));
+    p.lg_TL = lg_threads(1 << p.lg_T, 1, side);
+    p.lg_merge = lg_threads(pl.threads, p.groups, p.chunks);
     return pl;
 }
 

@@ -2,6 +2,7 @@
 // statistics from those of its chunks.
 #pragma once
 #include "elements.hpp"
+#include "igemm_i8.hpp"
 
 namespace tsx {
 
@@ -19,12 +20,15 @@ struct NormParams {
     int c, groups, d;
     int S, pieces;                     // pixels of a row; pieces of a row
     int lanes;                         // rows that a workgroup's threads take side by side (0: pieces in turns)
-    int run;                           // neighbours of a piece that lie in one group, whichever piece
+    int run, lg_run;                   // neighbours of a piece that lie in one group, whichever piece: a power of two
     int chunks;                        // of an image's rows: a workgroup's share of the statistics
     int places, parts;                 // n * chunks; workgroups that share a chunk of the norm itself
     int64_t chunk_rows, part_rows, part_pixels;
     float epsilon, slope;
     int act;
+    unsigned pieces_magic, chunks_magic, places_magic, d_magic;      // udiv
+    int lg_T, lg_TL;                   // threads that sum up one group's entries, of them on lanes of their own
+    int lg_merge;                      // threads that sum up one group's chunks
 };
 
 // the norm's values as int8 tokens, from the statistics in p.partial
@@ -32,6 +36,13 @@ int group_norm_tokens(const NormParams &p, int type, hipStream_t stream);
 
 // the norm in one launch, where that serves the call: *taken says whether
 int group_norm_held(const tsx_group_norm *g, const NormParams &p, hipStream_t stream, bool *taken);
+
+// Threads, as a power of two, that work on one group where `threads` share `groups` of `entries` each.
+inline int lg_threads(int threads, int groups, int entries) {
+    int lg = 0;
+    while (lg < 6 && (groups << lg) < threads && (1 << lg) < entries) ++lg;
+    return lg;
+}
 
 inline int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
@@ -44,23 +55,15 @@ struct Kind {
     static constexpr int SIZE = TYPE == TSX_TYPE_F32 ? 4 : 2;
 };
 
-// The sum over T consecutive lanes, T a power of two, in every one of them.
-__device__ __forceinline__ float sum_of(float v, int T) {
-    for (int far = 1; far < T; far *= 2) v += __shfl_xor(v, far);
-    return v;
-}
-// Threads that work on one group where `threads` share `groups` of `entries` each.
-__device__ __forceinline__ int threads_a_group(int threads, int groups, int entries) {
-    int T = 1;
-    while (T < 64 && T * groups < threads && T < entries) T *= 2;
-    return T;
-}
-
 // Where a workgroup of the two kernels below works: `of` = n * chunks places, consecutive ones on consecutive XCDs.
 struct Place {
     int64_t image;
     int chunk;
-    __device__ __forceinline__ Place(const NormParams &p, int at) : image(at / p.chunks), chunk(at % p.chunks) {}
+    __device__ __forceinline__ Place(const NormParams &p, int at) {
+        const int i = udiv(at, p.chunks, p.chunks_magic);
+        image = i;
+        chunk = at - i * p.chunks;
+    }
 };
 
 // Mean and 1 / sqrt(variance + epsilon) of the groups of one image, into LDS, from the chunks' means and squares, in one pass around
@@ -70,23 +73,23 @@ __device__ __forceinline__ void merge_chunks(const NormParams &p, int64_t image,
     const float whole = float(p.chunk_rows) * float(p.S) * float(p.d);
     const float last = float(p.pixels - (p.chunks - 1) * p.chunk_rows * p.S) * float(p.d);
     const float of_total = 1.f / (float(p.pixels) * float(p.d));
-    const int T = threads_a_group(blockDim.x, p.groups, p.chunks);
-    for (int g0 = 0; g0 < p.groups; g0 += blockDim.x / T) {
-        const int g = g0 + threadIdx.x / T;
+    const int lg = p.lg_merge, T = 1 << lg;
+    for (int g0 = 0; g0 < p.groups; g0 += blockDim.x >> lg) {
+        const int g = g0 + (threadIdx.x >> lg);
         if (g >= p.groups) continue;                         // T threads agree
         const float about = partial[g].x;
         float s = 0.f, m2 = 0.f;
-        for (int k = threadIdx.x % T; k < p.chunks; k += T) {
+        for (int k = threadIdx.x & (T - 1); k < p.chunks; k += T) {
             const float2 part = partial[int64_t(k) * p.groups + g];
             const float n = k == p.chunks - 1 ? last : whole, d = part.x - about;
             s = __builtin_fmaf(n, d, s);
             m2 += __builtin_fmaf(n * d, d, part.y);
         }
-        s = sum_of(s, T);
-        m2 = sum_of(m2, T);
+        s = sum_over_lanes(s, lg);
+        m2 = sum_over_lanes(m2, lg);
         const float shift = s * of_total, variance = fmaxf(__builtin_fmaf(-shift, s, m2), 0.f) * of_total;
         // a NaN among the squares stays one (fmaxf drops it)
-        if (threadIdx.x % T == 0) group[g] = float2{about + shift, 1.f / sqrtf((m2 == m2 ? variance : m2) + p.epsilon)};
+        if ((threadIdx.x & (T - 1)) == 0) group[g] = float2{about + shift, 1.f / sqrtf((m2 == m2 ? variance : m2) + p.epsilon)};
     }
 }
 
@@ -143,34 +146,39 @@ __device__ __forceinline__ void join_runs(int run, Join &&join) {
     if constexpr (V >= 8) { if (run % 8 == 0) static_for<0, V / 8>([&](auto ic) { join(std::integral_constant<int, 8 * decltype(ic)::value>{}, std::integral_constant<int, 4>{}); }); }
 }
 
-// Mean, scale and bias of the V channels of piece j of a row
+// Mean, scale and bias of V channels in a row, from channel ch on, of c that follow one another (behind the last one: the first) and
+// begin with a group's first one.  weight and bias: of those channels, or null.  The vectors are requested by the constructor, ahead of
+// the statistics, all behind one branch each: behind branches of their own they would wait for one another.
 template <int V>
 struct Affine {
     float mean[V], scale[V], shift[V];
-    // from channel ch on, of c that follow one another and begin with a group's first one; group[0]: that group
-    __device__ __forceinline__ Affine(const NormParams &p, const float2 *group, int ch, int c, const float *weight, const float *bias) {
-        int g = ch / p.d, left = (g + 1) * p.d - ch;         // channels left in the group
+    __device__ __forceinline__ Affine(int ch, int c, const float *weight, const float *bias) {
         int at[V];
+        static_for<0, V>([&](auto ec) {
+            constexpr int e = decltype(ec)::value;
+            at[e] = ch++;
+            if (ch == c) ch = 0;
+            scale[e] = 1.f;
+            shift[e] = 0.f;
+        });
+        if (bias) static_for<0, V>([&](auto ec) { shift[decltype(ec)::value] = bias[at[decltype(ec)::value]]; });
+        if (weight) static_for<0, V>([&](auto ec) { scale[decltype(ec)::value] = weight[at[decltype(ec)::value]]; });
+    }
+    // group[0]: the statistics of the first of the c channels
+    __device__ __forceinline__ void take(const float2 *group, int ch, int c, int d, unsigned d_magic) {
+        int g = udiv(ch, d, d_magic), left = (g + 1) * d - ch;             // channels left in the group
         static_for<0, V>([&](auto ec) {
             constexpr int e = decltype(ec)::value;
             const float2 stat = group[g];
             mean[e] = stat.x;
-            scale[e] = stat.y;
-            at[e] = ch++;
+            scale[e] *= stat.y;
+            ++ch;
             if (--left == 0) {
-                left = p.d;
+                left = d;
                 ++g;
                 if (ch == c) g = ch = 0;
             }
         });
-        // all requests behind one branch each: behind branches of their own they would wait for one another
-        static_for<0, V>([&](auto ec) { shift[decltype(ec)::value] = 0.f; });
-        if (bias) static_for<0, V>([&](auto ec) { shift[decltype(ec)::value] = bias[at[decltype(ec)::value]]; });
-        if (weight) {
-            float w[V];
-            static_for<0, V>([&](auto ec) { w[decltype(ec)::value] = weight[at[decltype(ec)::value]]; });
-            static_for<0, V>([&](auto ec) { scale[decltype(ec)::value] *= w[decltype(ec)::value]; });
-        }
     }
     template <int ACT, int TYPE>
     __device__ __forceinline__ void apply(int act, float slope, Piece<TYPE, V> &a) const {

@@ -11,8 +11,9 @@ namespace tsx {
 namespace {
 
 struct HeldParams : NormParams {
-    int B, pieces_a_pixel, held_lanes, bundles, per_xcd;
-    int TG, TL;                        // threads that sum one group's entries, of them on lanes of their own
+    int B, a_image, pieces_a_pixel, held_lanes, bundles, per_xcd;      // a_image: bundles of an image
+    int lg_TG;                         // threads that sum up one group's entries; lg_TL of them on lanes of their own
+    unsigned pixel_magic, image_magic; // udiv by pieces_a_pixel, by groups / B
 };
 
 template <int TYPE, int V, int NP, int ACT>
@@ -21,50 +22,49 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_held_kernel(Held
     __shared__ float2 group[NORM_MOST_THREADS];
     __shared__ float2 waves[NORM_MOST_THREADS / 64];
     constexpr int SIZE = Kind<TYPE>::SIZE;
-    const int t = threadIdx.x, lanes = p.held_lanes, channels = p.B * p.d, row_entries = channels / p.run, pitch = row_entries | 1;
+    const int t = threadIdx.x, lanes = p.held_lanes, channels = p.B * p.d, row_entries = channels >> p.lg_run, pitch = row_entries | 1;
     // consecutive bundles of an image on one XCD: they share cache lines
     const int id = int(blockIdx.x % 8) * p.per_xcd + int(blockIdx.x / 8);
     if (int(blockIdx.x / 8) >= p.per_xcd || id >= p.bundles) return;       // uniform
-    const int a_image = p.groups / p.B, image = id / a_image, ch0 = (id - image * a_image) * channels, pixels = int(p.pixels);
-    const int lane = t / p.pieces_a_pixel, j = t - lane * p.pieces_a_pixel;
+    const int a_image = p.a_image, image = udiv(id, a_image, p.image_magic), ch0 = (id - image * a_image) * channels, pixels = int(p.pixels);
+    const int lane = udiv(t, p.pieces_a_pixel, p.pixel_magic), j = t - lane * p.pieces_a_pixel;
     const bool mine = lane < lanes;
-    const char *const x = static_cast<const char *>(p.x) + (int64_t(image) * p.image_stride + ch0 + j * V) * SIZE;
+    // All requests at once, none behind a branch, where it would be waited for: threads without a pixel read another one again.
+    const int j_in = mine ? j : 0, lane_in = mine ? lane : 0;
+    const char *const x = static_cast<const char *>(p.x) + (int64_t(image) * p.image_stride + ch0 + j_in * V) * SIZE;
     Run<TYPE, V> v[NP];
-    static_for<0, NP>([&](auto ic) {
-        constexpr int i = decltype(ic)::value;
-        v[i].clear();
-        if (mine && lane + i * lanes < pixels) v[i].load(x + int64_t(lane + i * lanes) * p.pixel_stride * SIZE);
-    });
+    static_for<0, NP>([&](auto ic) { v[decltype(ic)::value].load(x + int64_t(min(lane_in + decltype(ic)::value * lanes, pixels - 1)) * p.pixel_stride * SIZE); });
+    Affine<V> affine(mine ? j * V : 0, channels, p.weight ? p.weight + ch0 : nullptr, p.bias ? p.bias + ch0 : nullptr);
     // The packed words anew for each pass over them: unpacked once for all three they would be twice as many registers.
     auto again = [&] { static_for<0, NP>([&](auto ic) { v[decltype(ic)::value].renew_words(); }); };
     // `leave`: a thread's V sums into LDS, neighbours of one group added up
     auto leave = [&](float *to, float (&s)[V]) __attribute__((always_inline)) {
         join_runs<V>(p.run, [&](auto ac, auto fc) { constexpr int a = decltype(ac)::value; s[a] += s[a + decltype(fc)::value]; });
         if (!mine) return;
-        int at = lane * pitch + j * V / p.run;
+        int at = lane * pitch + (j * V >> p.lg_run);
         static_for<0, V>([&](auto ec) { if ((decltype(ec)::value & (p.run - 1)) == 0) to[at++] = s[decltype(ec)::value]; });
     };
     // The sums of both arrays over a group's entries, for the TG threads of that group
-    const int g = t / p.TG, tg = t % p.TG, tl = tg % p.TL, te = tg / p.TL, TE = p.TG / p.TL, group_entries = p.d / p.run;
+    const int TG = 1 << p.lg_TG, TL = 1 << p.lg_TL, TE = TG >> p.lg_TL, group_entries = p.d >> p.lg_run;
+    const int g = t >> p.lg_TG, tg = t & (TG - 1), tl = tg & (TL - 1), te = tg >> p.lg_TL;
     const float *const second = entries + lanes * pitch;
     auto gather = [&](bool both) __attribute__((always_inline)) {
         float2 s = {0.f, 0.f};
         if (g < p.B)
-            for (int l = tl; l < lanes; l += p.TL)
+            for (int l = tl; l < lanes; l += TL)
                 for (int k = te; k < group_entries; k += TE) {
                     const int at = l * pitch + g * group_entries + k;
                     s.x += entries[at];
                     if (both) s.y += second[at];
                 }
-        const int width = min(p.TG, 64);
-        s.x = sum_of(s.x, width);
-        if (both) s.y = sum_of(s.y, width);
-        if (p.TG > 64) {                                     // uniform
+        s.x = sum_over_lanes(s.x, p.lg_TG);
+        if (both) s.y = sum_over_lanes(s.y, p.lg_TG);
+        if (TG > 64) {                                     // uniform
             if (t % 64 == 0) waves[t / 64] = s;
             __syncthreads();
             s = float2{0.f, 0.f};
-            for (int w = 0; w < p.TG / 64; ++w) {
-                const float2 part = waves[g * (p.TG / 64) + w];
+            for (int w = 0; w < TG / 64; ++w) {
+                const float2 part = waves[g * (TG / 64) + w];
                 s.x += part.x;
                 s.y += part.y;
             }
@@ -76,7 +76,7 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_held_kernel(Held
     static_for<0, V>([&](auto ec) { sum[decltype(ec)::value] = 0.f; });
     static_for<0, NP>([&](auto ic) {
         constexpr int i = decltype(ic)::value;
-        static_for<0, V>([&](auto ec) { constexpr int e = decltype(ec)::value; sum[e] += v[i].template get<e>(); });
+        if (lane + i * lanes < pixels) static_for<0, V>([&](auto ec) { constexpr int e = decltype(ec)::value; sum[e] += v[i].template get<e>(); });
     });
     leave(entries, sum);
     __syncthreads();
@@ -86,7 +86,7 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_held_kernel(Held
     again();
     float square[V], mean[V];
     {
-        int gi = mine ? j * V / p.d : 0, left = (gi + 1) * p.d - j * V;
+        int gi = mine ? udiv(j * V, p.d, p.d_magic) : 0, left = (gi + 1) * p.d - j * V;
         static_for<0, V>([&](auto ec) {
             constexpr int e = decltype(ec)::value;
             mean[e] = group[gi].x;
@@ -116,7 +116,7 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_held_kernel(Held
     __syncthreads();
     if (!mine) return;
     again();
-    const Affine<V> affine(p, group, j * V, channels, p.weight ? p.weight + ch0 : nullptr, p.bias ? p.bias + ch0 : nullptr);
+    affine.take(group, j * V, channels, p.d, p.d_magic);
     char *const out = static_cast<char *>(p.out) + (int64_t(image) * pixels * p.c + ch0 + j * V) * SIZE;
     static_for<0, NP>([&](auto ic) {
         constexpr int i = decltype(ic)::value;
@@ -146,12 +146,12 @@ HeldPlan held_plan(const tsx_group_norm *g, const NormParams &rows) {
     float best_cost = 0.f;
     if (g->pixels > 16384) return best;
     const int pixels = int(g->pixels), d = g->c / g->groups, whole = g->type == TSX_TYPE_F32 ? 4 : 8;
-    for (int V = whole; V >= 4; V -= 4)
+    for (int V = whole; V >= 2; V /= 2)
         for (int B = 1; B <= g->groups; ++B) {
             if (g->groups % B || B * d % V) continue;
             const int a_pixel = B * d / V;
             if (a_pixel > NORM_MOST_THREADS) break;
-            const int most = V == 8 ? 12 : g->type == TSX_TYPE_F32 ? 16 : 24;      // what 128 registers hold beside the rest
+            const int most = V == 8 ? 12 : g->type == TSX_TYPE_F32 && V == 4 ? 16 : 24;      // what 128 registers hold beside the rest
             int threads = 256;
             while (threads < NORM_MOST_THREADS && (threads < a_pixel || ceil_div(pixels, threads / a_pixel) > 4)) threads *= 2;
             const int lanes = threads / a_pixel, need = int(ceil_div(pixels, lanes));
@@ -173,8 +173,12 @@ HeldPlan held_plan(const tsx_group_norm *g, const NormParams &rows) {
             p.held_lanes = lanes;
             p.bundles = int(bundles);
             p.per_xcd = int(ceil_div(bundles, 8));
-            p.TG = threads / power_of_two(B);
-            p.TL = std::min(p.TG, power_of_two(lanes));
+            p.a_image = g->groups / B;
+            p.lg_run = lg_of(p.run);
+            p.lg_TG = lg_of(threads / power_of_two(B));
+            p.lg_TL = std::min(p.lg_TG, lg_of(power_of_two(lanes)));
+            p.pixel_magic = div_magic(a_pixel, NORM_MOST_THREADS);
+            p.image_magic = div_magic(p.a_image, bundles);
         }
     return best;
 }
@@ -200,7 +204,7 @@ int held(const HeldPlan &h, hipStream_t stream) {
         if (h.NP <= 12) return launch_held<TYPE, V, 12>(h, stream);
     } else {
         if (h.NP <= 16) return launch_held<TYPE, V, 16>(h, stream);
-        if constexpr (TYPE != TSX_TYPE_F32) return launch_held<TYPE, V, 24>(h, stream);
+        if constexpr (TYPE != TSX_TYPE_F32 || V == 2) return launch_held<TYPE, V, 24>(h, stream);
     }
     return fail(TSX_E_INVALID, "group_norm: %d pieces a thread", h.NP);
 }
@@ -210,7 +214,7 @@ int run_held(const HeldPlan &h, hipStream_t stream) {
     if constexpr (TYPE != TSX_TYPE_F32) {
         if (h.V == 8) return held<TYPE, 8>(h, stream);
     }
-    return held<TYPE, 4>(h, stream);
+    return h.V == 4 ? held<TYPE, 4>(h, stream) : held<TYPE, 2>(h, stream);
 }
 
 }  // namespace

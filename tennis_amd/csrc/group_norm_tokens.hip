@@ -15,12 +15,12 @@ __global__ __launch_bounds__(256) void group_norm_tokens_kernel(NormParams p) {
     constexpr int V = 8, SIZE = Kind<TYPE>::SIZE;
     const int pieces = (p.c + V - 1) / V, width = pieces * V;
     float *const means = reinterpret_cast<float *>(group + (p.groups + 1) / 2 * 2), *const scales = means + width, *const shifts = scales + width;
-    const int at = blockIdx.x % p.places, part = blockIdx.x / p.places;
+    const int part = udiv(blockIdx.x, p.places, p.places_magic), at = blockIdx.x - part * p.places;
     const Place place(p, p.places % 8 == 0 ? p.places - 8 - at / 8 * 8 + at % 8 : at);
     merge_chunks(p, place.image, group);
     __syncthreads();
     for (int ch = threadIdx.x; ch < width; ch += 256) {
-        const float2 g = ch < p.c ? group[ch / p.d] : float2{0.f, 0.f};
+        const float2 g = ch < p.c ? group[udiv(ch, p.d, p.d_magic)] : float2{0.f, 0.f};
         means[ch] = g.x;
         scales[ch] = ch < p.c && p.weight ? g.y * p.weight[ch] : g.y;
         shifts[ch] = ch < p.c && p.bias ? p.bias[ch] : 0.f;
@@ -35,13 +35,17 @@ __global__ __launch_bounds__(256) void group_norm_tokens_kernel(NormParams p) {
         const bool there = pixel < end;                      // a pixel's lanes agree
         const char *const from = x + (there ? pixel : end - 1) * p.pixel_stride * SIZE;
         Run<TYPE, V> in[P];
-        static_for<0, P>([&](auto ic) {
-            constexpr int i = decltype(ic)::value;
-            const int j = l + i * L;
-            in[i].clear();
-            if ((j + 1) * V <= p.c) in[i].load(from + j * (V * SIZE));
-            else if (j < pieces) in[i].load_some(from + j * (V * SIZE), p.c - j * V);
-        });
+        // all requests at once, none behind a branch, where it would be waited for
+        const int whole = p.c / V;
+        if (whole)       // uniform
+            static_for<0, P>([&](auto ic) { in[decltype(ic)::value].load(from + min(l + decltype(ic)::value * L, whole - 1) * (V * SIZE)); });
+        if (whole != pieces)
+            static_for<0, P>([&](auto ic) {
+                constexpr int i = decltype(ic)::value;
+                const int j = l + i * L;
+                if (j >= whole) in[i].clear();
+                if (j >= whole && j < pieces) in[i].load_some(from + j * (V * SIZE), p.c - j * V);
+            });
         float y[P][V];
         unsigned top = 0;
         static_for<0, P>([&](auto ic) {
@@ -64,8 +68,7 @@ __global__ __launch_bounds__(256) void group_norm_tokens_kernel(NormParams p) {
                     if ((pieces - 1) * V + e < p.c) top = max(top, __builtin_bit_cast(unsigned, y[i][e]) & 0x7fffffffu);
                 });
         });
-#pragma unroll
-        for (int far = 1; far < L; far *= 2) top = max(top, unsigned(__shfl_xor(int(top), far)));
+        top = over_lanes(top, lg_of(L), [](unsigned a, unsigned b) { return max(a, b); });
         const TokenScale s(__builtin_bit_cast(float, top));
         const int64_t token = place.image * p.pixels + pixel;
         if (there && l == 0) p.scales[token] = s.scale;
@@ -91,6 +94,8 @@ int launch_tokens(NormParams p, hipStream_t stream) {
     const int64_t chunk_pixels = p.chunk_rows * p.S, parts = std::max<int64_t>(1, std::min<int64_t>(ceil_div(1024, p.places), chunk_pixels / (2 * 256 / L)));
     p.part_pixels = ceil_div(chunk_pixels, parts);
     p.parts = int(ceil_div(chunk_pixels, p.part_pixels));
+    p.places_magic = div_magic(p.places, int64_t(p.places) * p.parts);
+    p.lg_merge = lg_threads(256, p.groups, p.chunks);
     const size_t lds = size_t(round_up(p.groups, 2)) * sizeof(float2) + size_t(round_up(p.c, 8)) * 3 * sizeof(float);
     const auto kernel = p.act == TSX_ACT_SILU ? group_norm_tokens_kernel<TYPE, L, P, TSX_ACT_SILU> : group_norm_tokens_kernel<TYPE, L, P, ANY_ACT>;
     if (lds > 64 * 1024)

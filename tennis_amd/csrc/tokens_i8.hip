@@ -32,13 +32,17 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void quantize_tokens_kernel(Toke
         const char *x = static_cast<const char *>(p.x) + (there ? row : p.rows - 1) * p.x_stride * SIZE;
         Values v[P];
         unsigned top = 0;
+        // All requests at once, none behind a branch, where it would be waited for: what lies behind the last whole piece is that piece
+        // again, and then zeros, or the values that are left there.
+        const int whole = p.cols / PIECE;
         auto fetch = [&](int first) __attribute__((always_inline)) {
+            if (whole)       // uniform
+                static_for<0, P>([&](auto ic) { v[decltype(ic)::value].load(x + int64_t(min(first + t + decltype(ic)::value * T, whole - 1)) * (PIECE * SIZE)); });
             static_for<0, P>([&](auto ic) {
                 constexpr int i = decltype(ic)::value;
                 const int piece = first + t + i * T;
-                v[i].clear();
-                if ((piece + 1) * PIECE <= p.cols) v[i].load(x + int64_t(piece) * (PIECE * SIZE));
-                else if (piece < pieces) v[i].load_some(x + int64_t(piece) * (PIECE * SIZE), p.cols - piece * PIECE);
+                if (piece >= whole) v[i].clear();
+                if (piece >= whole && piece < pieces) v[i].load_some(x + int64_t(piece) * (PIECE * SIZE), p.cols - piece * PIECE);
             });
         };
         const int turns = HELD ? 1 : (pieces_out + T * P - 1) / (T * P);
@@ -46,8 +50,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void quantize_tokens_kernel(Toke
             fetch(turn * T * P);
             static_for<0, P>([&](auto ic) { top = v[decltype(ic)::value].top(top); });
         }
-#pragma unroll
-        for (int far = 1; far < (T < 64 ? T : 64); far *= 2) top = Values::template larger<TYPE>(top, unsigned(__shfl_xor(int(top), far)));
+        top = over_lanes(top, lg_of(T < 64 ? T : 64), [](unsigned a, unsigned b) { return Values::template larger<TYPE>(a, b); });
         if constexpr (T > 64) {
             if (tid % 64 == 0) tops[tid / 64] = top;
             __syncthreads();
