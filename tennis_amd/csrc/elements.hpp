@@ -67,8 +67,8 @@ __device__ __forceinline__ void renew(unsigned &word) { asm volatile("" : "+v"(w
 // N consecutive values as they lie in memory
 template <int TYPE, int N>
 struct Run {
-    static constexpr int BYTES = N * (TYPE == TSX_TYPE_F32 ? 4 : 2), WORDS = BYTES / 4, PER_WORD = TYPE == TSX_TYPE_F32 ? 1 : 2;
-    static_assert(BYTES == 4 || BYTES % 8 == 0, "a word or whole pairs of words");
+    static constexpr int BYTES = N * (TYPE == TSX_TYPE_F32 ? 4 : 2), WORDS = (BYTES + 3) / 4, PER_WORD = TYPE == TSX_TYPE_F32 ? 1 : 2;
+    static_assert(BYTES <= 4 || BYTES % 8 == 0, "a word or whole pairs of words");
     unsigned word[WORDS];
 
     __device__ __forceinline__ void renew_words() {
@@ -78,7 +78,9 @@ struct Run {
         static_for<0, WORDS>([&](auto wc) { word[decltype(wc)::value] = 0; });
     }
     __device__ __forceinline__ void load(const void *at) {
-        if constexpr (BYTES == 4)
+        if constexpr (BYTES == 2)
+            word[0] = *reinterpret_cast<const unsigned short *>(at);
+        else if constexpr (BYTES == 4)
             word[0] = *reinterpret_cast<const u_any *>(at);
         else if constexpr (BYTES % 16 == 0)
             static_for<0, BYTES / 16>([&](auto wc) {
@@ -107,7 +109,9 @@ struct Run {
         });
     }
     __device__ __forceinline__ void store(void *at) const {
-        if constexpr (BYTES == 4)
+        if constexpr (BYTES == 2)
+            *reinterpret_cast<unsigned short *>(at) = (unsigned short)word[0];
+        else if constexpr (BYTES == 4)
             *reinterpret_cast<u_any *>(at) = word[0];
         else if constexpr (BYTES % 16 == 0)
             static_for<0, BYTES / 16>([&](auto wc) {
@@ -143,10 +147,10 @@ struct Run {
             } else if constexpr (TYPE == TSX_TYPE_BF16) {
                 typedef __bf16 pair __attribute__((ext_vector_type(2)));
                 typedef float two __attribute__((ext_vector_type(2)));
-                word[w] = __builtin_bit_cast(unsigned, __builtin_convertvector((two{v[2 * w], v[2 * w + 1]}), pair));
+                word[w] = __builtin_bit_cast(unsigned, __builtin_convertvector((two{v[2 * w], 2 * w + 1 < N ? v[(2 * w + 1) % N] : 0.f}), pair));
             } else {
                 typedef _Float16 pair __attribute__((ext_vector_type(2)));
-                word[w] = __builtin_bit_cast(unsigned, pair{_Float16(v[2 * w]), _Float16(v[2 * w + 1])});
+                word[w] = __builtin_bit_cast(unsigned, pair{_Float16(v[2 * w]), _Float16(2 * w + 1 < N ? v[(2 * w + 1) % N] : 0.f)});
             }
         });
     }

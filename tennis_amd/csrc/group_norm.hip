@@ -135,7 +135,7 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_statistics_kerne
             m2 += __builtin_fmaf(ni * d, d, squares[at]);
         });
         m2 = sum_over_lanes(m2, p.lg_T);
-        if ((t & (T - 1)) == 0) p.partial[int64_t(blockIdx.x) * p.groups + g] = float2{mean, m2};
+        if ((t & (T - 1)) == 0) p.partial[(place.image * p.groups + g) * p.chunks + place.chunk] = float2{mean, m2};
     }
 }
 
@@ -150,8 +150,6 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_apply_kernel(Nor
     // The last chunks first, since the statistics ended with them: what they read is still in the caches.  Each on the XCD that
     // read it.
     const Place place(p, p.places % 8 == 0 ? p.places - 8 - at / 8 * 8 + at % 8 : at);
-    merge_chunks(p, place.image, group);
-    __syncthreads();
     const char *const x = static_cast<const char *>(p.x) + place.image * p.image_stride * Kind<TYPE>::SIZE;
     char *const out = static_cast<char *>(p.out) + place.image * p.pixels * p.c * Kind<TYPE>::SIZE;
     const int64_t row_stride = p.S * p.pixel_stride;
@@ -159,45 +157,49 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_apply_kernel(Nor
     const int64_t first = place.chunk * p.chunk_rows + part * p.part_rows;
     const int rows = int(max(min(p.part_rows, chunk_end - first), int64_t(0)));
     const int tail = place.chunk == p.chunks - 1 && part == 0 ? int(p.pixels - p.rows * p.S) * p.c : 0;
+    constexpr int AHEAD = 4;
+    typedef Run<TYPE, V> Values;
+    // Requests of a batch leave together, the first ahead of the statistics; in the place of rows that are none the last one again.
+    const int64_t in_step = lanes * row_stride * Kind<TYPE>::SIZE, out_step = int64_t(lanes) * row_values * Kind<TYPE>::SIZE;
+    auto fetch = [&](Values (&v)[AHEAD], const char *at, int left) __attribute__((always_inline)) {
+        if (left > 0)
+            static_for<0, AHEAD>([&](auto uc) { v[decltype(uc)::value].load(at + min(decltype(uc)::value, left - 1) * in_step); });
+    };
     for (int j0 = 0; j0 < p.pieces; j0 += threads) {
         const int lane = p.lanes ? udiv(t, p.pieces, p.pieces_magic) : 0, j = p.lanes ? t - lane * p.pieces : j0 + t;
-        if (lane < lanes && j < p.pieces) {
-            const int ch = p.S > 1 ? j * V % p.c : j * V;
-            Affine<V> affine(ch, p.c, p.weight, p.bias);
-            affine.take(group, ch, p.c, p.d, p.d_magic);
-            const char *from = x + ((first + lane) * row_stride + j * V) * Kind<TYPE>::SIZE;
-            char *to = out + ((first + lane) * row_values + j * V) * Kind<TYPE>::SIZE;
-            const int64_t in_step = lanes * row_stride * Kind<TYPE>::SIZE, out_step = int64_t(lanes) * row_values * Kind<TYPE>::SIZE;
-            constexpr int AHEAD = 4;
-            int left = lane < rows ? (rows - lane - 1) / lanes + 1 : 0;
-            for (; left >= AHEAD; left -= AHEAD) {
-                Piece<TYPE, V> a[AHEAD];
-                static_for<0, AHEAD>([&](auto uc) { a[decltype(uc)::value].load(from + decltype(uc)::value * in_step, 0); });
-                static_for<0, AHEAD>([&](auto uc) {
-                    constexpr int u = decltype(uc)::value;
-                    affine.template apply<ACT>(p.act, p.slope, a[u]);
-                    a[u].store(to + u * out_step, 0, V);
-                });
-                from += AHEAD * in_step;
-                to += AHEAD * out_step;
-            }
-            if (left > 0) {                                  // the rest at once: its last row again in the place of those that are none
-                Piece<TYPE, V> a[AHEAD - 1];
-                static_for<0, AHEAD - 1>([&](auto uc) { a[decltype(uc)::value].load(from + min(decltype(uc)::value, left - 1) * in_step, 0); });
-                static_for<0, AHEAD - 1>([&](auto uc) {
-                    constexpr int u = decltype(uc)::value;
-                    if (u < left) {
-                        affine.template apply<ACT>(p.act, p.slope, a[u]);
-                        a[u].store(to + u * out_step, 0, V);
-                    }
-                });
-            }
-            if (lane == 0 && j * V < tail) {
-                Piece<TYPE, V> a;
-                a.load_some(x, p.rows * row_values + j * V, tail - j * V);
-                affine.template apply<ACT>(p.act, p.slope, a);
-                a.store(out, p.rows * row_values + j * V, tail - j * V);
-            }
+        const bool mine = lane < lanes && j < p.pieces;
+        const int ch = !mine ? 0 : p.S > 1 ? j * V % p.c : j * V;
+        const char *from = x + ((first + lane) * row_stride + j * V) * Kind<TYPE>::SIZE;
+        char *to = out + ((first + lane) * row_values + j * V) * Kind<TYPE>::SIZE;
+        int left = mine && lane < rows ? (rows - lane - 1) / lanes + 1 : 0;
+        Values v[AHEAD];
+        fetch(v, from, left);
+        Affine<V> affine(ch, p.c, p.weight, p.bias);
+        if (j0 == 0) {
+            merge_chunks(p, place.image, group);
+            __syncthreads();
+        }
+        affine.take(group, ch, p.c, p.d, p.d_magic);
+        auto apply = [&](auto uc) __attribute__((always_inline)) {
+            constexpr int u = decltype(uc)::value;
+            Piece<TYPE, V> a;
+            static_for<0, V>([&](auto ec) { a.v[decltype(ec)::value] = v[u].template get<decltype(ec)::value>(); });
+            affine.template apply<ACT>(p.act, p.slope, a);
+            a.store(to + u * out_step, 0, V);
+        };
+        while (left > AHEAD) {
+            static_for<0, AHEAD>(apply);
+            from += AHEAD * in_step;
+            to += AHEAD * out_step;
+            left -= AHEAD;
+            fetch(v, from, left);
+        }
+        static_for<0, AHEAD>([&](auto uc) { if (decltype(uc)::value < left) apply(uc); });
+        if (mine && lane == 0 && j * V < tail) {
+            Piece<TYPE, V> a;
+            a.load_some(x, p.rows * row_values + j * V, tail - j * V);
+            affine.template apply<ACT>(p.act, p.slope, a);
+            a.store(out, p.rows * row_values + j * V, tail - j * V);
         }
         if (p.lanes) break;
     }
@@ -243,7 +245,7 @@ NormPlan plan_of(const tsx_group_norm *g) {
     p.chunk_rows = std::max<int64_t>(1, ceil_div(p.rows, chunks));
     p.chunks = int(std::max<int64_t>(1, ceil_div(p.rows, p.chunk_rows)));
     p.places = n * p.chunks;
-    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(ceil_div(512, p.places), p.chunk_rows / (4 * side)));
+    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(ceil_div(256, p.places), p.chunk_rows / (4 * side)));
     p.part_rows = std::max<int64_t>(1, ceil_div(p.chunk_rows, parts));
     p.parts = int(std::max<int64_t>(1, ceil_div(p.chunk_rows, p.part_rows)));
     p.lg_run = lg_of(p.run);
@@ -274,8 +276,7 @@ int check(const tsx_group_norm *g, const char *what) {
 }
 
 size_t workspace_bytes(const tsx_group_norm *g) {
-    const NormPlan pl = plan_of(g);
-    return size_t(g->n) * pl.p.chunks * g->groups * sizeof(float2);
+    return size_t(g->n) * plan_of(g).p.chunks * g->groups * sizeof(float2);
 }
 
 template <int TYPE, int V>
@@ -329,8 +330,7 @@ int run_any(const tsx_group_norm *g, void *out, int8_t *q, float *scales, void *
         rc = group_norm_held(g, pl.p, stream, &taken);
         if (taken) return rc;
     }
-    return g->type == TSX_TYPE_F32 ? run<TSX_TYPE_F32>(pl, stream) : g->type == TSX_TYPE_F16 ? run<TSX_TYPE_F16>(pl, stream)
-                                                                                                : run<TSX_TYPE_BF16>(pl, stream);
+    return g->type == TSX_TYPE_F32 ? run<TSX_TYPE_F32>(pl, stream) : g->type == TSX_TYPE_F16 ? run<TSX_TYPE_F16>(pl, stream) : run<TSX_TYPE_BF16>(pl, stream);
 }
 
 }  // namespace

@@ -14,7 +14,7 @@ struct NormParams {
     int8_t *q;
     float *scales;
     const float *weight, *bias;
-    float2 *partial;                   // [n][chunks][groups]: mean, squares around it
+    float2 *partial;                   // [n][groups][chunks]: mean, squares around it (a group's chunks are read together)
     int64_t pixels, image_stride, pixel_stride;
     int64_t rows;                      // whole rows of S pixels
     int c, groups, d;
@@ -69,7 +69,6 @@ struct Place {
 // Mean and 1 / sqrt(variance + epsilon) of the groups of one image, into LDS, from the chunks' means and squares, in one pass around
 // the first chunk's mean: n_k (mean_k - mean_0)^2 is part of the variance, so what cancels is at most `chunks` times it.
 __device__ __forceinline__ void merge_chunks(const NormParams &p, int64_t image, float2 *group) {
-    const float2 *const partial = p.partial + image * p.chunks * p.groups;
     const float whole = float(p.chunk_rows) * float(p.S) * float(p.d);
     const float last = float(p.pixels - (p.chunks - 1) * p.chunk_rows * p.S) * float(p.d);
     const float of_total = 1.f / (float(p.pixels) * float(p.d));
@@ -77,13 +76,22 @@ __device__ __forceinline__ void merge_chunks(const NormParams &p, int64_t image,
     for (int g0 = 0; g0 < p.groups; g0 += blockDim.x >> lg) {
         const int g = g0 + (threadIdx.x >> lg);
         if (g >= p.groups) continue;                         // T threads agree
-        const float about = partial[g].x;
+        const float2 *const partial = p.partial + (image * p.groups + g) * p.chunks;
+        const float about = partial[0].x;
         float s = 0.f, m2 = 0.f;
-        for (int k = threadIdx.x & (T - 1); k < p.chunks; k += T) {
-            const float2 part = partial[int64_t(k) * p.groups + g];
-            const float n = k == p.chunks - 1 ? last : whole, d = part.x - about;
-            s = __builtin_fmaf(n, d, s);
-            m2 += __builtin_fmaf(n * d, d, part.y);
+        constexpr int AHEAD = 8;                             // requests that leave together
+        for (int k = threadIdx.x & (T - 1); k < p.chunks; k += AHEAD * T) {
+            float2 part[AHEAD];
+            static_for<0, AHEAD>([&](auto uc) { part[decltype(uc)::value] = partial[min(k + decltype(uc)::value * T, p.chunks - 1)]; });
+            static_for<0, AHEAD>([&](auto uc) {
+                constexpr int u = decltype(uc)::value;
+                const int at = k + u * T;
+                const float n = at < p.chunks - 1 ? whole : last, d = part[u].x - about;
+                if (at < p.chunks) {
+                    s = __builtin_fmaf(n, d, s);
+                    m2 += __builtin_fmaf(n * d, d, part[u].y);
+                }
+            });
         }
         s = sum_over_lanes(s, lg);
         m2 = sum_over_lanes(m2, lg);
@@ -98,43 +106,20 @@ template <int TYPE, int V>
 struct Piece {
     float v[V];
     __device__ __forceinline__ void load(const char *image, int64_t at) {
-        constexpr int SIZE = Kind<TYPE>::SIZE;
-        if constexpr (V == 1) {
-            if constexpr (TYPE == TSX_TYPE_F32) v[0] = *reinterpret_cast<const float *>(image + at * SIZE);
-            else v[0] = half_value<TYPE>(*reinterpret_cast<const unsigned short *>(image + at * SIZE));
-        } else {
-            Run<TYPE, V> r;
-            r.load(image + at * SIZE);
-            static_for<0, V>([&](auto ec) { v[decltype(ec)::value] = r.template get<decltype(ec)::value>(); });
-        }
+        Run<TYPE, V> r;
+        r.load(image + at * Kind<TYPE>::SIZE);
+        static_for<0, V>([&](auto ec) { v[decltype(ec)::value] = r.template get<decltype(ec)::value>(); });
     }
     __device__ __forceinline__ void load_some(const char *image, int64_t at, int left) {
-        constexpr int SIZE = Kind<TYPE>::SIZE;
-        if constexpr (V == 1) {
-            load(image, at);
-        } else {
-            Run<TYPE, V> r;
-            r.load_some(image + at * SIZE, left);
-            static_for<0, V>([&](auto ec) { v[decltype(ec)::value] = r.template get<decltype(ec)::value>(); });
-        }
-    }
-    template <int KIND>
-    static __device__ __forceinline__ float half_value(unsigned short bits) {
-        if constexpr (KIND == TSX_TYPE_BF16) return __builtin_bit_cast(float, unsigned(bits) << 16);
-        else return float(__builtin_bit_cast(_Float16, bits));
+        Run<TYPE, V> r;
+        r.load_some(image + at * Kind<TYPE>::SIZE, left);
+        static_for<0, V>([&](auto ec) { v[decltype(ec)::value] = r.template get<decltype(ec)::value>(); });
     }
     __device__ __forceinline__ void store(char *out, int64_t at, int left) const {
-        constexpr int SIZE = Kind<TYPE>::SIZE;
-        if constexpr (V == 1) {
-            if constexpr (TYPE == TSX_TYPE_F32) *reinterpret_cast<float *>(out + at * SIZE) = v[0];
-            else if constexpr (TYPE == TSX_TYPE_BF16) *reinterpret_cast<__bf16 *>(out + at * SIZE) = __bf16(v[0]);
-            else *reinterpret_cast<_Float16 *>(out + at * SIZE) = _Float16(v[0]);
-        } else {
-            Run<TYPE, V> r;
-            r.set(v);
-            if (left >= V) r.store(out + at * SIZE);
-            else r.store_some(out + at * SIZE, left);
-        }
+        Run<TYPE, V> r;
+        r.set(v);
+        if (left >= V) r.store(out + at * Kind<TYPE>::SIZE);
+        else r.store_some(out + at * Kind<TYPE>::SIZE, left);
     }
 };
 
