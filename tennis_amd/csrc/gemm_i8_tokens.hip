@@ -5,6 +5,8 @@
 // Rows of floats become int8 first (tokens_i8.hip), in the workspace, padded with zeros to whole chunks of K.  int32 sums are
 // exact, so every kernel here gives the same bits.
 #include <algorithm>
+#include <atomic>
+#include <cstdlib>
 
 #include "igemm_i8.hpp"
 #include "tokens_i8.hpp"
@@ -12,16 +14,16 @@
 namespace tsx {
 namespace {
 
-constexpr int CHUNK = 128;             // K bytes of a row per chunk: two packed K-steps
+constexpr int KSTEP = 64;              // K bytes of a packed K-step
 
 struct TokenGemmParams {
-    const int8_t *q;                   // [m][pitch], 16-byte aligned, pitch a multiple of CHUNK... or k itself where that is one
+    const int8_t *q;                   // [m][pitch], rows and their length multiples of 16 bytes
     const float *x_scales;
     const int8_t *wp;                  // as tsx_gemm_i8_pack_weights lays them out
     const float *w_scales, *bias;
     void *out;
     int64_t pitch, out_stride;
-    int m, n, frags, chunks;
+    int m, n, k, frags, ksteps;        // k: bytes of a row that are read, a multiple of 16
     int act;
     float slope;
     int row_tiles, col_tiles, tiles_per_xcd;
@@ -65,23 +67,42 @@ __device__ __forceinline__ void store_fragment(const TokenGemmParams &p, const v
     }
 }
 
-// the scales and biases of a lane's 16 accumulators
+// the scales and biases of a lane's 16 accumulators, all requested at once
 __device__ __forceinline__ void load_columns(const TokenGemmParams &p, int col0, float (&ws)[16], float (&bias)[16]) {
-    const int half = (threadIdx.x % 64) / 32;
-    static_for<0, 16>([&](auto rc) {
-        constexpr int r = decltype(rc)::value;
-        const int col = min(col0 + 8 * (r / 4) + 4 * half + r % 4, p.n - 1);
-        ws[r] = p.w_scales[col];
-        bias[r] = p.bias ? p.bias[col] : 0.f;
-    });
+    typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
+    const int first = col0 + 4 * ((threadIdx.x % 64) / 32);
+    auto load = [&](const float *from, float (&to)[16]) __attribute__((always_inline)) {
+        if (col0 + 32 <= p.n)       // uniform
+            static_for<0, 4>([&](auto gc) {
+                constexpr int g = decltype(gc)::value;
+                const v4f v = *reinterpret_cast<const v4f_any *>(from + first + 8 * g);
+                static_for<0, 4>([&](auto jc) { to[4 * g + decltype(jc)::value] = v[decltype(jc)::value]; });
+            });
+        else
+            static_for<0, 16>([&](auto rc) { constexpr int r = decltype(rc)::value; to[r] = from[min(first + 8 * (r / 4) + r % 4, p.n - 1)]; });
+    };
+    static_for<0, 16>([&](auto rc) { bias[decltype(rc)::value] = 0.f; });
+    load(p.w_scales, ws);
+    if (p.bias) load(p.bias, bias);
 }
 
-// WR x WC wavefronts, each with FR x FC fragments of 32 tokens x 32 columns.
-template <int WR, int WC, int FR, int FC, int OUT>
+// LDS is this workgroup's own: what was read from it is read, and what the wavefronts wrote is there, behind the barrier.  Requests to
+// memory stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+template <int N>
+__device__ __forceinline__ void wait_for_all_but() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+// WR x WC wavefronts, each with FR x FC fragments of 32 tokens x 32 columns; S chunks of KS K-steps in LDS.
+template <int WR, int WC, int FR, int FC, int KS, int S, int OUT>
 __global__ __launch_bounds__(WR *WC * 64) void gemm_i8_tokens_kernel(TokenGemmParams p) {
-    constexpr int WAVES = WR * WC, ROWS = 32 * WR * FR, COLS = 32 * WC * FC;
+    constexpr int CHUNK = KS * KSTEP, PIECES = CHUNK / 16, WAVES = WR * WC, ROWS = 32 * WR * FR, COLS = 32 * WC * FC, HALVES = 2 * KS;
     constexpr int A_BYTES = ROWS * CHUNK, B_BYTES = COLS * CHUNK, A_LOADS = A_BYTES / 1024 / WAVES, B_LOADS = B_BYTES / 1024 / WAVES;
-    __shared__ __attribute__((aligned(16))) int8_t lds[2][A_BYTES + B_BYTES];
+    static_assert(A_LOADS * 1024 * WAVES == A_BYTES && B_LOADS * 1024 * WAVES == B_BYTES && (S - 1) * (A_LOADS + B_LOADS) < 64, "whole loads, counted in six bits");
+    extern __shared__ __attribute__((aligned(16))) int8_t lds[];      // [S][A_BYTES + B_BYTES]
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int wave_r = wave / WC, wave_c = wave % WC;
     // blockIdx % 8 is the XCD: each takes a run of consecutive tiles, which walk four row tiles before the next column tile
@@ -93,25 +114,38 @@ __global__ __launch_bounds__(WR *WC * 64) void gemm_i8_tokens_kernel(TokenGemmPa
     const int tile_c = in_group / group_rows, tile_r = 4 * group + in_group - tile_c * group_rows;
     const int row0 = tile_r * ROWS, frag0 = tile_c * (COLS / 32);
 
-    // Rows in LDS are 128 bytes, their pieces of 16 XORed with bits 1 .. 3 of the row: 16 rows cover all banks for one piece.
-    // A load instruction fills 8 rows; rows beyond m are the last one again, never stored.
-    const int8_t *a_src[A_LOADS], *b_src[B_LOADS];
+    // A row in LDS is its CHUNK bytes, its pieces of 16 XORed with bits of the row that make 16 rows cover all banks for one piece.  A
+    // load instruction fills 1 KiB of such rows; rows beyond m are the last one again, never stored.  Pieces behind the end of a row are
+    // its first one, against weights that are zero.  Scalar bases and 32-bit lane offsets.
+    const auto key_of = [](int row) { return (row >> (KS == 1 ? 2 : 1)) & (PIECES - 1); };
+    const int chunks = (p.ksteps + KS - 1) / KS;
+    const int8_t *const a_base = p.q + int64_t(row0) * p.pitch;
+    unsigned a_off[A_LOADS], b_off[B_LOADS];
+    int a_piece[A_LOADS];
     static_for<0, A_LOADS>([&](auto ic) {
         constexpr int i = decltype(ic)::value;
-        const int r = (wave * A_LOADS + i) * 8 + lane / 8;
-        a_src[i] = p.q + int64_t(min(row0 + r, p.m - 1)) * p.pitch + ((lane % 8) ^ ((r >> 1) & 7)) * 16;
+        const int r = (wave * A_LOADS + i) * (64 / PIECES) + lane / PIECES;
+        a_piece[i] = ((lane % PIECES) ^ key_of(r)) * 16;
+        a_off[i] = unsigned(min(r, p.m - 1 - row0)) * unsigned(p.pitch);
     });
     // weights: packed[K-step][fragment][half][lane][16], in LDS [K-step of the chunk][fragment][half][lane][16]
     static_for<0, B_LOADS>([&](auto ic) {
         constexpr int i = decltype(ic)::value;
         const int unit = wave * B_LOADS + i, step = unit / (2 * COLS / 32), in_step = unit % (2 * COLS / 32);
         const int frag = min(frag0 + in_step / 2, p.frags - 1);
-        b_src[i] = p.wp + (int64_t(step) * p.frags + frag) * 2048 + (in_step % 2) * 1024 + lane * 16;
+        b_off[i] = unsigned(step * p.frags + frag) * 2048u + (in_step % 2) * 1024 + lane * 16;
     });
-    const int64_t b_step = int64_t(p.frags) * 4096;
-    auto fetch = [&](int c, int buf) __attribute__((always_inline)) {
-        static_for<0, A_LOADS>([&](auto ic) { constexpr int i = decltype(ic)::value; to_lds(a_src[i] + int64_t(c) * CHUNK, &lds[buf][(wave * A_LOADS + i) * 1024]); });
-        static_for<0, B_LOADS>([&](auto ic) { constexpr int i = decltype(ic)::value; to_lds(b_src[i] + c * b_step, &lds[buf][A_BYTES + (wave * B_LOADS + i) * 1024]); });
+    const int64_t b_step = int64_t(p.frags) * (KS * 2048);
+    auto fetch = [&](int chunk, int buf) __attribute__((always_inline)) {
+        const int c = min(chunk, chunks - 1);                // behind the last chunk: that one again, not read from LDS
+        int8_t *const at = lds + buf * (A_BYTES + B_BYTES);
+        const int8_t *const b = p.wp + c * b_step;
+        static_for<0, A_LOADS>([&](auto ic) {
+            constexpr int i = decltype(ic)::value;
+            const int k = c * CHUNK + a_piece[i];
+            to_lds(a_base + (a_off[i] + unsigned(k < p.k ? k : 0)), at + (wave * A_LOADS + i) * 1024);
+        });
+        static_for<0, B_LOADS>([&](auto ic) { constexpr int i = decltype(ic)::value; to_lds(b + b_off[i], at + A_BYTES + (wave * B_LOADS + i) * 1024); });
     };
 
     v16i acc[FR][FC];
@@ -119,31 +153,54 @@ __global__ __launch_bounds__(WR *WC * 64) void gemm_i8_tokens_kernel(TokenGemmPa
         constexpr int f = decltype(fc)::value;
         static_for<0, 16>([&](auto rc) { acc[f / FC][f % FC][decltype(rc)::value] = 0; });
     });
-    const int a_row = (wave_r * FR * 32 + lane % 32) * CHUNK, a_key = (lane >> 1) & 7;
-    fetch(0, 0);
-    for (int c = 0; c < p.chunks; ++c) {
-        const int buf = c & 1;
-        // chunk c is in LDS, for every wavefront, and the other buffer is read
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (c + 1 < p.chunks) fetch(c + 1, buf ^ 1);
-        static_for<0, CHUNK / 32>([&](auto hc) {
+    const int a_row = (wave_r * FR * 32 + lane % 32) * CHUNK, a_key = key_of(lane % 32);
+    v4i a[2][FR], b[2][FC];
+    auto read = [&](auto hc, int buf) __attribute__((always_inline)) {
+        constexpr int h = decltype(hc)::value, set = h % 2;
+        const int8_t *const at = lds + buf * (A_BYTES + B_BYTES);
+        static_for<0, FC>([&](auto fc) {
+            constexpr int f = decltype(fc)::value;
+            b[set][f] = *reinterpret_cast<const v4i *>(at + A_BYTES + (((h / 2) * (COLS / 32) + wave_c * FC + f) * 2 + h % 2) * 1024 + lane * 16);
+        });
+        static_for<0, FR>([&](auto ic) {
+            constexpr int i = decltype(ic)::value;
+            a[set][i] = *reinterpret_cast<const v4i *>(at + a_row + i * 32 * CHUNK + ((2 * h + lane / 32) ^ a_key) * 16);
+        });
+    };
+    static_for<0, S>([&](auto sc) { fetch(decltype(sc)::value, decltype(sc)::value); });
+    wait_for_all_but<(S - 1) * (A_LOADS + B_LOADS)>();
+    lds_barrier();
+    read(std::integral_constant<int, 0>{}, 0);
+    int buf = 0;
+    for (int c = 0; c < chunks; ++c) {
+        const int after = buf + 1 == S ? 0 : buf + 1;
+        static_for<0, HALVES>([&](auto hc) {
             constexpr int h = decltype(hc)::value;
-            v4i a[FR], b[FC];
-            static_for<0, FR>([&](auto ic) {
-                constexpr int i = decltype(ic)::value;
-                a[i] = *reinterpret_cast<const v4i *>(&lds[buf][a_row + i * 32 * CHUNK + ((2 * h + lane / 32) ^ a_key) * 16]);
-            });
-            static_for<0, FC>([&](auto fc) {
-                constexpr int f = decltype(fc)::value;
-                b[f] = *reinterpret_cast<const v4i *>(&lds[buf][A_BYTES + (((h / 2) * (COLS / 32) + wave_c * FC + f) * 2 + h % 2) * 1024 + lane * 16]);
-            });
+            if constexpr (h + 1 < HALVES) {
+                read(std::integral_constant<int, h + 1>{}, buf);
+            } else {
+                // Every wavefront has its operands of this chunk in registers: its buffer is free behind the barrier, and the next
+                // chunk is there for all.  The rest of this chunk's arithmetic covers the first reads behind it.
+                wait_for_all_but<(S - 2) * (A_LOADS + B_LOADS)>();
+                lds_barrier();
+                read(std::integral_constant<int, 0>{}, after);
+                fetch(c + S, buf);
+            }
             static_for<0, FR * FC>([&](auto fc) {
                 constexpr int i = decltype(fc)::value / FC, f = decltype(fc)::value % FC;
-                acc[i][f] = __builtin_amdgcn_mfma_i32_32x32x32_i8(b[f], a[i], acc[i][f], 0, 0, 0);
+                acc[i][f] = __builtin_amdgcn_mfma_i32_32x32x32_i8(b[h % 2][f], a[h % 2][i], acc[i][f], 0, 0, 0);
             });
+            // reads and requests between the multiplications
+            static_for<0, FR * FC>([&](auto fc) {
+                if constexpr (h + 1 == HALVES) __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            });
+            __builtin_amdgcn_sched_barrier(0);
         });
+        buf = after;
     }
+    wait_for_all_but<0>();                                   // nothing on its way into LDS when the workgroup gives it back
     static_for<0, FC>([&](auto fc) {
         constexpr int f = decltype(fc)::value;
         const int col0 = (frag0 + wave_c * FC + f) * 32;
@@ -159,22 +216,55 @@ __global__ __launch_bounds__(WR *WC * 64) void gemm_i8_tokens_kernel(TokenGemmPa
     });
 }
 
-template <int WR, int WC, int FR, int FC, int OUT>
+// more than 64 KiB of dynamic LDS, granted once per kernel and device
+int grant_lds(const void *kernel) {
+    struct Granted { std::atomic<const void *> kernel; std::atomic<uint64_t> devices; };
+    static Granted table[64];
+    int dev = 0;
+    TSX_HIP(hipGetDevice(&dev));
+    for (Granted &g : table) {
+        const void *none = nullptr;
+        if (g.kernel.load() != kernel && !g.kernel.compare_exchange_strong(none, kernel) && none != kernel) continue;
+        if (dev >= 64 || !(g.devices.load() >> dev & 1)) {
+            TSX_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+            if (dev < 64) g.devices.fetch_or(uint64_t(1) << dev);
+        }
+        return 0;
+    }
+    return check_hip(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024), "hipFuncSetAttribute");
+}
+
+template <int WR, int WC, int FR, int FC, int KS, int S, int OUT>
 int launch_tile(TokenGemmParams p, hipStream_t stream) {
     p.row_tiles = int(ceil_div(p.m, 32 * WR * FR));
     p.col_tiles = int(ceil_div(p.n, 32 * WC * FC));
     p.tiles_per_xcd = int(ceil_div(int64_t(p.row_tiles) * p.col_tiles, 8));
-    hipLaunchKernelGGL((gemm_i8_tokens_kernel<WR, WC, FR, FC, OUT>), dim3(unsigned(8 * p.tiles_per_xcd)), dim3(WR * WC * 64), 0, stream, p);
+    constexpr int LDS = S * 32 * (WR * FR + WC * FC) * KS * KSTEP;
+    const auto kernel = gemm_i8_tokens_kernel<WR, WC, FR, FC, KS, S, OUT>;
+    if (LDS > 64 * 1024) {
+        const int rc = grant_lds(reinterpret_cast<const void *>(kernel));
+        if (rc) return rc;
+    }
+    hipLaunchKernelGGL(kernel, dim3(unsigned(8 * p.tiles_per_xcd)), dim3(WR * WC * 64), LDS, stream, p);
     TSX_LAUNCH_CHECK("gemm_i8_tokens_kernel");
     return 0;
 }
 
 template <int OUT>
 int launch(const TokenGemmParams &p, hipStream_t stream) {
-    return launch_tile<2, 2, 2, 2, OUT>(p, stream);
+    const char *e = std::getenv("TSX_TOKENS_TILE");
+    switch (e ? e[0] - '0' : 1) {
+        case 0: return launch_tile<2, 2, 1, 1, 2, 4, OUT>(p, stream);
+        case 1: return launch_tile<2, 2, 2, 2, 2, 4, OUT>(p, stream);
+        case 2: return launch_tile<2, 2, 4, 4, 1, 4, OUT>(p, stream);
+        case 3: return launch_tile<2, 4, 4, 2, 1, 4, OUT>(p, stream);
+        case 4: return launch_tile<2, 4, 2, 2, 1, 6, OUT>(p, stream);
+        case 5: return launch_tile<2, 2, 2, 2, 1, 5, OUT>(p, stream);
+        default: return launch_tile<2, 2, 1, 1, 2, 8, OUT>(p, stream);
+    }
 }
 
-// rows of int8 tokens of another length, stride or alignment than the kernels read, copied to whole chunks
+// rows of int8 tokens of another length, stride or alignment than the kernels read, copied to whole pieces of 16
 __global__ __launch_bounds__(256) void copy_tokens_kernel(const int8_t *x, int64_t x_stride, int k, int8_t *q, int pitch, int64_t rows) {
     const int pieces = pitch / 16;
     for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < rows * pieces; i += int64_t(gridDim.x) * 256) {
@@ -202,10 +292,10 @@ int check(const tsx_token_gemm *g) {
     return 0;
 }
 
-int padded(int k) { return int(round_up(k, CHUNK)); }
+int padded(int k) { return int(round_up(k, 16)); }
 
 bool reads_in_place(const tsx_token_gemm *g) {
-    return g->x_type == TSX_TYPE_I8 && g->k % CHUNK == 0 && (g->m <= 1 || g->x_stride % 16 == 0) && reinterpret_cast<uintptr_t>(g->x_dev) % 16 == 0;
+    return g->x_type == TSX_TYPE_I8 && g->k % 16 == 0 && (g->m <= 1 || g->x_stride % 16 == 0) && reinterpret_cast<uintptr_t>(g->x_dev) % 16 == 0;
 }
 
 size_t scales_offset(const tsx_token_gemm *g) { return size_t(g->m) * padded(g->k); }
@@ -264,7 +354,8 @@ int tsx_gemm_i8_tokens(const tsx_token_gemm *g, void *workspace_dev, size_t work
     p.m = g->m;
     p.n = g->n;
     p.frags = int(tsx::round_up(g->n, 128) / 32);
-    p.chunks = kp / tsx::CHUNK;
+    p.k = kp;
+    p.ksteps = int(tsx::ceil_div(kp, tsx::KSTEP));
     p.act = g->act;
     p.slope = g->slope;
     return g->out_type == TSX_TYPE_F32 ? tsx::launch<TSX_TYPE_F32>(p, stream) : g->out_type == TSX_TYPE_F16 ? tsx::launch<TSX_TYPE_F16>(p, stream)
