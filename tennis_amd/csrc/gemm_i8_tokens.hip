@@ -39,15 +39,20 @@ __device__ __forceinline__ void to_lds(const int8_t *at, int8_t *lds) {
 
 // What leaves a fragment of 32 output columns x 32 tokens: accumulator r of lane l is column 8 (r / 4) + 4 (l / 32) + r % 4 of token
 // l % 32; swaps between the half-waves leave a lane with 16 consecutive columns, the lower ones with 0 .. 15, the upper ones with 16 .. 31.
-template <int OUT>
-__device__ __forceinline__ void store_fragment(const TokenGemmParams &p, const v16i &acc, const float (&ws)[16], const float (&bias)[16], float xs,
-                                               int row, int col0) {
-    const int lane = threadIdx.x % 64;
+// scales, biases: of the fragment's columns, in LDS; xs: the token's; out: the token's column 16 (l / 32) of the fragment, left: columns
+// from there on that exist, at most 0 where the token is none.
+template <int OUT, int ACT>
+__device__ __forceinline__ void store_fragment(const TokenGemmParams &p, const v16i &acc, const float *scales, const float *biases, float xs, char *out, int left) {
+    const int half = 4 * ((threadIdx.x % 64) / 32);
     float v[16];
-    static_for<0, 16>([&](auto rc) { constexpr int r = decltype(rc)::value; v[r] = __fmul_rn(__fmul_rn(float(acc[r]), ws[r]), xs); });
-    if (p.bias) static_for<0, 16>([&](auto rc) { constexpr int r = decltype(rc)::value; v[r] = __fadd_rn(v[r], bias[r]); });
-    activate_tokens(v, p.act, p.slope);
-    Run<OUT, 16> out, own;
+    static_for<0, 4>([&](auto gc) {
+        constexpr int g = decltype(gc)::value;
+        const v4f ws = *reinterpret_cast<const v4f *>(scales + 8 * g + half), bias = *reinterpret_cast<const v4f *>(biases + 8 * g + half);
+        // a missing bias is -0, which changes no sum
+        static_for<0, 4>([&](auto jc) { constexpr int j = decltype(jc)::value; v[4 * g + j] = __fadd_rn(__fmul_rn(__fmul_rn(float(acc[4 * g + j]), ws[j]), xs), bias[j]); });
+    });
+    activate_as<ACT>(v, p.slope);
+    Run<OUT, 16> to, own;
     own.set(v);
     constexpr int W = Run<OUT, 4>::WORDS;      // words of four values
     static_for<0, 2>([&](auto pc) {
@@ -55,35 +60,24 @@ __device__ __forceinline__ void store_fragment(const TokenGemmParams &p, const v
         static_for<0, W>([&](auto wc) {
             constexpr int w = decltype(wc)::value;
             const auto s = __builtin_amdgcn_permlane32_swap(own.word[a * W + w], own.word[(a + 2) * W + w], false, false);
-            out.word[2 * a * W + w] = s[0];
-            out.word[(2 * a + 1) * W + w] = s[1];
+            to.word[2 * a * W + w] = s[0];
+            to.word[(2 * a + 1) * W + w] = s[1];
         });
     });
-    const int col = col0 + 16 * (lane / 32), left = p.n - col;
-    if (row < p.m && left > 0) {
-        char *const at = static_cast<char *>(p.out) + (int64_t(row) * p.out_stride + col) * (OUT == TSX_TYPE_F32 ? 4 : 2);
-        if (left >= 16) out.store(at);
-        else out.store_some(at, left);
-    }
+    if (left >= 16) to.store(out);
+    else if (left > 0) to.store_some(out, left);
 }
 
-// the scales and biases of a lane's 16 accumulators, all requested at once
-__device__ __forceinline__ void load_columns(const TokenGemmParams &p, int col0, float (&ws)[16], float (&bias)[16]) {
-    typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
-    const int first = col0 + 4 * ((threadIdx.x % 64) / 32);
-    auto load = [&](const float *from, float (&to)[16]) __attribute__((always_inline)) {
-        if (col0 + 32 <= p.n)       // uniform
-            static_for<0, 4>([&](auto gc) {
-                constexpr int g = decltype(gc)::value;
-                const v4f v = *reinterpret_cast<const v4f_any *>(from + first + 8 * g);
-                static_for<0, 4>([&](auto jc) { to[4 * g + decltype(jc)::value] = v[decltype(jc)::value]; });
-            });
-        else
-            static_for<0, 16>([&](auto rc) { constexpr int r = decltype(rc)::value; to[r] = from[min(first + 8 * (r / 4) + r % 4, p.n - 1)]; });
-    };
-    static_for<0, 16>([&](auto rc) { bias[decltype(rc)::value] = 0.f; });
-    load(p.w_scales, ws);
-    if (p.bias) load(p.bias, bias);
+// f(the activation as a constant): one branch around all of a wavefront's values
+template <class F>
+__device__ __forceinline__ void by_act(int act, F &&f) {
+    switch (act) {
+        case TSX_ACT_RELU: f(std::integral_constant<int, TSX_ACT_RELU>{}); break;
+        case TSX_ACT_LEAKY_RELU: f(std::integral_constant<int, TSX_ACT_LEAKY_RELU>{}); break;
+        case TSX_ACT_MISH_FAST: f(std::integral_constant<int, TSX_ACT_MISH_FAST>{}); break;
+        case TSX_ACT_SILU: f(std::integral_constant<int, TSX_ACT_SILU>{}); break;
+        default: f(std::integral_constant<int, TSX_ACT_NONE>{}); break;
+    }
 }
 
 // LDS is this workgroup's own: what was read from it is read, and what the wavefronts wrote is there, behind the barrier.  Requests to
@@ -103,6 +97,9 @@ __global__ __launch_bounds__(WR *WC * 64) void gemm_i8_tokens_kernel(TokenGemmPa
     constexpr int A_BYTES = ROWS * CHUNK, B_BYTES = COLS * CHUNK, A_LOADS = A_BYTES / 1024 / WAVES, B_LOADS = B_BYTES / 1024 / WAVES;
     static_assert(A_LOADS * 1024 * WAVES == A_BYTES && B_LOADS * 1024 * WAVES == B_BYTES && (S - 1) * (A_LOADS + B_LOADS) < 64, "whole loads, counted in six bits");
     extern __shared__ __attribute__((aligned(16))) int8_t lds[];      // [S][A_BYTES + B_BYTES]
+    // the tile's scales and biases, requested ahead of everything: in the epilogue each request would be waited for
+    __shared__ __attribute__((aligned(16))) float of_cols[2][COLS], of_rows[ROWS];
+    constexpr int THREADS = WAVES * 64;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int wave_r = wave / WC, wave_c = wave % WC;
     // blockIdx % 8 is the XCD: each takes a run of consecutive tiles, which walk four row tiles before the next column tile
@@ -113,6 +110,17 @@ __global__ __launch_bounds__(WR *WC * 64) void gemm_i8_tokens_kernel(TokenGemmPa
     const int group_rows = min(4, p.row_tiles - 4 * group);
     const int tile_c = in_group / group_rows, tile_r = 4 * group + in_group - tile_c * group_rows;
     const int row0 = tile_r * ROWS, frag0 = tile_c * (COLS / 32);
+    static_for<0, (COLS + THREADS - 1) / THREADS>([&](auto ic) {
+        const int i = threadIdx.x + decltype(ic)::value * THREADS, col = min(frag0 * 32 + i, p.n - 1);
+        if (COLS % THREADS == 0 || i < COLS) {
+            of_cols[0][i] = p.w_scales[col];
+            of_cols[1][i] = p.bias ? p.bias[col] : -0.f;
+        }
+    });
+    static_for<0, (ROWS + THREADS - 1) / THREADS>([&](auto ic) {
+        const int i = threadIdx.x + decltype(ic)::value * THREADS;
+        if (ROWS % THREADS == 0 || i < ROWS) of_rows[i] = p.x_scales[min(row0 + i, p.m - 1)];
+    });
 
     // A row in LDS is its CHUNK bytes, its pieces of 16 XORed with bits of the row that make 16 rows cover all banks for one piece.  A
     // load instruction fills 1 KiB of such rows; rows beyond m are the last one again, never stored.  Pieces behind the end of a row are
@@ -201,23 +209,26 @@ __global__ __launch_bounds__(WR *WC * 64) void gemm_i8_tokens_kernel(TokenGemmPa
         buf = after;
     }
     wait_for_all_but<0>();                                   // nothing on its way into LDS when the workgroup gives it back
-    static_for<0, FC>([&](auto fc) {
-        constexpr int f = decltype(fc)::value;
-        const int col0 = (frag0 + wave_c * FC + f) * 32;
-        if (col0 < p.n) {                                    // uniform
-            float ws[16], bias[16];
-            load_columns(p, col0, ws, bias);
-            static_for<0, FR>([&](auto ic) {
-                constexpr int i = decltype(ic)::value;
-                const int row = row0 + (wave_r * FR + i) * 32 + lane % 32;
-                store_fragment<OUT>(p, acc[i][f], ws, bias, p.x_scales[min(row, p.m - 1)], row, col0);
+    by_act(p.act, [&](auto act) __attribute__((always_inline)) {
+        constexpr int SIZE = OUT == TSX_TYPE_F32 ? 4 : 2;
+        static_for<0, FR>([&](auto ic) {
+            constexpr int i = decltype(ic)::value;
+            const int in_tile = (wave_r * FR + i) * 32 + lane % 32, row = row0 + in_tile;
+            const float xs = of_rows[in_tile];
+            const int col = frag0 * 32 + wave_c * FC * 32 + 16 * (lane / 32);
+            char *const out = static_cast<char *>(p.out) + (int64_t(row) * p.out_stride + col) * SIZE;
+            static_for<0, FC>([&](auto fc) {
+                constexpr int f = decltype(fc)::value;
+                const int at = (wave_c * FC + f) * 32;
+                store_fragment<OUT, decltype(act)::value>(p, acc[i][f], of_cols[0] + at, of_cols[1] + at, xs, out + f * (32 * SIZE),
+                                                          row < p.m ? p.n - col - 32 * f : 0);
             });
-        }
+        });
     });
 }
 
 // more than 64 KiB of dynamic LDS, granted once per kernel and device
-int grant_lds(const void *kernel) {
+int grant_lds(const void *kernel, int bytes) {
     struct Granted { std::atomic<const void *> kernel; std::atomic<uint64_t> devices; };
     static Granted table[64];
     int dev = 0;
@@ -226,12 +237,12 @@ int grant_lds(const void *kernel) {
         const void *none = nullptr;
         if (g.kernel.load() != kernel && !g.kernel.compare_exchange_strong(none, kernel) && none != kernel) continue;
         if (dev >= 64 || !(g.devices.load() >> dev & 1)) {
-            TSX_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+            TSX_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
             if (dev < 64) g.devices.fetch_or(uint64_t(1) << dev);
         }
         return 0;
     }
-    return check_hip(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024), "hipFuncSetAttribute");
+    return check_hip(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "hipFuncSetAttribute");
 }
 
 template <int WR, int WC, int FR, int FC, int KS, int S, int OUT>
@@ -242,7 +253,7 @@ int launch_tile(TokenGemmParams p, hipStream_t stream) {
     constexpr int LDS = S * 32 * (WR * FR + WC * FC) * KS * KSTEP;
     const auto kernel = gemm_i8_tokens_kernel<WR, WC, FR, FC, KS, S, OUT>;
     if (LDS > 64 * 1024) {
-        const int rc = grant_lds(reinterpret_cast<const void *>(kernel));
+        const int rc = grant_lds(reinterpret_cast<const void *>(kernel), LDS);
         if (rc) return rc;
     }
     hipLaunchKernelGGL(kernel, dim3(unsigned(8 * p.tiles_per_xcd)), dim3(WR * WC * 64), LDS, stream, p);
