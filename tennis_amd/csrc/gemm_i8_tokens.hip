@@ -227,6 +227,143 @@ __global__ __launch_bounds__(WR *WC * 64) void gemm_i8_tokens_kernel(TokenGemmPa
     });
 }
 
+// ---- few tokens: a stream over the weights
+//
+// With up to 64 tokens the product reads n k bytes of weights and does little with each.  A workgroup owns 16 output columns (4096
+// columns: one workgroup a CU) and its 8 wavefronts split K, every eighth K-step each; a K-step of 16 columns is one 16-byte load a
+// lane, eight of them in flight from the first instruction on.  X, the type of the rows: TSX_TYPE_I8, or floats that the workgroup
+// quantizes itself while its weights are on their way (all of them do, out of the L2: one launch and its start less).  MT: groups of 16
+// tokens.  v_mfma_i32_16x16x64_i8: lane l supplies row (token or column) l % 16, K bytes 16 (l / 16) ..; accumulator r of lane l is
+// column 4 (l / 16) + r of token l % 16.  The eight partial sums meet in LDS.
+constexpr int FEW_THREADS = 512, FEW_WAVES = FEW_THREADS / 64;
+
+struct FewTokens : TokenGemmParams {
+    const void *x;
+    int64_t x_stride;
+    int lg_threads;                    // of a row that the workgroup quantizes
+    int cols;                          // values of a row; k: of its int8 row, as the K-steps are
+};
+
+template <int X, int MT, int NC, int AHEAD, int OUT>
+__global__ __launch_bounds__(FEW_THREADS) void gemm_i8_few_tokens_kernel(FewTokens p) {
+    typedef int v4i_ __attribute__((ext_vector_type(4)));
+    extern __shared__ __attribute__((aligned(16))) int8_t lds[];      // [8][MT][NC][4][64] partial sums, then the rows
+    __shared__ float scales[16 * MT];
+    __shared__ unsigned tops[FEW_WAVES];
+    int *const sums = reinterpret_cast<int *>(lds);
+    int8_t *const rows = lds + FEW_WAVES * MT * NC * 1024;
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), piece = lane / 16, row = lane % 16;
+    const int row0 = X == TSX_TYPE_I8 ? int(blockIdx.y) * 16 * MT : 0;
+    const int col16 = blockIdx.x * NC;                       // in columns of 16
+    const int8_t *w[NC];
+    static_for<0, NC>([&](auto nc) {
+        const int c = col16 + decltype(nc)::value;
+        w[decltype(nc)::value] = p.wp + int64_t(c >> 1) * 2048 + (piece >> 1) * 1024 + (16 * (c & 1) + row + 32 * (piece & 1)) * 16;
+    });
+    const int64_t w_step = int64_t(p.frags) * 2048;
+    v4i_ a[AHEAD][NC];
+    auto fetch = [&](int first) __attribute__((always_inline)) {
+        static_for<0, AHEAD>([&](auto uc) {
+            constexpr int u = decltype(uc)::value;
+            static_for<0, NC>([&](auto nc) { a[u][decltype(nc)::value] = *reinterpret_cast<const v4i_ *>(w[decltype(nc)::value] + min(first + FEW_WAVES * u, p.ksteps - 1) * w_step); });
+        });
+    };
+    fetch(wave);
+    const int pitch = p.ksteps * KSTEP + 16;                 // of a row in LDS: the 16 put the rows' pieces into different banks
+    if constexpr (X != TSX_TYPE_I8) {
+        constexpr int PIECE = 8, SIZE = X == TSX_TYPE_F32 ? 4 : 2, HELD = 4;
+        typedef Run<X, PIECE> Values;
+        const int lg = p.lg_threads, T = 1 << lg, whole = p.cols / PIECE, pieces = (p.cols + PIECE - 1) / PIECE;
+        const int t = threadIdx.x & (T - 1), side = FEW_THREADS >> lg, turns = (pieces + HELD * T - 1) / (HELD * T);
+        for (int r0 = 0; r0 < p.m; r0 += side) {
+            const int r = r0 + (threadIdx.x >> lg);
+            const char *const x = static_cast<const char *>(p.x) + min(r, p.m - 1) * p.x_stride * SIZE;
+            Values v[HELD];
+            auto load = [&](int first) __attribute__((always_inline)) {
+                if (whole)           // uniform
+                    static_for<0, HELD>([&](auto ic) { v[decltype(ic)::value].load(x + int64_t(min(first + t + decltype(ic)::value * T, whole - 1)) * (PIECE * SIZE)); });
+                static_for<0, HELD>([&](auto ic) {
+                    constexpr int i = decltype(ic)::value;
+                    const int at = first + t + i * T;
+                    if (at >= whole) v[i].clear();
+                    if (at >= whole && at < pieces) v[i].load_some(x + int64_t(at) * (PIECE * SIZE), p.cols - at * PIECE);
+                });
+            };
+            unsigned top = 0;
+            for (int turn = 0; turn < turns; ++turn) {
+                load(turn * HELD * T);
+                static_for<0, HELD>([&](auto ic) { top = v[decltype(ic)::value].top(top); });
+            }
+            top = over_lanes(top, lg, [](unsigned one, unsigned other) { return Values::template larger<X>(one, other); });
+            if (lg > 6) {            // uniform: wavefronts share a row, all rows are this turn's
+                if (lane == 0) tops[wave] = top;
+                __syncthreads();
+                for (int i = 0; i < T / 64; ++i) top = Values::template larger<X>(top, tops[(wave & ~(T / 64 - 1)) + i]);
+            }
+            const TokenScale s(top_value<X>(top));
+            if (t == 0 && r < p.m) scales[r] = s.scale;
+            for (int turn = 0; turn < turns; ++turn) {
+                if (turns > 1) load(turn * HELD * T);
+                static_for<0, HELD>([&](auto ic) {
+                    constexpr int i = decltype(ic)::value;
+                    const int at = turn * HELD * T + t + i * T;
+                    if (at >= pieces || r >= p.m) return;
+                    unsigned b[PIECE];
+                    static_for<0, PIECE>([&](auto ec) { constexpr int e = decltype(ec)::value; b[e] = s.bits(__fmul_rn(v[i].template get<e>(), s.lift)); });
+                    v2u out = {low_bytes(b[0], b[1], b[2], b[3]), low_bytes(b[4], b[5], b[6], b[7])};
+                    if (s.reciprocal == 0.f) out = v2u{0, 0};
+                    *reinterpret_cast<v2u *>(rows + r * pitch + at * PIECE) = out;       // behind the row's end: against weights that are zero
+                });
+            }
+        }
+        __syncthreads();
+    } else {
+        if (threadIdx.x < 16 * MT) scales[threadIdx.x] = p.x_scales[min(row0 + int(threadIdx.x), p.m - 1)];
+    }
+    v4i_ acc[MT][NC];
+    static_for<0, MT * NC>([&](auto mc) { acc[decltype(mc)::value / NC][decltype(mc)::value % NC] = v4i_{0, 0, 0, 0}; });
+    for (int first = wave; first < p.ksteps; first += FEW_WAVES * AHEAD) {
+        v4i_ b[AHEAD][MT];
+        static_for<0, AHEAD>([&](auto uc) {
+            constexpr int u = decltype(uc)::value;
+            const int k = min(first + FEW_WAVES * u, p.ksteps - 1) * KSTEP + piece * 16;
+            static_for<0, MT>([&](auto mc) {
+                constexpr int i = decltype(mc)::value;
+                const int token = min(row0 + 16 * i + row, p.m - 1);
+                if constexpr (X == TSX_TYPE_I8) b[u][i] = *reinterpret_cast<const v4i_ *>(p.q + token * p.pitch + (k < p.k ? k : 0));
+                else b[u][i] = *reinterpret_cast<const v4i_ *>(rows + token * pitch + k);
+            });
+        });
+        static_for<0, AHEAD>([&](auto uc) {
+            constexpr int u = decltype(uc)::value;
+            if (first + FEW_WAVES * u < p.ksteps)            // uniform
+                static_for<0, MT * NC>([&](auto mc) {
+                    constexpr int i = decltype(mc)::value / NC, c = decltype(mc)::value % NC;
+                    acc[i][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u][c], b[u][i], acc[i][c], 0, 0, 0);
+                });
+        });
+        if (first + FEW_WAVES * AHEAD < p.ksteps) fetch(first + FEW_WAVES * AHEAD);
+    }
+    static_for<0, MT * NC>([&](auto mc) {
+        constexpr int i = decltype(mc)::value / NC, c = decltype(mc)::value % NC;
+        static_for<0, 4>([&](auto rc) { sums[((wave * MT * NC + i * NC + c) * 4 + decltype(rc)::value) * 64 + lane] = acc[i][c][decltype(rc)::value]; });
+    });
+    __syncthreads();
+    for (int at = threadIdx.x; at < 256 * MT * NC; at += FEW_THREADS) {
+        const int in = at % (16 * NC), col = col16 * 16 + in, token = at / (16 * NC);
+        if (col >= p.n || row0 + token >= p.m) continue;
+        int sum = 0;
+#pragma unroll
+        for (int i = 0; i < FEW_WAVES; ++i) sum += sums[((i * MT * NC + token / 16 * NC + in / 16) * 4 + in % 4) * 64 + token % 16 + 16 * (in % 16 / 4)];
+        float v[1] = {__fmul_rn(__fmul_rn(float(sum), p.w_scales[col]), scales[token])};
+        if (p.bias) v[0] = __fadd_rn(v[0], p.bias[col]);
+        activate_tokens(v, p.act, p.slope);
+        Run<OUT, 1> out;
+        out.set(v);
+        out.store(static_cast<char *>(p.out) + ((row0 + token) * p.out_stride + col) * (OUT == TSX_TYPE_F32 ? 4 : 2));
+    }
+}
+
 // more than 64 KiB of dynamic LDS, granted once per kernel and device
 int grant_lds(const void *kernel, int bytes) {
     struct Granted { std::atomic<const void *> kernel; std::atomic<uint64_t> devices; };
@@ -261,9 +398,58 @@ int launch_tile(TokenGemmParams p, hipStream_t stream) {
     return 0;
 }
 
+int few_most() { const char *e = std::getenv("TSX_TOKENS_FEW"); return e ? std::atoi(e) : 32; }
+int fused_most() { const char *e = std::getenv("TSX_TOKENS_FUSED"); return e ? std::atoi(e) : 40; }
+// rows of LDS that the tokens of a call take where the product quantizes them
+constexpr int FEW_LDS = 152 * 1024;
+int64_t few_lds(int m, int k) { return int64_t(m) * (round_up(k, KSTEP) + 16); }
+
+template <int X, int MT, int NC, int AHEAD, int OUT>
+int launch_few_tokens(const FewTokens &p, hipStream_t stream) {
+    const int lds = FEW_WAVES * MT * NC * 1024 + (X == TSX_TYPE_I8 ? 0 : int(few_lds(p.m, p.cols)));
+    const auto kernel = gemm_i8_few_tokens_kernel<X, MT, NC, AHEAD, OUT>;
+    if (lds > 64 * 1024) {
+        const int rc = grant_lds(reinterpret_cast<const void *>(kernel), FEW_LDS);
+        if (rc) return rc;
+    }
+    const dim3 grid(unsigned(ceil_div(p.n, 16 * NC)), X == TSX_TYPE_I8 ? unsigned(ceil_div(p.m, 16 * MT)) : 1);
+    hipLaunchKernelGGL(kernel, grid, dim3(FEW_THREADS), lds, stream, p);
+    TSX_LAUNCH_CHECK("gemm_i8_few_tokens_kernel");
+    return 0;
+}
+
+template <int X, int OUT>
+int few_tokens_of(const FewTokens &p, hipStream_t stream) {
+    const bool deep = p.ksteps > 4 * FEW_WAVES;
+    if (p.m <= 16) return deep ? launch_few_tokens<X, 1, 1, 8, OUT>(p, stream) : launch_few_tokens<X, 1, 1, 4, OUT>(p, stream);
+    return deep ? launch_few_tokens<X, 2, 1, 8, OUT>(p, stream) : launch_few_tokens<X, 2, 1, 4, OUT>(p, stream);
+}
+
 template <int OUT>
-int launch(const TokenGemmParams &p, hipStream_t stream) {
+int few_tokens(const tsx_token_gemm *g, const TokenGemmParams &q, bool quantizes, int shape, hipStream_t stream) {
+    FewTokens p{};
+    static_cast<TokenGemmParams &>(p) = q;
+    p.x = g->x_dev;
+    p.x_stride = g->x_stride;
+    p.cols = g->k;
+    p.lg_threads = g->m <= 1 ? 9 : g->m <= 2 ? 8 : g->m <= 4 ? 7 : 6;
+    if (quantizes)
+        return g->x_type == TSX_TYPE_F32 ? few_tokens_of<TSX_TYPE_F32, OUT>(p, stream)
+               : g->x_type == TSX_TYPE_F16 ? few_tokens_of<TSX_TYPE_F16, OUT>(p, stream) : few_tokens_of<TSX_TYPE_BF16, OUT>(p, stream);
+    switch (shape) {
+        case 0: return few_tokens_of<TSX_TYPE_I8, OUT>(p, stream);
+        case 1: return launch_few_tokens<TSX_TYPE_I8, 2, 2, 4, OUT>(p, stream);
+        case 2: return launch_few_tokens<TSX_TYPE_I8, 4, 2, 4, OUT>(p, stream);
+        default: return launch_few_tokens<TSX_TYPE_I8, 4, 1, 4, OUT>(p, stream);
+    }
+}
+
+template <int OUT>
+int launch(const tsx_token_gemm *g, const TokenGemmParams &p, bool quantizes, hipStream_t stream) {
     const char *e = std::getenv("TSX_TOKENS_TILE");
+    if (quantizes) return few_tokens<OUT>(g, p, true, 0, stream);
+    if (e && e[0] >= 'A') return few_tokens<OUT>(g, p, false, e[0] - 'A', stream);
+    if (!e && g->m <= few_most()) return few_tokens<OUT>(g, p, false, 0, stream);
     switch (e ? e[0] - '0' : 1) {
         case 0: return launch_tile<2, 2, 1, 1, 2, 4, OUT>(p, stream);
         case 1: return launch_tile<2, 2, 2, 2, 2, 4, OUT>(p, stream);
@@ -305,6 +491,12 @@ int check(const tsx_token_gemm *g) {
 
 int padded(int k) { return int(round_up(k, 16)); }
 
+
+// Whether the product's workgroups quantize the rows themselves, each all of them
+bool quantizes_itself(const tsx_token_gemm *g) {
+    return g->x_type != TSX_TYPE_I8 && g->m <= 32 && int64_t(g->m) * g->k <= int64_t(fused_most()) * 1024 && few_lds(g->m, g->k) + FEW_WAVES * 2048 <= FEW_LDS;
+}
+
 bool reads_in_place(const tsx_token_gemm *g) {
     return g->x_type == TSX_TYPE_I8 && g->k % 16 == 0 && (g->m <= 1 || g->x_stride % 16 == 0) && reinterpret_cast<uintptr_t>(g->x_dev) % 16 == 0;
 }
@@ -312,7 +504,7 @@ bool reads_in_place(const tsx_token_gemm *g) {
 size_t scales_offset(const tsx_token_gemm *g) { return size_t(g->m) * padded(g->k); }
 
 size_t workspace_bytes(const tsx_token_gemm *g) {
-    if (g->m == 0 || reads_in_place(g)) return 0;
+    if (g->m == 0 || reads_in_place(g) || quantizes_itself(g)) return 0;
     return scales_offset(g) + (g->x_type == TSX_TYPE_I8 ? 0 : size_t(g->m) * 4);
 }
 
@@ -346,7 +538,10 @@ int tsx_gemm_i8_tokens(const tsx_token_gemm *g, void *workspace_dev, size_t work
     p.q = static_cast<const int8_t *>(need ? workspace_dev : g->x_dev);
     p.pitch = need ? kp : g->x_stride;
     p.x_scales = g->x_scales_dev;
-    if (g->x_type != TSX_TYPE_I8) {
+    const bool quantizes = tsx::quantizes_itself(g);
+    if (quantizes) {
+        // nothing ahead of the product
+    } else if (g->x_type != TSX_TYPE_I8) {
         float *const scales = reinterpret_cast<float *>(static_cast<char *>(workspace_dev) + tsx::scales_offset(g));
         rc = tsx::quantize_rows(g->m, g->k, kp, g->x_dev, g->x_type, g->x_stride, static_cast<int8_t *>(workspace_dev), kp, scales, stream);
         if (rc) return rc;
@@ -369,8 +564,8 @@ int tsx_gemm_i8_tokens(const tsx_token_gemm *g, void *workspace_dev, size_t work
     p.ksteps = int(tsx::ceil_div(kp, tsx::KSTEP));
     p.act = g->act;
     p.slope = g->slope;
-    return g->out_type == TSX_TYPE_F32 ? tsx::launch<TSX_TYPE_F32>(p, stream) : g->out_type == TSX_TYPE_F16 ? tsx::launch<TSX_TYPE_F16>(p, stream)
-                                                                                                          : tsx::launch<TSX_TYPE_BF16>(p, stream);
+    return g->out_type == TSX_TYPE_F32 ? tsx::launch<TSX_TYPE_F32>(g, p, quantizes, stream) : g->out_type == TSX_TYPE_F16 ? tsx::launch<TSX_TYPE_F16>(g, p, quantizes, stream)
+                                                                                                          : tsx::launch<TSX_TYPE_BF16>(g, p, quantizes, stream);
 }
 
 }  // extern "C"
