@@ -6,6 +6,7 @@
 // exact, so every kernel here gives the same bits.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdlib>
 
 #include "igemm_i8.hpp"
@@ -398,8 +399,6 @@ int launch_tile(TokenGemmParams p, hipStream_t stream) {
     return 0;
 }
 
-int few_most() { const char *e = std::getenv("TSX_TOKENS_FEW"); return e ? std::atoi(e) : 32; }
-int fused_most() { const char *e = std::getenv("TSX_TOKENS_FUSED"); return e ? std::atoi(e) : 40; }
 // rows of LDS that the tokens of a call take where the product quantizes them
 constexpr int FEW_LDS = 152 * 1024;
 int64_t few_lds(int m, int k) { return int64_t(m) * (round_up(k, KSTEP) + 16); }
@@ -426,7 +425,7 @@ int few_tokens_of(const FewTokens &p, hipStream_t stream) {
 }
 
 template <int OUT>
-int few_tokens(const tsx_token_gemm *g, const TokenGemmParams &q, bool quantizes, int shape, hipStream_t stream) {
+int few_tokens(const tsx_token_gemm *g, const TokenGemmParams &q, bool quantizes, bool wide, hipStream_t stream) {
     FewTokens p{};
     static_cast<TokenGemmParams &>(p) = q;
     p.x = g->x_dev;
@@ -436,28 +435,41 @@ int few_tokens(const tsx_token_gemm *g, const TokenGemmParams &q, bool quantizes
     if (quantizes)
         return g->x_type == TSX_TYPE_F32 ? few_tokens_of<TSX_TYPE_F32, OUT>(p, stream)
                : g->x_type == TSX_TYPE_F16 ? few_tokens_of<TSX_TYPE_F16, OUT>(p, stream) : few_tokens_of<TSX_TYPE_BF16, OUT>(p, stream);
-    switch (shape) {
-        case 0: return few_tokens_of<TSX_TYPE_I8, OUT>(p, stream);
-        case 1: return launch_few_tokens<TSX_TYPE_I8, 2, 2, 4, OUT>(p, stream);
-        case 2: return launch_few_tokens<TSX_TYPE_I8, 4, 2, 4, OUT>(p, stream);
-        default: return launch_few_tokens<TSX_TYPE_I8, 4, 1, 4, OUT>(p, stream);
-    }
+    return wide ? launch_few_tokens<TSX_TYPE_I8, 2, 2, 4, OUT>(p, stream) : few_tokens_of<TSX_TYPE_I8, OUT>(p, stream);
+}
+
+// The kernel a call takes, by an estimate of its time in us, fitted to products of 16 .. 32768 rows on K of 128 .. 8192 (bf16 output):
+// what a launch takes whatever its size, and for each 256 workgroups, one a CU, a fixed part and one for each 1024 of K.  Measured, few
+// tokens 16 x 32 and 32 x 32, tiles of 64, 128 and 256 (us): 32 x 1000, K = 2048: 4.4, 5.9, 7.3, 11.2, 22.6; 64 x 4096, K = 4096: 12.6, 9.9,
+// 12.1, 19.6, 40; 197 x 777, K = 1500: 5.0, 5.3, 6.8, 11, 25; 512 x 3840, K = 1280: 33, 26, 8.2, 9.4, 18.5; 2048^3: -, -, 19.7, 14.0,
+// 25.7; 4096^3: -, -, 110, 79, 65.
+enum class TokenKernel { few_16, few_32, tile_64, tile_128, tile_256 };
+
+TokenKernel choose(int m, int n, int k) {
+    if (m <= 16) return TokenKernel::few_16;
+    const float ks = float(k) / 1024.f;
+    const auto rounds = [&](int rows, int cols) { return float(ceil_div(m, rows) * ceil_div(n, cols)) / 256.f; };
+    const float few = rounds(32, 16), few_wide = rounds(32, 32), r64 = rounds(64, 64), r128 = rounds(128, 128), r256 = rounds(256, 256);
+    const float cost[] = {few <= 1.f ? 3.6f + ks * (k <= 2048 ? 0.5f : 1.25f * std::max(few, 0.5f)) : 3.6f + few * (0.25f + 1.1f * ks),
+                          4.2f + std::max(few_wide, 1.f) * (0.2f + 1.35f * ks), 3.f + std::max(r64, 1.f) * (0.5f + 1.8f * ks),
+                          3.f + std::ceil(r128) * (1.5f + 4.5f * ks), 3.f + std::ceil(r256) * (8.4f + 13.4f * ks * (0.75f + 0.25f * std::min(r256, 1.f)))};
+    int best = 0;
+    for (int i = 1; i < 5; ++i)
+        if (cost[i] < cost[best]) best = i;
+    return TokenKernel(best);
 }
 
 template <int OUT>
 int launch(const tsx_token_gemm *g, const TokenGemmParams &p, bool quantizes, hipStream_t stream) {
-    const char *e = std::getenv("TSX_TOKENS_TILE");
-    if (quantizes) return few_tokens<OUT>(g, p, true, 0, stream);
-    if (e && e[0] >= 'A') return few_tokens<OUT>(g, p, false, e[0] - 'A', stream);
-    if (!e && g->m <= few_most()) return few_tokens<OUT>(g, p, false, 0, stream);
-    switch (e ? e[0] - '0' : 1) {
-        case 0: return launch_tile<2, 2, 1, 1, 2, 4, OUT>(p, stream);
-        case 1: return launch_tile<2, 2, 2, 2, 2, 4, OUT>(p, stream);
-        case 2: return launch_tile<2, 2, 4, 4, 1, 4, OUT>(p, stream);
-        case 3: return launch_tile<2, 4, 4, 2, 1, 4, OUT>(p, stream);
-        case 4: return launch_tile<2, 4, 2, 2, 1, 6, OUT>(p, stream);
-        case 5: return launch_tile<2, 2, 2, 2, 1, 5, OUT>(p, stream);
-        default: return launch_tile<2, 2, 1, 1, 2, 8, OUT>(p, stream);
+    if (quantizes) return few_tokens<OUT>(g, p, true, false, stream);
+    // TSX_TOKENS_KERNEL: that kernel, by its place in the list above, whatever the call (tests, measurements)
+    const char *e = std::getenv("TSX_TOKENS_KERNEL");
+    switch (e && e[0] >= '0' && e[0] <= '4' ? TokenKernel(e[0] - '0') : choose(p.m, p.n, p.k)) {
+        case TokenKernel::few_16: return few_tokens<OUT>(g, p, false, false, stream);
+        case TokenKernel::few_32: return few_tokens<OUT>(g, p, false, true, stream);
+        case TokenKernel::tile_64: return launch_tile<2, 2, 1, 1, 2, 3, OUT>(p, stream);
+        case TokenKernel::tile_128: return launch_tile<2, 2, 2, 2, 1, 3, OUT>(p, stream);
+        default: return launch_tile<2, 4, 4, 2, 1, 4, OUT>(p, stream);
     }
 }
 
@@ -492,9 +504,11 @@ int check(const tsx_token_gemm *g) {
 int padded(int k) { return int(round_up(k, 16)); }
 
 
-// Whether the product's workgroups quantize the rows themselves, each all of them
+// Whether the product's workgroups quantize the rows themselves, each all of them: the launch that this saves is 2 us, and up to some
+// 40 K values its work hides behind the weights (us with and without, 4096 columns, K = 4096: 1 row 6.0 and 7.9, 8 rows 7.4 and 8.9, 16
+// rows 9.9 and 9.7; 1000 columns, K = 2048, 16 rows: 5.5 and 7.2).
 bool quantizes_itself(const tsx_token_gemm *g) {
-    return g->x_type != TSX_TYPE_I8 && g->m <= 32 && int64_t(g->m) * g->k <= int64_t(fused_most()) * 1024 && few_lds(g->m, g->k) + FEW_WAVES * 2048 <= FEW_LDS;
+    return g->x_type != TSX_TYPE_I8 && g->m <= 32 && int64_t(g->m) * g->k <= 40960 && few_lds(g->m, g->k) + FEW_WAVES * 2048 <= FEW_LDS;
 }
 
 bool reads_in_place(const tsx_token_gemm *g) {

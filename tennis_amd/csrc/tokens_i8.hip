@@ -96,9 +96,16 @@ int launch(const TokenParams &p, hipStream_t stream) {
 
 template <int TYPE>
 int launch_type(const TokenParams &p, hipStream_t stream) {
+    // A wavefront a row while there are rows for all CUs, with no barrier; more threads a row where there are few rows or it is long.
     const int64_t pieces = ceil_div(p.cols_out, PIECE);
     if (pieces <= 64) return launch<TYPE, 64, 1, true>(p, stream);
-    if (pieces <= 256) return launch<TYPE, 64, 4, true>(p, stream);
+    if (p.rows >= 512 || pieces <= 128) {
+        if (pieces <= 128) return launch<TYPE, 64, 2, true>(p, stream);
+        if (pieces <= 256) return launch<TYPE, 64, 4, true>(p, stream);
+        if (pieces <= 512) return launch<TYPE, 64, 8, true>(p, stream);
+    }
+    if (pieces <= 256) return launch<TYPE, 256, 1, true>(p, stream);
+    if (pieces <= 512) return launch<TYPE, 256, 2, true>(p, stream);
     if (pieces <= 1024) return launch<TYPE, 256, 4, true>(p, stream);
     if (pieces <= 4096) return launch<TYPE, 1024, 4, true>(p, stream);
     return launch<TYPE, 1024, 4, false>(p, stream);
