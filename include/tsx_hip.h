@@ -253,7 +253,7 @@ int tsx_gemm_i8_tokens(const tsx_token_gemm *g, void *workspace_dev, size_t work
 /* Group norm with an activation on channels-last tensors x[n][pixels][c], in groups of c / groups consecutive channels:
  *   y = act((x - mean) / sqrt(variance + epsilon) * weight[c] + bias[c]),  mean and variance over a group's channels of all pixels of
  * an image (the variance divides by their count).  Images and pixels lie at any stride (pixels at one of at least c); c is at
- * most 8192, n below 65536, pixels below 2^31; n or pixels may be 0.
+ * most 8192, n below 65536, pixels below 2^30 at a stride of at most 2^26; n or pixels may be 0.
  *   nhwc         the result in x's type, dense [n][pixels][c] (may be x itself where that is dense)
  *   tokens_nhwc  the result (as fp32, before any rounding) as int8 tokens, a pixel a token: q dense [n][pixels][c],
  *                scales [n][pixels], with the rule of tsx_quantize_tokens

@@ -20,32 +20,29 @@ namespace {
 template <int TYPE, int V>
 __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_statistics_kernel(NormParams p) {
     extern __shared__ float entries[];                       // [lanes + 1][pitch] means, then squares
-    const int threads = blockDim.x, t = threadIdx.x;
-    const int lanes = p.lanes ? p.lanes : 1, row_values = p.S * p.c, pixel_entries = p.c >> p.lg_run;
+    constexpr int SIZE = Kind<TYPE>::SIZE;
+    const int threads = blockDim.x, t = threadIdx.x, chunk = blockIdx.x, image = blockIdx.y;
+    const int lanes = p.lanes ? p.lanes : 1, pixel_entries = p.c >> p.lg_run, run = 1 << p.lg_run;
     const int pitch = (p.S * pixel_entries) | 1;             // odd: the lanes of one place lie in different banks
     float *const means = entries, *const squares = means + (lanes + 1) * pitch;
-    const Place place(p, blockIdx.x);
-    const char *const x = static_cast<const char *>(p.x) + place.image * p.image_stride * Kind<TYPE>::SIZE;
-    const int64_t row_stride = p.S * p.pixel_stride;
-    const int64_t first = place.chunk * p.chunk_rows;
-    const int rows = int(max(min(p.chunk_rows, p.rows - first), int64_t(0)));
+    const int first = chunk * p.chunk_rows, rows = min(p.chunk_rows, p.rows - first);
+    const char *const x = static_cast<const char *>(p.x) + image * p.image_bytes;
     // the incomplete row, with the last chunk: entries of its own behind the lanes'
-    const int tail = place.chunk == p.chunks - 1 ? int(p.pixels - p.rows * p.S) * p.c : 0;
+    const int tail = chunk == p.chunks - 1 ? p.tail : 0;
+    const int full = lanes == 1 ? rows : udiv(rows, lanes, p.lanes_magic), over = rows - full * lanes;      // rows of a lane: one more for the first `over`
     auto leave = [&](int lane, int j, const float (&mean)[V], const float (&square)[V]) __attribute__((always_inline)) {
-        const int at = lane * pitch + (j * V >> p.lg_run);
-        int k = 0;
+        int at = lane * pitch + (j * V >> p.lg_run);
         static_for<0, V>([&](auto ec) {
             constexpr int e = decltype(ec)::value;
-            if ((e & (p.run - 1)) == 0) {
-                means[at + k] = mean[e];
-                squares[at + k] = square[e];
-                ++k;
+            if ((e & (run - 1)) == 0) {
+                means[at] = mean[e];
+                squares[at++] = square[e];
             }
         });
     };
     // runs of values of one count become one entry: the mean of their means, their squares and n / 2 of the squared difference
     auto join = [&](float (&mean)[V], float (&square)[V], float count) __attribute__((always_inline)) {
-        join_runs<V>(p.run, [&](auto ac, auto fc) {
+        join_runs<V>(run, [&](auto ac, auto fc) {
             constexpr int a = decltype(ac)::value, b = a + decltype(fc)::value;
             const float d = mean[b] - mean[a];
             square[a] = square[a] + square[b] + (0.5f * decltype(fc)::value * count) * (d * d);
@@ -55,50 +52,51 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_statistics_kerne
     for (int j0 = 0; j0 < p.pieces; j0 += threads) {         // one turn where the threads cover a row
         const int lane = p.lanes ? udiv(t, p.pieces, p.pieces_magic) : 0, j = p.lanes ? t - lane * p.pieces : j0 + t;
         if (lane < lanes && j < p.pieces) {
+            const char *at = x + int64_t(first + lane) * p.row_bytes + j * (V * SIZE);
+            const int count = full + (lane < over ? 1 : 0);
+            // Requests of a batch leave together; the last one reads its last row again in the place of those that are none.
+            constexpr int AHEAD = 8;
+            typedef Run<TYPE, V> Values;
+            Values v[AHEAD];
+            auto fetch = [&](int left) __attribute__((always_inline)) {
+                static_for<0, AHEAD>([&](auto uc) { v[decltype(uc)::value].load(at + min(decltype(uc)::value, left - 1) * p.step_bytes); });
+            };
             float base[V], sum[V], square[V];
             static_for<0, V>([&](auto ec) { base[decltype(ec)::value] = sum[decltype(ec)::value] = square[decltype(ec)::value] = 0.f; });
-            const char *const from = x + (first * row_stride + j * V) * Kind<TYPE>::SIZE;
-            // requests of a batch leave together; the last one reads its last row again in the place of those that are none
-            constexpr int AHEAD = 8;
-            const int64_t step = lanes * row_stride * Kind<TYPE>::SIZE;
-            const char *at = from + lane * row_stride * Kind<TYPE>::SIZE;
-            int left = lane < rows ? (rows - lane - 1) / lanes + 1 : 0;
-            bool fresh = true;
-            auto batch = [&](auto whole) __attribute__((always_inline)) {
-                Piece<TYPE, V> a[AHEAD];
-                static_for<0, AHEAD>([&](auto uc) {
-                    constexpr int u = decltype(uc)::value;
-                    a[u].load(at + (whole ? u : min(u, left - 1)) * step, 0);
-                });
-                if (fresh) static_for<0, V>([&](auto ec) { base[decltype(ec)::value] = a[0].v[decltype(ec)::value]; });
-                fresh = false;
-                static_for<0, AHEAD>([&](auto uc) {
-                    constexpr int u = decltype(uc)::value;
-                    if (whole || u < left)
-                        static_for<0, V>([&](auto ec) {
-                            constexpr int e = decltype(ec)::value;
-                            const float d = a[u].v[e] - base[e];
-                            sum[e] += d;
-                            square[e] = __builtin_fmaf(d, d, square[e]);
-                        });
+            auto take = [&](auto uc) __attribute__((always_inline)) {
+                static_for<0, V>([&](auto ec) {
+                    constexpr int e = decltype(ec)::value;
+                    const float d = v[decltype(uc)::value].template get<e>() - base[e];
+                    sum[e] += d;
+                    square[e] = __builtin_fmaf(d, d, square[e]);
                 });
             };
-            for (; left >= AHEAD; left -= AHEAD, at += AHEAD * step) batch(std::true_type{});
-            if (left > 0) batch(std::false_type{});
-            const float count = float(lane < rows ? (rows - lane - 1) / lanes + 1 : 0), of_count = count > 0.f ? 1.f / count : 0.f;
+            int left = count;
+            if (left > 0) {
+                fetch(left);
+                static_for<0, V>([&](auto ec) { base[decltype(ec)::value] = v[0].template get<decltype(ec)::value>(); });
+            }
+            while (left > AHEAD) {
+                static_for<0, AHEAD>(take);
+                at += AHEAD * p.step_bytes;
+                left -= AHEAD;
+                fetch(left);
+            }
+            static_for<0, AHEAD>([&](auto uc) { if (decltype(uc)::value < left) take(uc); });
+            const float of_count = __builtin_amdgcn_rcpf(float(max(count, 1)));      // within a step: moves the mean by that much of the sum
             static_for<0, V>([&](auto ec) {
                 constexpr int e = decltype(ec)::value;
                 const float m = sum[e] * of_count;
-                square[e] = fmaxf(__builtin_fmaf(-m, sum[e], square[e]), 0.f);
+                // squares around base + m, whatever m is
+                square[e] = fmaxf(__builtin_fmaf(m, __builtin_fmaf(m, float(count), -2.f * sum[e]), square[e]), 0.f);
                 base[e] += m;
             });
-            join(base, square, count);
+            join(base, square, float(count));
             leave(lane, j, base, square);
             if (lane == 0 && tail) {
-                const int left = tail - j * V;
                 Piece<TYPE, V> a;
                 static_for<0, V>([&](auto ec) { a.v[decltype(ec)::value] = square[decltype(ec)::value] = 0.f; });
-                if (left > 0) a.load_some(x, p.rows * row_values + j * V, left);
+                if (tail > j * V) a.load_some(x, int64_t(p.rows) * (p.S * p.c) + j * V, tail - j * V);
                 join(a.v, square, 1.f);
                 leave(lanes, j, a.v, square);
             }
@@ -109,33 +107,32 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_statistics_kerne
     // T threads a group, TL of them on lanes of their own, which share the lane's entries of the group
     const int group_entries = p.d >> p.lg_run, sides = lanes + (tail ? 1 : 0);
     const int T = 1 << p.lg_T, TL = 1 << p.lg_TL, TE = T >> p.lg_TL;
-    const int tl = t & (TL - 1), te = (t & (T - 1)) >> p.lg_TL, tail_pixels = int(p.pixels - p.rows * p.S);
+    const int tl = t & (TL - 1), te = (t & (T - 1)) >> p.lg_TL, tail_pixels = p.pixels - p.rows * p.S;
     auto each = [&](int g, auto &&body) __attribute__((always_inline)) {
         for (int lane = tl; lane < sides; lane += TL) {
-            const float n = float(p.run * (lane == lanes ? 1 : lane < rows ? (rows - lane - 1) / lanes + 1 : 0));
+            const float n = float(run * (lane == lanes ? 1 : full + (lane < over ? 1 : 0)));
             const int pixels = n == 0.f ? 0 : lane == lanes ? tail_pixels : p.S;
             for (int pixel = 0; pixel < pixels; ++pixel)
                 for (int k = te; k < group_entries; k += TE) body(lane * pitch + pixel * pixel_entries + g * group_entries + k, n);
         }
     };
-    for (int g0 = 0; g0 < p.groups; g0 += threads >> p.lg_T) {
-        const int g = g0 + (t >> p.lg_T);
-        if (g >= p.groups) continue;                         // T threads agree
-        float n = 0.f, s = 0.f, m2 = 0.f;
+    const float of_values = __builtin_amdgcn_rcpf(chunk == p.chunks - 1 ? p.of_last : p.of_chunk);
+    for (int g = t >> p.lg_T; g < p.groups; g += threads >> p.lg_T) {      // T threads agree
+        float s = 0.f, n2 = 0.f, m2 = 0.f;
         const float about = means[(rows ? 0 : lanes * pitch) + g * group_entries];
-        each(g, [&](int at, float ni) __attribute__((always_inline)) {
-            n += ni;
-            s = __builtin_fmaf(ni, means[at] - about, s);
-        });
-        n = sum_over_lanes(n, p.lg_T);
+        each(g, [&](int at, float ni) __attribute__((always_inline)) { s = __builtin_fmaf(ni, means[at] - about, s); });
         s = sum_over_lanes(s, p.lg_T);
-        const float mean = about + (n > 0.f ? s / n : 0.f);
+        const float mean = about + s * of_values;
+        // around that mean, and what the values are off it on the whole (its rounding)
         each(g, [&](int at, float ni) __attribute__((always_inline)) {
             const float d = means[at] - mean;
+            n2 = __builtin_fmaf(ni, d, n2);
             m2 += __builtin_fmaf(ni * d, d, squares[at]);
         });
+        n2 = sum_over_lanes(n2, p.lg_T);
         m2 = sum_over_lanes(m2, p.lg_T);
-        if ((t & (T - 1)) == 0) p.partial[(place.image * p.groups + g) * p.chunks + place.chunk] = float2{mean, m2};
+        const float shift = n2 * of_values;
+        if ((t & (T - 1)) == 0) p.partial[int64_t(image * p.groups + g) * p.chunks + chunk] = float2{mean + shift, __builtin_fmaf(-shift, n2, m2)};
     }
 }
 
@@ -144,39 +141,35 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_statistics_kerne
 template <int TYPE, int V, int ACT>
 __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_apply_kernel(NormParams p) {
     extern __shared__ float2 group[];
-    const int threads = blockDim.x, t = threadIdx.x;
-    const int lanes = p.lanes ? p.lanes : 1, row_values = p.S * p.c;
-    const int part = udiv(blockIdx.x, p.places, p.places_magic), at = blockIdx.x - part * p.places;
-    // The last chunks first, since the statistics ended with them: what they read is still in the caches.  Each on the XCD that
-    // read it.
-    const Place place(p, p.places % 8 == 0 ? p.places - 8 - at / 8 * 8 + at % 8 : at);
-    const char *const x = static_cast<const char *>(p.x) + place.image * p.image_stride * Kind<TYPE>::SIZE;
-    char *const out = static_cast<char *>(p.out) + place.image * p.pixels * p.c * Kind<TYPE>::SIZE;
-    const int64_t row_stride = p.S * p.pixel_stride;
-    const int64_t chunk_end = min((place.chunk + 1) * p.chunk_rows, p.rows);
-    const int64_t first = place.chunk * p.chunk_rows + part * p.part_rows;
-    const int rows = int(max(min(p.part_rows, chunk_end - first), int64_t(0)));
-    const int tail = place.chunk == p.chunks - 1 && part == 0 ? int(p.pixels - p.rows * p.S) * p.c : 0;
-    constexpr int AHEAD = 4;
+    constexpr int SIZE = Kind<TYPE>::SIZE, AHEAD = 4;
     typedef Run<TYPE, V> Values;
-    // Requests of a batch leave together, the first ahead of the statistics; in the place of rows that are none the last one again.
-    const int64_t in_step = lanes * row_stride * Kind<TYPE>::SIZE, out_step = int64_t(lanes) * row_values * Kind<TYPE>::SIZE;
-    auto fetch = [&](Values (&v)[AHEAD], const char *at, int left) __attribute__((always_inline)) {
-        if (left > 0)
-            static_for<0, AHEAD>([&](auto uc) { v[decltype(uc)::value].load(at + min(decltype(uc)::value, left - 1) * in_step); });
-    };
+    const int threads = blockDim.x, t = threadIdx.x, lanes = p.lanes ? p.lanes : 1;
+    // The last chunks first, since the statistics ended with them: what they read is still in the caches.  Each on the XCD that
+    // read it: workgroups go to the XCDs in turn.
+    const bool turned = p.chunks % 8 == 0;
+    const int chunk = turned ? p.chunks - 8 - (blockIdx.x & ~7u) + (blockIdx.x & 7) : blockIdx.x, image = turned ? p.images - 1 - blockIdx.y : blockIdx.y;
+    const int in_chunk = blockIdx.z * p.part_rows, first = chunk * p.chunk_rows + in_chunk;
+    const int rows = min(min(p.part_rows, p.chunk_rows - in_chunk), p.rows - first);      // may be none
+    const int tail = chunk == p.chunks - 1 && blockIdx.z == 0 ? p.tail : 0;
+    const char *const x = static_cast<const char *>(p.x) + image * p.image_bytes;
+    char *const out = static_cast<char *>(p.out) + image * p.out_image_bytes;
     for (int j0 = 0; j0 < p.pieces; j0 += threads) {
         const int lane = p.lanes ? udiv(t, p.pieces, p.pieces_magic) : 0, j = p.lanes ? t - lane * p.pieces : j0 + t;
         const bool mine = lane < lanes && j < p.pieces;
-        const int ch = !mine ? 0 : p.S > 1 ? j * V % p.c : j * V;
-        const char *from = x + ((first + lane) * row_stride + j * V) * Kind<TYPE>::SIZE;
-        char *to = out + ((first + lane) * row_values + j * V) * Kind<TYPE>::SIZE;
-        int left = mine && lane < rows ? (rows - lane - 1) / lanes + 1 : 0;
+        const char *from = x + int64_t(first + lane) * p.row_bytes + j * (V * SIZE);
+        char *to = out + int64_t(first + lane) * p.out_row_bytes + j * (V * SIZE);
+        const int out_step = lanes * p.out_row_bytes, out_steps = AHEAD * out_step;
+        // Requests of a batch leave together, the first ahead of the statistics; in the place of rows that are none the last one again.
+        const int most = lanes == 1 ? rows - lane : udiv(max(rows - lane, 0) + lanes - 1, lanes, p.lanes_magic);
+        int left = mine ? most : 0;
         Values v[AHEAD];
-        fetch(v, from, left);
+        auto fetch = [&] { static_for<0, AHEAD>([&](auto uc) { v[decltype(uc)::value].load(from + min(decltype(uc)::value, left - 1) * p.step_bytes); }); };
+        if (left > 0) fetch();
+        int ch = mine ? j * V : 0;
+        if (p.S > 1) ch -= udiv(ch, p.c, p.c_magic) * p.c;
         Affine<V> affine(ch, p.c, p.weight, p.bias);
         if (j0 == 0) {
-            merge_chunks(p, place.image, group);
+            merge_chunks(p, image, group);
             __syncthreads();
         }
         affine.take(group, ch, p.c, p.d, p.d_magic);
@@ -189,17 +182,18 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_apply_kernel(Nor
         };
         while (left > AHEAD) {
             static_for<0, AHEAD>(apply);
-            from += AHEAD * in_step;
-            to += AHEAD * out_step;
+            from += AHEAD * p.step_bytes;
+            to += out_steps;
             left -= AHEAD;
-            fetch(v, from, left);
+            fetch();
         }
         static_for<0, AHEAD>([&](auto uc) { if (decltype(uc)::value < left) apply(uc); });
         if (mine && lane == 0 && j * V < tail) {
             Piece<TYPE, V> a;
-            a.load_some(x, p.rows * row_values + j * V, tail - j * V);
+            const int64_t at = int64_t(p.rows) * (p.S * p.c) + j * V;
+            a.load_some(x, at, tail - j * V);
             affine.template apply<ACT>(p.act, p.slope, a);
-            a.store(out, p.rows * row_values + j * V, tail - j * V);
+            a.store(out, at, tail - j * V);
         }
         if (p.lanes) break;
     }
@@ -208,6 +202,12 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_apply_kernel(Nor
 // ---- host side
 
 constexpr int MOST_CHUNKS = 256;
+#ifndef NORM_THREADS
+#define NORM_THREADS 512
+#endif
+#ifndef NORM_WORKGROUPS
+#define NORM_WORKGROUPS 512
+#endif
 
 // Rows, threads and chunks of a call; V: values of a piece (1: a channel a thread, for pixels apart that are no whole pieces).
 struct NormPlan {
@@ -218,42 +218,50 @@ struct NormPlan {
 NormPlan plan_of(const tsx_group_norm *g) {
     NormPlan pl{};
     NormParams &p = pl.p;
-    const int whole = g->type == TSX_TYPE_F32 ? 4 : 8;
+    const int whole = g->type == TSX_TYPE_F32 ? 4 : 8, size = int(element_bytes(g->type));
     const bool dense = g->pixel_stride == g->c || g->pixels <= 1;
-    const int S = whole / gcd(g->c, whole);
+    const int S = whole / gcd(g->c, whole), n = std::max(g->n, 1), d = g->c / g->groups;
+    const int64_t pixel_stride = g->pixels <= 1 ? g->c : g->pixel_stride;
     pl.V = S == 1 || (dense && S * g->c <= NORM_MOST_CHANNELS) ? whole : 1;
     p.S = pl.V == 1 ? 1 : S;
     p.x = g->x_dev;
     p.weight = g->weight_dev;
     p.bias = g->bias_dev;
-    p.pixels = g->pixels;
-    p.image_stride = g->image_stride;
-    p.pixel_stride = g->pixels <= 1 ? g->c : g->pixel_stride;
     p.c = g->c;
     p.groups = g->groups;
-    p.d = g->c / g->groups;
+    p.d = d;
+    p.pixels = int(g->pixels);
     p.epsilon = g->epsilon;
     p.slope = g->slope;
     p.act = g->act;
-    p.rows = g->pixels / p.S;
+    p.images = n;
+    p.rows = p.pixels / p.S;
+    p.tail = (p.pixels - p.rows * p.S) * p.c;
     p.pieces = p.S * p.c / pl.V;
-    p.run = gcd(p.d, pl.V);
-    pl.threads = NORM_MOST_THREADS;
+    p.image_bytes = g->image_stride * size;
+    p.out_image_bytes = g->pixels * g->c * size;
+    p.row_bytes = int(p.S * pixel_stride * size);
+    p.out_row_bytes = p.S * p.c * size;
+    p.pixel_bytes = int(pixel_stride * size);
+    pl.threads = p.pieces <= NORM_THREADS ? NORM_THREADS : NORM_MOST_THREADS;
     p.lanes = p.pieces <= pl.threads ? pl.threads / p.pieces : 0;
-    const int side = p.lanes ? p.lanes : 1, n = std::max(g->n, 1);
-    const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>({ceil_div(256, n), int64_t(MOST_CHUNKS), p.rows / (4 * side)}));
-    p.chunk_rows = std::max<int64_t>(1, ceil_div(p.rows, chunks));
+    const int side = p.lanes ? p.lanes : 1;
+    p.step_bytes = int64_t(side) * p.row_bytes;
+    const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>({ceil_div(NORM_WORKGROUPS, n), int64_t(MOST_CHUNKS), p.rows / (4 * side)}));
+    p.chunk_rows = int(std::max<int64_t>(1, ceil_div(p.rows, chunks)));
     p.chunks = int(std::max<int64_t>(1, ceil_div(p.rows, p.chunk_rows)));
-    p.places = n * p.chunks;
-    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(ceil_div(256, p.places), p.chunk_rows / (4 * side)));
-    p.part_rows = std::max<int64_t>(1, ceil_div(p.chunk_rows, parts));
+    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(ceil_div(NORM_WORKGROUPS, int64_t(n) * p.chunks), p.chunk_rows / (4 * side)));
+    p.part_rows = int(std::max<int64_t>(1, ceil_div(p.chunk_rows, parts)));
     p.parts = int(std::max<int64_t>(1, ceil_div(p.chunk_rows, p.part_rows)));
-    p.lg_run = lg_of(p.run);
+    p.of_chunk = float(int64_t(p.chunk_rows) * p.S * d);
+    p.of_last = float((g->pixels - int64_t(p.chunks - 1) * p.chunk_rows * p.S) * d);
+    p.of_image = float(1.0 / (double(g->pixels) * d));
+    p.lg_run = lg_of(gcd(d, pl.V));
     p.pieces_magic = div_magic(p.pieces, NORM_MOST_THREADS);
-    p.chunks_magic = div_magic(p.chunks, p.places);
-    p.places_magic = div_magic(p.places, int64_t(p.places) * p.parts);
-    p.d_magic = div_magic(p.d, NORM_MOST_CHANNELS);
-    p.lg_T = lg_threads(pl.threads, p.groups, (side + 1) * p.S * (p.d / p.run));
+    p.lanes_magic = div_magic(side, int64_t(p.chunk_rows) + side);
+    p.c_magic = div_magic(p.c, NORM_MOST_CHANNELS);
+    p.d_magic = div_magic(d, NORM_MOST_CHANNELS);
+    p.lg_T = lg_threads(pl.threads, p.groups, (side + 1) * p.S * (d >> p.lg_run));
     p.lg_TL = lg_threads(1 << p.lg_T, 1, side);
     p.lg_merge = lg_threads(pl.threads, p.groups, p.chunks);
     return pl;
@@ -265,8 +273,9 @@ int check(const tsx_group_norm *g, const char *what) {
     TSX_REQUIRE(g->c % g->groups == 0, "%s: %d channels are no %d groups", what, g->c, g->groups);
     TSX_REQUIRE(g->c <= NORM_MOST_CHANNELS, "%s: %d channels (at most %d)", what, g->c, NORM_MOST_CHANNELS);
     TSX_REQUIRE(is_float_type(g->type), "%s: element type %d (fp32, fp16 or bf16)", what, g->type);
-    TSX_REQUIRE(g->n < 65536 && g->pixels < int64_t(1) << 31, "%s: %d images of %lld pixels", what, g->n, (long long)g->pixels);
+    TSX_REQUIRE(g->n < 65536 && g->pixels < int64_t(1) << 30, "%s: %d images of %lld pixels", what, g->n, (long long)g->pixels);
     TSX_REQUIRE(g->pixels <= 1 || g->pixel_stride >= g->c, "%s: pixels of %d channels overlap at a stride of %lld", what, g->c, (long long)g->pixel_stride);
+    TSX_REQUIRE(g->pixels <= 1 || g->pixel_stride <= 1 << 26, "%s: pixels at a stride of %lld (at most 2^26)", what, (long long)g->pixel_stride);
     TSX_REQUIRE(g->n <= 1 || g->image_stride >= 0, "%s: negative image stride", what);
     TSX_REQUIRE(is_token_act(g->act), "%s: activation %d", what, g->act);
     TSX_REQUIRE(g->epsilon >= 0.f, "%s: epsilon is negative or NaN", what);
@@ -282,10 +291,10 @@ size_t workspace_bytes(const tsx_group_norm *g) {
 template <int TYPE, int V>
 int launch_statistics(const NormPlan &pl, hipStream_t stream) {
     const NormParams &p = pl.p;
-    const size_t lds = size_t((p.lanes ? p.lanes : 1) + 1) * ((p.S * (p.c / p.run)) | 1) * 2 * sizeof(float);
+    const size_t lds = size_t((p.lanes ? p.lanes : 1) + 1) * ((p.S * (p.c >> p.lg_run)) | 1) * 2 * sizeof(float);
     if (lds > 64 * 1024)
         TSX_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(group_norm_statistics_kernel<TYPE, V>), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
-    hipLaunchKernelGGL((group_norm_statistics_kernel<TYPE, V>), dim3(unsigned(p.places)), dim3(pl.threads), lds, stream, p);
+    hipLaunchKernelGGL((group_norm_statistics_kernel<TYPE, V>), dim3(unsigned(p.chunks), unsigned(p.images)), dim3(pl.threads), lds, stream, p);
     TSX_LAUNCH_CHECK("group_norm_statistics_kernel");
     return 0;
 }
@@ -294,7 +303,7 @@ template <int TYPE, int V>
 int launch_apply(const NormPlan &pl, hipStream_t stream) {
     const NormParams &p = pl.p;
     with_act(p.act, [&](auto act) {
-        hipLaunchKernelGGL((group_norm_apply_kernel<TYPE, V, decltype(act)::value>), dim3(unsigned(p.places) * unsigned(p.parts)), dim3(pl.threads),
+        hipLaunchKernelGGL((group_norm_apply_kernel<TYPE, V, decltype(act)::value>), dim3(unsigned(p.chunks), unsigned(p.images), unsigned(p.parts)), dim3(pl.threads),
                            size_t(p.groups) * sizeof(float2), stream, p);
     });
     TSX_LAUNCH_CHECK("group_norm_apply_kernel");

@@ -1,4 +1,4 @@
-// What the kernels of the group norm share (group_norm.hip, group_norm_tokens.hip): how an image's pixels are dealt out, and its
+// What the kernels of the group norm share (group_norm.hip, group_norm_held.hip, group_norm_tokens.hip): how an image's pixels are dealt out, and its
 // statistics from those of its chunks.
 #pragma once
 #include "elements.hpp"
@@ -8,6 +8,8 @@ namespace tsx {
 
 constexpr int NORM_MOST_CHANNELS = 8192, NORM_MOST_THREADS = 1024;
 
+// Everything a kernel would otherwise work out from the sizes: sixteen wavefronts share a CU's scalar unit, and a prologue of 600
+// instructions, most of them 64-bit products of strides, kept the last of them waiting for 8 us.
 struct NormParams {
     const void *x;
     void *out;
@@ -15,18 +17,19 @@ struct NormParams {
     float *scales;
     const float *weight, *bias;
     float2 *partial;                   // [n][groups][chunks]: mean, squares around it (a group's chunks are read together)
-    int64_t pixels, image_stride, pixel_stride;
-    int64_t rows;                      // whole rows of S pixels
-    int c, groups, d;
-    int S, pieces;                     // pixels of a row; pieces of a row
+    int64_t image_bytes, out_image_bytes, step_bytes;      // from image to image; from a thread's row to its next one
+    int c, groups, d, pixels;
+    int S, pieces, rows;               // pixels of a row; pieces of a row; whole rows of an image
+    int row_bytes, out_row_bytes, pixel_bytes;
     int lanes;                         // rows that a workgroup's threads take side by side (0: pieces in turns)
-    int run, lg_run;                   // neighbours of a piece that lie in one group, whichever piece: a power of two
-    int chunks;                        // of an image's rows: a workgroup's share of the statistics
-    int places, parts;                 // n * chunks; workgroups that share a chunk of the norm itself
-    int64_t chunk_rows, part_rows, part_pixels;
-    float epsilon, slope;
+    int lg_run;                        // neighbours of a piece that lie in one group, whichever piece: 2^lg_run
+    int images, chunks, parts;         // chunks of an image's rows: a workgroup's share of the statistics; parts of them: of the norm
+    int chunk_rows, part_rows, part_pixels;
+    int tail;                          // values of an image behind its last whole row
     int act;
-    unsigned pieces_magic, chunks_magic, places_magic, d_magic;      // udiv
+    float epsilon, slope;
+    float of_chunk, of_last, of_image; // values of a group in a chunk, in the last one; 1 / those in an image
+    unsigned pieces_magic, lanes_magic, c_magic, d_magic;  // udiv
     int lg_T, lg_TL;                   // threads that sum up one group's entries, of them on lanes of their own
     int lg_merge;                      // threads that sum up one group's chunks
 };
@@ -55,38 +58,28 @@ struct Kind {
     static constexpr int SIZE = TYPE == TSX_TYPE_F32 ? 4 : 2;
 };
 
-// Where a workgroup of the two kernels below works: `of` = n * chunks places, consecutive ones on consecutive XCDs.
-struct Place {
-    int64_t image;
-    int chunk;
-    __device__ __forceinline__ Place(const NormParams &p, int at) {
-        const int i = udiv(at, p.chunks, p.chunks_magic);
-        image = i;
-        chunk = at - i * p.chunks;
-    }
-};
+// 1 / sqrt(v) by the hardware's, within a step; its argument is no denormal
+__device__ __forceinline__ float reciprocal_root(float v) {
+    const bool tiny = v < 0x1p-100f;
+    return __fmul_rn(__builtin_amdgcn_rsqf(tiny ? __fmul_rn(v, 0x1p100f) : v), tiny ? 0x1p50f : 1.f);
+}
 
 // Mean and 1 / sqrt(variance + epsilon) of the groups of one image, into LDS, from the chunks' means and squares, in one pass around
 // the first chunk's mean: n_k (mean_k - mean_0)^2 is part of the variance, so what cancels is at most `chunks` times it.
-__device__ __forceinline__ void merge_chunks(const NormParams &p, int64_t image, float2 *group) {
-    const float whole = float(p.chunk_rows) * float(p.S) * float(p.d);
-    const float last = float(p.pixels - (p.chunks - 1) * p.chunk_rows * p.S) * float(p.d);
-    const float of_total = 1.f / (float(p.pixels) * float(p.d));
-    const int lg = p.lg_merge, T = 1 << lg;
-    for (int g0 = 0; g0 < p.groups; g0 += blockDim.x >> lg) {
-        const int g = g0 + (threadIdx.x >> lg);
-        if (g >= p.groups) continue;                         // T threads agree
-        const float2 *const partial = p.partial + (image * p.groups + g) * p.chunks;
+__device__ __forceinline__ void merge_chunks(const NormParams &p, int image, float2 *group) {
+    const int lg = p.lg_merge, T = 1 << lg, t = threadIdx.x & (T - 1);
+    const float2 *const partials = p.partial + int64_t(image * p.groups) * p.chunks;
+    for (int g = threadIdx.x >> lg; g < p.groups; g += blockDim.x >> lg) {      // T threads agree
+        const float2 *const partial = partials + g * p.chunks;
         const float about = partial[0].x;
         float s = 0.f, m2 = 0.f;
-        constexpr int AHEAD = 8;                             // requests that leave together
-        for (int k = threadIdx.x & (T - 1); k < p.chunks; k += AHEAD * T) {
-            float2 part[AHEAD];
-            static_for<0, AHEAD>([&](auto uc) { part[decltype(uc)::value] = partial[min(k + decltype(uc)::value * T, p.chunks - 1)]; });
-            static_for<0, AHEAD>([&](auto uc) {
+        for (int k = t; k < p.chunks; k += 4 * T) {          // four requests that leave together
+            float2 part[4];
+            static_for<0, 4>([&](auto uc) { part[decltype(uc)::value] = partial[min(k + decltype(uc)::value * T, p.chunks - 1)]; });
+            static_for<0, 4>([&](auto uc) {
                 constexpr int u = decltype(uc)::value;
                 const int at = k + u * T;
-                const float n = at < p.chunks - 1 ? whole : last, d = part[u].x - about;
+                const float n = at < p.chunks - 1 ? p.of_chunk : p.of_last, d = part[u].x - about;
                 if (at < p.chunks) {
                     s = __builtin_fmaf(n, d, s);
                     m2 += __builtin_fmaf(n * d, d, part[u].y);
@@ -95,9 +88,9 @@ __device__ __forceinline__ void merge_chunks(const NormParams &p, int64_t image,
         }
         s = sum_over_lanes(s, lg);
         m2 = sum_over_lanes(m2, lg);
-        const float shift = s * of_total, variance = fmaxf(__builtin_fmaf(-shift, s, m2), 0.f) * of_total;
+        const float shift = s * p.of_image, variance = fmaxf(__builtin_fmaf(-shift, s, m2), 0.f) * p.of_image;
         // a NaN among the squares stays one (fmaxf drops it)
-        if ((threadIdx.x & (T - 1)) == 0) group[g] = float2{about + shift, 1.f / sqrtf((m2 == m2 ? variance : m2) + p.epsilon)};
+        if (t == 0) group[g] = float2{about + shift, reciprocal_root((m2 == m2 ? variance : m2) + p.epsilon)};
     }
 }
 
@@ -138,20 +131,39 @@ template <int V>
 struct Affine {
     float mean[V], scale[V], shift[V];
     __device__ __forceinline__ Affine(int ch, int c, const float *weight, const float *bias) {
-        int at[V];
         static_for<0, V>([&](auto ec) {
-            constexpr int e = decltype(ec)::value;
-            at[e] = ch++;
-            if (ch == c) ch = 0;
-            scale[e] = 1.f;
-            shift[e] = 0.f;
+            scale[decltype(ec)::value] = 1.f;
+            shift[decltype(ec)::value] = 0.f;
         });
-        if (bias) static_for<0, V>([&](auto ec) { shift[decltype(ec)::value] = bias[at[decltype(ec)::value]]; });
-        if (weight) static_for<0, V>([&](auto ec) { scale[decltype(ec)::value] = weight[at[decltype(ec)::value]]; });
+        const bool wraps = ch + V > c;
+        auto load = [&](const float *from, float (&to)[V]) __attribute__((always_inline)) {
+            if (wraps) {
+                static_for<0, V>([&](auto ec) { const int at = ch + decltype(ec)::value; to[decltype(ec)::value] = from[at - (at >= c ? at / c * c : 0)]; });
+            } else if constexpr (V % 4 == 0) {
+                typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
+                static_for<0, V / 4>([&](auto gc) {
+                    constexpr int g = decltype(gc)::value;
+                    const v4f v = *reinterpret_cast<const v4f_any *>(from + ch + 4 * g);
+                    static_for<0, 4>([&](auto jc) { to[4 * g + decltype(jc)::value] = v[decltype(jc)::value]; });
+                });
+            } else {
+                static_for<0, V>([&](auto ec) { to[decltype(ec)::value] = from[ch + decltype(ec)::value]; });
+            }
+        };
+        if (bias) load(bias, shift);
+        if (weight) load(weight, scale);
     }
     // group[0]: the statistics of the first of the c channels
     __device__ __forceinline__ void take(const float2 *group, int ch, int c, int d, unsigned d_magic) {
         int g = udiv(ch, d, d_magic), left = (g + 1) * d - ch;             // channels left in the group
+        if (d % V == 0) {                                    // uniform: a piece lies in one group
+            const float2 stat = group[g];
+            static_for<0, V>([&](auto ec) {
+                mean[decltype(ec)::value] = stat.x;
+                scale[decltype(ec)::value] *= stat.y;
+            });
+            return;
+        }
         static_for<0, V>([&](auto ec) {
             constexpr int e = decltype(ec)::value;
             const float2 stat = group[g];

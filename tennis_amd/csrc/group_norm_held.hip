@@ -26,23 +26,23 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_held_kernel(Held
     // consecutive bundles of an image on one XCD: they share cache lines
     const int id = int(blockIdx.x % 8) * p.per_xcd + int(blockIdx.x / 8);
     if (int(blockIdx.x / 8) >= p.per_xcd || id >= p.bundles) return;       // uniform
-    const int a_image = p.a_image, image = udiv(id, a_image, p.image_magic), ch0 = (id - image * a_image) * channels, pixels = int(p.pixels);
+    const int a_image = p.a_image, image = udiv(id, a_image, p.image_magic), ch0 = (id - image * a_image) * channels, pixels = p.pixels;
     const int lane = udiv(t, p.pieces_a_pixel, p.pixel_magic), j = t - lane * p.pieces_a_pixel;
     const bool mine = lane < lanes;
     // All requests at once, none behind a branch, where it would be waited for: threads without a pixel read another one again.
     const int j_in = mine ? j : 0, lane_in = mine ? lane : 0;
-    const char *const x = static_cast<const char *>(p.x) + (int64_t(image) * p.image_stride + ch0 + j_in * V) * SIZE;
+    const char *const x = static_cast<const char *>(p.x) + image * p.image_bytes + (ch0 + j_in * V) * SIZE;
     Run<TYPE, V> v[NP];
-    static_for<0, NP>([&](auto ic) { v[decltype(ic)::value].load(x + int64_t(min(lane_in + decltype(ic)::value * lanes, pixels - 1)) * p.pixel_stride * SIZE); });
+    static_for<0, NP>([&](auto ic) { v[decltype(ic)::value].load(x + int64_t(min(lane_in + decltype(ic)::value * lanes, pixels - 1)) * p.pixel_bytes); });
     Affine<V> affine(mine ? j * V : 0, channels, p.weight ? p.weight + ch0 : nullptr, p.bias ? p.bias + ch0 : nullptr);
     // The packed words anew for each pass over them: unpacked once for all three they would be twice as many registers.
     auto again = [&] { static_for<0, NP>([&](auto ic) { v[decltype(ic)::value].renew_words(); }); };
     // `leave`: a thread's V sums into LDS, neighbours of one group added up
     auto leave = [&](float *to, float (&s)[V]) __attribute__((always_inline)) {
-        join_runs<V>(p.run, [&](auto ac, auto fc) { constexpr int a = decltype(ac)::value; s[a] += s[a + decltype(fc)::value]; });
+        join_runs<V>(1 << p.lg_run, [&](auto ac, auto fc) { constexpr int a = decltype(ac)::value; s[a] += s[a + decltype(fc)::value]; });
         if (!mine) return;
         int at = lane * pitch + (j * V >> p.lg_run);
-        static_for<0, V>([&](auto ec) { if ((decltype(ec)::value & (p.run - 1)) == 0) to[at++] = s[decltype(ec)::value]; });
+        static_for<0, V>([&](auto ec) { if ((decltype(ec)::value & ((1 << p.lg_run) - 1)) == 0) to[at++] = s[decltype(ec)::value]; });
     };
     // The sums of both arrays over a group's entries, for the TG threads of that group
     const int TG = 1 << p.lg_TG, TL = 1 << p.lg_TL, TE = TG >> p.lg_TL, group_entries = p.d >> p.lg_run;
@@ -71,7 +71,7 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_held_kernel(Held
         }
         return s;
     };
-    const float of_count = 1.f / (float(pixels) * float(p.d));
+    const float of_count = p.of_image;
     float sum[V];
     static_for<0, V>([&](auto ec) { sum[decltype(ec)::value] = 0.f; });
     static_for<0, NP>([&](auto ic) {
@@ -111,13 +111,13 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_held_kernel(Held
     if (tg == 0 && g < p.B) {
         const float shift = total.x * of_count, squares = __builtin_fmaf(-shift, total.x, total.y);
         // a NaN stays one (fmaxf drops it)
-        group[g] = float2{rough + shift, 1.f / sqrtf((squares == squares ? fmaxf(squares, 0.f) * of_count : squares) + p.epsilon)};
+        group[g] = float2{rough + shift, reciprocal_root((squares == squares ? fmaxf(squares, 0.f) * of_count : squares) + p.epsilon)};
     }
     __syncthreads();
     if (!mine) return;
     again();
     affine.take(group, j * V, channels, p.d, p.d_magic);
-    char *const out = static_cast<char *>(p.out) + (int64_t(image) * pixels * p.c + ch0 + j * V) * SIZE;
+    char *const out = static_cast<char *>(p.out) + image * p.out_image_bytes + (ch0 + j * V) * SIZE;
     static_for<0, NP>([&](auto ic) {
         constexpr int i = decltype(ic)::value;
         if (lane + i * lanes < pixels) {
@@ -167,14 +167,13 @@ HeldPlan held_plan(const tsx_group_norm *g, const NormParams &rows) {
             best.threads = threads;
             HeldParams &p = best.p;
             static_cast<NormParams &>(p) = rows;
-            p.run = gcd(d, V);
             p.B = B;
             p.pieces_a_pixel = a_pixel;
             p.held_lanes = lanes;
             p.bundles = int(bundles);
             p.per_xcd = int(ceil_div(bundles, 8));
             p.a_image = g->groups / B;
-            p.lg_run = lg_of(p.run);
+            p.lg_run = lg_of(gcd(d, V));
             p.lg_TG = lg_of(threads / power_of_two(B));
             p.lg_TL = std::min(p.lg_TG, lg_of(power_of_two(lanes)));
             p.pixel_magic = div_magic(a_pixel, NORM_MOST_THREADS);
@@ -186,7 +185,7 @@ HeldPlan held_plan(const tsx_group_norm *g, const NormParams &rows) {
 template <int TYPE, int V, int NP>
 int launch_held(const HeldPlan &h, hipStream_t stream) {
     const HeldParams &p = h.p;
-    const size_t lds = size_t(p.held_lanes) * ((p.B * p.d / p.run) | 1) * 2 * sizeof(float);
+    const size_t lds = size_t(p.held_lanes) * ((p.B * p.d >> p.lg_run) | 1) * 2 * sizeof(float);
     const auto kernel = p.act == TSX_ACT_SILU ? group_norm_held_kernel<TYPE, V, NP, TSX_ACT_SILU> : group_norm_held_kernel<TYPE, V, NP, ANY_ACT>;
     if (lds > 48 * 1024)
         TSX_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024));

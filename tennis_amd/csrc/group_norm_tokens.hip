@@ -15,9 +15,9 @@ __global__ __launch_bounds__(256) void group_norm_tokens_kernel(NormParams p) {
     constexpr int V = 8, SIZE = Kind<TYPE>::SIZE;
     const int pieces = (p.c + V - 1) / V, width = pieces * V;
     float *const means = reinterpret_cast<float *>(group + (p.groups + 1) / 2 * 2), *const scales = means + width, *const shifts = scales + width;
-    const int part = udiv(blockIdx.x, p.places, p.places_magic), at = blockIdx.x - part * p.places;
-    const Place place(p, p.places % 8 == 0 ? p.places - 8 - at / 8 * 8 + at % 8 : at);
-    merge_chunks(p, place.image, group);
+    const bool turned = p.chunks % 8 == 0;      // as in the norm to its own type
+    const int chunk = turned ? p.chunks - 8 - (blockIdx.x & ~7u) + (blockIdx.x & 7) : blockIdx.x, image = turned ? p.images - 1 - blockIdx.y : blockIdx.y;
+    merge_chunks(p, image, group);
     __syncthreads();
     for (int ch = threadIdx.x; ch < width; ch += 256) {
         const float2 g = ch < p.c ? group[udiv(ch, p.d, p.d_magic)] : float2{0.f, 0.f};
@@ -26,14 +26,14 @@ __global__ __launch_bounds__(256) void group_norm_tokens_kernel(NormParams p) {
         shifts[ch] = ch < p.c && p.bias ? p.bias[ch] : 0.f;
     }
     __syncthreads();
-    const int64_t chunk_pixels = p.chunk_rows * p.S, chunk_end = place.chunk == p.chunks - 1 ? p.pixels : (place.chunk + 1) * chunk_pixels;
-    const int64_t first = place.chunk * chunk_pixels + part * p.part_pixels, end = part == p.parts - 1 ? chunk_end : min(first + p.part_pixels, chunk_end);
+    const int chunk_pixels = p.chunk_rows * p.S, chunk_first = chunk * chunk_pixels, chunk_end = chunk == p.chunks - 1 ? p.pixels : chunk_first + chunk_pixels;
+    const int first = chunk_first + int(blockIdx.z) * p.part_pixels, end = int(blockIdx.z) == p.parts - 1 ? chunk_end : min(first + p.part_pixels, chunk_end);
     const int l = threadIdx.x % L;
-    const char *const x = static_cast<const char *>(p.x) + place.image * p.image_stride * SIZE;
-    for (int64_t base = first; base < end; base += 256 / L) {
-        const int64_t pixel = base + threadIdx.x / L;
+    const char *const x = static_cast<const char *>(p.x) + image * p.image_bytes;
+    for (int base = first; base < end; base += 256 / L) {
+        const int pixel = base + threadIdx.x / L;
         const bool there = pixel < end;                      // a pixel's lanes agree
-        const char *const from = x + (there ? pixel : end - 1) * p.pixel_stride * SIZE;
+        const char *const from = x + int64_t(there ? pixel : end - 1) * p.pixel_bytes;
         Run<TYPE, V> in[P];
         // all requests at once, none behind a branch, where it would be waited for
         const int whole = p.c / V;
@@ -70,7 +70,7 @@ __global__ __launch_bounds__(256) void group_norm_tokens_kernel(NormParams p) {
         });
         top = over_lanes(top, lg_of(L), [](unsigned a, unsigned b) { return max(a, b); });
         const TokenScale s(__builtin_bit_cast(float, top));
-        const int64_t token = place.image * p.pixels + pixel;
+        const int64_t token = int64_t(image) * p.pixels + pixel;
         if (there && l == 0) p.scales[token] = s.scale;
         if (there)
             static_for<0, P>([&](auto ic) {
@@ -91,16 +91,15 @@ __global__ __launch_bounds__(256) void group_norm_tokens_kernel(NormParams p) {
 template <int TYPE, int L, int P>
 int launch_tokens(NormParams p, hipStream_t stream) {
     // four workgroups a CU, of two turns at least
-    const int64_t chunk_pixels = p.chunk_rows * p.S, parts = std::max<int64_t>(1, std::min<int64_t>(ceil_div(1024, p.places), chunk_pixels / (2 * 256 / L)));
-    p.part_pixels = ceil_div(chunk_pixels, parts);
+    const int chunk_pixels = p.chunk_rows * p.S, parts = int(std::max<int64_t>(1, std::min<int64_t>(ceil_div(1024, int64_t(p.images) * p.chunks), chunk_pixels / (2 * 256 / L))));
+    p.part_pixels = int(ceil_div(chunk_pixels, parts));
     p.parts = int(ceil_div(chunk_pixels, p.part_pixels));
-    p.places_magic = div_magic(p.places, int64_t(p.places) * p.parts);
     p.lg_merge = lg_threads(256, p.groups, p.chunks);
     const size_t lds = size_t(round_up(p.groups, 2)) * sizeof(float2) + size_t(round_up(p.c, 8)) * 3 * sizeof(float);
     const auto kernel = p.act == TSX_ACT_SILU ? group_norm_tokens_kernel<TYPE, L, P, TSX_ACT_SILU> : group_norm_tokens_kernel<TYPE, L, P, ANY_ACT>;
     if (lds > 64 * 1024)
         TSX_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
-    hipLaunchKernelGGL(kernel, dim3(unsigned(p.places) * unsigned(p.parts)), dim3(256), lds, stream, p);
+    hipLaunchKernelGGL(kernel, dim3(unsigned(p.chunks), unsigned(p.images), unsigned(p.parts)), dim3(256), lds, stream, p);
     TSX_LAUNCH_CHECK("group_norm_tokens_kernel");
     return 0;
 }
