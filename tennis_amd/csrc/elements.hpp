@@ -108,6 +108,8 @@ struct Run {
             }
         });
     }
+    // STREAMS: not to be kept in the caches
+    template <bool STREAMS = false>
     __device__ __forceinline__ void store(void *at) const {
         if constexpr (BYTES == 2)
             *reinterpret_cast<unsigned short *>(at) = (unsigned short)word[0];
@@ -116,7 +118,9 @@ struct Run {
         else if constexpr (BYTES % 16 == 0)
             static_for<0, BYTES / 16>([&](auto wc) {
                 constexpr int w = decltype(wc)::value;
-                reinterpret_cast<v4u_any *>(at)[w] = v4u{word[4 * w], word[4 * w + 1], word[4 * w + 2], word[4 * w + 3]};
+                const v4u_any v = v4u{word[4 * w], word[4 * w + 1], word[4 * w + 2], word[4 * w + 3]};
+                if constexpr (STREAMS) __builtin_nontemporal_store(v, reinterpret_cast<v4u_any *>(at) + w);
+                else reinterpret_cast<v4u_any *>(at)[w] = v;
             });
         else
             static_for<0, BYTES / 8>([&](auto wc) {

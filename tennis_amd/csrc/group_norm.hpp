@@ -108,10 +108,11 @@ struct Piece {
         r.load_some(image + at * Kind<TYPE>::SIZE, left);
         static_for<0, V>([&](auto ec) { v[decltype(ec)::value] = r.template get<decltype(ec)::value>(); });
     }
+    template <bool STREAMS = false>
     __device__ __forceinline__ void store(char *out, int64_t at, int left) const {
         Run<TYPE, V> r;
         r.set(v);
-        if (left >= V) r.store(out + at * Kind<TYPE>::SIZE);
+        if (left >= V) r.template store<STREAMS>(out + at * Kind<TYPE>::SIZE);
         else r.store_some(out + at * Kind<TYPE>::SIZE, left);
     }
 };
