@@ -49,7 +49,6 @@ __device__ __forceinline__ void store_fragment(const TokenGemmParams &p, const v
     static_for<0, 4>([&](auto gc) {
         constexpr int g = decltype(gc)::value;
         const v4f ws = *reinterpret_cast<const v4f *>(scales + 8 * g + half), bias = *reinterpret_cast<const v4f *>(biases + 8 * g + half);
-        // a missing bias is -0, which changes no sum
         static_for<0, 4>([&](auto jc) { constexpr int j = decltype(jc)::value; v[4 * g + j] = __fadd_rn(__fmul_rn(__fmul_rn(float(acc[4 * g + j]), ws[j]), xs), bias[j]); });
     });
     activate_as<ACT>(v, p.slope);
@@ -98,7 +97,8 @@ __global__ __launch_bounds__(WR *WC * 64) void gemm_i8_tokens_kernel(TokenGemmPa
     constexpr int A_BYTES = ROWS * CHUNK, B_BYTES = COLS * CHUNK, A_LOADS = A_BYTES / 1024 / WAVES, B_LOADS = B_BYTES / 1024 / WAVES;
     static_assert(A_LOADS * 1024 * WAVES == A_BYTES && B_LOADS * 1024 * WAVES == B_BYTES && (S - 1) * (A_LOADS + B_LOADS) < 64, "whole loads, counted in six bits");
     extern __shared__ __attribute__((aligned(16))) int8_t lds[];      // [S][A_BYTES + B_BYTES]
-    // the tile's scales and biases, requested ahead of everything: in the epilogue each request would be waited for
+    // The tile's scales and biases, requested ahead of everything and here by the time the first chunk is: in the epilogue each request
+    // would be waited for.
     __shared__ __attribute__((aligned(16))) float of_cols[2][COLS], of_rows[ROWS];
     constexpr int THREADS = WAVES * 64;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -111,17 +111,15 @@ __global__ __launch_bounds__(WR *WC * 64) void gemm_i8_tokens_kernel(TokenGemmPa
     const int group_rows = min(4, p.row_tiles - 4 * group);
     const int tile_c = in_group / group_rows, tile_r = 4 * group + in_group - tile_c * group_rows;
     const int row0 = tile_r * ROWS, frag0 = tile_c * (COLS / 32);
-    static_for<0, (COLS + THREADS - 1) / THREADS>([&](auto ic) {
-        const int i = threadIdx.x + decltype(ic)::value * THREADS, col = min(frag0 * 32 + i, p.n - 1);
-        if (COLS % THREADS == 0 || i < COLS) {
-            of_cols[0][i] = p.w_scales[col];
-            of_cols[1][i] = p.bias ? p.bias[col] : -0.f;
-        }
+    constexpr int COL_TURNS = (COLS + THREADS - 1) / THREADS, ROW_TURNS = (ROWS + THREADS - 1) / THREADS;
+    float col_scale[COL_TURNS], col_bias[COL_TURNS], row_scale[ROW_TURNS];
+    static_for<0, COL_TURNS>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        col_scale[i] = p.w_scales[min(frag0 * 32 + int(threadIdx.x) + i * THREADS, p.n - 1)];
+        col_bias[i] = -0.f;                                  // changes no sum
     });
-    static_for<0, (ROWS + THREADS - 1) / THREADS>([&](auto ic) {
-        const int i = threadIdx.x + decltype(ic)::value * THREADS;
-        if (ROWS % THREADS == 0 || i < ROWS) of_rows[i] = p.x_scales[min(row0 + i, p.m - 1)];
-    });
+    if (p.bias) static_for<0, COL_TURNS>([&](auto ic) { col_bias[decltype(ic)::value] = p.bias[min(frag0 * 32 + int(threadIdx.x) + decltype(ic)::value * THREADS, p.n - 1)]; });
+    static_for<0, ROW_TURNS>([&](auto ic) { row_scale[decltype(ic)::value] = p.x_scales[min(row0 + int(threadIdx.x) + decltype(ic)::value * THREADS, p.m - 1)]; });
 
     // A row in LDS is its CHUNK bytes, its pieces of 16 XORed with bits of the row that make 16 rows cover all banks for one piece.  A
     // load instruction fills 1 KiB of such rows; rows beyond m are the last one again, never stored.  Pieces behind the end of a row are
@@ -178,6 +176,15 @@ __global__ __launch_bounds__(WR *WC * 64) void gemm_i8_tokens_kernel(TokenGemmPa
     };
     static_for<0, S>([&](auto sc) { fetch(decltype(sc)::value, decltype(sc)::value); });
     wait_for_all_but<(S - 1) * (A_LOADS + B_LOADS)>();
+    static_for<0, COL_TURNS>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        const int at = threadIdx.x + i * THREADS;
+        if (COLS % THREADS == 0 || at < COLS) of_cols[0][at] = col_scale[i], of_cols[1][at] = col_bias[i];
+    });
+    static_for<0, ROW_TURNS>([&](auto ic) {
+        const int at = threadIdx.x + decltype(ic)::value * THREADS;
+        if (ROWS % THREADS == 0 || at < ROWS) of_rows[at] = row_scale[decltype(ic)::value];
+    });
     lds_barrier();
     read(std::integral_constant<int, 0>{}, 0);
     int buf = 0;

@@ -9,6 +9,10 @@
 namespace tsx {
 namespace {
 
+#ifndef TOKENS_WORKGROUPS
+#define TOKENS_WORKGROUPS 512
+#endif
+
 template <int TYPE, int L, int P, int ACT>
 __global__ __launch_bounds__(256) void group_norm_tokens_kernel(NormParams p) {
     extern __shared__ float2 group[];                        // [groups], behind them [3][channels in whole pieces]
@@ -17,26 +21,15 @@ __global__ __launch_bounds__(256) void group_norm_tokens_kernel(NormParams p) {
     float *const means = reinterpret_cast<float *>(group + (p.groups + 1) / 2 * 2), *const scales = means + width, *const shifts = scales + width;
     const bool turned = p.chunks % 8 == 0;      // as in the norm to its own type
     const int chunk = turned ? p.chunks - 8 - (blockIdx.x & ~7u) + (blockIdx.x & 7) : blockIdx.x, image = turned ? p.images - 1 - blockIdx.y : blockIdx.y;
-    merge_chunks(p, image, group);
-    __syncthreads();
-    for (int ch = threadIdx.x; ch < width; ch += 256) {
-        const float2 g = ch < p.c ? group[udiv(ch, p.d, p.d_magic)] : float2{0.f, 0.f};
-        means[ch] = g.x;
-        scales[ch] = ch < p.c && p.weight ? g.y * p.weight[ch] : g.y;
-        shifts[ch] = ch < p.c && p.bias ? p.bias[ch] : 0.f;
-    }
-    __syncthreads();
     const int chunk_pixels = p.chunk_rows * p.S, chunk_first = chunk * chunk_pixels, chunk_end = chunk == p.chunks - 1 ? p.pixels : chunk_first + chunk_pixels;
     const int first = chunk_first + int(blockIdx.z) * p.part_pixels, end = int(blockIdx.z) == p.parts - 1 ? chunk_end : min(first + p.part_pixels, chunk_end);
-    const int l = threadIdx.x % L;
+    const int l = threadIdx.x % L, whole = p.c / V;
     const char *const x = static_cast<const char *>(p.x) + image * p.image_bytes;
-    for (int base = first; base < end; base += 256 / L) {
-        const int pixel = base + threadIdx.x / L;
-        const bool there = pixel < end;                      // a pixel's lanes agree
-        const char *const from = x + int64_t(there ? pixel : end - 1) * p.pixel_bytes;
-        Run<TYPE, V> in[P];
-        // all requests at once, none behind a branch, where it would be waited for
-        const int whole = p.c / V;
+    // All requests at once, none behind a branch, where it would be waited for; the first pixels' ahead of the statistics, and the
+    // vectors' of the first 1024 channels.
+    Run<TYPE, V> in[P];
+    auto fetch = [&](int base) __attribute__((always_inline)) {
+        const char *const from = x + int64_t(min(base + int(threadIdx.x / L), end - 1)) * p.pixel_bytes;
         if (whole)       // uniform
             static_for<0, P>([&](auto ic) { in[decltype(ic)::value].load(from + min(l + decltype(ic)::value * L, whole - 1) * (V * SIZE)); });
         if (whole != pieces)
@@ -46,6 +39,35 @@ __global__ __launch_bounds__(256) void group_norm_tokens_kernel(NormParams p) {
                 if (j >= whole) in[i].clear();
                 if (j >= whole && j < pieces) in[i].load_some(from + j * (V * SIZE), p.c - j * V);
             });
+    };
+    float w[4], b[4];
+    auto fetch_vectors = [&](int ch) __attribute__((always_inline)) {
+        static_for<0, 4>([&](auto uc) { w[decltype(uc)::value] = 1.f, b[decltype(uc)::value] = 0.f; });
+        if (p.weight) static_for<0, 4>([&](auto uc) { w[decltype(uc)::value] = p.weight[min(ch + 256 * decltype(uc)::value, p.c - 1)]; });
+        if (p.bias) static_for<0, 4>([&](auto uc) { b[decltype(uc)::value] = p.bias[min(ch + 256 * decltype(uc)::value, p.c - 1)]; });
+    };
+    if (first < end) fetch(first);
+    fetch_vectors(threadIdx.x);
+    merge_chunks(p, image, group);
+    __syncthreads();
+    for (int ch0 = threadIdx.x; ch0 < width; ch0 += 1024) {
+        if (ch0 >= 1024) fetch_vectors(ch0);
+        static_for<0, 4>([&](auto uc) {
+            constexpr int u = decltype(uc)::value;
+            const int ch = ch0 + 256 * u;
+            if (ch < width) {
+                const float2 g = group[udiv(min(ch, p.c - 1), p.d, p.d_magic)];
+                means[ch] = g.x;
+                scales[ch] = g.y * w[u];
+                shifts[ch] = b[u];
+            }
+        });
+    }
+    __syncthreads();
+    for (int base = first; base < end; base += 256 / L) {
+        const int pixel = base + threadIdx.x / L;
+        const bool there = pixel < end;                      // a pixel's lanes agree
+        if (base != first) fetch(base);
         float y[P][V];
         unsigned top = 0;
         static_for<0, P>([&](auto ic) {
@@ -67,6 +89,7 @@ __global__ __launch_bounds__(256) void group_norm_tokens_kernel(NormParams p) {
                     constexpr int e = decltype(ec)::value;
                     if ((pieces - 1) * V + e < p.c) top = max(top, __builtin_bit_cast(unsigned, y[i][e]) & 0x7fffffffu);
                 });
+            __builtin_amdgcn_sched_barrier(0);               // a piece at a time: all at once they take twice the registers
         });
         top = over_lanes(top, lg_of(L), [](unsigned a, unsigned b) { return max(a, b); });
         const TokenScale s(__builtin_bit_cast(float, top));
@@ -90,8 +113,7 @@ __global__ __launch_bounds__(256) void group_norm_tokens_kernel(NormParams p) {
 
 template <int TYPE, int L, int P>
 int launch_tokens(NormParams p, hipStream_t stream) {
-    // four workgroups a CU, of two turns at least
-    const int chunk_pixels = p.chunk_rows * p.S, parts = int(std::max<int64_t>(1, std::min<int64_t>(ceil_div(1024, int64_t(p.images) * p.chunks), chunk_pixels / (2 * 256 / L))));
+    const int chunk_pixels = p.chunk_rows * p.S, parts = int(std::max<int64_t>(1, std::min<int64_t>(ceil_div(TOKENS_WORKGROUPS, int64_t(p.images) * p.chunks), ceil_div(chunk_pixels, 256 / L))));
     p.part_pixels = int(ceil_div(chunk_pixels, parts));
     p.parts = int(ceil_div(chunk_pixels, p.part_pixels));
     p.lg_merge = lg_threads(256, p.groups, p.chunks);
