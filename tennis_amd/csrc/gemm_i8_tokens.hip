@@ -38,12 +38,11 @@ __device__ __forceinline__ void to_lds(const int8_t *at, int8_t *lds) {
     __builtin_amdgcn_global_load_lds((global_void *)at, (lds_void *)lds, 16, 0, 0);
 }
 
-// What leaves a fragment of 32 output columns x 32 tokens: accumulator r of lane l is column 8 (r / 4) + 4 (l / 32) + r % 4 of token
-// l % 32; swaps between the half-waves leave a lane with 16 consecutive columns, the lower ones with 0 .. 15, the upper ones with 16 .. 31.
-// scales, biases: of the fragment's columns, in LDS; xs: the token's; out: the token's column 16 (l / 32) of the fragment, left: columns
-// from there on that exist, at most 0 where the token is none.
+// A fragment's values of 32 output columns x 32 tokens in the output's type: accumulator r of lane l is column 8 (r / 4) + 4 (l / 32) +
+// r % 4 of token l % 32; swaps between the half-waves leave a lane with 16 consecutive columns, the lower ones with 0 .. 15, the upper
+// ones with 16 .. 31.  scales, biases: of the fragment's columns, in LDS; xs: the token's.
 template <int OUT, int ACT>
-__device__ __forceinline__ void store_fragment(const TokenGemmParams &p, const v16i &acc, const float *scales, const float *biases, float xs, char *out, int left) {
+__device__ __forceinline__ Run<OUT, 16> fragment_values(const TokenGemmParams &p, const v16i &acc, const float *scales, const float *biases, float xs) {
     const int half = 4 * ((threadIdx.x % 64) / 32);
     float v[16];
     static_for<0, 4>([&](auto gc) {
@@ -64,8 +63,7 @@ __device__ __forceinline__ void store_fragment(const TokenGemmParams &p, const v
             to.word[(2 * a + 1) * W + w] = s[1];
         });
     });
-    if (left >= 16) to.store(out);
-    else if (left > 0) to.store_some(out, left);
+    return to;
 }
 
 // f(the activation as a constant): one branch around all of a wavefront's values
@@ -174,7 +172,7 @@ __global__ __launch_bounds__(WR *WC * 64) void gemm_i8_tokens_kernel(TokenGemmPa
             a[set][i] = *reinterpret_cast<const v4i *>(at + a_row + i * 32 * CHUNK + ((2 * h + lane / 32) ^ a_key) * 16);
         });
     };
-    static_for<0, S>([&](auto sc) { fetch(decltype(sc)::value, decltype(sc)::value); });
+    static_for<0, S>([&](auto sc) { fetch(decltype(sc)::value, decltype(sc)::value); });     // behind the last chunk: that one again
     wait_for_all_but<(S - 1) * (A_LOADS + B_LOADS)>();
     static_for<0, COL_TURNS>([&](auto ic) {
         constexpr int i = decltype(ic)::value;
@@ -187,8 +185,9 @@ __global__ __launch_bounds__(WR *WC * 64) void gemm_i8_tokens_kernel(TokenGemmPa
     });
     lds_barrier();
     read(std::integral_constant<int, 0>{}, 0);
-    int buf = 0;
-    for (int c = 0; c < chunks; ++c) {
+    int buf = 0, c = 0;
+    auto multiply = [&](auto fetching) __attribute__((always_inline)) {
+        constexpr bool FETCHES = decltype(fetching)::value;
         const int after = buf + 1 == S ? 0 : buf + 1;
         static_for<0, HALVES>([&](auto hc) {
             constexpr int h = decltype(hc)::value;
@@ -197,10 +196,10 @@ __global__ __launch_bounds__(WR *WC * 64) void gemm_i8_tokens_kernel(TokenGemmPa
             } else {
                 // Every wavefront has its operands of this chunk in registers: its buffer is free behind the barrier, and the next
                 // chunk is there for all.  The rest of this chunk's arithmetic covers the first reads behind it.
-                wait_for_all_but<(S - 2) * (A_LOADS + B_LOADS)>();
+                wait_for_all_but<FETCHES ? (S - 2) * (A_LOADS + B_LOADS) : 0>();
                 lds_barrier();
                 read(std::integral_constant<int, 0>{}, after);
-                fetch(c + S, buf);
+                if constexpr (FETCHES) fetch(c + S, buf);
             }
             static_for<0, FR * FC>([&](auto fc) {
                 constexpr int i = decltype(fc)::value / FC, f = decltype(fc)::value % FC;
@@ -208,29 +207,49 @@ __global__ __launch_bounds__(WR *WC * 64) void gemm_i8_tokens_kernel(TokenGemmPa
             });
             // reads and requests between the multiplications
             static_for<0, FR * FC>([&](auto fc) {
-                if constexpr (h + 1 == HALVES) __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);
+                if constexpr (FETCHES && h + 1 == HALVES) __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
             });
             __builtin_amdgcn_sched_barrier(0);
         });
         buf = after;
-    }
-    wait_for_all_but<0>();                                   // nothing on its way into LDS when the workgroup gives it back
+    };
+    for (; c + S < chunks; ++c) multiply(std::true_type{});
+    for (; c < chunks; ++c) multiply(std::false_type{});      // the last S chunks are all on their way
+    // The chunks' LDS is free: nothing is on its way into it, and behind this barrier nobody reads it.  A wavefront's 32 tokens x 32 FC
+    // columns go through it, so that a store instruction writes whole cache lines (straight from the registers it would write 16 bytes of
+    // each of 64 runs).
+    wait_for_all_but<0>();
+    lds_barrier();
     by_act(p.act, [&](auto act) __attribute__((always_inline)) {
-        constexpr int SIZE = OUT == TSX_TYPE_F32 ? 4 : 2;
+        constexpr int SIZE = OUT == TSX_TYPE_F32 ? 4 : 2, ROW = FC * 32 * SIZE, PITCH = ROW + 16, IN_ROW = ROW / 16, AT_ONCE = 64 / IN_ROW, EACH = 16 / SIZE;
+        static_assert(WAVES * 32 * PITCH <= S * (A_BYTES + B_BYTES), "room for all wavefronts");
+        int8_t *const mine = lds + wave * (32 * PITCH);
+        const int col = (frag0 + wave_c * FC) * 32 + lane % IN_ROW * EACH, left = p.n - col;      // where a lane stores
         static_for<0, FR>([&](auto ic) {
             constexpr int i = decltype(ic)::value;
-            const int in_tile = (wave_r * FR + i) * 32 + lane % 32, row = row0 + in_tile;
-            const float xs = of_rows[in_tile];
-            const int col = frag0 * 32 + wave_c * FC * 32 + 16 * (lane / 32);
-            char *const out = static_cast<char *>(p.out) + (int64_t(row) * p.out_stride + col) * SIZE;
+            const int in_tile = (wave_r * FR + i) * 32;
+            const float xs = of_rows[in_tile + lane % 32];
             static_for<0, FC>([&](auto fc) {
                 constexpr int f = decltype(fc)::value;
                 const int at = (wave_c * FC + f) * 32;
-                store_fragment<OUT, decltype(act)::value>(p, acc[i][f], of_cols[0] + at, of_cols[1] + at, xs, out + f * (32 * SIZE),
-                                                          row < p.m ? p.n - col - 32 * f : 0);
+                const Run<OUT, 16> v = fragment_values<OUT, decltype(act)::value>(p, acc[i][f], of_cols[0] + at, of_cols[1] + at, xs);
+                v4u *const to = reinterpret_cast<v4u *>(mine + lane % 32 * PITCH + (f * 32 + 16 * (lane / 32)) * SIZE);
+                static_for<0, SIZE>([&](auto wc) { constexpr int w = 4 * decltype(wc)::value; to[w / 4] = v4u{v.word[w], v.word[w + 1], v.word[w + 2], v.word[w + 3]}; });
             });
+            static_for<0, 32 / AT_ONCE>([&](auto kc) {
+                const int r = decltype(kc)::value * AT_ONCE + lane / IN_ROW, row = row0 + in_tile + r;
+                Run<OUT, EACH> v;
+                const v4u got = *reinterpret_cast<const v4u *>(mine + r * PITCH + lane % IN_ROW * 16);
+                static_for<0, 4>([&](auto wc) { v.word[decltype(wc)::value] = got[decltype(wc)::value]; });
+                char *const out = static_cast<char *>(p.out) + (int64_t(row) * p.out_stride + col) * SIZE;
+                if (row < p.m) {
+                    if (left >= EACH) v.store(out);
+                    else if (left > 0) v.store_some(out, left);
+                }
+            });
+            __builtin_amdgcn_sched_barrier(0);               // 32 tokens at a time: their values would fill the registers
         });
     });
 }
@@ -448,8 +467,8 @@ int few_tokens(const tsx_token_gemm *g, const TokenGemmParams &q, bool quantizes
 // The kernel a call takes, by an estimate of its time in us, fitted to products of 16 .. 32768 rows on K of 128 .. 8192 (bf16 output):
 // what a launch takes whatever its size, and for each 256 workgroups, one a CU, a fixed part and one for each 1024 of K.  Measured, few
 // tokens 16 x 32 and 32 x 32, tiles of 64, 128 and 256 (us): 32 x 1000, K = 2048: 4.4, 5.9, 7.3, 11.2, 22.6; 64 x 4096, K = 4096: 12.6, 9.9,
-// 12.1, 19.6, 40; 197 x 777, K = 1500: 5.0, 5.3, 6.8, 11, 25; 512 x 3840, K = 1280: 33, 26, 8.2, 9.4, 18.5; 2048^3: -, -, 19.7, 14.0,
-// 25.7; 4096^3: -, -, 110, 79, 65.
+// 12.1, 19.6, 40; 197 x 777, K = 1500: 5.0, 5.3, 6.8, 11, 25; 512 x 3840, K = 1280: 33, 26, 7.3, 9.2, 17.4; 2048^3: -, -, 17.8, 13.8,
+// 24.3; 4096^3: -, -, 108, 77, 62.
 enum class TokenKernel { few_16, few_32, tile_64, tile_128, tile_256 };
 
 TokenKernel choose(int m, int n, int k) {
@@ -458,8 +477,8 @@ TokenKernel choose(int m, int n, int k) {
     const auto rounds = [&](int rows, int cols) { return float(ceil_div(m, rows) * ceil_div(n, cols)) / 256.f; };
     const float few = rounds(32, 16), few_wide = rounds(32, 32), r64 = rounds(64, 64), r128 = rounds(128, 128), r256 = rounds(256, 256);
     const float cost[] = {few <= 1.f ? 3.6f + ks * (k <= 2048 ? 0.5f : 1.25f * std::max(few, 0.5f)) : 3.6f + few * (0.25f + 1.1f * ks),
-                          4.2f + std::max(few_wide, 1.f) * (0.2f + 1.35f * ks), 3.f + std::max(r64, 1.f) * (0.5f + 1.8f * ks),
-                          3.f + std::ceil(r128) * (1.5f + 4.5f * ks), 3.f + std::ceil(r256) * (8.4f + 13.4f * ks * (0.75f + 0.25f * std::min(r256, 1.f)))};
+                          4.2f + std::max(few_wide, 1.f) * (0.2f + 1.35f * ks), 3.f + std::max(r64, 1.f) * (0.5f + 1.75f * ks),
+                          3.f + std::ceil(r128) * (1.9f + 4.2f * ks), 3.f + std::ceil(r256) * (7.4f + 13.f * ks * (0.75f + 0.25f * std::min(r256, 1.f)))};
     int best = 0;
     for (int i = 1; i < 5; ++i)
         if (cost[i] < cost[best]) best = i;
