@@ -135,7 +135,11 @@ int power_of_two(int v) {      // the next one up
     return p;
 }
 
-// Whether the one-launch kernel takes the call, on which pieces and threads: V = 0, it does not.
+// Whether the one-launch kernel takes the call, on which pieces and threads (V = 0: it does not), by estimates of the times in us, fitted
+// to bf16 with SiLU.  Here a workgroup's own values take their time, and all workgroups' that of the cache lines they share with one
+// another (runs of less than 40 bytes at a pixel cost as much as 40).  Two kernels: two starts and the tensor's bytes.  Measured, one launch
+// and two: 64 pixels x 1280 channels on 2 images 6.2 and 9.6, on 32 images 7.2 and 10.4; 1024 x 640 on 8 10.8 and 16, on 32 27.6 and 24.8;
+// 4096 x 320 (groups of 10: runs of 20 bytes) on 1 20 and 12, on 8 22 and 18; 4096 x 128 on 1 9.5 and 10.3, on 8 14.6 and 11.5.
 struct HeldPlan {
     HeldParams p;
     int V, NP, threads;
@@ -143,7 +147,8 @@ struct HeldPlan {
 
 HeldPlan held_plan(const tsx_group_norm *g, const NormParams &rows) {
     HeldPlan best{};
-    float best_cost = 0.f;
+    const float size = float(element_bytes(g->type));
+    float best_cost = 10.f + 0.4e-6f * float(g->n) * float(g->pixels) * float(g->c) * size;
     if (g->pixels > 16384) return best;
     const int pixels = int(g->pixels), d = g->c / g->groups, whole = g->type == TSX_TYPE_F32 ? 4 : 8;
     for (int V = whole; V >= 2; V /= 2)
@@ -159,8 +164,9 @@ HeldPlan held_plan(const tsx_group_norm *g, const NormParams &rows) {
             if (power_of_two(B) > threads) continue;
             const int64_t bundles = int64_t(g->n) * (g->groups / B);
             if (bundles > 1 << 24) continue;
-            const float cost = float(ceil_div(bundles, 256)) * float(pixels) * float(B * d) / 8000.f;
-            if (best.V && cost >= best_cost) continue;
+            const float run = float(B * d) * size, pixel = float(pixels) / 20480.f;
+            const float cost = 5.f + std::max(1.7f * pixel * run, 2.6f * float(bundles) / 256.f * pixel * std::max(run, 40.f)) * (V == 2 ? 2.f : 1.f);
+            if (cost >= best_cost) continue;
             best_cost = cost;
             best.V = V;
             best.NP = need;
