@@ -95,16 +95,17 @@ struct Run {
                 static_for<0, 2>([&](auto jc) { word[2 * w + decltype(jc)::value] = v[decltype(jc)::value]; });
             });
     }
-    // the first `left` values, behind them zeros
+    // the first `left` values, one at least, behind them zeros; all requested at once, the last one again in the place of those
     __device__ __forceinline__ void load_some(const void *at, int left) {
         static_for<0, WORDS>([&](auto wc) {
             constexpr int w = decltype(wc)::value;
             if constexpr (TYPE == TSX_TYPE_F32) {
-                word[w] = w < left ? reinterpret_cast<const unsigned *>(at)[w] : 0u;
+                const unsigned v = reinterpret_cast<const unsigned *>(at)[min(w, left - 1)];
+                word[w] = w < left ? v : 0u;
             } else {
                 const unsigned short *h = reinterpret_cast<const unsigned short *>(at);
-                const unsigned lo = 2 * w < left ? h[2 * w] : 0, hi = 2 * w + 1 < left ? h[2 * w + 1] : 0;
-                word[w] = lo | hi << 16;
+                const unsigned lo = h[min(2 * w, left - 1)], hi = h[min(2 * w + 1, left - 1)];
+                word[w] = (2 * w < left ? lo : 0u) | (2 * w + 1 < left ? hi << 16 : 0u);
             }
         });
     }

@@ -309,11 +309,14 @@ __global__ __launch_bounds__(FEW_THREADS) void gemm_i8_few_tokens_kernel(FewToke
             auto load = [&](int first) __attribute__((always_inline)) {
                 if (whole)           // uniform
                     static_for<0, HELD>([&](auto ic) { v[decltype(ic)::value].load(x + int64_t(min(first + t + decltype(ic)::value * T, whole - 1)) * (PIECE * SIZE)); });
+                Values last;
+                last.clear();
+                if (whole != pieces) last.load_some(x + int64_t(whole) * (PIECE * SIZE), p.cols - whole * PIECE);       // uniform
                 static_for<0, HELD>([&](auto ic) {
                     constexpr int i = decltype(ic)::value;
                     const int at = first + t + i * T;
                     if (at >= whole) v[i].clear();
-                    if (at >= whole && at < pieces) v[i].load_some(x + int64_t(at) * (PIECE * SIZE), p.cols - at * PIECE);
+                    if (at == whole) v[i] = last;
                 });
             };
             unsigned top = 0;

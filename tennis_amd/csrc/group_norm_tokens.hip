@@ -32,13 +32,11 @@ __global__ __launch_bounds__(256) void group_norm_tokens_kernel(NormParams p) {
         const char *const from = x + int64_t(min(base + int(threadIdx.x / L), end - 1)) * p.pixel_bytes;
         if (whole)       // uniform
             static_for<0, P>([&](auto ic) { in[decltype(ic)::value].load(from + min(l + decltype(ic)::value * L, whole - 1) * (V * SIZE)); });
-        if (whole != pieces)
-            static_for<0, P>([&](auto ic) {
-                constexpr int i = decltype(ic)::value;
-                const int j = l + i * L;
-                if (j >= whole) in[i].clear();
-                if (j >= whole && j < pieces) in[i].load_some(from + j * (V * SIZE), p.c - j * V);
-            });
+        if (whole != pieces) {   // uniform: the pixel's last, incomplete piece
+            Run<TYPE, V> last;
+            last.load_some(from + whole * (V * SIZE), p.c - whole * V);
+            static_for<0, P>([&](auto ic) { if (l + decltype(ic)::value * L == whole) in[decltype(ic)::value] = last; });
+        }
     };
     float w[4], b[4];
     auto fetch_vectors = [&](int ch) __attribute__((always_inline)) {

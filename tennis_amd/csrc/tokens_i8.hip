@@ -38,11 +38,14 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void quantize_tokens_kernel(Toke
         auto fetch = [&](int first) __attribute__((always_inline)) {
             if (whole)       // uniform
                 static_for<0, P>([&](auto ic) { v[decltype(ic)::value].load(x + int64_t(min(first + t + decltype(ic)::value * T, whole - 1)) * (PIECE * SIZE)); });
+            Values last;
+            last.clear();
+            if (whole != pieces) last.load_some(x + int64_t(whole) * (PIECE * SIZE), p.cols - whole * PIECE);       // uniform
             static_for<0, P>([&](auto ic) {
                 constexpr int i = decltype(ic)::value;
                 const int piece = first + t + i * T;
                 if (piece >= whole) v[i].clear();
-                if (piece >= whole && piece < pieces) v[i].load_some(x + int64_t(piece) * (PIECE * SIZE), p.cols - piece * PIECE);
+                if (piece == whole) v[i] = last;
             });
         };
         const int turns = HELD ? 1 : (pieces_out + T * P - 1) / (T * P);
@@ -96,8 +99,11 @@ int launch(const TokenParams &p, hipStream_t stream) {
 
 template <int TYPE>
 int launch_type(const TokenParams &p, hipStream_t stream) {
-    // A wavefront a row while there are rows for all CUs, with no barrier; more threads a row where there are few rows or it is long.
+    // Several rows a wavefront where they are short, one while there are rows for all CUs, with no barrier; more threads a row where there are few rows or it is long.
     const int64_t pieces = ceil_div(p.cols_out, PIECE);
+    if (pieces <= 1) return launch<TYPE, 1, 1, true>(p, stream);
+    if (pieces <= 4) return launch<TYPE, 4, 1, true>(p, stream);
+    if (pieces <= 16) return launch<TYPE, 16, 1, true>(p, stream);
     if (pieces <= 64) return launch<TYPE, 64, 1, true>(p, stream);
     if (p.rows >= 512 || pieces <= 128) {
         if (pieces <= 128) return launch<TYPE, 64, 2, true>(p, stream);

@@ -102,6 +102,17 @@ def test_quantize_tokens(torch, capi, name, m, k):
 
 
 @pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("m,k", [(3000, 1), (1000, 8), (999, 9), (777, 31), (700, 128), (700, 129), (600, 1000), (600, 4096), (513, 4000), (2000, 600)])
+def test_quantize_many_tokens(torch, capi, name, m, k):
+    """Several rows to a wavefront, and one."""
+    rng = np.random.default_rng(m + k)
+    x, x64 = values(torch, rng, (m, k + 3), name)
+    q, s = capi.quantize_tokens(x[:, 1:k + 1])
+    eq, es = tokens64(x64[:, 1:k + 1])
+    assert np.array_equal(q.cpu().numpy(), eq) and np.array_equal(s.cpu().numpy(), es)
+
+
+@pytest.mark.parametrize("name", TYPES)
 def test_quantize_tokens_strides(torch, capi, name):
     rng = np.random.default_rng(4)
     wide, wide64 = values(torch, rng, (37, 300), name)
@@ -167,6 +178,54 @@ def test_product(torch, capi, name, m, n, k):
     # its own tokens, quantized ahead, are the same bits
     qd, sd = capi.quantize_tokens(x)
     assert torch.equal(layer(qd, x_scales=sd, act=act, slope=0.1, out_dtype=x.dtype), out)
+
+
+@pytest.mark.parametrize("kernel", "01234")
+@pytest.mark.parametrize("m,n,k", [(1, 1, 16), (5, 17, 64), (33, 31, 100), (64, 130, 192), (65, 129, 257), (130, 70, 1040), (257, 257, 640), (300, 520, 2048), (260, 100, 48)])
+def test_every_product_kernel(torch, capi, monkeypatch, kernel, m, n, k):
+    """Each kernel on sizes that end inside its tiles and K of fewer and more chunks than it keeps in flight: the same bits."""
+    rng = np.random.default_rng(m + n + k)
+    w, sw, bias = weights(torch, rng, n, k)
+    q = rng.integers(-128, 128, (m, k)).astype(np.int8)
+    sx = rng.uniform(0.01, 0.1, m).astype(np.float32)
+    layer = capi.TokenGemmI8(torch.from_numpy(w).cuda(), torch.from_numpy(sw).cuda(), torch.from_numpy(bias).cuda())
+    x, s = torch.from_numpy(q).cuda(), torch.from_numpy(sx).cuda()
+    monkeypatch.setenv("TSX_TOKENS_KERNEL", kernel)
+    for name, act in zip(TYPES, ("silu", None, "leaky_relu")):
+        want, error = product64(q, sx, w, sw, bias, act)
+        got = layer(x, x_scales=s, act=act, slope=0.1, out_dtype=dtype(torch, name))
+        close(torch, got, want, error, name)
+        monkeypatch.delenv("TSX_TOKENS_KERNEL")
+        assert torch.equal(got, layer(x, x_scales=s, act=act, slope=0.1, out_dtype=got.dtype))
+        monkeypatch.setenv("TSX_TOKENS_KERNEL", kernel)
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("m,n,k", [(1, 40, 40960), (2, 33, 20479), (3, 20, 9000), (5, 20, 8192), (9, 50, 4551), (20, 70, 2048), (32, 40, 1279), (17, 16, 7)])
+def test_product_quantizes_few_tokens_itself(torch, capi, name, m, n, k):
+    """Rows that one workgroup's threads hold and rows read in turns, shared by all, several or one of its wavefronts."""
+    rng = np.random.default_rng(m + k)
+    w, sw, bias = weights(torch, rng, n, k)
+    x, x64 = values(torch, rng, (m, k), name, 0.3)
+    x[m - 1, k // 2] = math.inf
+    q, sx = tokens64(x.double().cpu().numpy())
+    layer = capi.TokenGemmI8(torch.from_numpy(w).cuda(), torch.from_numpy(sw).cuda(), torch.from_numpy(bias).cuda())
+    out = layer(x)
+    assert out[m - 1].isnan().all()
+    if m > 1:
+        want, error = product64(q[:-1], sx[:-1], w, sw, bias, None)
+        close(torch, out[:-1], want, error, name)
+
+
+def test_product_of_the_longest_rows(torch, capi):
+    """The largest sums: 127 * 127 * (2^17 - 1) is 2 % short of what 32 bits hold."""
+    k = (1 << 17) - 1
+    for m in (2, 40):
+        q = torch.full((m, k), 127, dtype=torch.int8, device="cuda")
+        layer = capi.TokenGemmI8(torch.full((3, k), 127, dtype=torch.int8, device="cuda"), torch.ones(3, device="cuda"))
+        assert (layer(q, x_scales=torch.ones(m, device="cuda")) == float(np.float32(127 * 127 * k))).all()
+    with pytest.raises(capi.TsxError, match="2\\^17"):
+        capi.TokenGemmI8(torch.ones((3, k + 1), dtype=torch.int8, device="cuda"), torch.ones(3, device="cuda"))(torch.ones((2, k + 1), device="cuda"))
 
 
 @pytest.mark.parametrize("act", ACTS)
