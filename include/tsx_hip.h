@@ -218,7 +218,8 @@ int tsx_gemm_i8(int32_t m, int32_t n, int32_t k, const int8_t *a_dev, const void
 #define TSX_TYPE_I8   3   /* where a call says so */
 /* x / (1 + exp(-x)), on the hardware's exponential and reciprocal; only in the calls on tokens and in the group norm, which take
  * TSX_ACT_NONE, _RELU, _LEAKY_RELU, _MISH_FAST and this (the exact Mish is the host's bits for a given fp32 number: there is
- * none to match here).  A negative zero and a NaN become 0 under ReLU, as in the activations' SIMD body. */
+ * none to match here).  A negative zero and a NaN become 0 under ReLU, a NaN 0 under LeakyReLU, as in the activations' SIMD body: so does
+ * what a row or a group with a NaN gives. */
 #define TSX_ACT_SILU 5
 
 /* Each row to int8 by its own largest magnitude a:  scale = fp32(a / 127),  q = x * fp32(127 / a) rounded to nearest even (the
@@ -231,7 +232,7 @@ int tsx_quantize_tokens(int64_t rows, int32_t cols, const void *x_dev, int32_t x
  *   out[i][j] = act(float(sum_k q[i][k] w[k][j]) * w_scales[j] * x_scales[i] + bias[j])
  * x_type TSX_TYPE_I8: x holds q, x_scales its scales, as tsx_quantize_tokens or tsx_group_norm_tokens_nhwc write them.  Another type:
  * the rows are quantized by the call, with the values of tsx_quantize_tokens (x_scales is not read).  Weights as
- * tsx_gemm_i8_pack_weights packs them; k is below 2^17, m may be 0.  The workspace (16-byte aligned, its contents written and read by
+ * tsx_gemm_i8_pack_weights packs them; k is below 2^17, n below 2^24, m below 2^28 and may be 0.  The workspace (16-byte aligned, its contents written and read by
  * each call: calls that share one must not overlap) may be asked for as 0 bytes. */
 typedef struct tsx_token_gemm {
     int32_t m, n, k;

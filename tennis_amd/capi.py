@@ -614,7 +614,7 @@ def _token_operand(what, x, types):
         raise TsxError("%s: expected a device tensor" % what)
     if x.dtype not in types:
         raise TsxError("%s: %s (one of %s)" % (what, x.dtype, ", ".join(str(t) for t in types)))
-    return x
+    return x.resolve_neg()
 
 
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
@@ -661,9 +661,9 @@ def quantize_tokens(x):
     out = _native().quantize_tokens(x)
     if out is not NotImplemented:
         return out
-    _token_operand("quantize_tokens", x, _FLOATS)
-    if x.dim() < 1 or x.shape[-1] == 0:
-        raise TsxError("quantize_tokens: rows without values, %s" % (tuple(x.shape),))
+    x = _token_operand("quantize_tokens", x, _FLOATS)
+    if x.dim() < 1 or not 0 < x.shape[-1] <= 1 << 30:
+        raise TsxError("quantize_tokens: shape %s (rows of 1 to 2^30 values)" % (tuple(x.shape),))
     q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
     scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
     if x.numel():
@@ -679,7 +679,7 @@ class TokenGemmI8:
 
     def __init__(self, w_i8, w_scales, bias=None, transpose=True):
         self.w = _dev(_token_operand("weights", w_i8, (torch.int8,)), torch.int8)
-        if self.w.dim() != 2 or 0 in self.w.shape:
+        if self.w.dim() != 2 or 0 in self.w.shape or max(self.w.shape) >= 1 << 24:
             raise TsxError("weights of shape %s" % (tuple(self.w.shape),))
         self.transpose = bool(transpose)
         self.n, self.k = (self.w.shape if self.transpose else self.w.shape[::-1])
@@ -707,7 +707,7 @@ class TokenGemmI8:
                                         -1 if out_dtype is None else _TYPES.get(out_dtype, 3))
         if out is not NotImplemented:
             return out
-        _token_operand("token product", x, _FLOATS + (torch.int8,))
+        x = _token_operand("token product", x, _FLOATS + (torch.int8,))
         if x.device != self.w.device:
             raise TsxError("tokens on %s, weights on %s" % (x.device, self.w.device))
         if x.dim() < 1 or x.shape[-1] != self.k:
@@ -717,6 +717,8 @@ class TokenGemmI8:
         out_dtype = out_dtype or x.dtype
         if out_dtype not in _FLOATS:
             raise TsxError("token product: output type %s" % out_dtype)
+        if x.numel() // self.k >= 1 << 28:
+            raise TsxError("token product: %d rows (below 2^28)" % (x.numel() // self.k))
         out = torch.empty(x.shape[:-1] + (self.n,), dtype=out_dtype, device=x.device)
         x_scales = _vector("x_scales", x_scales, x.numel() // self.k, x)
         if x.numel() == 0:
@@ -736,10 +738,12 @@ def _group_norm(x, groups, weight, bias, epsilon, act, slope, tokens):
     out = _native().group_norm(x, groups, weight, bias, epsilon, act, slope, tokens)
     if out is not NotImplemented:
         return out
-    _token_operand("group_norm", x, _FLOATS)
+    x = _token_operand("group_norm", x, _FLOATS)
     if x.dim() < 2 or x.shape[-1] == 0:
         raise TsxError("group_norm: shape %s ([n, ..., c] expected)" % (tuple(x.shape),))
-    n, c = x.shape[0], x.shape[-1]
+    n, c, groups = x.shape[0], x.shape[-1], int(groups)
+    if n >= 65536 or c > 8192 or not 0 < groups <= c:
+        raise TsxError("group_norm: %d images of %d channels in %d groups (below 65536, at most 8192)" % (n, c, groups))
     weight, bias = _vector("weight", weight, c, x), _vector("bias", bias, c, x)
     out = torch.empty(x.shape, dtype=torch.int8 if tokens else x.dtype, device=x.device)
     scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if tokens else None
@@ -748,7 +752,7 @@ def _group_norm(x, groups, weight, bias, epsilon, act, slope, tokens):
         if pixels is None or (c > 1 and x.stride(-1) != 1) or (pixels[0] > 1 and pixels[1] < c) or x.stride(0) < 0:
             x = x.contiguous()
             pixels = _axis(x, 1, x.dim() - 1)
-        g = GroupNorm(n, c, int(groups), _TYPES[x.dtype], pixels[0], x.stride(0), pixels[1] if pixels[0] > 1 else c, _ptr(x), _ptr(weight),
+        g = GroupNorm(n, c, groups, _TYPES[x.dtype], pixels[0], x.stride(0), pixels[1] if pixels[0] > 1 else c, _ptr(x), _ptr(weight),
                       _ptr(bias), float(epsilon), act, float(slope))
         nbytes = lib().tsx_group_norm_workspace_bytes(ctypes.byref(g))
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None

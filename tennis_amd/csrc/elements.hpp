@@ -1,6 +1,8 @@
 // Tensors of fp32, fp16 and bf16 values: runs of them to and from registers, their magnitudes, and their rows as int8 tokens.
 // All arithmetic on them is in fp32; a result is rounded once, to nearest even, when it is stored.
 #pragma once
+#include <atomic>
+
 #include "tsx_common.hpp"
 
 namespace tsx {
@@ -9,6 +11,26 @@ inline size_t element_bytes(int type) { return type == TSX_TYPE_F32 ? 4 : type =
 inline bool is_float_type(int type) { return type == TSX_TYPE_F32 || type == TSX_TYPE_F16 || type == TSX_TYPE_BF16; }
 inline bool is_token_act(int act) {      // the exact Mish is the host's bits for a given fp32 number, which no sum here has
     return act == TSX_ACT_NONE || act == TSX_ACT_RELU || act == TSX_ACT_LEAKY_RELU || act == TSX_ACT_MISH_FAST || act == TSX_ACT_SILU;
+}
+
+// Dynamic LDS beyond 64 KiB is granted per kernel and device: once for each, of a kernel always the same bytes.
+inline int grant_lds(const void *kernel, int bytes) {
+    struct Granted { std::atomic<const void *> kernel; std::atomic<uint64_t> devices; };
+    constexpr unsigned PLACES = 256;       // more than there are kernels that ask
+    static Granted table[PLACES];
+    int dev = 0;
+    TSX_HIP(hipGetDevice(&dev));
+    const unsigned first = unsigned(reinterpret_cast<uintptr_t>(kernel) >> 4);
+    for (unsigned i = 0; i < PLACES; ++i) {
+        Granted &g = table[(first + i) % PLACES];
+        const void *none = nullptr;
+        if (g.kernel.load() != kernel && !g.kernel.compare_exchange_strong(none, kernel) && none != kernel) continue;
+        if (dev < 64 && g.devices.load() >> dev & 1) return 0;
+        TSX_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        if (dev < 64) g.devices.fetch_or(uint64_t(1) << dev);
+        return 0;
+    }
+    return fail(TSX_E_INVALID, "no place for another kernel's LDS");
 }
 
 // f(the activation as a constant)

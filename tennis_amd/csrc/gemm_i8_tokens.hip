@@ -5,7 +5,6 @@
 // Rows of floats become int8 first (tokens_i8.hip), in the workspace, padded with zeros to whole chunks of K.  int32 sums are
 // exact, so every kernel here gives the same bits.
 #include <algorithm>
-#include <atomic>
 #include <cmath>
 #include <cstdlib>
 
@@ -394,29 +393,13 @@ __global__ __launch_bounds__(FEW_THREADS) void gemm_i8_few_tokens_kernel(FewToke
     }
 }
 
-// more than 64 KiB of dynamic LDS, granted once per kernel and device
-int grant_lds(const void *kernel, int bytes) {
-    struct Granted { std::atomic<const void *> kernel; std::atomic<uint64_t> devices; };
-    static Granted table[64];
-    int dev = 0;
-    TSX_HIP(hipGetDevice(&dev));
-    for (Granted &g : table) {
-        const void *none = nullptr;
-        if (g.kernel.load() != kernel && !g.kernel.compare_exchange_strong(none, kernel) && none != kernel) continue;
-        if (dev >= 64 || !(g.devices.load() >> dev & 1)) {
-            TSX_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-            if (dev < 64) g.devices.fetch_or(uint64_t(1) << dev);
-        }
-        return 0;
-    }
-    return check_hip(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "hipFuncSetAttribute");
-}
-
 template <int WR, int WC, int FR, int FC, int KS, int S, int OUT>
 int launch_tile(TokenGemmParams p, hipStream_t stream) {
     p.row_tiles = int(ceil_div(p.m, 32 * WR * FR));
     p.col_tiles = int(ceil_div(p.n, 32 * WC * FC));
-    p.tiles_per_xcd = int(ceil_div(int64_t(p.row_tiles) * p.col_tiles, 8));
+    const int64_t per_xcd = ceil_div(int64_t(p.row_tiles) * p.col_tiles, 8);
+    TSX_REQUIRE(8 * per_xcd * WR * WC * 64 < int64_t(1) << 32, "gemm_i8_tokens: %d x %d outputs are more than a launch holds", p.m, p.n);
+    p.tiles_per_xcd = int(per_xcd);
     constexpr int LDS = S * 32 * (WR * FR + WC * FC) * KS * KSTEP;
     const auto kernel = gemm_i8_tokens_kernel<WR, WC, FR, FC, KS, S, OUT>;
     if (LDS > 64 * 1024) {
@@ -474,6 +457,8 @@ int few_tokens(const tsx_token_gemm *g, const TokenGemmParams &q, bool quantizes
 // 24.3; 4096^3: -, -, 108, 77, 62.
 enum class TokenKernel { few_16, few_32, tile_64, tile_128, tile_256 };
 
+constexpr int FEW_MOST = 1 << 14;      // rows of the kernels for few tokens: with more their groups of rows leave a launch's second axis
+
 TokenKernel choose(int m, int n, int k) {
     if (m <= 16) return TokenKernel::few_16;
     const float ks = float(k) / 1024.f;
@@ -482,8 +467,8 @@ TokenKernel choose(int m, int n, int k) {
     const float cost[] = {few <= 1.f ? 3.6f + ks * (k <= 2048 ? 0.5f : 1.25f * std::max(few, 0.5f)) : 3.6f + few * (0.25f + 1.1f * ks),
                           4.2f + std::max(few_wide, 1.f) * (0.2f + 1.35f * ks), 3.f + std::max(r64, 1.f) * (0.5f + 1.75f * ks),
                           3.f + std::ceil(r128) * (1.9f + 4.2f * ks), 3.f + std::ceil(r256) * (7.4f + 13.f * ks * (0.75f + 0.25f * std::min(r256, 1.f)))};
-    int best = 0;
-    for (int i = 1; i < 5; ++i)
+    int best = m <= FEW_MOST ? 0 : 2;
+    for (int i = best + 1; i < 5; ++i)
         if (cost[i] < cost[best]) best = i;
     return TokenKernel(best);
 }
@@ -493,7 +478,8 @@ int launch(const tsx_token_gemm *g, const TokenGemmParams &p, bool quantizes, hi
     if (quantizes) return few_tokens<OUT>(g, p, true, false, stream);
     // TSX_TOKENS_KERNEL: that kernel, by its place in the list above, whatever the call (tests, measurements)
     const char *e = std::getenv("TSX_TOKENS_KERNEL");
-    switch (e && e[0] >= '0' && e[0] <= '4' ? TokenKernel(e[0] - '0') : choose(p.m, p.n, p.k)) {
+    const bool named = e && e[0] >= (p.m <= FEW_MOST ? '0' : '2') && e[0] <= '4';
+    switch (named ? TokenKernel(e[0] - '0') : choose(p.m, p.n, p.k)) {
         case TokenKernel::few_16: return few_tokens<OUT>(g, p, false, false, stream);
         case TokenKernel::few_32: return few_tokens<OUT>(g, p, false, true, stream);
         case TokenKernel::tile_64: return launch_tile<2, 2, 1, 1, 2, 3, OUT>(p, stream);
@@ -521,7 +507,7 @@ int check(const tsx_token_gemm *g) {
     TSX_REQUIRE(g, "gemm_i8_tokens: null argument");
     TSX_REQUIRE(g->m >= 0 && g->n > 0 && g->k > 0, "gemm_i8_tokens: bad extents");
     TSX_REQUIRE(g->k < 1 << 17, "gemm_i8_tokens: K = %d (below 2^17: longer sums leave 32 bits)", g->k);
-    TSX_REQUIRE(g->m < (1 << 30) && g->n < (1 << 30), "gemm_i8_tokens: extents of 2^30 and more");
+    TSX_REQUIRE(g->m < 1 << 28 && g->n < 1 << 24, "gemm_i8_tokens: %d rows and %d columns (below 2^28 and 2^24)", g->m, g->n);
     TSX_REQUIRE(is_float_type(g->x_type) || g->x_type == TSX_TYPE_I8, "gemm_i8_tokens: element type %d", g->x_type);
     TSX_REQUIRE(is_float_type(g->out_type), "gemm_i8_tokens: output type %d (fp32, fp16 or bf16)", g->out_type);
     TSX_REQUIRE(is_token_act(g->act), "gemm_i8_tokens: activation %d", g->act);
@@ -532,7 +518,6 @@ int check(const tsx_token_gemm *g) {
 
 int padded(int k) { return int(round_up(k, 16)); }
 
-
 // Whether the product's workgroups quantize the rows themselves, each all of them: the launch that this saves is 2 us, and up to some
 // 40 K values its work hides behind the weights (us with and without, 4096 columns, K = 4096: 1 row 6.0 and 7.9, 8 rows 7.4 and 8.9, 16
 // rows 9.9 and 9.7; 1000 columns, K = 2048, 16 rows: 5.5 and 7.2).
@@ -540,8 +525,9 @@ bool quantizes_itself(const tsx_token_gemm *g) {
     return g->x_type != TSX_TYPE_I8 && g->m <= 32 && int64_t(g->m) * g->k <= 40960 && few_lds(g->m, g->k) + FEW_WAVES * 2048 <= FEW_LDS;
 }
 
+// A tile's rows are reached by 32-bit offsets: 256 of them at 2^23.
 bool reads_in_place(const tsx_token_gemm *g) {
-    return g->x_type == TSX_TYPE_I8 && g->k % 16 == 0 && (g->m <= 1 || g->x_stride % 16 == 0) && reinterpret_cast<uintptr_t>(g->x_dev) % 16 == 0;
+    return g->x_type == TSX_TYPE_I8 && g->k % 16 == 0 && (g->m <= 1 || (g->x_stride % 16 == 0 && g->x_stride <= 1 << 23)) && reinterpret_cast<uintptr_t>(g->x_dev) % 16 == 0;
 }
 
 size_t scales_offset(const tsx_token_gemm *g) { return size_t(g->m) * padded(g->k); }
@@ -579,7 +565,7 @@ int tsx_gemm_i8_tokens(const tsx_token_gemm *g, void *workspace_dev, size_t work
     tsx::TokenGemmParams p{};
     const int kp = tsx::padded(g->k);
     p.q = static_cast<const int8_t *>(need ? workspace_dev : g->x_dev);
-    p.pitch = need ? kp : g->x_stride;
+    p.pitch = need ? kp : g->m <= 1 ? 0 : g->x_stride;
     p.x_scales = g->x_scales_dev;
     const bool quantizes = tsx::quantizes_itself(g);
     if (quantizes) {

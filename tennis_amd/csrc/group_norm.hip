@@ -203,13 +203,10 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_apply_kernel(Nor
 
 // ---- host side
 
-constexpr int MOST_CHUNKS = 256;
-#ifndef NORM_THREADS
-#define NORM_THREADS 512
-#endif
-#ifndef NORM_WORKGROUPS
-#define NORM_WORKGROUPS 512
-#endif
+// One workgroup of 512 threads a CU: with more, each has its prologue and its reductions, and the caches hold more streams.  us (bf16) at
+// 256, 512 and 2048 workgroups: 16384 pixels x 128 channels on 4 images 15.7, 17.8 and 17.9, 65536 x 64 on 2 16.6, 19.8 and 19.8, 262144 x
+// 128 on 4 133, 138 and 141; 256 workgroups of 1024 threads: 16.5, 17, 142, and 16384 x 128 on 1 14 where 512 threads take 11.9.
+constexpr int NORM_THREADS = 512, NORM_WORKGROUPS = 256, MOST_CHUNKS = 256;
 
 // Rows, threads and chunks of a call; V: values of a piece (1: a channel a thread, for pixels apart that are no whole pieces).
 struct NormPlan {
@@ -294,8 +291,10 @@ template <int TYPE, int V>
 int launch_statistics(const NormPlan &pl, hipStream_t stream) {
     const NormParams &p = pl.p;
     const size_t lds = size_t((p.lanes ? p.lanes : 1) + 1) * ((p.S * (p.c >> p.lg_run)) | 1) * 2 * sizeof(float);
-    if (lds > 64 * 1024)
-        TSX_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(group_norm_statistics_kernel<TYPE, V>), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+    if (lds > 64 * 1024) {
+        const int rc = grant_lds(reinterpret_cast<const void *>(group_norm_statistics_kernel<TYPE, V>), 160 * 1024);
+        if (rc) return rc;
+    }
     hipLaunchKernelGGL((group_norm_statistics_kernel<TYPE, V>), dim3(unsigned(p.chunks), unsigned(p.images)), dim3(pl.threads), lds, stream, p);
     TSX_LAUNCH_CHECK("group_norm_statistics_kernel");
     return 0;

@@ -2,7 +2,7 @@
 //
 // A workgroup takes B groups of one image, B * d channels of every pixel: whole pieces of V values.  Its threads hold them from the one
 // read to the one write; in between the mean, as the sum over all of them, and then the sums of x - mean and of its square, whose first
-// corrects the mean's rounding.  Two kernels read the tensor twice and wait for each other: 8 x 8 x 1280 on 2 images 21 us there.
+// corrects the mean's rounding.  Two kernels read the tensor twice and wait for each other: 8 x 8 x 1280 on 2 images 10.2 us there, 6.3 here.
 #include <algorithm>
 
 #include "group_norm.hpp"
@@ -138,8 +138,8 @@ int power_of_two(int v) {      // the next one up
 // Whether the one-launch kernel takes the call, on which pieces and threads (V = 0: it does not), by estimates of the times in us, fitted
 // to bf16 with SiLU.  Here a workgroup's own values take their time, and all workgroups' that of the cache lines they share with one
 // another (runs of less than 40 bytes at a pixel cost as much as 40).  Two kernels: two starts and the tensor's bytes.  Measured, one launch
-// and two: 64 pixels x 1280 channels on 2 images 6.2 and 9.6, on 32 images 7.2 and 10.4; 1024 x 640 on 8 10.8 and 16, on 32 27.6 and 24.8;
-// 4096 x 320 (groups of 10: runs of 20 bytes) on 1 20 and 12, on 8 22 and 18; 4096 x 128 on 1 9.5 and 10.3, on 8 14.6 and 11.5.
+// and two: 64 pixels x 1280 channels on 2 images 6.3 and 10.2, on 32 images 7.3 and 11.1; 1024 x 640 on 8 10.8 and 13.1, on 32 27.9 and 26.3;
+// 4096 x 320 (groups of 10: runs of 20 bytes) on 1 21.4 and 11.8, on 8 21.8 and 17.5; 4096 x 128 on 1 9.6 and 10.3, on 16 18.4 and 14.7.
 struct HeldPlan {
     HeldParams p;
     int V, NP, threads;
@@ -148,7 +148,7 @@ struct HeldPlan {
 HeldPlan held_plan(const tsx_group_norm *g, const NormParams &rows) {
     HeldPlan best{};
     const float size = float(element_bytes(g->type));
-    float best_cost = 10.f + 0.4e-6f * float(g->n) * float(g->pixels) * float(g->c) * size;
+    float best_cost = 10.f + 0.28e-6f * float(g->n) * float(g->pixels) * float(g->c) * size;
     if (g->pixels > 16384) return best;
     const int pixels = int(g->pixels), d = g->c / g->groups, whole = g->type == TSX_TYPE_F32 ? 4 : 8;
     for (int V = whole; V >= 2; V /= 2)
@@ -163,7 +163,7 @@ HeldPlan held_plan(const tsx_group_norm *g, const NormParams &rows) {
             if (need > most) break;
             if (power_of_two(B) > threads) continue;
             const int64_t bundles = int64_t(g->n) * (g->groups / B);
-            if (bundles > 1 << 24) continue;
+            if (bundles > 1 << 21) continue;      // with 1024 threads each, half of what a launch holds
             const float run = float(B * d) * size, pixel = float(pixels) / 20480.f;
             const float cost = 5.f + std::max(1.7f * pixel * run, 2.6f * float(bundles) / 256.f * pixel * std::max(run, 40.f)) * (V == 2 ? 2.f : 1.f);
             if (cost >= best_cost) continue;
@@ -193,8 +193,10 @@ int launch_held(const HeldPlan &h, hipStream_t stream) {
     const HeldParams &p = h.p;
     const size_t lds = size_t(p.held_lanes) * ((p.B * p.d >> p.lg_run) | 1) * 2 * sizeof(float);
     const auto kernel = p.act == TSX_ACT_SILU ? group_norm_held_kernel<TYPE, V, NP, TSX_ACT_SILU> : group_norm_held_kernel<TYPE, V, NP, ANY_ACT>;
-    if (lds > 48 * 1024)
-        TSX_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024));
+    if (lds > 48 * 1024) {      // 9 KiB beside them are the kernel's own
+        const int rc = grant_lds(reinterpret_cast<const void *>(kernel), 128 * 1024);
+        if (rc) return rc;
+    }
     hipLaunchKernelGGL(kernel, dim3(unsigned(8 * p.per_xcd)), dim3(h.threads), lds, stream, p);
     TSX_LAUNCH_CHECK("group_norm_held_kernel");
     return 0;

@@ -9,9 +9,9 @@
 namespace tsx {
 namespace {
 
-#ifndef TOKENS_WORKGROUPS
-#define TOKENS_WORKGROUPS 512
-#endif
+// us (bf16) at 512 and 1024: 262144 pixels x 128 channels on 2 images 82 and 76, 1024 x 640 on 32 28.4 and 27.3, 4096 x 320 on 8 18.8 and 18.9;
+// at 2048 the second takes 38
+constexpr int TOKENS_WORKGROUPS = 1024;
 
 template <int TYPE, int L, int P, int ACT>
 __global__ __launch_bounds__(256) void group_norm_tokens_kernel(NormParams p) {
@@ -117,8 +117,10 @@ int launch_tokens(NormParams p, hipStream_t stream) {
     p.lg_merge = lg_threads(256, p.groups, p.chunks);
     const size_t lds = size_t(round_up(p.groups, 2)) * sizeof(float2) + size_t(round_up(p.c, 8)) * 3 * sizeof(float);
     const auto kernel = p.act == TSX_ACT_SILU ? group_norm_tokens_kernel<TYPE, L, P, TSX_ACT_SILU> : group_norm_tokens_kernel<TYPE, L, P, ANY_ACT>;
-    if (lds > 64 * 1024)
-        TSX_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+    if (lds > 64 * 1024) {
+        const int rc = grant_lds(reinterpret_cast<const void *>(kernel), 160 * 1024);
+        if (rc) return rc;
+    }
     hipLaunchKernelGGL(kernel, dim3(unsigned(p.chunks), unsigned(p.images), unsigned(p.parts)), dim3(256), lds, stream, p);
     TSX_LAUNCH_CHECK("group_norm_tokens_kernel");
     return 0;

@@ -753,7 +753,7 @@ PyObject *token_gemm(PyObject *const *a, Py_ssize_t) {                // packed,
     g.k = int32_t(integer(a[1]));
     g.n = int32_t(integer(a[2]));
     const Rows r(x);
-    if (r.cols != g.k || r.rows >= 1 << 30 || packed.get_device() != x.get_device()) throw Decline{};
+    if (r.cols != g.k || r.rows >= 1 << 28 || packed.get_device() != x.get_device()) throw Decline{};
     g.m = int32_t(r.rows);
     g.x_type = type_code(x.scalar_type());
     g.x_stride = r.stride;
@@ -789,11 +789,12 @@ PyObject *group_norm(PyObject *const *a, Py_ssize_t) {                // x, grou
     tsx_group_norm g{};
     g.type = type_code(x.scalar_type());
     const int64_t c = x.size(-1);
-    if (g.type == TSX_TYPE_I8 || (c > 1 && x.stride(-1) != 1) || c > 1 << 20 || x.size(0) >= 65536) throw Decline{};
+    const long groups = integer(a[1]);
+    if (g.type == TSX_TYPE_I8 || (c > 1 && x.stride(-1) != 1) || c > 1 << 20 || x.size(0) >= 65536 || groups < 1 || groups > c) throw Decline{};
     const Axis pixels(x, 1, x.dim() - 1);
     g.n = int32_t(x.size(0));
     g.c = int32_t(c);
-    g.groups = int32_t(integer(a[1]));
+    g.groups = int32_t(groups);
     g.pixels = pixels.count;
     g.pixel_stride = pixels.count > 1 ? pixels.stride : c;
     g.image_stride = x.stride(0);

@@ -228,6 +228,97 @@ def test_product_of_the_longest_rows(torch, capi):
         capi.TokenGemmI8(torch.ones((3, k + 1), dtype=torch.int8, device="cuda"), torch.ones(3, device="cuda"))(torch.ones((2, k + 1), device="cuda"))
 
 
+def test_product_of_many_short_tokens(torch, capi):
+    """More groups of tokens than a launch has places along its second axis; 32-bit offsets would end at 2^31 bytes of rows and outputs."""
+    rng = np.random.default_rng(13)
+    for m, n, k in ((1 << 21, 16, 64), ((1 << 21) + 77, 1040, 1040)):
+        w, sw, bias = weights(torch, rng, n, k)
+        layer = capi.TokenGemmI8(torch.from_numpy(w).cuda(), torch.from_numpy(sw).cuda(), torch.from_numpy(bias).cuda())
+        q = torch.randint(-128, 128, (m, k), dtype=torch.int8, device="cuda")
+        sx = torch.rand(m, device="cuda") * 0.1 + 0.01
+        out = layer(q, x_scales=sx, out_dtype=torch.bfloat16)
+        at = torch.tensor([0, 1, 255, 256, m // 2, m - 257, m - 256, m - 2, m - 1], device="cuda")
+        want, error = product64(q[at].cpu().numpy(), sx[at].cpu().numpy(), w, sw, bias, None)
+        close(torch, out[at], want, error, "bf16")
+        for first in range(0, m, 1 << 19):       # the same by parts
+            assert torch.equal(out[first:first + (1 << 19)], layer(q[first:first + (1 << 19)], x_scales=sx[first:first + (1 << 19)], out_dtype=torch.bfloat16))
+
+
+def test_product_of_rows_far_apart(torch, capi):
+    """int8 tokens at strides on both sides of the longest that a tile reads in place, the last of them behind 2^32 bytes."""
+    rng = np.random.default_rng(14)
+    w, sw, _ = weights(torch, rng, 40, 64)
+    layer = capi.TokenGemmI8(torch.from_numpy(w).cuda(), torch.from_numpy(sw).cuda())
+    for m, stride in ((300, 1 << 23), (300, (1 << 23) + 16), (2, 1 << 31)):
+        whole = torch.empty((m - 1) * stride + 64, dtype=torch.int8, device="cuda")
+        x = whole.as_strided((m, 64), (stride, 1))
+        q = torch.from_numpy(rng.integers(-128, 128, (m, 64)).astype(np.int8)).cuda()
+        x.copy_(q)
+        s = torch.ones(m, device="cuda")
+        assert torch.equal(layer(x, x_scales=s), layer(q, x_scales=s))
+
+
+@pytest.mark.parametrize("m", [1, 16, 70])
+def test_rows_without_a_number_and_activations(torch, capi, m):
+    """ReLU and LeakyReLU make 0 of a NaN, the others keep it, in the products and in the norm."""
+    layer = capi.TokenGemmI8(torch.ones((33, 24), dtype=torch.int8, device="cuda"), torch.ones(33, device="cuda"))
+    x = torch.full((m, 24), math.nan, device="cuda")
+    planes = torch.full((2, m, 24), math.nan, device="cuda")
+    for act in ACTS:
+        for y in (layer(x, act=act, slope=0.1), capi.group_norm(planes, 3, act=act, slope=0.1)):
+            assert (y == 0).all() if act in ("relu", "leaky_relu") else y.isnan().all()
+        q, s = capi.group_norm_tokens(planes, 3, act=act, slope=0.1)
+        assert (q == 0).all() and ((s == 0).all() if act in ("relu", "leaky_relu") else s.isnan().all())
+
+
+def test_layers_are_copied_and_stored(torch, capi):
+    import copy
+    import io
+    import pickle
+    rng = np.random.default_rng(15)
+    w, sw, bias = weights(torch, rng, 30, 50)
+    layer = capi.TokenGemmI8(torch.from_numpy(w).cuda(), torch.from_numpy(sw).cuda(), torch.from_numpy(bias).cuda())
+    x, _ = values(torch, rng, (7, 50), "bf16", 0.3)
+    want = layer(x)
+    for other in (copy.copy(layer), copy.deepcopy(layer), pickle.loads(pickle.dumps(layer))):
+        assert torch.equal(other(x), want)
+    buf = io.BytesIO()
+    torch.save({"q": layer.w, "s": layer.w_scales, "b": layer.bias}, buf)
+    buf.seek(0)
+    state = torch.load(buf, weights_only=True)
+    assert torch.equal(capi.TokenGemmI8(state["q"], state["s"], state["b"])(x), want)
+
+
+def test_tensors_of_other_kinds(torch, capi):
+    """Views that stand for their negation, leaves that want gradients, vectors of another type, calls that carry no gradient."""
+    rng = np.random.default_rng(16)
+    z = torch.complex(torch.randn(6, 48, device="cuda"), torch.randn(6, 48, device="cuda"))
+    x = z.conj().imag
+    assert x.is_neg()
+    for a, b in ((capi.quantize_tokens(x), capi.quantize_tokens(x.clone())), (capi.group_norm_tokens(x, 4), capi.group_norm_tokens(x.clone(), 4))):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    assert torch.equal(capi.group_norm(x, 4), capi.group_norm(x.clone(), 4))
+    w, sw, bias = weights(torch, rng, 30, 48)
+    layer = capi.TokenGemmI8(torch.from_numpy(w).cuda(), torch.from_numpy(sw).cuda().double(), torch.from_numpy(bias).cuda().double())
+    assert torch.equal(layer(x), layer(x.clone()))
+    leaf = torch.randn(6, 48, device="cuda", requires_grad=True)
+    for y in (layer(leaf), capi.group_norm(leaf, 4, torch.ones(48, device="cuda", requires_grad=True)), capi.quantize_tokens(leaf)[1]):
+        assert not y.requires_grad
+
+
+def test_product_refuses_on_the_device(torch, capi):
+    layer = capi.TokenGemmI8(torch.ones((5, 16), dtype=torch.int8, device="cuda"), torch.ones(5, device="cuda"))
+    x, q = torch.ones((3, 16), device="cuda"), torch.ones((3, 16), dtype=torch.int8, device="cuda")
+    for call in (lambda: layer(x[:, :15]), lambda: layer(q), lambda: layer(x, x_scales=torch.ones(3, device="cuda")), lambda: layer(q, x_scales=torch.ones(2, device="cuda")),
+                 lambda: layer(x, out_dtype=torch.int8), lambda: layer(x.double()), lambda: layer(x, act="mish"), lambda: layer(x.cpu()), lambda: layer(torch.ones((), device="cuda")),
+                 lambda: capi.quantize_tokens(x[:, :0]), lambda: capi.quantize_tokens(q), lambda: capi.group_norm(x, 5), lambda: capi.group_norm(x, 0), lambda: capi.group_norm(x, -4),
+                 lambda: capi.group_norm(x, (1 << 32) + 4), lambda: capi.group_norm(x[:, :0], 1), lambda: capi.group_norm(x[0], 4), lambda: capi.group_norm(x, 4, torch.ones(15, device="cuda")),
+                 lambda: capi.group_norm(x, 4, epsilon=math.nan), lambda: capi.group_norm(torch.ones((1, 8193), device="cuda"), 1),
+                 lambda: capi.group_norm(torch.ones((65536, 1), device="cuda"), 1), lambda: capi.group_norm_tokens(x, 4, None, torch.ones(17, device="cuda"))):
+        with pytest.raises(capi.TsxError):
+            call()
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("out", TYPES)
 @pytest.mark.parametrize("m,n,k", [(3, 50, 70), (40, 136, 200), (130, 200, 140)])
@@ -398,6 +489,46 @@ def test_group_norm_far_from_zero(torch, capi, name):
     x[1, 20, 3, 9] = -1000.0
     want, error = norm64(x.double().numpy(), 4, None, None, 1e-5, None)
     close(torch, capi.group_norm(x.cuda(), 4), want, error, name)
+
+
+def test_group_norm_in_place(torch, capi):
+    """Through the C ABI the result may take the tensor's place, in one launch and in two."""
+    import ctypes
+    rng = np.random.default_rng(25)
+    for shape, groups in (((2, 8, 8, 320), 32), ((1, 5, 9, 60), 4), ((1, 200, 200, 24), 4), ((2, 90, 91, 13), 1), ((3, 1, 8192), 1)):
+        for name, code in (("f32", 0), ("f16", 1), ("bf16", 2)):
+            x = torch.from_numpy(rng.standard_normal(shape)).to(dtype(torch, name)).cuda()
+            want = capi.group_norm(x, groups, act="silu")
+            c = shape[-1]
+            pixels = x[0].numel() // c
+            g = capi.GroupNorm(shape[0], c, groups, code, pixels, pixels * c, c, capi._ptr(x), None, None, 1e-5, 5, 0.0)
+            nbytes = capi.lib().tsx_group_norm_workspace_bytes(ctypes.byref(g))
+            ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+            capi.check(capi.lib().tsx_group_norm_nhwc(ctypes.byref(g), capi._ptr(x), capi._ptr(ws), nbytes, capi._stream()))
+            assert torch.equal(x, want)
+
+
+def test_group_norm_of_large_images(torch, capi):
+    """Outputs that go past the caches, and images of more than 2^32 bytes, channels in odd numbers among them."""
+    for shape, groups, name in (((1, 1200, 1300, 40), 5, "bf16"), ((1, 1, (1 << 28) + 3, 9), 3, "bf16"), ((1, 1, (1 << 26) + 5, 24), 2, "f32")):
+        x = torch.randn(shape, device="cuda", dtype=dtype(torch, name)).mul_(2).add_(0.5)
+        out = capi.group_norm(x, groups, epsilon=1e-5)
+        q, s = capi.group_norm_tokens(x, groups)
+        d = shape[-1] // groups
+        for g in range(groups):
+            part = x[..., g * d:(g + 1) * d]
+            count = part.numel()
+            mean = sum(p.double().sum() for p in part.flatten(1, 2).split(1 << 24, 1)) / count
+            variance = sum((p.double() - mean).square().sum() for p in part.flatten(1, 2).split(1 << 24, 1)) / count
+            pixels = out.shape[1] * out.shape[2]
+            for at in (0, pixels // 2, pixels - 1000):
+                xs = part.flatten(1, 2)[:, at:at + 1000].double()
+                want = ((xs - mean) / torch.sqrt(variance + 1e-5)).cpu().numpy()
+                # the bar of norm64: threads add up to 2400 values here, sqrt(2400) / 2 roundings' worth, and 10^5 threads' errors average
+                close(torch, out.flatten(1, 2)[:, at:at + 1000, g * d:(g + 1) * d], want, (600 + 160 * np.abs(want)) * U, name)
+                got = q.flatten(1, 2)[:, at:at + 1000, g * d:(g + 1) * d].double() * s.flatten(1, 2)[:, at:at + 1000, None].double()
+                step = s.flatten(1, 2)[:, at:at + 1000, None].double().cpu().numpy()
+                assert (np.abs(got.cpu().numpy() - want) <= 0.501 * step + (600 + 160 * np.abs(want)) * U).all()
 
 
 def test_group_norm_of_constants(torch, capi):

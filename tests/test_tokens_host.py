@@ -39,10 +39,10 @@ def gemm(capi, **change):
 
 def test_product_refuses(capi):
     L = capi.lib()
-    need = L.tsx_gemm_i8_tokens_workspace_bytes(ctypes.byref(gemm(capi)))
-    assert need >= 4 * 16 + 16
+    need = L.tsx_gemm_i8_tokens_workspace_bytes(ctypes.byref(gemm(capi, m=100)))
+    assert need >= 100 * 16 + 100 * 4
     assert L.tsx_gemm_i8_tokens(ctypes.byref(gemm(capi, m=0)), None, 0, None) == 0
-    for change, word in ((dict(m=-1), "extents"), (dict(n=0), "extents"), (dict(k=0), "extents"), (dict(k=1 << 17, x_stride=1 << 17), "2^17"),
+    for change, word in ((dict(m=-1), "extents"), (dict(n=0), "extents"), (dict(m=1 << 28), "below 2^28"), (dict(n=1 << 24, out_stride=1 << 24), "below 2^28"), (dict(k=0), "extents"), (dict(k=1 << 17, x_stride=1 << 17), "2^17"),
                          (dict(x_type=4), "element type"), (dict(out_type=3), "output type"), (dict(act=3), "activation 3"), (dict(act=6), "activation 6"),
                          (dict(x_stride=15), "overlap"), (dict(out_stride=7), "overlap"), (dict(x_dev=None), "null"), (dict(packed_w_dev=None), "null"),
                          (dict(w_scales_dev=None), "null"), (dict(out_dev=None), "null"), (dict(x_type=3), "scales"), (dict(packed_w_dev=AT + 8), "aligned"),
@@ -71,7 +71,7 @@ def test_group_norm_refuses(capi):
         assert call(norm(capi, n=0)) == 0 and call(norm(capi, pixels=0)) == 0
         for change, word in ((dict(n=-1), "extents"), (dict(c=0), "extents"), (dict(groups=0), "extents"), (dict(pixels=-1), "extents"),
                              (dict(groups=5), "5 groups"), (dict(c=8200, groups=1, pixel_stride=8200), "at most 8192"), (dict(type=3), "element type"),
-                             (dict(n=65536), "65536 images"), (dict(pixel_stride=15), "overlap"), (dict(image_stride=-1), "negative"), (dict(act=3), "activation 3"),
+                             (dict(n=65536), "65536 images"), (dict(pixels=1 << 30), "pixels"), (dict(pixel_stride=(1 << 26) + 1), "2^26"), (dict(pixel_stride=15), "overlap"), (dict(image_stride=-1), "negative"), (dict(act=3), "activation 3"),
                              (dict(epsilon=-1.0), "epsilon"), (dict(epsilon=float("nan")), "epsilon"), (dict(x_dev=None), "null"), (dict(x_dev=AT + 1), "multiple")):
             assert call(norm(capi, **change)) == -1 and word in said(capi), (change, said(capi))
     g = norm(capi, pixels=1 << 20, image_stride=16 << 20)
