@@ -39,15 +39,24 @@ __device__ __forceinline__ void to_lds(const int8_t *at, int8_t *lds) {
 
 // A fragment's values of 32 output columns x 32 tokens in the output's type: accumulator r of lane l is column 8 (r / 4) + 4 (l / 32) +
 // r % 4 of token l % 32; swaps between the half-waves leave a lane with 16 consecutive columns, the lower ones with 0 .. 15, the upper
-// ones with 16 .. 31.  scales, biases: of the fragment's columns, in LDS; xs: the token's.
+// ones with 16 .. 31.  xs: the token's scale.
+struct OfColumns {                     // scales and biases of a lane's columns of a fragment
+    v4f scale[4], bias[4];
+    __device__ __forceinline__ void read(const float *scales, const float *biases) {      // the fragment's, in LDS
+        const int half = 4 * ((threadIdx.x % 64) / 32);
+        static_for<0, 4>([&](auto gc) {
+            constexpr int g = decltype(gc)::value;
+            scale[g] = *reinterpret_cast<const v4f *>(scales + 8 * g + half);
+            bias[g] = *reinterpret_cast<const v4f *>(biases + 8 * g + half);
+        });
+    }
+};
 template <int OUT, int ACT>
-__device__ __forceinline__ Run<OUT, 16> fragment_values(const TokenGemmParams &p, const v16i &acc, const float *scales, const float *biases, float xs) {
-    const int half = 4 * ((threadIdx.x % 64) / 32);
+__device__ __forceinline__ Run<OUT, 16> fragment_values(const TokenGemmParams &p, const v16i &acc, const OfColumns &of, float xs) {
     float v[16];
     static_for<0, 4>([&](auto gc) {
         constexpr int g = decltype(gc)::value;
-        const v4f ws = *reinterpret_cast<const v4f *>(scales + 8 * g + half), bias = *reinterpret_cast<const v4f *>(biases + 8 * g + half);
-        static_for<0, 4>([&](auto jc) { constexpr int j = decltype(jc)::value; v[4 * g + j] = __fadd_rn(__fmul_rn(__fmul_rn(float(acc[4 * g + j]), ws[j]), xs), bias[j]); });
+        static_for<0, 4>([&](auto jc) { constexpr int j = decltype(jc)::value; v[4 * g + j] = __fadd_rn(__fmul_rn(__fmul_rn(float(acc[4 * g + j]), of.scale[g][j]), xs), of.bias[g][j]); });
     });
     activate_as<ACT>(v, p.slope);
     Run<OUT, 16> to, own;
@@ -88,8 +97,15 @@ template <int N>
 __device__ __forceinline__ void wait_for_all_but() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
 // WR x WC wavefronts, each with FR x FC fragments of 32 tokens x 32 columns; S chunks of KS K-steps in LDS.
+//
+// Bound: the matrix cores where K is long.  256 x 256, K in chunks of 64, four of them on their way: a chunk's 64 multiplications of a
+// wavefront take 2048 cycles of its SIMD and 24 LDS reads; 4096^3 62 us, 8192^3 445 us (2.2 and 2.5 P operations/s; the library's plain
+// int8 product 69 and 432), where the card holds its power by a clock of 1.5 .. 1.7 GHz.  Where K is short, its start and its outputs,
+// which wait for no other tile's arithmetic on the same CU: 32768 x 960, K = 320 25 us, of which 12 are the two turns' epilogues.  Tiles
+// of 128: three of them a CU in 168 registers, which fill each other's waits (two of them: 29 us for 25, 131072 x 512, K = 128 37 for 29).
+// Requests to memory fill LDS past the registers, and a wavefront waits for all but the newest chunks' of them.
 template <int WR, int WC, int FR, int FC, int KS, int S, int OUT>
-__global__ __launch_bounds__(WR *WC * 64) void gemm_i8_tokens_kernel(TokenGemmParams p) {
+__global__ __launch_bounds__(WR *WC * 64, WR * FR == 4 ? 3 : 1) void gemm_i8_tokens_kernel(TokenGemmParams p) {
     constexpr int CHUNK = KS * KSTEP, PIECES = CHUNK / 16, WAVES = WR * WC, ROWS = 32 * WR * FR, COLS = 32 * WC * FC, HALVES = 2 * KS;
     constexpr int A_BYTES = ROWS * CHUNK, B_BYTES = COLS * CHUNK, A_LOADS = A_BYTES / 1024 / WAVES, B_LOADS = B_BYTES / 1024 / WAVES;
     static_assert(A_LOADS * 1024 * WAVES == A_BYTES && B_LOADS * 1024 * WAVES == B_BYTES && (S - 1) * (A_LOADS + B_LOADS) < 64, "whole loads, counted in six bits");
@@ -226,14 +242,22 @@ __global__ __launch_bounds__(WR *WC * 64) void gemm_i8_tokens_kernel(TokenGemmPa
         static_assert(WAVES * 32 * PITCH <= S * (A_BYTES + B_BYTES), "room for all wavefronts");
         int8_t *const mine = lds + wave * (32 * PITCH);
         const int col = (frag0 + wave_c * FC) * 32 + lane % IN_ROW * EACH, left = p.n - col;      // where a lane stores
+        // Read once where the registers hold them: each time they are as many LDS cycles as the values take.
+        constexpr bool ONCE = FR > 2 || OUT == TSX_TYPE_BF16;
+        OfColumns of[ONCE ? FC : 1];
+        auto read_columns = [&](auto fc) {
+            constexpr int f = decltype(fc)::value;
+            of[ONCE ? f : 0].read(of_cols[0] + (wave_c * FC + f) * 32, of_cols[1] + (wave_c * FC + f) * 32);
+        };
+        if constexpr (ONCE) static_for<0, FC>(read_columns);
         static_for<0, FR>([&](auto ic) {
             constexpr int i = decltype(ic)::value;
             const int in_tile = (wave_r * FR + i) * 32;
             const float xs = of_rows[in_tile + lane % 32];
             static_for<0, FC>([&](auto fc) {
                 constexpr int f = decltype(fc)::value;
-                const int at = (wave_c * FC + f) * 32;
-                const Run<OUT, 16> v = fragment_values<OUT, decltype(act)::value>(p, acc[i][f], of_cols[0] + at, of_cols[1] + at, xs);
+                if constexpr (!ONCE) read_columns(fc);
+                const Run<OUT, 16> v = fragment_values<OUT, decltype(act)::value>(p, acc[i][f], of[ONCE ? f : 0], xs);
                 v4u *const to = reinterpret_cast<v4u *>(mine + lane % 32 * PITCH + (f * 32 + 16 * (lane / 32)) * SIZE);
                 static_for<0, SIZE>([&](auto wc) { constexpr int w = 4 * decltype(wc)::value; to[w / 4] = v4u{v.word[w], v.word[w + 1], v.word[w + 2], v.word[w + 3]}; });
             });
@@ -451,10 +475,11 @@ int few_tokens(const tsx_token_gemm *g, const TokenGemmParams &q, bool quantizes
 }
 
 // The kernel a call takes, by an estimate of its time in us, fitted to products of 16 .. 32768 rows on K of 128 .. 8192 (bf16 output):
-// what a launch takes whatever its size, and for each 256 workgroups, one a CU, a fixed part and one for each 1024 of K.  Measured, few
-// tokens 16 x 32 and 32 x 32, tiles of 64, 128 and 256 (us): 32 x 1000, K = 2048: 4.4, 5.9, 7.3, 11.2, 22.6; 64 x 4096, K = 4096: 12.6, 9.9,
-// 12.1, 19.6, 40; 197 x 777, K = 1500: 5.0, 5.3, 6.8, 11, 25; 512 x 3840, K = 1280: 33, 26, 7.3, 9.2, 17.4; 2048^3: -, -, 17.8, 13.8,
-// 24.3; 4096^3: -, -, 108, 77, 62.
+// what a launch takes whatever its size, and for each 256 workgroups, one a CU, a fixed part and one for each 1024 of K (tiles of 256: a
+// CU's only workgroup, in whole turns).  Measured, few tokens 16 x 32 and 32 x 32, tiles of 64, 128 and 256 (us): 32 x 1000, K = 2048: 4.4,
+// 5.9, 7.3, 11.2, 22.6; 64 x 4096, K = 4096: 12.6, 9.9, 12.1, 19.6, 40; 197 x 777, K = 1500: 5.0, 5.3, 6.8, 11, 25; 512 x 3840, K = 1280:
+// 33, 26, 7.2, 9.1, 17.7; tiles alone: 2048^3 17.3, 13.8, 24.7; 8192 x 1280, K = 640 18.1, 14.5, 15.5; 32768 x 960, K = 320 41, 24.7, 25.4;
+// 131072 x 512, K = 128 58, 29.4, 33.7; 4096^3 107, 77, 62.
 enum class TokenKernel { few_16, few_32, tile_64, tile_128, tile_256 };
 
 constexpr int FEW_MOST = 1 << 14;      // rows of the kernels for few tokens: with more their groups of rows leave a launch's second axis
@@ -466,7 +491,7 @@ TokenKernel choose(int m, int n, int k) {
     const float few = rounds(32, 16), few_wide = rounds(32, 32), r64 = rounds(64, 64), r128 = rounds(128, 128), r256 = rounds(256, 256);
     const float cost[] = {few <= 1.f ? 3.6f + ks * (k <= 2048 ? 0.5f : 1.25f * std::max(few, 0.5f)) : 3.6f + few * (0.25f + 1.1f * ks),
                           4.2f + std::max(few_wide, 1.f) * (0.2f + 1.35f * ks), 3.f + std::max(r64, 1.f) * (0.5f + 1.75f * ks),
-                          3.f + std::ceil(r128) * (1.9f + 4.2f * ks), 3.f + std::ceil(r256) * (7.4f + 13.f * ks * (0.75f + 0.25f * std::min(r256, 1.f)))};
+                          4.6f + std::max(r128, 1.f) * (1.3f + 4.2f * ks), 3.f + std::ceil(r256) * (7.4f + 13.f * ks * (0.75f + 0.25f * std::min(r256, 1.f)))};
     int best = m <= FEW_MOST ? 0 : 2;
     for (int i = best + 1; i < 5; ++i)
         if (cost[i] < cost[best]) best = i;
