@@ -279,9 +279,10 @@ __global__ __launch_bounds__(WR *WC * 64, WR * FR == 4 ? 3 : 1) void gemm_i8_tok
 
 // ---- few tokens: a stream over the weights
 //
-// With up to 64 tokens the product reads n k bytes of weights and does little with each.  A workgroup owns 16 output columns (4096
-// columns: one workgroup a CU) and its 8 wavefronts split K, every eighth K-step each; a K-step of 16 columns is one 16-byte load a
-// lane, eight of them in flight from the first instruction on.  X, the type of the rows: TSX_TYPE_I8, or floats that the workgroup
+// There the product reads n k bytes of weights and does little with each.  A workgroup owns 16 NC output columns (4096 columns: one
+// workgroup a CU) and its 8 wavefronts split K, every eighth K-step each; a K-step of 16 columns is one 16-byte load a lane, AHEAD of them
+// in flight from the first instruction on (4096 columns, K = 4096, one row of bf16: 5.1 .. 6.8 us in the kernel, 16.8 MB, of which 2 are the
+// launch and 1 the first load's way; a call 6.3, which took 24 on tiles).  X, the type of the rows: TSX_TYPE_I8, or floats that the workgroup
 // quantizes itself while its weights are on their way (all of them do, out of the L2: one launch and its start less).  MT: groups of 16
 // tokens.  v_mfma_i32_16x16x64_i8: lane l supplies row (token or column) l % 16, K bytes 16 (l / 16) ..; accumulator r of lane l is
 // column 4 (l / 16) + r of token l % 16.  The eight partial sums meet in LDS.

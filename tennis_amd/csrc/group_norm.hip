@@ -3,6 +3,10 @@
 // A group is `d` consecutive channels of all pixels of one image: mean and variance over them, then
 // y = act((x - mean) / sqrt(variance + epsilon) * weight[c] + bias[c]).  Bound: HBM, one read and one write of the tensor.
 //
+// Two kernels, the statistics of chunks and the norm: 512 x 512 x 128 bf16 on 4 images, 268 MB, 45 and 82 us (6.0 and 6.5 TB/s: the second
+// finds part of its input in the caches); 64 x 64 x 320 fp16 on 8, 21 MB, 6.3 and 9.4 us, of which each has 2 of launch and about 2 of
+// prologue and reductions.
+//
 // Pixels are taken `rows` at a time: S pixels whose S * c values are whole pieces of 16 bytes (S = 1 where c is a multiple of a
 // piece), so that a thread that steps by whole rows keeps the channels of its piece, whatever c is, and a wavefront reads consecutive
 // bytes.  Sums of a channel are taken around the channel's first value that the thread sees: the difference of two large sums that
@@ -20,6 +24,7 @@ namespace {
 template <int TYPE, int V>
 __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_statistics_kernel(NormParams p) {
     extern __shared__ float entries[];                       // [lanes + 1][pitch] means, then squares
+    __shared__ float waves[NORM_MOST_THREADS / 64];
     constexpr int SIZE = Kind<TYPE>::SIZE;
     const int threads = blockDim.x, t = threadIdx.x, chunk = blockIdx.x, image = blockIdx.y;
     const int lanes = p.lanes ? p.lanes : 1, pixel_entries = p.c >> p.lg_run, run = 1 << p.lg_run;
@@ -117,11 +122,23 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_statistics_kerne
         }
     };
     const float of_values = __builtin_amdgcn_rcpf(chunk == p.chunks - 1 ? p.of_last : p.of_chunk);
-    for (int g = t >> p.lg_T; g < p.groups; g += threads >> p.lg_T) {      // T threads agree
+    // Over the T threads of a group: of one wavefront, or of several, then through LDS
+    auto sum_group = [&](float v) __attribute__((always_inline)) {
+        v = sum_over_lanes(v, p.lg_T);
+        if (T <= 64) return v;                             // uniform
+        __syncthreads();
+        if (t % 64 == 0) waves[t / 64] = v;
+        __syncthreads();
+        v = 0.f;
+        for (int w = 0; w < T / 64; ++w) v += waves[(t >> p.lg_T) * (T / 64) + w];
+        return v;
+    };
+    for (int g0 = 0; g0 < p.groups; g0 += threads >> p.lg_T) {
+        const int g = min(g0 + (t >> p.lg_T), p.groups - 1); // T threads agree; behind the last group: that one again, not stored
         float s = 0.f, n2 = 0.f, m2 = 0.f;
         const float about = means[(rows ? 0 : lanes * pitch) + g * group_entries];
         each(g, [&](int at, float ni) __attribute__((always_inline)) { s = __builtin_fmaf(ni, means[at] - about, s); });
-        s = sum_over_lanes(s, p.lg_T);
+        s = sum_group(s);
         const float mean = about + s * of_values;
         // around that mean, and what the values are off it on the whole (its rounding)
         each(g, [&](int at, float ni) __attribute__((always_inline)) {
@@ -129,10 +146,10 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_statistics_kerne
             n2 = __builtin_fmaf(ni, d, n2);
             m2 += __builtin_fmaf(ni * d, d, squares[at]);
         });
-        n2 = sum_over_lanes(n2, p.lg_T);
-        m2 = sum_over_lanes(m2, p.lg_T);
+        n2 = sum_group(n2);
+        m2 = sum_group(m2);
         const float shift = n2 * of_values;
-        if ((t & (T - 1)) == 0) p.partial[int64_t(image * p.groups + g) * p.chunks + chunk] = float2{mean + shift, __builtin_fmaf(-shift, n2, m2)};
+        if ((t & (T - 1)) == 0 && g == g0 + (t >> p.lg_T)) p.partial[int64_t(image * p.groups + g) * p.chunks + chunk] = float2{mean + shift, __builtin_fmaf(-shift, n2, m2)};
     }
 }
 
@@ -260,7 +277,9 @@ NormPlan plan_of(const tsx_group_norm *g) {
     p.lanes_magic = div_magic(side, int64_t(p.chunk_rows) + side);
     p.c_magic = div_magic(p.c, NORM_MOST_CHANNELS);
     p.d_magic = div_magic(d, NORM_MOST_CHANNELS);
-    p.lg_T = lg_threads(pl.threads, p.groups, (side + 1) * p.S * (d >> p.lg_run));
+    // as far as a group's threads have eight entries each (9 pixels x 809 channels in one group: a call 14 us, with 64 threads 22)
+    p.lg_T = lg_threads(pl.threads, p.groups, (side + 1) * p.S * (d >> p.lg_run) / 8, 9);
+    if (p.lg_T < 6) p.lg_T = lg_threads(pl.threads, p.groups, (side + 1) * p.S * (d >> p.lg_run));
     p.lg_TL = lg_threads(1 << p.lg_T, 1, side);
     p.lg_merge = lg_threads(pl.threads, p.groups, p.chunks);
     return pl;
@@ -292,7 +311,7 @@ int launch_statistics(const NormPlan &pl, hipStream_t stream) {
     const NormParams &p = pl.p;
     const size_t lds = size_t((p.lanes ? p.lanes : 1) + 1) * ((p.S * (p.c >> p.lg_run)) | 1) * 2 * sizeof(float);
     if (lds > 64 * 1024) {
-        const int rc = grant_lds(reinterpret_cast<const void *>(group_norm_statistics_kernel<TYPE, V>), 160 * 1024);
+        const int rc = grant_lds(reinterpret_cast<const void *>(group_norm_statistics_kernel<TYPE, V>), 136 * 1024);
         if (rc) return rc;
     }
     hipLaunchKernelGGL((group_norm_statistics_kernel<TYPE, V>), dim3(unsigned(p.chunks), unsigned(p.images)), dim3(pl.threads), lds, stream, p);

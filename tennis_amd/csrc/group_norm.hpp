@@ -40,10 +40,10 @@ int group_norm_tokens(const NormParams &p, int type, hipStream_t stream);
 // the norm in one launch, where that serves the call: *taken says whether
 int group_norm_held(const tsx_group_norm *g, const NormParams &p, hipStream_t stream, bool *taken);
 
-// Threads, as a power of two, that work on one group where `threads` share `groups` of `entries` each.
-inline int lg_threads(int threads, int groups, int entries) {
+// Threads, as a power of two and at most 2^most, that work on one group where `threads` share `groups` of `entries` each.
+inline int lg_threads(int threads, int groups, int entries, int most = 6) {
     int lg = 0;
-    while (lg < 6 && (groups << lg) < threads && (1 << lg) < entries) ++lg;
+    while (lg < most && (groups << lg) < threads && (1 << lg) < entries) ++lg;
     return lg;
 }
 

