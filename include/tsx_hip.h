@@ -233,7 +233,8 @@ int tsx_quantize_tokens(int64_t rows, int32_t cols, const void *x_dev, int32_t x
  * x_type TSX_TYPE_I8: x holds q, x_scales its scales, as tsx_quantize_tokens or tsx_group_norm_tokens_nhwc write them.  Another type:
  * the rows are quantized by the call, with the values of tsx_quantize_tokens (x_scales is not read).  Weights as
  * tsx_gemm_i8_pack_weights packs them; k is below 2^17, n below 2^24, m below 2^28 and may be 0.  The workspace (16-byte aligned, its contents written and read by
- * each call: calls that share one must not overlap) may be asked for as 0 bytes. */
+ * each call: calls that share one must not overlap) may be asked for as 0 bytes; how many goes by the sizes, x_type and the
+ * stride and alignment of x_dev. */
 typedef struct tsx_token_gemm {
     int32_t m, n, k;
     int32_t x_type, out_type;
@@ -258,6 +259,7 @@ int tsx_gemm_i8_tokens(const tsx_token_gemm *g, void *workspace_dev, size_t work
  *   nhwc         the result in x's type, dense [n][pixels][c] (may be x itself where that is dense)
  *   tokens_nhwc  the result (as fp32, before any rounding) as int8 tokens, a pixel a token: q dense [n][pixels][c],
  *                scales [n][pixels], with the rule of tsx_quantize_tokens
+ * Statistics are fp32: where epsilon and the variance are both 0, or the sum of the squared deviations leaves fp32, so does the result.
  * The workspace (8-byte aligned) is written and read by each call: calls that share one must not overlap. */
 typedef struct tsx_group_norm {
     int32_t n, c, groups;

@@ -297,7 +297,6 @@ struct FewTokens : TokenGemmParams {
 
 template <int X, int MT, int NC, int AHEAD, int OUT>
 __global__ __launch_bounds__(FEW_THREADS) void gemm_i8_few_tokens_kernel(FewTokens p) {
-    typedef int v4i_ __attribute__((ext_vector_type(4)));
     extern __shared__ __attribute__((aligned(16))) int8_t lds[];      // [8][MT][NC][4][64] partial sums, then the rows
     __shared__ float scales[16 * MT];
     __shared__ unsigned tops[FEW_WAVES];
@@ -312,11 +311,11 @@ __global__ __launch_bounds__(FEW_THREADS) void gemm_i8_few_tokens_kernel(FewToke
         w[decltype(nc)::value] = p.wp + int64_t(c >> 1) * 2048 + (piece >> 1) * 1024 + (16 * (c & 1) + row + 32 * (piece & 1)) * 16;
     });
     const int64_t w_step = int64_t(p.frags) * 2048;
-    v4i_ a[AHEAD][NC];
+    v4i a[AHEAD][NC];
     auto fetch = [&](int first) __attribute__((always_inline)) {
         static_for<0, AHEAD>([&](auto uc) {
             constexpr int u = decltype(uc)::value;
-            static_for<0, NC>([&](auto nc) { a[u][decltype(nc)::value] = *reinterpret_cast<const v4i_ *>(w[decltype(nc)::value] + min(first + FEW_WAVES * u, p.ksteps - 1) * w_step); });
+            static_for<0, NC>([&](auto nc) { a[u][decltype(nc)::value] = *reinterpret_cast<const v4i *>(w[decltype(nc)::value] + min(first + FEW_WAVES * u, p.ksteps - 1) * w_step); });
         });
     };
     fetch(wave);
@@ -374,18 +373,18 @@ __global__ __launch_bounds__(FEW_THREADS) void gemm_i8_few_tokens_kernel(FewToke
     } else {
         if (threadIdx.x < 16 * MT) scales[threadIdx.x] = p.x_scales[min(row0 + int(threadIdx.x), p.m - 1)];
     }
-    v4i_ acc[MT][NC];
-    static_for<0, MT * NC>([&](auto mc) { acc[decltype(mc)::value / NC][decltype(mc)::value % NC] = v4i_{0, 0, 0, 0}; });
+    v4i acc[MT][NC];
+    static_for<0, MT * NC>([&](auto mc) { acc[decltype(mc)::value / NC][decltype(mc)::value % NC] = v4i{0, 0, 0, 0}; });
     for (int first = wave; first < p.ksteps; first += FEW_WAVES * AHEAD) {
-        v4i_ b[AHEAD][MT];
+        v4i b[AHEAD][MT];
         static_for<0, AHEAD>([&](auto uc) {
             constexpr int u = decltype(uc)::value;
             const int k = min(first + FEW_WAVES * u, p.ksteps - 1) * KSTEP + piece * 16;
             static_for<0, MT>([&](auto mc) {
                 constexpr int i = decltype(mc)::value;
                 const int token = min(row0 + 16 * i + row, p.m - 1);
-                if constexpr (X == TSX_TYPE_I8) b[u][i] = *reinterpret_cast<const v4i_ *>(p.q + token * p.pitch + (k < p.k ? k : 0));
-                else b[u][i] = *reinterpret_cast<const v4i_ *>(rows + token * pitch + k);
+                if constexpr (X == TSX_TYPE_I8) b[u][i] = *reinterpret_cast<const v4i *>(p.q + token * p.pitch + (k < p.k ? k : 0));
+                else b[u][i] = *reinterpret_cast<const v4i *>(rows + token * pitch + k);
             });
         });
         static_for<0, AHEAD>([&](auto uc) {
@@ -502,7 +501,7 @@ TokenKernel choose(int m, int n, int k) {
 template <int OUT>
 int launch(const tsx_token_gemm *g, const TokenGemmParams &p, bool quantizes, hipStream_t stream) {
     if (quantizes) return few_tokens<OUT>(g, p, true, false, stream);
-    // TSX_TOKENS_KERNEL: that kernel, by its place in the list above, whatever the call (tests, measurements)
+    // TSX_TOKENS_KERNEL: that kernel, by its place in the list above, for any call it can take (tests, measurements)
     const char *e = std::getenv("TSX_TOKENS_KERNEL");
     const bool named = e && e[0] >= (p.m <= FEW_MOST ? '0' : '2') && e[0] <= '4';
     switch (named ? TokenKernel(e[0] - '0') : choose(p.m, p.n, p.k)) {

@@ -98,11 +98,6 @@ __device__ __forceinline__ void merge_chunks(const NormParams &p, int image, flo
 template <int TYPE, int V>
 struct Piece {
     float v[V];
-    __device__ __forceinline__ void load(const char *image, int64_t at) {
-        Run<TYPE, V> r;
-        r.load(image + at * Kind<TYPE>::SIZE);
-        static_for<0, V>([&](auto ec) { v[decltype(ec)::value] = r.template get<decltype(ec)::value>(); });
-    }
     __device__ __forceinline__ void load_some(const char *image, int64_t at, int left) {
         Run<TYPE, V> r;
         r.load_some(image + at * Kind<TYPE>::SIZE, left);
