@@ -431,7 +431,8 @@ def norm64(x, groups, weight, bias, eps, act):
 NORMS = [((2, 8, 8, 1280), 32), ((1, 1, 1, 32), 8), ((3, 1, 64), 64), ((2, 5, 7, 30), 3), ((1, 37, 29, 15), 5), ((4, 33, 10), 1), ((2, 16, 16, 320), 32),
          ((1, 64, 48, 96), 32), ((5, 3, 3, 7), 7), ((2, 100, 1), 1), ((3, 17, 2), 2), ((1, 9, 9, 2560), 32), ((2, 4, 4, 4096), 32), ((1, 6, 8191), 1),
          ((1, 300, 1030), 10), ((2, 12), 4), ((1, 128, 128, 128), 32), ((20, 40, 24), 6), ((1, 3, 5000), 8), ((2, 11, 13, 1025), 5), ((1, 70, 50, 3), 1), ((1, 3, 3, 809), 1), ((3, 9, 9, 51), 1),
-         ((8, 10, 10, 7), 1), ((1, 89, 89, 1059), 3), ((2, 5, 127, 138), 2), ((1, 2, 2, 8190), 3)]
+         ((8, 10, 10, 7), 1), ((1, 89, 89, 1059), 3), ((2, 5, 127, 138), 2), ((1, 2, 2, 8190), 3),
+         ((1, 2, 8192), 8192), ((2, 3, 8192), 4096), ((1, 40, 8192), 1)]
 
 
 @pytest.mark.parametrize("name", TYPES)
