@@ -9,9 +9,12 @@
 //
 // Pixels are taken `rows` at a time: S pixels whose S * c values are whole pieces of 16 bytes (S = 1 where c is a multiple of a
 // piece), so that a thread that steps by whole rows keeps the channels of its piece, whatever c is, and a wavefront reads consecutive
-// bytes.  Sums of a channel are taken around the channel's first value that the thread sees: the difference of two large sums that
-// would cancel never forms, since the value itself is part of the variance that the error is measured by.  Partial results are
-// merged as (count, mean, squares around the mean), in an order that the sizes fix.
+// bytes.  Sums of a channel are taken around its mean so far, which is brought up to date after 8, 16, 32, 64 rows and every 64 from there on:
+// a batch is no longer than what came before it, so at most half of its squares cancels (of the first eight, around the first value, seven
+// eighths).  Sums around one value for all n rows of a thread leave 1 / n of the squares where that value is far from the rest: with 1000 ahead
+// of 1000 small ones the norm was off by a hundredth.  Of a mean's update what its rounding drops is kept, since it would add up where an image
+// grows along its rows.  This takes 0.4 us (64 x 64 x 320).  Partial results are merged as (count, mean, squares around the mean), in an order
+// that the sizes fix.
 #include <algorithm>
 
 #include "group_norm.hpp"
@@ -59,45 +62,56 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_statistics_kerne
         if (lane < lanes && j < p.pieces) {
             const char *at = x + int64_t(first + lane) * p.row_bytes + j * (V * SIZE);
             const int count = full + (lane < over ? 1 : 0);
-            // Requests of a batch leave together; the last one reads its last row again in the place of those that are none.
-            constexpr int AHEAD = 8;
-            typedef Run<TYPE, V> Values;
-            Values v[AHEAD];
+            // Requests of eight rows leave together; in the place of those that are none the last one is read again.
+            constexpr int AHEAD = 8, LONGEST = 64;
+            Run<TYPE, V> v[AHEAD];
             auto fetch = [&](int left) __attribute__((always_inline)) {
                 static_for<0, AHEAD>([&](auto uc) { v[decltype(uc)::value].load(at + min(decltype(uc)::value, left - 1) * p.step_bytes); });
             };
-            float base[V], sum[V], square[V];
-            static_for<0, V>([&](auto ec) { base[decltype(ec)::value] = sum[decltype(ec)::value] = square[decltype(ec)::value] = 0.f; });
+            // mean + low and the squares around it of the `closed` rows so far; sums and squares of the differences from `mean` since
+            float mean[V], low[V], square[V], sum[V], around[V];
             auto take = [&](auto uc) __attribute__((always_inline)) {
                 static_for<0, V>([&](auto ec) {
                     constexpr int e = decltype(ec)::value;
-                    const float d = v[decltype(uc)::value].template get<e>() - base[e];
+                    const float d = v[decltype(uc)::value].template get<e>() - mean[e];
                     sum[e] += d;
-                    square[e] = __builtin_fmaf(d, d, square[e]);
+                    around[e] = __builtin_fmaf(d, d, around[e]);
+                });
+            };
+            auto close = [&](int closed, int rows) __attribute__((always_inline)) {
+                const float n = float(closed), of_rows = __builtin_amdgcn_rcpf(float(rows));      // within a step: moves the mean by that much of its step
+                static_for<0, V>([&](auto ec) {
+                    constexpr int e = decltype(ec)::value;
+                    const float nl = n * low[e], s = sum[e] + nl, step = s * of_rows, moved = mean[e] + step;
+                    square[e] += __builtin_fmaf(-step, s, __builtin_fmaf(nl, low[e], around[e]));
+                    low[e] = step - (moved - mean[e]);
+                    mean[e] = moved;
+                    sum[e] = around[e] = 0.f;
                 });
             };
             int left = count;
-            if (left > 0) {
-                fetch(left);
-                static_for<0, V>([&](auto ec) { base[decltype(ec)::value] = v[0].template get<decltype(ec)::value>(); });
-            }
-            while (left > AHEAD) {
+            if (left > 0) fetch(left);
+            static_for<0, V>([&](auto ec) {
+                constexpr int e = decltype(ec)::value;
+                mean[e] = left > 0 ? v[0].template get<e>() : 0.f;
+                low[e] = square[e] = sum[e] = around[e] = 0.f;
+            });
+            int closed = 0, end = AHEAD;                     // the next batch's: as many rows as all before, at most LONGEST
+            for (int rows = AHEAD; left > AHEAD; rows += AHEAD) {
                 static_for<0, AHEAD>(take);
                 at += AHEAD * p.step_bytes;
                 left -= AHEAD;
                 fetch(left);
+                if (rows == end) {                           // uniform
+                    close(closed, rows);
+                    closed = rows;
+                    end += min(rows, LONGEST);
+                }
             }
             static_for<0, AHEAD>([&](auto uc) { if (decltype(uc)::value < left) take(uc); });
-            const float of_count = __builtin_amdgcn_rcpf(float(max(count, 1)));      // within a step: moves the mean by that much of the sum
-            static_for<0, V>([&](auto ec) {
-                constexpr int e = decltype(ec)::value;
-                const float m = sum[e] * of_count;
-                // squares around base + m, whatever m is
-                square[e] = fmaxf(__builtin_fmaf(m, __builtin_fmaf(m, float(count), -2.f * sum[e]), square[e]), 0.f);
-                base[e] += m;
-            });
-            join(base, square, float(count));
-            leave(lane, j, base, square);
+            if (count > 0) close(closed, count);
+            join(mean, square, float(count));
+            leave(lane, j, mean, square);
             if (lane == 0 && tail) {
                 Piece<TYPE, V> a;
                 static_for<0, V>([&](auto ec) { a.v[decltype(ec)::value] = square[decltype(ec)::value] = 0.f; });
