@@ -1,5 +1,5 @@
-"""Statistics of the channels-last group norm where fp32 sums lose them: means far from zero, single values far from the
-rest, means that drift along an image; on images of up to a thousand pixels a thread, in one launch and in two, with their definition in
+"""Statistics of the channels-last group norm where fp32 sums lose them: means far from zero, single values and blocks of pixels far from
+the rest, means that drift along an image; on images of up to a thousand pixels a thread, in one launch and in two, with their definition in
 64 bits.
 
 Bars.  u = 2^-24 is half a step of fp32 relative to the value.  Ahead of the rounding to the output's type, (x - mean) r is off by
@@ -50,6 +50,8 @@ def image(torch, kind, shape, groups, name):
         x += 1000.0
     elif kind == "drift":
         x = x * 0.03 + 1000.0 + torch.linspace(0, 1, pixels, device="cuda").view(1, -1, 1, 1)
+    elif kind == "block":        # of pixels: what a chunk of them has, or less
+        x[:, :max(1, pixels // 256)] += 1000.0
     elif kind == "outlier":      # in front of zeros, of small values and of a constant
         for k in range(groups):
             if k % 3 == 0:
@@ -80,7 +82,7 @@ SHAPES = [((1, 2048, 2048, 128), 32), ((300, 64, 64, 64), 8), ((1, 300, 512, 102
           ((1, 9000, 320), 32), ((2, 40, 40, 16), 4), ((2, 8, 8, 1280), 32)]
 
 
-@pytest.mark.parametrize("kind", ["normal", "far", "drift", "outlier"])
+@pytest.mark.parametrize("kind", ["normal", "far", "drift", "block", "outlier"])
 @pytest.mark.parametrize("name", ["f32", "bf16"])
 @pytest.mark.parametrize("shape,groups", SHAPES)
 def test_statistics(torch, capi, shape, groups, name, kind):
