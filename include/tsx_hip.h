@@ -259,7 +259,9 @@ int tsx_gemm_i8_tokens(const tsx_token_gemm *g, void *workspace_dev, size_t work
  *   nhwc         the result in x's type, dense [n][pixels][c] (may be x itself where that is dense)
  *   tokens_nhwc  the result (as fp32, before any rounding) as int8 tokens, a pixel a token: q dense [n][pixels][c],
  *                scales [n][pixels], with the rule of tsx_quantize_tokens
- * Statistics are fp32: where epsilon and the variance are both 0, or the sum of the squared deviations leaves fp32, so does the result.
+ * Statistics are fp32.  Where epsilon and the variance are both 0 the result is infinite or NaN.  Where the count of a group's values times
+ * the square of the largest leaves fp32 (3.4e38: values from some 10^15 on in large groups) its statistics may: then the group is NaN, and what
+ * the activation makes of that.
  * The workspace (8-byte aligned) is written and read by each call: calls that share one must not overlap. */
 typedef struct tsx_group_norm {
     int32_t n, c, groups;

@@ -64,6 +64,13 @@ __device__ __forceinline__ float reciprocal_root(float v) {
     return __fmul_rn(__builtin_amdgcn_rsqf(tiny ? __fmul_rn(v, 0x1p100f) : v), tiny ? 0x1p50f : 1.f);
 }
 
+// 1 / sqrt(variance + epsilon) of an image's group.  Squares that left fp32, of which an infinity or a NaN is left, make it NaN: 1 / infinity
+// would make the group its bias.
+__device__ __forceinline__ float root_of(float squares, const NormParams &p) {
+    const float r = reciprocal_root(__builtin_fmaf(fmaxf(squares, 0.f), p.of_image, p.epsilon));
+    return squares < __builtin_inff() ? r : __builtin_nanf("");
+}
+
 // Mean and 1 / sqrt(variance + epsilon) of the groups of one image, into LDS, from the chunks' means and squares, in one pass around
 // the average of the means that a group's threads request first, 4 T of them or all.  n_k (mean_k - average)^2 is part of the variance but for
 // the average's own distance from the mean, of which a chunk far from the rest makes a (4 T)-th of its distance at most: what cancels is within
@@ -97,9 +104,8 @@ __device__ __forceinline__ void merge_chunks(const NormParams &p, int image, flo
         }
         s = sum_over_lanes(s, lg);
         m2 = sum_over_lanes(m2, lg);
-        const float shift = s * p.of_image, variance = fmaxf(__builtin_fmaf(-shift, s, m2), 0.f) * p.of_image;
-        // a NaN among the squares stays one (fmaxf drops it)
-        if (t == 0) group[g] = float2{about + shift, reciprocal_root((m2 == m2 ? variance : m2) + p.epsilon)};
+        const float shift = s * p.of_image;
+        if (t == 0) group[g] = float2{about + shift, root_of(__builtin_fmaf(-shift, s, m2), p)};
     }
 }
 

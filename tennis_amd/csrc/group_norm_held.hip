@@ -109,9 +109,8 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_held_kernel(Held
     __syncthreads();
     const float2 total = gather(true);
     if (tg == 0 && g < p.B) {
-        const float shift = total.x * of_count, squares = __builtin_fmaf(-shift, total.x, total.y);
-        // a NaN stays one (fmaxf drops it)
-        group[g] = float2{rough + shift, reciprocal_root((squares == squares ? fmaxf(squares, 0.f) * of_count : squares) + p.epsilon)};
+        const float shift = total.x * of_count;
+        group[g] = float2{rough + shift, root_of(__builtin_fmaf(-shift, total.x, total.y), p)};
     }
     __syncthreads();
     if (!mine) return;

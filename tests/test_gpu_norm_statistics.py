@@ -111,3 +111,29 @@ def test_statistics_of_many_images(torch, capi):
         assert torch.equal(got[0], got[255])
         off = (got[0].double() - want[i]).abs() - (error[i] * (1 + h) + h * want[i].abs() + TINY["bf16"])
         assert float(off.max()) <= 0
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("shape,groups", [((2, 8, 8, 64), 8), ((2, 130, 130, 16), 4), ((2, 40, 40, 15), 5), ((300, 64, 64, 64), 8)])
+def test_statistics_that_leave_fp32(torch, capi, shape, groups, name):
+    """A group whose squares leave fp32 is NaN, in one launch and in two, and nothing finite in its place; the others do not notice.  Up to there
+    the norm is that of smaller values."""
+    x = image(torch, "normal", shape, groups, name)
+    d = shape[-1] // groups
+    bias = torch.linspace(-1, 1, shape[-1], device="cuda")
+    want, (q, s) = capi.group_norm(x, groups, None, bias), capi.group_norm_tokens(x, groups)
+    for size in (1e20, 1e25, 1e30, 1e37):
+        y = x.clone()
+        y[1, ..., d:2 * d] *= size
+        got = capi.group_norm(y, groups, None, bias)
+        assert got[1, ..., d:2 * d].isnan().all()
+        got[1, ..., d:2 * d] = want[1, ..., d:2 * d]
+        assert torch.equal(got, want)
+        qt, st = capi.group_norm_tokens(y, groups)
+        assert (qt[1] == 0).all() and st[1].isnan().all() and torch.equal(qt[0], q[0]) and torch.equal(st[0], s[0])
+    # 67600 squares of at most (6e15)^2 are within 3.4e38
+    y = x * 1e15
+    want, error = norm64(torch, y, groups, 1e-5, "normal")
+    got = capi.group_norm(y, groups)
+    h = torch.finfo(x.dtype).eps / 2
+    assert float(((got.double() - want).abs() - (error * (1 + h) + h * want.abs() + TINY[name])).max()) <= 0
