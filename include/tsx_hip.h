@@ -216,7 +216,8 @@ int tsx_gemm_i8(int32_t m, int32_t n, int32_t k, const int8_t *a_dev, const void
 #define TSX_TYPE_F16  1
 #define TSX_TYPE_BF16 2
 #define TSX_TYPE_I8   3   /* where a call says so */
-/* x / (1 + exp(-x)), on the hardware's exponential and reciprocal; only in the calls on tokens and in the group norm, which take
+/* x / (1 + exp(-x)), on the hardware's exponential and reciprocal, within 8 2^-24 of itself where the result is fp32 and (8 + |x|) 2^-24
+ * ahead of another type's rounding (below -87, where it is less than 10^-35, it may be 0); only in the calls on tokens and in the group norm, which take
  * TSX_ACT_NONE, _RELU, _LEAKY_RELU, _MISH_FAST and this (the exact Mish is the host's bits for a given fp32 number: there is
  * none to match here).  A negative zero and a NaN become 0 under ReLU, a NaN 0 under LeakyReLU, as in the activations' SIMD body: so does
  * what a row or a group with a NaN gives. */

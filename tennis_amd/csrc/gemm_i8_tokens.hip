@@ -58,7 +58,7 @@ __device__ __forceinline__ Run<OUT, 16> fragment_values(const TokenGemmParams &p
         constexpr int g = decltype(gc)::value;
         static_for<0, 4>([&](auto jc) { constexpr int j = decltype(jc)::value; v[4 * g + j] = __fadd_rn(__fmul_rn(__fmul_rn(float(acc[4 * g + j]), of.scale[g][j]), xs), of.bias[g][j]); });
     });
-    activate_as<ACT>(v, p.slope);
+    activate_as<OUT, ACT>(v, p.slope);
     Run<OUT, 16> to, own;
     own.set(v);
     constexpr int W = Run<OUT, 4>::WORDS;      // words of four values
@@ -410,7 +410,7 @@ __global__ __launch_bounds__(FEW_THREADS) void gemm_i8_few_tokens_kernel(FewToke
         for (int i = 0; i < FEW_WAVES; ++i) sum += sums[((i * MT * NC + token / 16 * NC + in / 16) * 4 + in % 4) * 64 + token % 16 + 16 * (in % 16 / 4)];
         float v[1] = {__fmul_rn(__fmul_rn(float(sum), p.w_scales[col]), scales[token])};
         if (p.bias) v[0] = __fadd_rn(v[0], p.bias[col]);
-        activate_tokens(v, p.act, p.slope);
+        activate_tokens<OUT>(v, p.act, p.slope);
         Run<OUT, 1> out;
         out.set(v);
         out.store(static_cast<char *>(p.out) + ((row0 + token) * p.out_stride + col) * (OUT == TSX_TYPE_F32 ? 4 : 2));

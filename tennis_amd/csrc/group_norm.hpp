@@ -191,8 +191,8 @@ struct Affine {
     template <int ACT, int TYPE>
     __device__ __forceinline__ void apply(int act, float slope, Piece<TYPE, V> &a) const {
         static_for<0, V>([&](auto ec) { constexpr int e = decltype(ec)::value; a.v[e] = __builtin_fmaf(a.v[e] - mean[e], scale[e], shift[e]); });
-        if constexpr (ACT == ANY_ACT) activate_tokens(a.v, act, slope);
-        else activate_as<ACT>(a.v, slope);
+        if constexpr (ACT == ANY_ACT) activate_tokens<TYPE>(a.v, act, slope);
+        else activate_as<TYPE, ACT>(a.v, slope);
     }
 };
 

@@ -81,8 +81,8 @@ __global__ __launch_bounds__(256) void group_norm_tokens_kernel(NormParams p) {
                           b = *reinterpret_cast<const v4f *>(shifts + j * V + h);
                 static_for<0, 4>([&](auto ec) { constexpr int e = decltype(ec)::value; y[i][h + e] = __builtin_fmaf(in[i].template get<h + e>() - m[e], a[e], b[e]); });
             });
-            if constexpr (ACT == ANY_ACT) activate_tokens(y[i], p.act, p.slope);
-            else activate_as<ACT>(y[i], p.slope);
+            if constexpr (ACT == ANY_ACT) activate_tokens<TSX_TYPE_I8>(y[i], p.act, p.slope);
+            else activate_as<TSX_TYPE_I8, ACT>(y[i], p.slope);
             if (l + i * L < pieces - 1 || (l + i * L == pieces - 1 && width == p.c))
                 static_for<0, V>([&](auto ec) { top = max(top, __builtin_bit_cast(unsigned, y[i][decltype(ec)::value]) & 0x7fffffffu); });
             else if (l + i * L < pieces)
