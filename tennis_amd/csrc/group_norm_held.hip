@@ -150,9 +150,16 @@ HeldPlan held_plan(const tsx_group_norm *g, const NormParams &rows) {
     float best_cost = 10.f + 0.28e-6f * float(g->n) * float(g->pixels) * float(g->c) * size;
     if (g->pixels > 16384) return best;
     const int pixels = int(g->pixels), d = g->c / g->groups, whole = g->type == TSX_TYPE_F32 ? 4 : 8;
+    // The divisors of the groups in ascending order, looked for up to their root: each B up to 8192 for itself was 10 .. 50 us of the call.
+    int divisors[64], count = 0, root = 1;                   // no number up to NORM_MOST_CHANNELS has more than 64
+    for (; root * root <= g->groups; ++root)
+        if (g->groups % root == 0) divisors[count++] = root;
+    for (int i = count - 1; i >= 0; --i)
+        if (divisors[i] * divisors[i] != g->groups) divisors[count++] = g->groups / divisors[i];
     for (int V = whole; V >= 2; V /= 2)
-        for (int B = 1; B <= g->groups; ++B) {
-            if (g->groups % B || B * d % V) continue;
+        for (int i = 0; i < count; ++i) {
+            const int B = divisors[i];
+            if (B * d % V) continue;
             const int a_pixel = B * d / V;
             if (a_pixel > NORM_MOST_THREADS) break;
             const int most = V == 8 ? 12 : g->type == TSX_TYPE_F32 && V == 4 ? 16 : 24;      // what 128 registers hold beside the rest
