@@ -599,7 +599,9 @@ class GemmI8:
 
 
 # ---------------------------------------------------------------- tokens and channels-last tensors
-# Tensors of fp32, fp16 or bf16 values on one device, taken at their strides; the calls run on the current stream of that device.
+# Tensors of fp32, fp16 or bf16 values on one device, taken at their strides where the last axis is dense and the others are one axis of
+# rows (of a norm: images, and one axis of pixels); others are copied first, by torch: NCHW tensors permuted are.  The calls run on the
+# current stream of that device.
 # They allocate their workspace for the call, so calls on several streams or in several captured graphs share none.  Results carry
 # no gradient.
 
@@ -765,7 +767,8 @@ def _group_norm(x, groups, weight, bias, epsilon, act, slope, tokens):
 
 def group_norm(x, groups, weight=None, bias=None, epsilon=1e-5, act=None, slope=0.0):
     """tsx_group_norm_nhwc: group norm and an activation on channels-last x [n, ..., c] in fp32, fp16 or bf16 (a tensor of torch's
-    channels_last format is one as x.permute(0, 2, 3, 1)); weight and bias [c].  Returns a dense tensor of x's shape and type."""
+    channels_last format is one as x.permute(0, 2, 3, 1); of a dense NCHW tensor that is copied first); weight and bias [c].  Returns a
+    dense tensor of x's shape and type."""
     return _group_norm(x, groups, weight, bias, epsilon, act, slope, False)
 
 

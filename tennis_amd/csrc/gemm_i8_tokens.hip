@@ -99,8 +99,9 @@ __device__ __forceinline__ void wait_for_all_but() { asm volatile("s_waitcnt vmc
 // WR x WC wavefronts, each with FR x FC fragments of 32 tokens x 32 columns; S chunks of KS K-steps in LDS.
 //
 // Bound: the matrix cores where K is long.  256 x 256, K in chunks of 64, four of them on their way: a chunk's 64 multiplications of a
-// wavefront take 2048 cycles of its SIMD and 24 LDS reads; 4096^3 62 us, 8192^3 445 us (2.2 and 2.5 P operations/s; the library's plain
-// int8 product 69 and 432), where the card holds its power by a clock of 1.5 .. 1.7 GHz.  Where K is short, its start and its outputs,
+// wavefront take 2048 cycles of its SIMD and 24 LDS reads.  On int8 tokens, 20 calls in a row, the means of ten such rows: 4096^3 59 .. 67 us,
+// 8192^3 422 .. 432 (2.3 and 2.6 P operations/s; the library's plain int8 product 63 .. 69 and 422), where the card holds its power by a clock of
+// 1.5 .. 1.7 GHz; in a trace, each behind rows that become int8, 65 and 498 (440 at the least).  Where K is short, its start and its outputs,
 // which wait for no other tile's arithmetic on the same CU: 32768 x 960, K = 320 25 us, of which 12 are the two turns' epilogues.  Tiles
 // of 128: three of them a CU in 168 registers, which fill each other's waits (two of them: 29 us for 25, 131072 x 512, K = 128 37 for 29).
 // Requests to memory fill LDS past the registers, and a wavefront waits for all but the newest chunks' of them.

@@ -3,8 +3,8 @@
 // A group is `d` consecutive channels of all pixels of one image: mean and variance over them, then
 // y = act((x - mean) / sqrt(variance + epsilon) * weight[c] + bias[c]).  Bound: HBM, one read and one write of the tensor.
 //
-// Two kernels, the statistics of chunks and the norm: 512 x 512 x 128 bf16 on 4 images, 268 MB, 45 and 82 us (6.0 and 6.5 TB/s: the second
-// finds part of its input in the caches); 64 x 64 x 320 fp16 on 8, 21 MB, 6.3 and 9.4 us, of which each has 2 of launch and about 2 of
+// Two kernels, the statistics of chunks and the norm, the least of 24 launches: 512 x 512 x 128 bf16 on 4 images, 268 MB, 45 and 81 us (6.0 and
+// 6.6 TB/s: the second finds part of its input in the caches); 64 x 64 x 320 fp16 on 8, 21 MB, 7.4 and 9.8 us, of which each has 2 of launch and about 2 of
 // prologue and reductions.
 //
 // Pixels are taken `rows` at a time: S pixels whose S * c values are whole pieces of 16 bytes (S = 1 where c is a multiple of a
@@ -170,7 +170,7 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_statistics_kerne
 // ---- the norm itself: a part of a chunk's rows
 
 // STREAMS: the output goes past the caches, which then keep more of what the statistics read (four images of 512 x 512 x 128 bf16, 268 MB:
-// 159 us without, 136 with; one of them, 67 MB: 42 and 40).
+// 156 us without, 132 with; one of them, 67 MB: 42 and 40).
 template <int TYPE, int V, int ACT, bool STREAMS>
 __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_apply_kernel(NormParams p) {
     extern __shared__ float2 group[];
@@ -235,8 +235,8 @@ __global__ __launch_bounds__(NORM_MOST_THREADS) void group_norm_apply_kernel(Nor
 // ---- host side
 
 // One workgroup of 512 threads a CU: with more, each has its prologue and its reductions, and the caches hold more streams.  us (bf16) at
-// 256, 512 and 2048 workgroups: 16384 pixels x 128 channels on 4 images 15.7, 17.8 and 17.9, 65536 x 64 on 2 16.6, 19.8 and 19.8, 262144 x
-// 128 on 4 133, 138 and 141; 256 workgroups of 1024 threads: 16.5, 17, 142, and 16384 x 128 on 1 14 where 512 threads take 11.9.
+// 256, 512 and 2048 workgroups: 16384 pixels x 128 channels on 4 images 15.8, 17.4 and 17.4, 65536 x 64 on 2 16.4, 18.9 and 18.7, 262144 x
+// 128 on 4 132, 137 and 140; 256 workgroups of 1024 threads: 16.3, 16.9, 144, and 16384 x 128 on 1 13.6 where 512 threads take 11.0.
 constexpr int NORM_THREADS = 512, NORM_WORKGROUPS = 256, MOST_CHUNKS = 256;
 
 // Rows, threads and chunks of a call; V: values of a piece (1: a channel a thread, for pixels apart that are no whole pieces).

@@ -2,7 +2,7 @@
 //
 // A workgroup takes B groups of one image, B * d channels of every pixel: whole pieces of V values.  Its threads hold them from the one
 // read to the one write; in between the mean, as the sum over all of them, and then the sums of x - mean and of its square, whose first
-// corrects the mean's rounding.  Two kernels read the tensor twice and wait for each other: 8 x 8 x 1280 on 2 images 10.2 us there, 6.3 here.
+// corrects the mean's rounding.  Two kernels read the tensor twice and wait for each other: 8 x 8 x 1280 on 2 images 9.8 us there, 5.2 here.
 #include <algorithm>
 
 #include "group_norm.hpp"
@@ -137,8 +137,8 @@ int power_of_two(int v) {      // the next one up
 // Whether the one-launch kernel takes the call, on which pieces and threads (V = 0: it does not), by estimates of the times in us, fitted
 // to bf16 with SiLU.  Here a workgroup's own values take their time, and all workgroups' that of the cache lines they share with one
 // another (runs of less than 40 bytes at a pixel cost as much as 40).  Two kernels: two starts and the tensor's bytes.  Measured, one launch
-// and two: 64 pixels x 1280 channels on 2 images 6.3 and 10.2, on 32 images 7.3 and 11.1; 1024 x 640 on 8 10.8 and 13.1, on 32 27.9 and 26.3;
-// 4096 x 320 (groups of 10: runs of 20 bytes) on 1 21.4 and 11.8, on 8 21.8 and 17.5; 4096 x 128 on 1 9.6 and 10.3, on 16 18.4 and 14.7.
+// and two: 64 pixels x 1280 channels on 2 images 5.2 and 9.8, on 32 images 6.9 and 10.8; 1024 x 640 on 8 10.5 and 13.0, on 32 26.6 and 26.3;
+// 4096 x 320 (groups of 10: runs of 20 bytes) on 1 21.5 and 11.4, on 8 21.2 and 17.7; 4096 x 128 on 1 9.4 and 10.0, on 16 18.1 and 15.7.
 struct HeldPlan {
     HeldParams p;
     int V, NP, threads;

@@ -1,6 +1,6 @@
 // The group norm's values as int8 tokens: a pixel's largest value decides its scale, so a pixel stays with one wavefront.
 //
-// Bound: HBM, one read and half of a write behind the statistics' read: 64 x 64 x 320 bf16 on 8 images 10 us behind 7, as much by the
+// Bound: HBM, one read and half of a write behind the statistics' read: 64 x 64 x 320 bf16 on 8 images 10.2 us behind 7.6 at the least, as much by the
 // prologue (the vectors into LDS, the chunks' statistics) as by its 31 MB.
 //
 // L lanes of a wavefront share a pixel, each with P pieces of eight of its channels, which they hold from the load to the store.
@@ -12,8 +12,8 @@
 namespace tsx {
 namespace {
 
-// us (bf16) at 512 and 1024: 262144 pixels x 128 channels on 2 images 82 and 76, 1024 x 640 on 32 28.4 and 27.3, 4096 x 320 on 8 18.8 and 18.9;
-// at 2048 the second takes 38
+// us (bf16) at 512, 1024 and 2048: 262144 pixels x 128 channels on 2 images 82.7, 73.2 and 75.0, 1024 x 640 on 32 27.7, 26.3 and 28.7, 4096 x 320
+// on 8 18.4, 18.3 and 18.4
 constexpr int TOKENS_WORKGROUPS = 1024;
 
 template <int TYPE, int L, int P, int ACT>
