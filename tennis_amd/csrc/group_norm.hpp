@@ -74,7 +74,7 @@ __device__ __forceinline__ float root_of(float squares, const NormParams &p) {
 // Mean and 1 / sqrt(variance + epsilon) of the groups of one image, into LDS, from the chunks' means and squares, in one pass around
 // the average of the means that a group's threads request first, 4 T of them or all.  n_k (mean_k - average)^2 is part of the variance but for
 // the average's own distance from the mean, of which a chunk far from the rest makes a (4 T)-th of its distance at most: what cancels is within
-// chunks / (4 T)^2 times the variance, 16 for one thread a group and less than one from four threads on.  (Around one chunk's mean it is `chunks`
+// chunks / (4 T)^2 times the variance, 16 for one thread a group and at most one from four threads on.  (Around one chunk's mean it is `chunks`
 // times the variance where that chunk is the far one.  A second pass instead, around the mean, takes 0.2 us more.)
 __device__ __forceinline__ void merge_chunks(const NormParams &p, int image, float2 *group) {
     const int lg = p.lg_merge, T = 1 << lg, t = threadIdx.x & (T - 1);
