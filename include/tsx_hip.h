@@ -253,6 +253,80 @@ typedef struct tsx_token_gemm {
 size_t tsx_gemm_i8_tokens_workspace_bytes(const tsx_token_gemm *g);
 int tsx_gemm_i8_tokens(const tsx_token_gemm *g, void *workspace_dev, size_t workspace_bytes, void *stream);
 
+/* int8 tokens to values: out[i][j] = q[i][j] * scales[i] in fp32, rounded to out_type.  Rows as for tsx_quantize_tokens. */
+int tsx_dequantize_tokens(int64_t rows, int32_t cols, const int8_t *q_dev, int64_t q_stride, const float *scales_dev, void *out_dev,
+                          int32_t out_type, int64_t out_stride, void *stream);
+
+/* Rows in microscaled 4-bit floating point (MXFP4): blocks of 32 consecutive values share a scale 2^(s - 127), s a byte, and a value is
+ * four bits c: its sign (bit 3) and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (bits 0 .. 2), so that c * 2^(s - 127) stands for it.  A row of cols values is
+ * ceil(cols / 2) bytes of codes, the value at an even place in a byte's lower half (behind an odd row's end a zero), and ceil(cols / 32)
+ * bytes of scales, its last block being what is left; strides count bytes.
+ *   quantize    s = the exponent of the block's largest magnitude a (that of the power of two at or below it, + 127) - 2, at least 0: a lies in
+ *               [4, 8) steps; each value over 2^(s - 127), to nearest, ties to even codes, beyond 6 to 6.  A block with an infinity or a NaN has
+ *               s = 255 and codes 0.
+ *   dequantize  the values, rounded once to out_type; NaN where s = 255
+ * rows may be 0; cols is at most 2^30. */
+int tsx_quantize_mxfp4(int64_t rows, int32_t cols, const void *x_dev, int32_t x_type, int64_t x_stride, uint8_t *codes_dev,
+                       int64_t codes_stride, uint8_t *scales_dev, int64_t scales_stride, void *stream);
+int tsx_dequantize_mxfp4(int64_t rows, int32_t cols, const uint8_t *codes_dev, int64_t codes_stride, const uint8_t *scales_dev,
+                         int64_t scales_stride, void *out_dev, int32_t out_type, int64_t out_stride, void *stream);
+
+/* Product of MXFP4 rows, sums in fp32:
+ *   out[i][j] = act(sum_k x[i][k] w[j][k] + bias[j])
+ * x_type TSX_TYPE_MXFP4: x holds codes at x_stride bytes, x_scales their scales at x_scales_stride, as tsx_quantize_mxfp4 or tsx_rms_norm_mxfp4
+ * write them.  Another type: the rows are quantized by the call, with the values of tsx_quantize_mxfp4 (x_scales is not read).  Weights
+ * [n][k] as tsx_gemm_mxfp4_pack_weights packs them from their codes and scales.  k is below 2^21, n below 2^24, m below 2^28 and may be 0.  A
+ * row of x or w with a block of scale 255 gives NaN (and what the activation makes of that).  Sums of different kernels, which go by the
+ * sizes, may round differently; of one call on the same operands never.  The matrix cores' sums of subnormal fp32 numbers may lose them.
+ * The workspace: as for tsx_gemm_i8_tokens. */
+#define TSX_TYPE_MXFP4 4
+typedef struct tsx_mxfp4_gemm {
+    int32_t m, n, k;
+    int32_t x_type, out_type;
+    int32_t act;                 /* TSX_ACT_* as above */
+    float slope;                 /* leaky_relu */
+    const void *x_dev;
+    int64_t x_stride;
+    const uint8_t *x_scales_dev; /* [m][ceil(k / 32)], MXFP4 rows only */
+    int64_t x_scales_stride;
+    const void *packed_w_dev;
+    const float *bias_dev;       /* [n] or NULL */
+    void *out_dev;
+    int64_t out_stride;
+} tsx_mxfp4_gemm;
+size_t tsx_gemm_mxfp4_packed_weight_bytes(int32_t k, int32_t n);
+int tsx_gemm_mxfp4_pack_weights(int32_t k, int32_t n, const uint8_t *codes_dev, int64_t codes_stride, const uint8_t *scales_dev,
+                                int64_t scales_stride, void *packed_dev, void *stream);
+size_t tsx_gemm_mxfp4_workspace_bytes(const tsx_mxfp4_gemm *g);
+int tsx_gemm_mxfp4(const tsx_mxfp4_gemm *g, void *workspace_dev, size_t workspace_bytes, void *stream);
+
+/* Root-mean-square norm of rows, with the residual's addition in front of it:
+ *   h = x + residual, rounded to their type (h = x without a residual);  y = h / sqrt(mean(h^2) + epsilon) * weight
+ * x and residual in one type, each at a stride of its own; where sum_dev is given h is written there (x or residual themselves may be
+ * that memory, at the same stride), which a residual needs.  Sums of squares are fp32 or more and do not overflow or vanish: rows whose mean square leaves
+ * [2^-120, 3.4e38] are scaled first.  Where epsilon and a row are 0, and where a row has an infinity or NaN, y is what the formula gives:
+ * NaN for the zeros, the infinities and every value beside a NaN, 0 for finite values beside infinities.
+ *   rows    y in x's type, at out_stride
+ *   tokens  y (as fp32, before any rounding) as int8 tokens, dense, with the rule of tsx_quantize_tokens
+ *   mxfp4   y as MXFP4 rows, with the rule of tsx_quantize_mxfp4, codes [rows][ceil(cols / 2)] and scales [rows][ceil(cols / 32)] dense
+ * rows may be 0; cols is at most 2^30. */
+typedef struct tsx_rms_norm {
+    int64_t rows;
+    int32_t cols;
+    int32_t type;
+    const void *x_dev;
+    int64_t x_stride;
+    const void *residual_dev;    /* or NULL */
+    int64_t residual_stride;
+    void *sum_dev;               /* or NULL without a residual */
+    int64_t sum_stride;
+    const float *weight_dev;     /* [cols] or NULL */
+    float epsilon;
+} tsx_rms_norm;
+int tsx_rms_norm_rows(const tsx_rms_norm *g, void *out_dev, int64_t out_stride, void *stream);
+int tsx_rms_norm_tokens(const tsx_rms_norm *g, int8_t *q_dev, float *scales_dev, void *stream);
+int tsx_rms_norm_mxfp4(const tsx_rms_norm *g, uint8_t *codes_dev, uint8_t *scales_dev, void *stream);
+
 /* Group norm with an activation on channels-last tensors x[n][pixels][c], in groups of c / groups consecutive channels:
  *   y = act((x - mean) / sqrt(variance + epsilon) * weight[c] + bias[c]),  mean and variance over a group's channels of all pixels of
  * an image (the variance divides by their count).  Images and pixels lie at any stride (pixels at one of at least c); c is at

@@ -63,6 +63,19 @@ class GroupNorm(ctypes.Structure):
                 ("slope", _f32)]
 
 
+class Mxfp4Gemm(ctypes.Structure):
+    """tsx_mxfp4_gemm."""
+    _fields_ = [("m", _i32), ("n", _i32), ("k", _i32), ("x_type", _i32), ("out_type", _i32), ("act", _i32), ("slope", _f32),
+                ("x_dev", _vp), ("x_stride", _i64), ("x_scales_dev", _vp), ("x_scales_stride", _i64), ("packed_w_dev", _vp),
+                ("bias_dev", _vp), ("out_dev", _vp), ("out_stride", _i64)]
+
+
+class RmsNorm(ctypes.Structure):
+    """tsx_rms_norm."""
+    _fields_ = [("rows", _i64), ("cols", _i32), ("type", _i32), ("x_dev", _vp), ("x_stride", _i64), ("residual_dev", _vp),
+                ("residual_stride", _i64), ("sum_dev", _vp), ("sum_stride", _i64), ("weight_dev", _vp), ("epsilon", _f32)]
+
+
 class TsxError(RuntimeError):
     pass
 
@@ -127,6 +140,16 @@ SIGNATURES = {
     "tsx_quantize_tokens": (ctypes.c_int, [_i64, _i32, _vp, _i32, _i64, _vp, _i64, _vp, _vp]),
     "tsx_gemm_i8_tokens_workspace_bytes": (_sz, [ctypes.POINTER(TokenGemm)]),
     "tsx_gemm_i8_tokens": (ctypes.c_int, [ctypes.POINTER(TokenGemm), _vp, _sz, _vp]),
+    "tsx_dequantize_tokens": (ctypes.c_int, [_i64, _i32, _vp, _i64, _vp, _vp, _i32, _i64, _vp]),
+    "tsx_quantize_mxfp4": (ctypes.c_int, [_i64, _i32, _vp, _i32, _i64, _vp, _i64, _vp, _i64, _vp]),
+    "tsx_dequantize_mxfp4": (ctypes.c_int, [_i64, _i32, _vp, _i64, _vp, _i64, _vp, _i32, _i64, _vp]),
+    "tsx_gemm_mxfp4_packed_weight_bytes": (_sz, [_i32, _i32]),
+    "tsx_gemm_mxfp4_pack_weights": (ctypes.c_int, [_i32, _i32, _vp, _i64, _vp, _i64, _vp, _vp]),
+    "tsx_gemm_mxfp4_workspace_bytes": (_sz, [ctypes.POINTER(Mxfp4Gemm)]),
+    "tsx_gemm_mxfp4": (ctypes.c_int, [ctypes.POINTER(Mxfp4Gemm), _vp, _sz, _vp]),
+    "tsx_rms_norm_rows": (ctypes.c_int, [ctypes.POINTER(RmsNorm), _vp, _i64, _vp]),
+    "tsx_rms_norm_tokens": (ctypes.c_int, [ctypes.POINTER(RmsNorm), _vp, _vp, _vp]),
+    "tsx_rms_norm_mxfp4": (ctypes.c_int, [ctypes.POINTER(RmsNorm), _vp, _vp, _vp]),
     "tsx_group_norm_workspace_bytes": (_sz, [ctypes.POINTER(GroupNorm)]),
     "tsx_group_norm_nhwc": (ctypes.c_int, [ctypes.POINTER(GroupNorm), _vp, _vp, _sz, _vp]),
     "tsx_group_norm_tokens_nhwc": (ctypes.c_int, [ctypes.POINTER(GroupNorm), _vp, _vp, _vp, _sz, _vp]),
@@ -776,6 +799,199 @@ def group_norm_tokens(x, groups, weight=None, bias=None, epsilon=1e-5, act=None,
     """tsx_group_norm_tokens_nhwc: the same as int8 tokens, a pixel a token: (q of x's shape, scales of x.shape[:-1]), what
     TokenGemmI8 takes."""
     return _group_norm(x, groups, weight, bias, epsilon, act, slope, True)
+
+
+# ---------------------------------------------------------------- MXFP4 rows, root-mean-square norm
+# As above.  MXFP4 rows of k values are codes uint8 [..., ceil(k / 2)], two values a byte, and scales uint8 [..., ceil(k / 32)].
+
+MXFP4_BLOCK = 32
+_MXFP4 = 4
+
+
+def _float_dtype(what, dtype):
+    if dtype not in _FLOATS:
+        raise TsxError("%s: output type %s" % (what, dtype))
+    return _TYPES[dtype]
+
+
+def _mxfp4_shape(x, k):
+    return x.shape[:-1] + ((k + 1) // 2,), x.shape[:-1] + ((k + MXFP4_BLOCK - 1) // MXFP4_BLOCK,)
+
+
+def _mxfp4_rows(what, codes, scales, k):
+    """Checked codes and scales of rows of k values (None: two for each byte); k, too."""
+    codes = _token_operand(what, codes, (torch.uint8,))
+    scales = _token_operand(what, scales, (torch.uint8,))
+    if codes.device != scales.device:
+        raise TsxError("%s: codes on %s, scales on %s" % (what, codes.device, scales.device))
+    k = 2 * codes.shape[-1] if k is None and codes.dim() else k
+    if codes.dim() < 1 or not 0 < k <= 1 << 30 or (codes.shape, scales.shape) != _mxfp4_shape(codes, k):
+        raise TsxError("%s: codes of shape %s, scales of shape %s, rows of %s values" % (what, tuple(codes.shape), tuple(scales.shape), k))
+    return codes, scales, k
+
+
+def dequantize_tokens(q, scales, dtype=torch.float32):
+    """tsx_dequantize_tokens: q * scales[..., None] in dtype (fp32, fp16 or bf16) for int8 q [..., k] and fp32 scales [...], as
+    quantize_tokens gives them."""
+    out = _native().dequantize(q, scales, -1, _TYPES.get(dtype, 3))
+    if out is not NotImplemented:
+        return out
+    q = _token_operand("dequantize_tokens", q, (torch.int8,))
+    kind = _float_dtype("dequantize_tokens", dtype)
+    if q.dim() < 1 or not 0 < q.shape[-1] <= 1 << 30:
+        raise TsxError("dequantize_tokens: shape %s (rows of 1 to 2^30 values)" % (tuple(q.shape),))
+    if scales is None:
+        raise TsxError("int8 tokens come with their scales")
+    scales = _vector("scales", scales, q.numel() // q.shape[-1], q)
+    out = torch.empty(q.shape, dtype=dtype, device=q.device)
+    if q.numel():
+        with torch.cuda.device(q.device):
+            q, rows, stride = _rows(q)
+            check(lib().tsx_dequantize_tokens(rows, q.shape[-1], _ptr(q), stride, _ptr(scales), _ptr(out), kind, q.shape[-1], _stream()))
+    return out
+
+
+def quantize_mxfp4(x):
+    """tsx_quantize_mxfp4: (codes, scales) of x [..., k] in fp32, fp16 or bf16: codes uint8 [..., ceil(k / 2)], the value at an even place in a
+    byte's lower half, scales uint8 [..., ceil(k / 32)], so that a code's value (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) times
+    2^(scale - 127) stands for x."""
+    out = _native().quantize_mxfp4(x)
+    if out is not NotImplemented:
+        return out
+    x = _token_operand("quantize_mxfp4", x, _FLOATS)
+    if x.dim() < 1 or not 0 < x.shape[-1] <= 1 << 30:
+        raise TsxError("quantize_mxfp4: shape %s (rows of 1 to 2^30 values)" % (tuple(x.shape),))
+    codes, scales = (torch.empty(shape, dtype=torch.uint8, device=x.device) for shape in _mxfp4_shape(x, x.shape[-1]))
+    if x.numel():
+        with torch.cuda.device(x.device):
+            x, rows, stride = _rows(x)
+            check(lib().tsx_quantize_mxfp4(rows, x.shape[-1], _ptr(x), _TYPES[x.dtype], stride, _ptr(codes), codes.shape[-1], _ptr(scales),
+                                           scales.shape[-1], _stream()))
+    return codes, scales
+
+
+def dequantize_mxfp4(codes, scales, k=None, dtype=torch.float32):
+    """tsx_dequantize_mxfp4: the values [..., k] in dtype (fp32, fp16 or bf16) of codes and scales as quantize_mxfp4 gives them; k, by default two
+    values for each byte, says where it is odd."""
+    out = _native().dequantize(codes, scales, 0 if k is None else k, _TYPES.get(dtype, 3))
+    if out is not NotImplemented:
+        return out
+    kind = _float_dtype("dequantize_mxfp4", dtype)
+    codes, scales, k = _mxfp4_rows("dequantize_mxfp4", codes, scales, k)
+    out = torch.empty(codes.shape[:-1] + (k,), dtype=dtype, device=codes.device)
+    if out.numel():
+        with torch.cuda.device(codes.device):
+            (codes, rows, stride), (scales, _, scales_stride) = _rows(codes), _rows(scales)
+            check(lib().tsx_dequantize_mxfp4(rows, k, _ptr(codes), stride, _ptr(scales), scales_stride, _ptr(out), kind, k, _stream()))
+    return out
+
+
+class TokenGemmMxfp4:
+    """Product of MXFP4 rows with packed MXFP4 weights: codes [n][ceil(k / 2)] and scales [n][ceil(k / 32)] of the weights [n][k], as quantize_mxfp4
+    gives them (k says where it is odd); bias [n]."""
+
+    def __init__(self, codes, scales, bias=None, k=None):
+        codes, scales, self.k = _mxfp4_rows("weights", codes, scales, k)
+        self.n = codes.shape[0]
+        if codes.dim() != 2 or self.n == 0 or self.n >= 1 << 24 or self.k >= 1 << 21:
+            raise TsxError("weights of shape %s (below 2^24 rows of below 2^21 values)" % ((codes.shape[0], self.k),))
+        self.bias = _vector("bias", bias, self.n, codes)
+        with torch.cuda.device(codes.device):
+            (codes, _, stride), (scales, _, scales_stride) = _rows(codes), _rows(scales)
+            self.packed = torch.empty(lib().tsx_gemm_mxfp4_packed_weight_bytes(self.k, self.n), dtype=torch.uint8, device=codes.device)
+            check(lib().tsx_gemm_mxfp4_pack_weights(self.k, self.n, _ptr(codes), stride, _ptr(scales), scales_stride, _ptr(self.packed), _stream()))
+
+    @classmethod
+    def from_float(cls, w, bias=None):
+        """Weights [n][k] in fp32, fp16 or bf16, quantized by quantize_mxfp4."""
+        return cls(*quantize_mxfp4(w), bias, w.shape[-1])
+
+    def __call__(self, x, x_scales=None, act=None, slope=0.0, out_dtype=None):
+        """x [..., k] in fp32, fp16 or bf16, quantized to MXFP4 in the call; or codes [..., ceil(k / 2)] with x_scales [..., ceil(k / 32)], as
+        quantize_mxfp4 and rms_norm_mxfp4 give them.  Returns [..., n] in out_dtype, by default x's type (codes: fp32)."""
+        act = _token_act(act)
+        if out_dtype is None and x_scales is not None:
+            out_dtype = torch.float32
+        out = _native_module.mxfp4_gemm(self.packed, self.k, self.n, self.bias, x, x_scales, act, slope, -1 if out_dtype is None else _TYPES.get(out_dtype, 3))
+        if out is not NotImplemented:
+            return out
+        x = _token_operand("MXFP4 product", x, _FLOATS + (torch.uint8,))
+        if (x.dtype == torch.uint8) != (x_scales is not None):
+            raise TsxError("MXFP4 codes come with their scales, others without")
+        if x.device != self.packed.device:
+            raise TsxError("tokens on %s, weights on %s" % (x.device, self.packed.device))
+        if x_scales is not None:
+            x, x_scales, _ = _mxfp4_rows("MXFP4 product", x, x_scales, self.k)
+        elif x.dim() < 1 or x.shape[-1] != self.k:
+            raise TsxError("tokens of shape %s, weights of %d rows" % (tuple(x.shape), self.k))
+        out_dtype = out_dtype or x.dtype
+        out_type = _float_dtype("MXFP4 product", out_dtype)
+        rows = x.numel() // x.shape[-1]
+        if rows >= 1 << 28:
+            raise TsxError("MXFP4 product: %d rows (below 2^28)" % rows)
+        out = torch.empty(x.shape[:-1] + (self.n,), dtype=out_dtype, device=x.device)
+        if rows == 0:
+            return out
+        with torch.cuda.device(x.device):
+            x, rows, stride = _rows(x)
+            scales_stride = 0
+            if x_scales is not None:
+                x_scales, _, scales_stride = _rows(x_scales)
+            g = Mxfp4Gemm(rows, self.n, self.k, _TYPES.get(x.dtype, _MXFP4), out_type, act, float(slope), _ptr(x), stride, _ptr(x_scales), scales_stride,
+                          _ptr(self.packed), _ptr(self.bias), _ptr(out), self.n)
+            nbytes = lib().tsx_gemm_mxfp4_workspace_bytes(ctypes.byref(g))
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+            check(lib().tsx_gemm_mxfp4(ctypes.byref(g), _ptr(workspace), nbytes, _stream()))
+        return out
+
+
+def _rms_norm(x, weight, epsilon, residual, to):
+    out = _native().rms_norm(x, weight, epsilon, residual, to)
+    if out is not NotImplemented:
+        return out
+    x = _token_operand("rms_norm", x, _FLOATS)
+    if x.dim() < 1 or not 0 < x.shape[-1] <= 1 << 30:
+        raise TsxError("rms_norm: shape %s (rows of 1 to 2^30 values)" % (tuple(x.shape),))
+    k = x.shape[-1]
+    weight = _vector("weight", weight, k, x)
+    if residual is not None:
+        residual = _token_operand("residual", residual, (x.dtype,))
+        if residual.device != x.device or residual.shape != x.shape:
+            raise TsxError("residual of shape %s on %s, x of shape %s on %s" % (tuple(residual.shape), residual.device, tuple(x.shape), x.device))
+    total = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    shape, scales_shape = {0: (x.shape, None), 1: (x.shape, x.shape[:-1]), 2: _mxfp4_shape(x, k)}[to]
+    out = torch.empty(shape, dtype=(x.dtype, torch.int8, torch.uint8)[to], device=x.device)
+    scales = torch.empty(scales_shape, dtype=torch.float32 if to == 1 else torch.uint8, device=x.device) if to else None
+    if x.numel():
+        with torch.cuda.device(x.device):
+            x, rows, stride = _rows(x)
+            residual, _, residual_stride = (None, 0, 0) if residual is None else _rows(residual)
+            g = RmsNorm(rows, k, _TYPES[x.dtype], _ptr(x), stride, _ptr(residual), residual_stride, _ptr(total), k, _ptr(weight), float(epsilon))
+            if to == 0:
+                check(lib().tsx_rms_norm_rows(ctypes.byref(g), _ptr(out), k, _stream()))
+            else:
+                call = lib().tsx_rms_norm_tokens if to == 1 else lib().tsx_rms_norm_mxfp4
+                check(call(ctypes.byref(g), _ptr(out), _ptr(scales), _stream()))
+    every = [t for t in (out, scales, total) if t is not None]
+    return every[0] if len(every) == 1 else tuple(every)
+
+
+def rms_norm(x, weight=None, epsilon=1e-6, residual=None):
+    """tsx_rms_norm_rows: x / sqrt(mean(x^2) + epsilon) * weight over the last axis of x [..., k] in fp32, fp16 or bf16, weight fp32 [k] (another type
+    is converted in each call).  With a residual of x's shape and type it is the norm of h = x + residual, rounded to their type, and the call
+    returns (the norm, h)."""
+    return _rms_norm(x, weight, epsilon, residual, 0)
+
+
+def rms_norm_tokens(x, weight=None, epsilon=1e-6, residual=None):
+    """tsx_rms_norm_tokens: the same as int8 tokens: (q of x's shape, scales of x.shape[:-1]), what TokenGemmI8 takes, and h behind them
+    with a residual."""
+    return _rms_norm(x, weight, epsilon, residual, 1)
+
+
+def rms_norm_mxfp4(x, weight=None, epsilon=1e-6, residual=None):
+    """tsx_rms_norm_mxfp4: the same as MXFP4 rows: (codes, scales), what TokenGemmMxfp4 takes, and h behind them with a residual."""
+    return _rms_norm(x, weight, epsilon, residual, 2)
 
 
 def conv2d_f32(x, w, pads=(0, 0, 0, 0), strides=(1, 1), dilations=(1, 1), padding_value=0.0, bias=None, act=None,

@@ -9,6 +9,7 @@
 #include <cstdlib>
 
 #include "igemm_i8.hpp"
+#include "token_tiles.hpp"
 #include "tokens_i8.hpp"
 
 namespace tsx {
@@ -28,14 +29,6 @@ struct TokenGemmParams {
     float slope;
     int row_tiles, col_tiles, tiles_per_xcd;
 };
-
-typedef __attribute__((address_space(3))) void lds_void;
-typedef const __attribute__((address_space(1))) void global_void;
-
-// 64 lanes x 16 bytes, from an address for each lane to consecutive bytes of LDS.  Complete when vmcnt says so.
-__device__ __forceinline__ void to_lds(const int8_t *at, int8_t *lds) {
-    __builtin_amdgcn_global_load_lds((global_void *)at, (lds_void *)lds, 16, 0, 0);
-}
 
 // A fragment's values of 32 output columns x 32 tokens in the output's type: accumulator r of lane l is column 8 (r / 4) + 4 (l / 32) +
 // r % 4 of token l % 32; swaps between the half-waves leave a lane with 16 consecutive columns, the lower ones with 0 .. 15, the upper
@@ -73,28 +66,6 @@ __device__ __forceinline__ Run<OUT, 16> fragment_values(const TokenGemmParams &p
     });
     return to;
 }
-
-// f(the activation as a constant): one branch around all of a wavefront's values
-template <class F>
-__device__ __forceinline__ void by_act(int act, F &&f) {
-    switch (act) {
-        case TSX_ACT_RELU: f(std::integral_constant<int, TSX_ACT_RELU>{}); break;
-        case TSX_ACT_LEAKY_RELU: f(std::integral_constant<int, TSX_ACT_LEAKY_RELU>{}); break;
-        case TSX_ACT_MISH_FAST: f(std::integral_constant<int, TSX_ACT_MISH_FAST>{}); break;
-        case TSX_ACT_SILU: f(std::integral_constant<int, TSX_ACT_SILU>{}); break;
-        default: f(std::integral_constant<int, TSX_ACT_NONE>{}); break;
-    }
-}
-
-// LDS is this workgroup's own: what was read from it is read, and what the wavefronts wrote is there, behind the barrier.  Requests to
-// memory stay in flight.
-__device__ __forceinline__ void lds_barrier() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
-template <int N>
-__device__ __forceinline__ void wait_for_all_but() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
 // WR x WC wavefronts, each with FR x FC fragments of 32 tokens x 32 columns; S chunks of KS K-steps in LDS.
 //

@@ -1,0 +1,627 @@
+// Product of MXFP4 rows (mxfp4.hpp) with MXFP4 weights, on rows of fp32, fp16, bf16 or MXFP4.
+//
+//     out[i][j] = act(sum over blocks b of 2^(s_x[i][b] + s_w[j][b] - 254) sum_k x[i][k] w[j][k] + bias[j]),  rounded once to the output's type
+//
+// The scaled matrix instructions take both scales with the codes: v_mfma_scale_f32_32x32x64_f8f6f4, where a lane supplies row l % 32 of block
+// l / 32 of two, its 16 bytes of codes and its scale, and v_mfma_scale_f32_16x16x128_f8f6f4, row l % 16 of block l / 16 of four.  Sums are fp32.
+#include <algorithm>
+#include <cmath>
+#include <cstdlib>
+
+#include "mxfp4.hpp"
+#include "token_tiles.hpp"
+
+namespace tsx {
+namespace {
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+constexpr int KSTEP = MX_STEP / 2;     // bytes of codes
+constexpr int FP4 = 4;                 // the instructions' number for this type
+
+// Packed weights: codes [K-step][fragment of 32 columns][half of the K-step][lane][16], as the 32x32x64 instruction takes them, behind
+// them scales [K-step][column][4].  Columns in whole groups of 128, K-steps in pairs; zeros behind n and k, whose scales are 2^-127.
+int frags_of(int n) { return int(round_up(n, 128) / 32); }
+int ksteps_of(int k) { return int(round_up(ceil_div(k, MX_STEP), 2)); }
+int64_t packed_codes(int k, int n) { return int64_t(ksteps_of(k)) * frags_of(n) * 2048; }
+
+struct MxGemmParams {
+    const uint8_t *x, *x_scales;       // codes [m] at x_pitch, a multiple of 16; scales: a K-step's word of a row at row scale_row + step scale_step
+    const int8_t *w, *w_scales;
+    const float *bias;
+    void *out;
+    int64_t x_pitch, scale_row, scale_step, out_stride;
+    int m, n, k, frags, ksteps;        // k: bytes of codes of a row that are there, a multiple of 16; ksteps: of the weights
+    int x_steps;                       // K-steps of x's scales
+    float slope;
+    int act;
+    int row_tiles, col_tiles, tiles_per_xcd;
+};
+
+__device__ __forceinline__ v8i operand(v4i v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
+
+// A fragment's values of 32 output columns x 32 tokens in the output's type: accumulator r of lane l is column 8 (r / 4) + 4 (l / 32) +
+// r % 4 of token l % 32; swaps between the half-waves leave a lane with 16 consecutive columns, the lower ones with 0 .. 15, the upper
+// ones with 16 .. 31.
+template <int OUT>
+__device__ __forceinline__ Run<OUT, 16> fragment_values(const float (&v)[16]) {
+    Run<OUT, 16> to, own;
+    own.set(v);
+    constexpr int W = Run<OUT, 4>::WORDS;      // words of four values
+    static_for<0, 2>([&](auto pc) {
+        constexpr int a = decltype(pc)::value;
+        static_for<0, W>([&](auto wc) {
+            constexpr int w = decltype(wc)::value;
+            const auto s = __builtin_amdgcn_permlane32_swap(own.word[a * W + w], own.word[(a + 2) * W + w], false, false);
+            to.word[2 * a * W + w] = s[0];
+            to.word[(2 * a + 1) * W + w] = s[1];
+        });
+    });
+    return to;
+}
+
+__device__ __forceinline__ void word_to_lds(const uint8_t *at, int8_t *lds) {
+    __builtin_amdgcn_global_load_lds((global_void *)at, (lds_void *)lds, 4, 0, 0);
+}
+
+// A sum, taken from the accumulators here and not before: all of them taken at once would not fit the other registers.
+__device__ __forceinline__ float sum_of(float v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+// WR x WC wavefronts, each with FR x FC fragments of 32 tokens x 32 columns; S chunks of KS K-steps in LDS, a K-step's scales behind its codes.
+template <int WR, int WC, int FR, int FC, int KS, int S, int OUT>
+__global__ __launch_bounds__(WR *WC * 64, WR * FR == 4 ? 3 : 1) void gemm_mxfp4_kernel(MxGemmParams p) {
+    constexpr int CHUNK = KS * KSTEP, PIECES = CHUNK / 16, WAVES = WR * WC, ROWS = 32 * WR * FR, COLS = 32 * WC * FC, HALVES = 2 * KS;
+    constexpr int A_BYTES = ROWS * CHUNK, B_BYTES = COLS * CHUNK, A_LOADS = A_BYTES / 1024 / WAVES, B_LOADS = B_BYTES / 1024 / WAVES;
+    constexpr int A_WORDS = KS * ROWS / 64, S_LOADS = KS * (ROWS + COLS) / 64 / WAVES;      // requests of 64 words of scales
+    constexpr int SCALES = A_BYTES + B_BYTES, BUFFER = SCALES + KS * (ROWS + COLS) * 4, LOADS = A_LOADS + B_LOADS + S_LOADS;
+    static_assert(A_LOADS * 1024 * WAVES == A_BYTES && B_LOADS * 1024 * WAVES == B_BYTES && S_LOADS * 64 * WAVES == KS * (ROWS + COLS) && (S - 1) * LOADS < 64,
+                  "whole loads, counted in six bits");
+    extern __shared__ __attribute__((aligned(16))) int8_t lds[];      // [S][BUFFER]
+    __shared__ __attribute__((aligned(16))) float of_cols[COLS];      // biases, requested ahead of everything
+    constexpr int THREADS = WAVES * 64;
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int wave_r = wave / WC, wave_c = wave % WC;
+    // blockIdx % 8 is the XCD: each takes a run of consecutive tiles, which walk four row tiles before the next column tile
+    const int tiles = p.row_tiles * p.col_tiles;
+    const int t = int(blockIdx.x % 8) * p.tiles_per_xcd + int(blockIdx.x / 8);
+    if (int(blockIdx.x / 8) >= p.tiles_per_xcd || t >= tiles) return;      // uniform, ahead of every barrier
+    const int group = t / (4 * p.col_tiles), in_group = t - group * 4 * p.col_tiles;
+    const int group_rows = min(4, p.row_tiles - 4 * group);
+    const int tile_c = in_group / group_rows, tile_r = 4 * group + in_group - tile_c * group_rows;
+    const int row0 = tile_r * ROWS, frag0 = tile_c * (COLS / 32);
+    constexpr int COL_TURNS = (COLS + THREADS - 1) / THREADS;
+    float col_bias[COL_TURNS];
+    static_for<0, COL_TURNS>([&](auto ic) { col_bias[decltype(ic)::value] = -0.f; });      // changes no sum
+    if (p.bias) static_for<0, COL_TURNS>([&](auto ic) { col_bias[decltype(ic)::value] = p.bias[min(frag0 * 32 + int(threadIdx.x) + decltype(ic)::value * THREADS, p.n - 1)]; });
+
+    // A row in LDS is its CHUNK bytes, its pieces of 16 XORed with bits of the row that make 16 rows cover all banks for one piece.  A
+    // load instruction fills 1 KiB of such rows; rows beyond m are the last one again, never stored.  Pieces behind the end of a row are
+    // its first one, against weights that are zero.  Scalar bases and 32-bit lane offsets.
+    const auto key_of = [](int row) { return (row >> (KS == 1 ? 2 : 1)) & (PIECES - 1); };
+    const int chunks = p.ksteps / KS;
+    const uint8_t *const a_base = p.x + int64_t(row0) * p.x_pitch;
+    unsigned a_off[A_LOADS], b_off[B_LOADS], s_off[S_LOADS];
+    int a_piece[A_LOADS];
+    static_for<0, A_LOADS>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        const int r = (wave * A_LOADS + i) * (64 / PIECES) + lane / PIECES;
+        a_piece[i] = ((lane % PIECES) ^ key_of(r)) * 16;
+        a_off[i] = unsigned(min(r, p.m - 1 - row0)) * unsigned(p.x_pitch);
+    });
+    static_for<0, B_LOADS>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        const int unit = wave * B_LOADS + i, step = unit / (2 * COLS / 32), in_step = unit % (2 * COLS / 32);
+        const int frag = min(frag0 + in_step / 2, p.frags - 1);
+        b_off[i] = unsigned(step * p.frags + frag) * 2048u + (in_step % 2) * 1024 + lane * 16;
+    });
+    // Scales in LDS: [K-step of the chunk][row], then [K-step of the chunk][column].  A request's K-steps lie s_stride apart, the last of them is
+    // s_last; selects, no branches: all requests of a chunk are one run of instructions.
+    const uint8_t *s_base[S_LOADS];
+    int64_t s_stride[S_LOADS];
+    int s_step[S_LOADS], s_last[S_LOADS];
+    static_for<0, S_LOADS>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        const int unit = wave * S_LOADS + i, of_w = unit - A_WORDS;
+        const bool is_x = unit < A_WORDS;
+        s_step[i] = is_x ? unit / (ROWS / 64) : of_w / (COLS / 64);
+        s_base[i] = is_x ? p.x_scales + int64_t(row0) * p.scale_row : reinterpret_cast<const uint8_t *>(p.w_scales) + frag0 * 128;
+        s_stride[i] = is_x ? p.scale_step : int64_t(p.frags) * 128;
+        s_last[i] = is_x ? p.x_steps - 1 : p.ksteps - 1;
+        s_off[i] = is_x ? unsigned(min(unit % (ROWS / 64) * 64 + lane, p.m - 1 - row0)) * unsigned(p.scale_row)
+                        : unsigned(min(of_w % (COLS / 64) * 64 + lane, (p.frags - frag0) * 32 - 1)) * 4u;
+    });
+    const int64_t b_step = int64_t(p.frags) * (KS * 2048);
+    auto fetch = [&](int chunk, int buf) __attribute__((always_inline)) {
+        const int c = min(chunk, chunks - 1);                // behind the last chunk: that one again, not read from LDS
+        int8_t *const at = lds + buf * BUFFER;
+        const int8_t *const b = p.w + c * b_step;
+        static_for<0, A_LOADS>([&](auto ic) {
+            constexpr int i = decltype(ic)::value;
+            const int k = c * CHUNK + a_piece[i];
+            to_lds(reinterpret_cast<const int8_t *>(a_base) + (a_off[i] + unsigned(k < p.k ? k : 0)), at + (wave * A_LOADS + i) * 1024);
+        });
+        static_for<0, B_LOADS>([&](auto ic) { constexpr int i = decltype(ic)::value; to_lds(b + b_off[i], at + A_BYTES + (wave * B_LOADS + i) * 1024); });
+        static_for<0, S_LOADS>([&](auto ic) {
+            constexpr int i = decltype(ic)::value;
+            word_to_lds(s_base[i] + min(c * KS + s_step[i], s_last[i]) * s_stride[i] + s_off[i], at + SCALES + (wave * S_LOADS + i) * 256);
+        });
+    };
+
+    v16f acc[FR][FC];
+    static_for<0, FR * FC>([&](auto fc) {
+        constexpr int f = decltype(fc)::value;
+        static_for<0, 16>([&](auto rc) { acc[f / FC][f % FC][decltype(rc)::value] = 0.f; });
+    });
+    const int a_row = (wave_r * FR * 32 + lane % 32) * CHUNK, a_key = key_of(lane % 32);
+    v4i a[2][FR], b[2][FC];
+    int a_scale[2][FR], b_scale[2][FC];      // of a K-step: blocks l / 32 and 2 + l / 32 in bytes 0 and 2
+    auto read = [&](auto hc, int buf) __attribute__((always_inline)) {
+        constexpr int h = decltype(hc)::value, set = h % 2, step = h / 2;
+        const int8_t *const at = lds + buf * BUFFER;
+        if constexpr (h % 2 == 0) {
+            static_for<0, FC>([&](auto fc) {
+                constexpr int f = decltype(fc)::value;
+                b_scale[step % 2][f] = *reinterpret_cast<const int *>(at + SCALES + (KS * ROWS + step * COLS + (wave_c * FC + f) * 32 + lane % 32) * 4);
+            });
+            static_for<0, FR>([&](auto ic) {
+                constexpr int i = decltype(ic)::value;
+                a_scale[step % 2][i] = *reinterpret_cast<const int *>(at + SCALES + (step * ROWS + (wave_r * FR + i) * 32 + lane % 32) * 4);
+            });
+        }
+        static_for<0, FC>([&](auto fc) {
+            constexpr int f = decltype(fc)::value;
+            b[set][f] = *reinterpret_cast<const v4i *>(at + A_BYTES + ((step * (COLS / 32) + wave_c * FC + f) * 2 + h % 2) * 1024 + lane * 16);
+        });
+        static_for<0, FR>([&](auto ic) {
+            constexpr int i = decltype(ic)::value;
+            a[set][i] = *reinterpret_cast<const v4i *>(at + a_row + i * 32 * CHUNK + ((2 * h + lane / 32) ^ a_key) * 16);
+        });
+    };
+    static_for<0, S>([&](auto sc) { fetch(decltype(sc)::value, decltype(sc)::value); });     // behind the last chunk: that one again
+    wait_for_all_but<(S - 1) * LOADS>();
+    static_for<0, COL_TURNS>([&](auto ic) {
+        const int at = threadIdx.x + decltype(ic)::value * THREADS;
+        if (COLS % THREADS == 0 || at < COLS) of_cols[at] = col_bias[decltype(ic)::value];
+    });
+    lds_barrier();
+    read(std::integral_constant<int, 0>{}, 0);
+    const int upper = 8 * (lane / 32);
+    int buf = 0, c = 0;
+    auto multiply = [&](auto fetching) __attribute__((always_inline)) {
+        constexpr bool FETCHES = decltype(fetching)::value;
+        const int after = buf + 1 == S ? 0 : buf + 1;
+        static_for<0, HALVES>([&](auto hc) {
+            constexpr int h = decltype(hc)::value;
+            int as[FR], bs[FC];
+            static_for<0, FR>([&](auto ic) { as[decltype(ic)::value] = int(unsigned(a_scale[h / 2 % 2][decltype(ic)::value]) >> upper); });
+            static_for<0, FC>([&](auto fc) { bs[decltype(fc)::value] = int(unsigned(b_scale[h / 2 % 2][decltype(fc)::value]) >> upper); });
+            if constexpr (h + 1 < HALVES) {
+                read(std::integral_constant<int, h + 1>{}, buf);
+            } else {
+                // Every wavefront has its operands of this chunk in registers: its buffer is free behind the barrier, and the next
+                // chunk is there for all.  The rest of this chunk's arithmetic covers the first reads behind it.
+                wait_for_all_but<FETCHES ? (S - 2) * LOADS : 0>();
+                lds_barrier();
+                read(std::integral_constant<int, 0>{}, after);
+                if constexpr (FETCHES) fetch(c + S, buf);
+            }
+            static_for<0, FR * FC>([&](auto fc) {
+                constexpr int i = decltype(fc)::value / FC, f = decltype(fc)::value % FC;
+                acc[i][f] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(b[h % 2][f]), operand(a[h % 2][i]), acc[i][f], FP4, FP4, 2 * (h % 2), bs[f],
+                                                                            2 * (h % 2), as[i]);
+            });
+            // reads and requests between the multiplications
+            static_for<0, FR * FC>([&](auto fc) {
+                if constexpr (FETCHES && h + 1 == HALVES) __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        buf = after;
+    };
+    for (; c + S < chunks; ++c) multiply(std::true_type{});
+    for (; c < chunks; ++c) multiply(std::false_type{});      // the last S chunks are all on their way
+    // The chunks' LDS is free: nothing is on its way into it, and behind this barrier nobody reads it.  A wavefront's 32 tokens x 32 FC
+    // columns go through it, so that a store instruction writes whole cache lines (straight from the registers it would write 16 bytes of
+    // each of 64 runs).
+    wait_for_all_but<0>();
+    lds_barrier();
+    constexpr int SIZE = OUT == TSX_TYPE_F32 ? 4 : 2, ROW = FC * 32 * SIZE, PITCH = ROW + 16, IN_ROW = ROW / 16, AT_ONCE = 64 / IN_ROW, EACH = 16 / SIZE;
+    static_assert(WAVES * 32 * PITCH <= S * BUFFER, "room for all wavefronts");
+    int8_t *const mine = lds + wave * (32 * PITCH);
+    const int col = (frag0 + wave_c * FC) * 32 + lane % IN_ROW * EACH, left = p.n - col;      // where a lane stores
+    static_for<0, FR>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        const int in_tile = (wave_r * FR + i) * 32;
+        float v[FC][16];
+        static_for<0, FC>([&](auto fc) {
+            constexpr int f = decltype(fc)::value;
+            static_for<0, 4>([&](auto gc) {
+                constexpr int g = decltype(gc)::value;
+                const v4f bias = *reinterpret_cast<const v4f *>(of_cols + (wave_c * FC + f) * 32 + 8 * g + 4 * (lane / 32));
+                static_for<0, 4>([&](auto jc) { constexpr int j = decltype(jc)::value; v[f][4 * g + j] = __fadd_rn(sum_of(acc[i][f][4 * g + j]), bias[j]); });
+            });
+        });
+        by_act(p.act, [&](auto act) __attribute__((always_inline)) {
+            static_for<0, FC>([&](auto fc) { activate_as<OUT, decltype(act)::value>(v[decltype(fc)::value], p.slope); });
+        });
+        static_for<0, FC>([&](auto fc) {
+            constexpr int f = decltype(fc)::value;
+            const Run<OUT, 16> to = fragment_values<OUT>(v[f]);
+            v4u *const at = reinterpret_cast<v4u *>(mine + lane % 32 * PITCH + (f * 32 + 16 * (lane / 32)) * SIZE);
+            static_for<0, SIZE>([&](auto wc) { constexpr int w = 4 * decltype(wc)::value; at[w / 4] = v4u{to.word[w], to.word[w + 1], to.word[w + 2], to.word[w + 3]}; });
+        });
+        static_for<0, 32 / AT_ONCE>([&](auto kc) {
+            const int r = decltype(kc)::value * AT_ONCE + lane / IN_ROW, row = row0 + in_tile + r;
+            Run<OUT, EACH> to;
+            const v4u got = *reinterpret_cast<const v4u *>(mine + r * PITCH + lane % IN_ROW * 16);
+            static_for<0, 4>([&](auto wc) { to.word[decltype(wc)::value] = got[decltype(wc)::value]; });
+            char *const out = static_cast<char *>(p.out) + (int64_t(row) * p.out_stride + col) * SIZE;
+            if (row < p.m) {
+                if (left >= EACH) to.store(out);
+                else if (left > 0) to.store_some(out, left);
+            }
+        });
+        __builtin_amdgcn_sched_barrier(0);               // 32 tokens at a time: their values would fill the registers
+    });
+}
+
+// ---- few tokens: a stream over the weights
+//
+// There the product reads 17 / 32 n k bytes of weights and does little with each.  A workgroup owns 16 output columns and its 8 wavefronts split K, every
+// eighth K-step each; a K-step of 16 columns is one 16-byte load a lane and a word of scales, AHEAD of them in flight from the first instruction
+// on.  X, the type of the rows: MXFP4, or floats, which a lane quantizes where it needs them, 32 values of one token, a block: nothing has to meet
+// for a block's scale, so there is no launch ahead of the product and no barrier in it before the partial sums meet in LDS.  MT: groups of 16 tokens.
+// 16x16x128 instruction: accumulator r of lane l is column 4 (l / 16) + r of token l % 16.
+constexpr int FEW_THREADS = 512, FEW_WAVES = FEW_THREADS / 64;
+
+struct FewTokens : MxGemmParams {
+    const void *values;                // rows of floats
+    int64_t x_stride;
+    int cols;                          // values of such a row
+};
+
+template <int X, int MT, int AHEAD, int OUT>
+__global__ __launch_bounds__(FEW_THREADS) void gemm_mxfp4_few_kernel(FewTokens p) {
+    __shared__ float sums[FEW_WAVES][MT][4][64];
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), block = lane / 16, row = lane % 16;
+    const int row0 = int(blockIdx.y) * 16 * MT, col16 = blockIdx.x;      // in columns of 16
+    const int8_t *const w = p.w + int64_t(col16 >> 1) * 2048 + (block >> 1) * 1024 + (16 * (col16 & 1) + row + 32 * (block & 1)) * 16;
+    const int8_t *const ws = p.w_scales + (col16 * 16 + row) * 4;
+    const int64_t w_step = int64_t(p.frags) * 2048, ws_step = int64_t(p.frags) * 128;
+    v4i a[AHEAD];
+    unsigned as[AHEAD];
+    auto fetch = [&](int first) __attribute__((always_inline)) {
+        static_for<0, AHEAD>([&](auto uc) {
+            constexpr int u = decltype(uc)::value;
+            const int step = min(first + FEW_WAVES * u, p.ksteps - 1);
+            a[u] = *reinterpret_cast<const v4i *>(w + step * w_step);
+            as[u] = *reinterpret_cast<const unsigned *>(ws + step * ws_step);
+        });
+    };
+    fetch(wave);
+    v4f acc[MT];
+    static_for<0, MT>([&](auto mc) { acc[decltype(mc)::value] = v4f{0.f, 0.f, 0.f, 0.f}; });
+    for (int first = wave; first < p.ksteps; first += FEW_WAVES * AHEAD) {
+        v4i b[AHEAD][MT];
+        unsigned bs[AHEAD][MT];
+        static_for<0, AHEAD>([&](auto uc) {
+            constexpr int u = decltype(uc)::value;
+            const int step = min(first + FEW_WAVES * u, p.ksteps - 1);
+            static_for<0, MT>([&](auto mc) {
+                constexpr int i = decltype(mc)::value;
+                const int token = min(row0 + 16 * i + row, p.m - 1);
+                if constexpr (X == TSX_TYPE_MXFP4) {
+                    const int k = step * KSTEP + block * 16;
+                    b[u][i] = *reinterpret_cast<const v4i *>(p.x + token * p.x_pitch + (k < p.k ? k : 0));
+                    bs[u][i] = p.x_scales[token * p.scale_row + min(step, p.x_steps - 1) * p.scale_step + block];
+                } else {
+                    constexpr int SIZE = X == TSX_TYPE_F32 ? 4 : 2;
+                    typedef Run<X, 8> Values;
+                    const int k = step * MX_STEP + block * MX_BLOCK;
+                    const char *const x = static_cast<const char *>(p.values) + token * p.x_stride * SIZE;
+                    Values v[4];
+                    unsigned top = 0;
+                    if (p.cols >= 8)             // uniform
+                        static_for<0, 4>([&](auto pc) { constexpr int q = decltype(pc)::value; v[q].load(x + int64_t(min(k + 8 * q, p.cols - 8)) * SIZE); });
+                    if (k + MX_BLOCK > p.cols)   // the row's end, and blocks behind it
+                        static_for<0, 4>([&](auto pc) {
+                            constexpr int q = decltype(pc)::value;
+                            const int left = p.cols - k - 8 * q;
+                            if (left < 8) v[q].clear();
+                            if (left > 0 && left < 8) v[q].load_some(x + int64_t(k + 8 * q) * SIZE, left);
+                        });
+                    static_for<0, 4>([&](auto pc) { top = v[decltype(pc)::value].top(top); });
+                    bs[u][i] = mx_scale(top_value<X>(top));
+                    static_for<0, 4>([&](auto pc) { constexpr int q = decltype(pc)::value; b[u][i][q] = int(mx_codes<X>(v[q], bs[u][i])); });
+                }
+            });
+        });
+        static_for<0, AHEAD>([&](auto uc) {
+            constexpr int u = decltype(uc)::value;
+            if (first + FEW_WAVES * u < p.ksteps)            // uniform
+                static_for<0, MT>([&](auto mc) {
+                    constexpr int i = decltype(mc)::value;
+                    acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(a[u]), operand(b[u][i]), acc[i], FP4, FP4, 0, int(as[u] >> (8 * block)), 0, int(bs[u][i]));
+                });
+        });
+        if (first + FEW_WAVES * AHEAD < p.ksteps) fetch(first + FEW_WAVES * AHEAD);
+    }
+    static_for<0, MT>([&](auto mc) {
+        constexpr int i = decltype(mc)::value;
+        static_for<0, 4>([&](auto rc) { sums[wave][i][decltype(rc)::value][lane] = acc[i][decltype(rc)::value]; });
+    });
+    __syncthreads();
+    for (int at = threadIdx.x; at < 256 * MT; at += FEW_THREADS) {
+        const int in = at % 16, col = col16 * 16 + in, token = at / 16;
+        if (col >= p.n || row0 + token >= p.m) continue;
+        float v[1] = {0.f};
+#pragma unroll
+        for (int i = 0; i < FEW_WAVES; ++i) v[0] = __fadd_rn(v[0], sums[i][token / 16][in % 4][token % 16 + 16 * (in / 4)]);
+        if (p.bias) v[0] = __fadd_rn(v[0], p.bias[col]);
+        activate_tokens<OUT>(v, p.act, p.slope);
+        Run<OUT, 1> out;
+        out.set(v);
+        out.store(static_cast<char *>(p.out) + ((row0 + token) * p.out_stride + col) * (OUT == TSX_TYPE_F32 ? 4 : 2));
+    }
+}
+
+// codes and scales of weights [n][k] to the layout above
+__global__ __launch_bounds__(256) void pack_mxfp4_kernel(const uint8_t *codes, int64_t codes_stride, const uint8_t *scales, int64_t scales_stride, int n,
+                                                         int bytes, int blocks, int frags, int64_t pieces, int64_t words, int8_t *packed) {
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < pieces + words; i += int64_t(gridDim.x) * 256) {
+        if (i < pieces) {
+            const int lane = int(i % 64);
+            const int64_t unit = i / 64, step = unit / 2 / frags;
+            const int half = int(unit % 2), frag = int(unit / 2 - step * frags);
+            const int col = frag * 32 + lane % 32;
+            const int64_t at = step * KSTEP + (2 * half + lane / 32) * 16;
+            v4i v = {0, 0, 0, 0};
+            if (col < n) {
+                const uint8_t *const from = codes + col * codes_stride + at;
+                if (at + 16 <= bytes) v = __builtin_bit_cast(v4i, v4u(*reinterpret_cast<const v4u_any *>(from)));
+                else
+                    for (int b = 0; b < 16 && at + b < bytes; ++b) v[b / 4] |= int(unsigned(from[b]) << (8 * (b % 4)));
+            }
+            reinterpret_cast<v4i *>(packed)[i] = v;
+        } else {
+            const int64_t word = i - pieces, step = word / (frags * 32);
+            const int col = int(word - step * (frags * 32));
+            unsigned v = 0;
+            for (int b = 0; b < 4; ++b)
+                if (col < n && step * 4 + b < blocks) v |= unsigned(scales[col * scales_stride + step * 4 + b]) << (8 * b);
+            reinterpret_cast<unsigned *>(packed + pieces * 16)[word] = v;
+        }
+    }
+}
+
+// MXFP4 rows of another length, stride or alignment than the kernels read: codes to whole K-steps at `pitch`, scales to words of K-steps
+__global__ __launch_bounds__(256) void copy_mxfp4_kernel(const uint8_t *codes, int64_t codes_stride, const uint8_t *scales, int64_t scales_stride, int bytes,
+                                                         int blocks, int64_t rows, int steps, uint8_t *to, uint8_t *to_scales) {
+    const int64_t pitch = int64_t(steps) * KSTEP, pieces = rows * steps * 4, words = rows * steps;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < pieces + words; i += int64_t(gridDim.x) * 256) {
+        if (i < pieces) {
+            const int64_t row = i / (steps * 4);
+            const int at = int(i - row * (steps * 4)) * 16;
+            v4i v = {0, 0, 0, 0};
+            const uint8_t *const from = codes + row * codes_stride + at;
+            if (at + 16 <= bytes) v = __builtin_bit_cast(v4i, v4u(*reinterpret_cast<const v4u_any *>(from)));
+            else
+                for (int b = 0; b < 16 && at + b < bytes; ++b) v[b / 4] |= int(unsigned(from[b]) << (8 * (b % 4)));
+            *reinterpret_cast<v4i *>(to + row * pitch + at) = v;
+        } else {
+            const int64_t word = i - pieces, step = word / rows, row = word - step * rows;
+            unsigned v = 0;
+            for (int b = 0; b < 4; ++b)
+                if (step * 4 + b < blocks) v |= unsigned(scales[row * scales_stride + step * 4 + b]) << (8 * b);
+            reinterpret_cast<unsigned *>(to_scales)[word] = v;
+        }
+    }
+}
+
+template <int WR, int WC, int FR, int FC, int KS, int S, int OUT>
+int launch_tile(MxGemmParams p, hipStream_t stream) {
+    p.row_tiles = int(ceil_div(p.m, 32 * WR * FR));
+    p.col_tiles = int(ceil_div(p.n, 32 * WC * FC));
+    const int64_t per_xcd = ceil_div(int64_t(p.row_tiles) * p.col_tiles, 8);
+    TSX_REQUIRE(8 * per_xcd * WR * WC * 64 < int64_t(1) << 32, "gemm_mxfp4: %d x %d outputs are more than a launch holds", p.m, p.n);
+    p.tiles_per_xcd = int(per_xcd);
+    constexpr int LDS = S * 32 * (WR * FR + WC * FC) * KS * (KSTEP + 4);
+    const auto kernel = gemm_mxfp4_kernel<WR, WC, FR, FC, KS, S, OUT>;
+    if (LDS > 64 * 1024) {
+        const int rc = grant_lds(reinterpret_cast<const void *>(kernel), LDS);
+        if (rc) return rc;
+    }
+    hipLaunchKernelGGL(kernel, dim3(unsigned(8 * p.tiles_per_xcd)), dim3(WR * WC * 64), LDS, stream, p);
+    TSX_LAUNCH_CHECK("gemm_mxfp4_kernel");
+    return 0;
+}
+
+template <int X, int MT, int AHEAD, int OUT>
+int launch_few(const FewTokens &p, hipStream_t stream) {
+    const dim3 grid(unsigned(ceil_div(p.n, 16)), unsigned(ceil_div(p.m, 16 * MT)));
+    hipLaunchKernelGGL((gemm_mxfp4_few_kernel<X, MT, AHEAD, OUT>), grid, dim3(FEW_THREADS), 0, stream, p);
+    TSX_LAUNCH_CHECK("gemm_mxfp4_few_kernel");
+    return 0;
+}
+template <int X, int OUT>
+int few_of(const FewTokens &p, hipStream_t stream) {
+    if constexpr (X == TSX_TYPE_MXFP4)
+        if (p.m > 16) return launch_few<X, 2, 4, OUT>(p, stream);
+    return launch_few<X, 1, 4, OUT>(p, stream);      // rows of floats: 16 at most
+}
+template <int OUT>
+int few_tokens(const tsx_mxfp4_gemm *g, const MxGemmParams &q, bool quantizes, hipStream_t stream) {
+    FewTokens p{};
+    static_cast<MxGemmParams &>(p) = q;
+    p.values = g->x_dev;
+    p.x_stride = g->m <= 1 ? 0 : g->x_stride;
+    p.cols = g->k;
+    if (quantizes)
+        return g->x_type == TSX_TYPE_F32 ? few_of<TSX_TYPE_F32, OUT>(p, stream)
+               : g->x_type == TSX_TYPE_F16 ? few_of<TSX_TYPE_F16, OUT>(p, stream) : few_of<TSX_TYPE_BF16, OUT>(p, stream);
+    return few_of<TSX_TYPE_MXFP4, OUT>(p, stream);
+}
+
+constexpr int FEW_MOST = 1 << 14;      // rows of the kernel for few tokens: with more their groups of rows leave a launch's second axis
+
+enum class Kernel { few, tile_64, tile_128, tile_256 };
+
+Kernel choose(int m, int n, int k) {
+    if (m <= 32) return Kernel::few;
+    if (int64_t(m) * n >= int64_t(2048) * 2048) return Kernel::tile_256;
+    if (int64_t(m) * n >= int64_t(1024) * 1024) return Kernel::tile_128;
+    return Kernel::tile_64;
+}
+
+template <int OUT>
+int launch(const tsx_mxfp4_gemm *g, const MxGemmParams &p, bool quantizes, hipStream_t stream) {
+    if (quantizes) return few_tokens<OUT>(g, p, true, stream);
+    // TSX_MXFP4_KERNEL: that kernel, by its place in the list above, for any call it can take (tests, measurements)
+    const char *e = std::getenv("TSX_MXFP4_KERNEL");
+    const bool named = e && e[0] >= (p.m <= FEW_MOST ? '0' : '1') && e[0] <= '3';
+    switch (named ? Kernel(e[0] - '0') : choose(p.m, p.n, p.k)) {
+        case Kernel::few: return few_tokens<OUT>(g, p, false, stream);
+        case Kernel::tile_64: return launch_tile<2, 2, 1, 1, 2, 3, OUT>(p, stream);
+        case Kernel::tile_128: return launch_tile<2, 2, 2, 2, 1, 3, OUT>(p, stream);
+        default:
+            if constexpr (OUT == TSX_TYPE_F32) return launch_tile<2, 4, 4, 2, 1, 4, OUT>(p, stream);
+            else return launch_tile<2, 2, 4, 4, 1, 4, OUT>(p, stream);
+    }
+}
+
+int check(const tsx_mxfp4_gemm *g) {
+    TSX_REQUIRE(g, "gemm_mxfp4: null argument");
+    TSX_REQUIRE(g->m >= 0 && g->n > 0 && g->k > 0, "gemm_mxfp4: bad extents");
+    TSX_REQUIRE(g->m < 1 << 28 && g->n < 1 << 24 && g->k < 1 << 21, "gemm_mxfp4: %d rows, %d columns, K = %d (below 2^28, 2^24 and 2^21)", g->m, g->n, g->k);
+    TSX_REQUIRE(is_float_type(g->x_type) || g->x_type == TSX_TYPE_MXFP4, "gemm_mxfp4: element type %d", g->x_type);
+    TSX_REQUIRE(is_float_type(g->out_type), "gemm_mxfp4: output type %d (fp32, fp16 or bf16)", g->out_type);
+    TSX_REQUIRE(is_token_act(g->act), "gemm_mxfp4: activation %d", g->act);
+    const bool codes = g->x_type == TSX_TYPE_MXFP4;
+    TSX_REQUIRE(g->m <= 1 || (g->x_stride >= (codes ? (g->k + 1) / 2 : g->k) && g->out_stride >= g->n && (!codes || g->x_scales_stride >= (g->k + 31) / 32)),
+                "gemm_mxfp4: rows of %d and %d columns overlap at strides %lld, %lld and %lld", g->k, g->n, (long long)g->x_stride, (long long)g->x_scales_stride,
+                (long long)g->out_stride);
+    return 0;
+}
+
+bool is_multiple(const void *at, size_t bytes) { return reinterpret_cast<uintptr_t>(at) % bytes == 0; }
+
+// Whether the product's workgroups quantize the rows themselves
+bool quantizes_itself(const tsx_mxfp4_gemm *g) { return g->x_type != TSX_TYPE_MXFP4 && g->m <= 16; }
+
+// A tile's rows are reached by 32-bit offsets: 256 of them at 2^23.
+bool reads_in_place(const tsx_mxfp4_gemm *g) {
+    return g->x_type == TSX_TYPE_MXFP4 && g->k % MX_STEP == 0 && is_multiple(g->x_dev, 16) && is_multiple(g->x_scales_dev, 4) &&
+           (g->m <= 1 || (g->x_stride % 16 == 0 && g->x_stride <= 1 << 23 && g->x_scales_stride % 4 == 0 && g->x_scales_stride <= 1 << 23));
+}
+
+// the workspace: codes [m][steps][64], scales [steps][m][4]
+int64_t steps_of(int k) { return ceil_div(k, MX_STEP); }
+size_t workspace_bytes(const tsx_mxfp4_gemm *g) {
+    if (g->m == 0 || reads_in_place(g) || quantizes_itself(g)) return 0;
+    return size_t(g->m) * steps_of(g->k) * (KSTEP + 4);
+}
+
+int check_weights(int32_t k, int32_t n) {
+    TSX_REQUIRE(k > 0 && n > 0 && k < 1 << 21 && n < 1 << 24, "gemm_mxfp4: weights of %d columns, K = %d (below 2^24 and 2^21)", n, k);
+    return 0;
+}
+
+}  // namespace
+}  // namespace tsx
+
+extern "C" {
+
+size_t tsx_gemm_mxfp4_packed_weight_bytes(int32_t k, int32_t n) {
+    if (tsx::check_weights(k, n)) return 0;
+    return size_t(tsx::packed_codes(k, n)) + size_t(tsx::ksteps_of(k)) * tsx::frags_of(n) * 128;
+}
+
+int tsx_gemm_mxfp4_pack_weights(int32_t k, int32_t n, const uint8_t *codes_dev, int64_t codes_stride, const uint8_t *scales_dev, int64_t scales_stride,
+                                void *packed_dev, void *stream) {
+    if (const int rc = tsx::check_weights(k, n)) return rc;
+    TSX_REQUIRE(n <= 1 || (codes_stride >= (k + 1) / 2 && scales_stride >= (k + 31) / 32), "gemm_mxfp4: rows of K = %d overlap at strides %lld and %lld", k,
+                (long long)codes_stride, (long long)scales_stride);
+    TSX_REQUIRE(codes_dev && scales_dev && packed_dev, "gemm_mxfp4: null pointer");
+    TSX_REQUIRE(tsx::is_multiple(packed_dev, 16), "gemm_mxfp4: packed weights must be 16-byte aligned");
+    const int64_t pieces = tsx::packed_codes(k, n) / 16, words = int64_t(tsx::ksteps_of(k)) * tsx::frags_of(n) * 32;
+    const int64_t blocks = std::min<int64_t>(tsx::ceil_div(pieces + words, 256), 1 << 16);
+    hipLaunchKernelGGL(tsx::pack_mxfp4_kernel, dim3(unsigned(blocks)), dim3(256), 0, tsx::as_stream(stream), codes_dev, codes_stride, scales_dev, scales_stride,
+                       n, (k + 1) / 2, (k + 31) / 32, tsx::frags_of(n), pieces, words, static_cast<int8_t *>(packed_dev));
+    TSX_LAUNCH_CHECK("pack_mxfp4_kernel");
+    return 0;
+}
+
+size_t tsx_gemm_mxfp4_workspace_bytes(const tsx_mxfp4_gemm *g) {
+    if (tsx::check(g)) return 0;
+    return tsx::workspace_bytes(g);
+}
+
+int tsx_gemm_mxfp4(const tsx_mxfp4_gemm *g, void *workspace_dev, size_t workspace_bytes, void *stream_) {
+    int rc = tsx::check(g);
+    if (rc || g->m == 0) return rc;
+    const bool codes = g->x_type == TSX_TYPE_MXFP4;
+    TSX_REQUIRE(g->x_dev && g->packed_w_dev && g->out_dev, "gemm_mxfp4: null pointer");
+    TSX_REQUIRE(!codes || g->x_scales_dev, "gemm_mxfp4: MXFP4 rows need their scales");
+    TSX_REQUIRE(tsx::is_multiple(g->packed_w_dev, 16), "gemm_mxfp4: packed weights must be 16-byte aligned");
+    TSX_REQUIRE((codes || tsx::is_multiple(g->x_dev, tsx::element_bytes(g->x_type))) && tsx::is_multiple(g->out_dev, tsx::element_bytes(g->out_type)) &&
+                    tsx::is_multiple(g->bias_dev, 4), "gemm_mxfp4: pointer is no multiple of its elements");
+    const size_t need = tsx::workspace_bytes(g);
+    if (need) {
+        if (!workspace_dev || workspace_bytes < need)
+            return tsx::fail(TSX_E_WORKSPACE, "gemm_mxfp4: workspace %zu < %zu bytes", workspace_dev ? workspace_bytes : size_t(0), need);
+        TSX_REQUIRE(tsx::is_multiple(workspace_dev, 16), "gemm_mxfp4: workspace must be 16-byte aligned");
+    }
+    hipStream_t stream = tsx::as_stream(stream_);
+    tsx::MxGemmParams p{};
+    const int steps = int(tsx::steps_of(g->k));
+    p.x_steps = steps;
+    p.k = steps * tsx::KSTEP;
+    const bool quantizes = tsx::quantizes_itself(g);
+    if (need) {
+        uint8_t *const to = static_cast<uint8_t *>(workspace_dev), *const to_scales = to + int64_t(g->m) * p.k;
+        p.x = to;
+        p.x_scales = to_scales;
+        p.x_pitch = p.k;
+        p.scale_row = 4;
+        p.scale_step = int64_t(g->m) * 4;
+        if (codes) {
+            const int64_t units = int64_t(g->m) * steps * 5, blocks = tsx::ceil_div(units, 256);
+            hipLaunchKernelGGL(tsx::copy_mxfp4_kernel, dim3(unsigned(std::min<int64_t>(blocks, 1 << 16))), dim3(256), 0, stream, static_cast<const uint8_t *>(g->x_dev),
+                               g->x_stride, g->x_scales_dev, g->x_scales_stride, (g->k + 1) / 2, (g->k + 31) / 32, int64_t(g->m), steps, to, to_scales);
+            TSX_LAUNCH_CHECK("copy_mxfp4_kernel");
+        } else {
+            rc = tsx::quantize_mxfp4_rows(g->m, g->k, steps * tsx::MX_STEP, g->x_dev, g->x_type, g->x_stride,
+                                          tsx::MxRows{to, to_scales, p.x_pitch, p.scale_row, p.scale_step}, stream);
+            if (rc) return rc;
+        }
+    } else if (!quantizes) {
+        p.x = static_cast<const uint8_t *>(g->x_dev);
+        p.x_scales = g->x_scales_dev;
+        p.x_pitch = g->m <= 1 ? 0 : g->x_stride;
+        p.scale_row = g->m <= 1 ? 0 : g->x_scales_stride;
+        p.scale_step = 4;
+    }
+    p.w = static_cast<const int8_t *>(g->packed_w_dev);
+    p.w_scales = p.w + tsx::packed_codes(g->k, g->n);
+    p.bias = g->bias_dev;
+    p.out = g->out_dev;
+    p.out_stride = g->out_stride;
+    p.m = g->m;
+    p.n = g->n;
+    p.frags = tsx::frags_of(g->n);
+    p.ksteps = tsx::ksteps_of(g->k);
+    p.act = g->act;
+    p.slope = g->slope;
+    return g->out_type == TSX_TYPE_F32 ? tsx::launch<TSX_TYPE_F32>(g, p, quantizes, stream) : g->out_type == TSX_TYPE_F16 ? tsx::launch<TSX_TYPE_F16>(g, p, quantizes, stream)
+                                                                                                          : tsx::launch<TSX_TYPE_BF16>(g, p, quantizes, stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,231 @@
+// Root-mean-square norm of rows, with the residual's addition in front of it; the result in the rows' type, as int8 tokens or as MXFP4.
+//
+//     h = x + residual, rounded to their type;  y = h w r,  r = 1 / sqrt(mean(h^2) + epsilon)
+//
+// Bound: HBM, four times the element size a value with a residual.  A row is read once: T threads share it and hold h and the weight in registers, eight values to a piece, while they find
+// the sum of its squares.  As int8 tokens a row's codes do not know r: with A the largest |h w|, y's largest magnitude is A r, and
+// y 127 / (A r) = h w 127 / A; so the search for A shares the one exchange between the threads with the sum, and only the scale, A r / 127, waits for r.
+#pragma once
+#include "mxfp4.hpp"
+
+namespace tsx {
+
+constexpr int NORM_ROWS = 0, NORM_TOKENS = 1, NORM_MXFP4 = 2;      // what leaves
+
+struct RmsNormParams {
+    const void *x, *residual;
+    void *sum;
+    const float *weight;
+    void *out;                    // rows of x's type, int8 or codes
+    void *scales;                 // fp32, or a byte a block
+    int64_t rows, x_stride, residual_stride, sum_stride, out_stride, scales_stride;
+    int cols;
+    float inv_cols, epsilon;
+};
+
+int rms_norm_rows(const RmsNormParams &p, int type, hipStream_t stream);
+int rms_norm_tokens(const RmsNormParams &p, int type, hipStream_t stream);
+int rms_norm_mxfp4(const RmsNormParams &p, int type, hipStream_t stream);
+
+#ifdef __HIPCC__
+
+// A row whose mean square (with epsilon) leaves [2^-120, infinity) in fp32 is taken times a power of two instead; inside, what squares below 2^-126
+// lose is 2^-30 of the mean.  Above: by 2^-80, so that 2^30 squares of the largest number stay below 2^126.  Below: by 2^105; the largest
+// number that can be there, 2^-45 alone among 2^30 columns, becomes 2^60, and the mean with the least one, 2^-149 alone among them, 2^-118.
+constexpr float NORM_LEAST = 0x1p-120f, NORM_DOWN = 0x1p-80f, NORM_UP = 0x1p105f;
+
+template <int TYPE, int TO, int T, int P, bool HELD>
+__global__ __launch_bounds__(T < 256 ? 256 : T) void rms_norm_kernel(RmsNormParams p) {
+    constexpr int PIECE = 8, THREADS = T < 256 ? 256 : T, ROWS = THREADS / T, SIZE = TYPE == TSX_TYPE_F32 ? 4 : 2, WAVES = T / 64;
+    constexpr int LG = lg_of(T < 64 ? T : 64);
+    typedef Run<TYPE, PIECE> Values;
+    typedef Run<TSX_TYPE_F32, PIECE> Weights;
+    __shared__ float sums[T > 64 ? WAVES : 1], tops[T > 64 ? WAVES : 1];
+    const int tid = threadIdx.x, t = tid % T;
+    const int pieces = (p.cols + PIECE - 1) / PIECE, whole = p.cols / PIECE, in_last = p.cols - whole * PIECE;
+    const int turns = HELD ? 1 : (pieces + T * P - 1) / (T * P);
+    for (int64_t row0 = int64_t(blockIdx.x) * ROWS; row0 < p.rows; row0 += int64_t(gridDim.x) * ROWS) {
+        const int64_t row = row0 + tid / T;
+        const bool there = row < p.rows;      // a row's threads agree; only T <= 64 has rows beyond the last one, which are that one again
+        const int64_t at = there ? row : p.rows - 1;
+        const char *const x = static_cast<const char *>(p.x) + at * p.x_stride * SIZE;
+        const char *const residual = static_cast<const char *>(p.residual) + at * p.residual_stride * SIZE;
+        char *const sum = static_cast<char *>(p.sum) + at * p.sum_stride * SIZE;
+        Values h[P];
+        Weights w[P];
+        // P pieces of a row of values; all requests at once, none behind a branch, where it would be waited for: what lies behind the last whole piece is that
+        // piece again, and then zeros, or the values that are left there
+        auto load = [&](auto &v, const char *from, int first) __attribute__((always_inline)) {
+            typedef std::remove_reference_t<decltype(v[0])> Piece;
+            constexpr int BYTES = Piece::BYTES;
+            if (whole)       // uniform
+                static_for<0, P>([&](auto ic) { v[decltype(ic)::value].load(from + int64_t(min(first + t + decltype(ic)::value * T, whole - 1)) * BYTES); });
+            if (in_last || pieces < turns * T * P) {       // uniform
+                Piece last;
+                last.clear();
+                if (in_last) last.load_some(from + int64_t(whole) * BYTES, in_last);
+                static_for<0, P>([&](auto ic) {
+                    constexpr int i = decltype(ic)::value;
+                    const int piece = first + t + i * T;
+                    if (piece >= whole) v[i].clear();
+                    if (piece == whole) v[i] = last;
+                });
+            }
+        };
+        auto store = [&](const Values &v, char *to, int piece) __attribute__((always_inline)) {
+            if (!there || piece >= pieces) return;
+            if (piece < whole) v.store(to + int64_t(piece) * (PIECE * SIZE));
+            else v.store_some(to + int64_t(piece) * (PIECE * SIZE), in_last);
+        };
+        auto fetch_weight = [&](int first) __attribute__((always_inline)) {
+            if (p.weight) load(w, reinterpret_cast<const char *>(p.weight), first);
+            else static_for<0, P>([&](auto ic) { static_for<0, PIECE>([&](auto ec) { w[decltype(ic)::value].word[decltype(ec)::value] = 0x3f800000u; }); });
+        };
+        // h of a turn; again: as it was kept
+        auto fetch = [&](int first, bool again) __attribute__((always_inline)) {
+            if (again && p.sum) {
+                load(h, sum, first);
+            } else {
+                load(h, x, first);
+                if (p.residual) {
+                    Values r[P];
+                    load(r, residual, first);
+                    static_for<0, P>([&](auto ic) {
+                        constexpr int i = decltype(ic)::value;
+                        float v[PIECE];
+                        static_for<0, PIECE>([&](auto ec) { constexpr int e = decltype(ec)::value; v[e] = __fadd_rn(h[i].template get<e>(), r[i].template get<e>()); });
+                        h[i].set(v);
+                    });
+                }
+                if (p.sum) static_for<0, P>([&](auto ic) { store(h[decltype(ic)::value], sum, first + t + decltype(ic)::value * T); });
+            }
+        };
+        // the sum of (h lift)^2 and the largest |h lift w| over the row, in all its threads
+        float squares, top;
+        auto statistics = [&](auto lifted, float lift, bool again) __attribute__((always_inline)) {
+            constexpr bool LIFTED = decltype(lifted)::value;
+            double long_sum = 0;                  // over turns
+            unsigned most = 0;                    // magnitudes' bits sort as they do, infinities and NaN last
+            for (int turn = 0; turn < turns; ++turn) {
+                if (!HELD || !again) fetch(turn * T * P, again);
+                if (TO == NORM_TOKENS && (!HELD || !again)) fetch_weight(turn * T * P);
+                float s[2] = {0.f, 0.f};
+                static_for<0, P>([&](auto ic) {
+                    constexpr int i = decltype(ic)::value;
+                    static_for<0, PIECE>([&](auto ec) {
+                        constexpr int e = decltype(ec)::value;
+                        float v = h[i].template get<e>();
+                        if (LIFTED) v = __fmul_rn(v, lift);
+                        s[e % 2] = __builtin_fmaf(v, v, s[e % 2]);
+                        if constexpr (TO == NORM_TOKENS) most = max(most, __builtin_bit_cast(unsigned, __fmul_rn(v, w[i].template get<e>())) & 0x7fffffffu);
+                    });
+                });
+                if (HELD) squares = s[0] + s[1];
+                else long_sum += double(s[0]) + double(s[1]);
+            }
+            if (!HELD) squares = float(long_sum);
+            squares = sum_over_lanes(squares, LG);
+            if constexpr (TO == NORM_TOKENS) most = over_lanes(most, LG, [](unsigned a, unsigned b) { return max(a, b); });
+            if constexpr (T > 64) {
+                if (tid % 64 == 0) sums[tid / 64] = squares, tops[tid / 64] = __builtin_bit_cast(float, most);
+                __syncthreads();
+                squares = 0.f;
+#pragma unroll
+                for (int i = 0; i < WAVES; ++i) squares += sums[i], most = max(most, __builtin_bit_cast(unsigned, tops[i]));
+                __syncthreads();                  // the next row writes them
+            }
+            top = __builtin_bit_cast(float, most);
+        };
+        if (TO != NORM_TOKENS && HELD) fetch_weight(0);
+        statistics(std::false_type{}, 1.f, false);
+        float mean = __builtin_fmaf(squares, p.inv_cols, p.epsilon), lift = 1.f;
+        if (!(mean >= NORM_LEAST && mean < __builtin_inff())) {       // a row's threads agree
+            lift = mean < NORM_LEAST ? NORM_UP : NORM_DOWN;
+            statistics(std::true_type{}, lift, true);
+            mean = __builtin_fmaf(squares, p.inv_cols, __fmul_rn(__fmul_rn(p.epsilon, lift), lift));
+        }
+        const float r = __builtin_amdgcn_rsqf(mean);
+        const TokenScale token(top);
+        if (TO == NORM_TOKENS && there && t == 0)
+            static_cast<float *>(p.scales)[row] = top < __builtin_inff() ? __fdiv_rn(__fmul_rn(top, r), 127.f) : __builtin_nanf("");
+        char *const out = static_cast<char *>(p.out) + at * p.out_stride * (TO == NORM_ROWS ? SIZE : 1);
+        for (int turn = 0; turn < turns; ++turn) {
+            if (!HELD) fetch(turn * T * P, true), fetch_weight(turn * T * P);
+            static_for<0, P>([&](auto ic) {
+                constexpr int i = decltype(ic)::value;
+                const int piece = turn * T * P + t + i * T;
+                float y[PIECE];
+                static_for<0, PIECE>([&](auto ec) { constexpr int e = decltype(ec)::value; y[e] = __fmul_rn(__fmul_rn(h[i].template get<e>(), lift), w[i].template get<e>()); });
+                if constexpr (TO == NORM_ROWS) {
+                    static_for<0, PIECE>([&](auto ec) { constexpr int e = decltype(ec)::value; y[e] = __fmul_rn(y[e], r); });
+                    Values v;
+                    v.set(y);
+                    store(v, out, piece);
+                } else if constexpr (TO == NORM_TOKENS) {
+                    if (!there || piece >= pieces) return;
+                    unsigned b[PIECE];
+                    static_for<0, PIECE>([&](auto ec) { constexpr int e = decltype(ec)::value; b[e] = token.bits(__fmul_rn(y[e], token.lift)); });
+                    v2u q = {low_bytes(b[0], b[1], b[2], b[3]), low_bytes(b[4], b[5], b[6], b[7])};
+                    if (token.reciprocal == 0.f) q = v2u{0, 0};
+                    char *const to = out + int64_t(piece) * PIECE;
+                    if (piece < whole) {
+                        *reinterpret_cast<v2u_any *>(to) = q;
+                    } else {
+                        static_for<0, PIECE - 1>([&](auto ec) {
+                            constexpr int e = decltype(ec)::value;
+                            if (e < in_last) to[e] = char(q[e / 4] >> (8 * (e % 4)));
+                        });
+                    }
+                } else {
+                    static_for<0, PIECE>([&](auto ec) { constexpr int e = decltype(ec)::value; y[e] = __fmul_rn(y[e], r); });
+                    Weights v;
+                    v.set(y);
+                    // a block's four lanes: pieces behind the row's end are zeros, but for r: NaN and infinities have to come from the row itself
+                    const unsigned own = piece < pieces ? v.top(0) : 0u;
+                    const unsigned scale = mx_scale(__builtin_bit_cast(float, over_lanes(own, T < 4 ? 0 : 2, [](unsigned a, unsigned b) { return max(a, b); })));
+                    const unsigned codes = mx_codes<TSX_TYPE_F32>(v, scale);
+                    if (!there || piece >= pieces) return;
+                    store_codes(reinterpret_cast<uint8_t *>(out) + int64_t(piece) * (PIECE / 2), codes, piece < whole ? PIECE : in_last);
+                    if (piece % 4 == 0) static_cast<uint8_t *>(p.scales)[at * p.scales_stride + piece / 4] = uint8_t(scale);
+                }
+            });
+        }
+    }
+}
+
+template <int TYPE, int TO, int T, int P, bool HELD>
+int launch_rms_norm(const RmsNormParams &p, hipStream_t stream) {
+    constexpr int THREADS = T < 256 ? 256 : T, ROWS = THREADS / T;
+    const int64_t blocks = ceil_div(p.rows, ROWS), most = int64_t(1) << 20;       // beyond that a workgroup takes several rows
+    hipLaunchKernelGGL((rms_norm_kernel<TYPE, TO, T, P, HELD>), dim3(unsigned(blocks < most ? blocks : most)), dim3(THREADS), 0, stream, p);
+    TSX_LAUNCH_CHECK("rms_norm_kernel");
+    return 0;
+}
+
+template <int TYPE, int TO>
+int rms_norm_type(const RmsNormParams &p, hipStream_t stream) {
+    // Several rows a wavefront where they are short, a wavefront a row, with no barrier, while there are rows for all CUs; more threads a
+    // row where there are few rows or it is long.
+    const int64_t pieces = ceil_div(p.cols, 8);
+    if (pieces <= 4) return launch_rms_norm<TYPE, TO, 4, 1, true>(p, stream);
+    if (pieces <= 16) return launch_rms_norm<TYPE, TO, 16, 1, true>(p, stream);
+    if (pieces <= 64) return launch_rms_norm<TYPE, TO, 64, 1, true>(p, stream);
+    if (p.rows >= 512 || pieces <= 128) {
+        if (pieces <= 128) return launch_rms_norm<TYPE, TO, 64, 2, true>(p, stream);
+        if (pieces <= 256) return launch_rms_norm<TYPE, TO, 64, 4, true>(p, stream);
+    }
+    if (pieces <= 256) return launch_rms_norm<TYPE, TO, 256, 1, true>(p, stream);
+    if (pieces <= 512) return launch_rms_norm<TYPE, TO, 256, 2, true>(p, stream);
+    if (pieces <= 1024) return launch_rms_norm<TYPE, TO, 256, 4, true>(p, stream);
+    if (pieces <= 2048) return launch_rms_norm<TYPE, TO, 1024, 2, true>(p, stream);
+    return launch_rms_norm<TYPE, TO, 1024, 2, false>(p, stream);
+}
+template <int TO>
+int rms_norm_of(const RmsNormParams &p, int type, hipStream_t stream) {
+    return type == TSX_TYPE_F32 ? rms_norm_type<TSX_TYPE_F32, TO>(p, stream) : type == TSX_TYPE_F16 ? rms_norm_type<TSX_TYPE_F16, TO>(p, stream)
+                                                                                                    : rms_norm_type<TSX_TYPE_BF16, TO>(p, stream);
+}
+
+#endif  // __HIPCC__
+
+}  // namespace tsx

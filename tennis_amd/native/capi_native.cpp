@@ -35,7 +35,8 @@ namespace {
     X(tsx_winograd_f63_fast_workspace_bytes) X(tsx_winograd_f23_workspace_bytes) X(tsx_conv2d_winograd_f63_nchw)            \
     X(tsx_conv2d_winograd_f63_fast_nchw) X(tsx_conv2d_winograd_f23_nchw) X(tsx_quantize_tokens)                             \
     X(tsx_gemm_i8_tokens_workspace_bytes) X(tsx_gemm_i8_tokens) X(tsx_group_norm_workspace_bytes) X(tsx_group_norm_nhwc)    \
-    X(tsx_group_norm_tokens_nhwc)
+    X(tsx_group_norm_tokens_nhwc) X(tsx_dequantize_tokens) X(tsx_quantize_mxfp4) X(tsx_dequantize_mxfp4)                    \
+    X(tsx_gemm_mxfp4_workspace_bytes) X(tsx_gemm_mxfp4) X(tsx_rms_norm_rows) X(tsx_rms_norm_tokens) X(tsx_rms_norm_mxfp4)
 
 struct Library {
 #define X(name) decltype(&::name) name;
@@ -819,6 +820,158 @@ PyObject *group_norm(PyObject *const *a, Py_ssize_t) {                // x, grou
     return tokens ? results(out, scales) : wrap(out);
 }
 
+// ---- MXFP4 rows, root-mean-square norm
+
+c10::ScalarType float_type(int32_t code) { return code == TSX_TYPE_F32 ? c10::kFloat : code == TSX_TYPE_F16 ? c10::kHalf : c10::kBFloat16; }
+
+// x's shape with another last axis
+c10::SmallVector<int64_t, 6> with_last(const at::Tensor &x, int64_t last) {
+    c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = last;
+    return shape;
+}
+int64_t code_bytes(int64_t k) { return (k + 1) / 2; }
+int64_t blocks(int64_t k) { return (k + 31) / 32; }
+
+const at::Tensor &bytes(PyObject *o) {
+    const at::Tensor &t = strided(o);
+    if (t.scalar_type() != c10::kByte) throw Decline{};
+    return t;
+}
+// MXFP4 rows' scales, a row for each of theirs
+Rows scale_rows(const at::Tensor &scales, const at::Tensor &codes, int64_t k) {
+    if (scales.dim() != codes.dim() || scales.sizes().slice(0, scales.dim() - 1) != codes.sizes().slice(0, codes.dim() - 1) || scales.size(-1) != blocks(k))
+        throw Decline{};
+    return Rows(scales);
+}
+
+PyObject *quantize_mxfp4(PyObject *const *a, Py_ssize_t) {            // x
+    const at::Tensor &x = strided(a[0]);
+    const int32_t type = type_code(x.scalar_type());
+    if (type == TSX_TYPE_I8) throw Decline{};
+    const Rows r(x);
+    at::TensorBase codes, scales;
+    launch([&] {
+        codes = empty(with_last(x, code_bytes(r.cols)), c10::kByte, x);
+        scales = empty(with_last(x, blocks(r.cols)), c10::kByte, x);
+        return L.tsx_quantize_mxfp4(r.rows, r.cols, x.const_data_ptr(), type, r.stride, data<uint8_t>(codes), code_bytes(r.cols), data<uint8_t>(scales),
+                                    blocks(r.cols), stream());
+    });
+    return results(codes, scales);
+}
+
+PyObject *dequantize(PyObject *const *a, Py_ssize_t) {                // int8 tokens or codes, scales, k (codes; else below 0), output type
+    const at::Tensor &q = strided(a[0]);
+    long k = integer(a[2]);
+    const long type = integer(a[3]);
+    if (type < 0 || type > TSX_TYPE_BF16) throw Decline{};
+    const Rows r(q);
+    at::TensorBase out;
+    if (k < 0) {
+        if (q.scalar_type() != c10::kChar) throw Decline{};
+        const float *scales = f32_of(a[1], r.rows);
+        if (!scales) throw Decline{};
+        launch([&] {
+            out = empty(q.sizes(), float_type(int32_t(type)), q);
+            return L.tsx_dequantize_tokens(r.rows, r.cols, q.const_data_ptr<int8_t>(), r.stride, scales, out.mutable_data_ptr(), int32_t(type), r.cols, stream());
+        });
+        return wrap(out);
+    }
+    const at::Tensor &codes = bytes(a[0]), &scales = bytes(a[1]);
+    if (k == 0) k = 2 * long(r.cols);
+    if (k > 1 << 30 || code_bytes(k) != r.cols) throw Decline{};
+    const Rows s = scale_rows(scales, codes, k);
+    launch([&] {
+        out = empty(with_last(codes, k), float_type(int32_t(type)), codes);
+        return L.tsx_dequantize_mxfp4(r.rows, int32_t(k), codes.const_data_ptr<uint8_t>(), r.stride, scales.const_data_ptr<uint8_t>(), s.stride,
+                                      out.mutable_data_ptr(), int32_t(type), k, stream());
+    });
+    return wrap(out);
+}
+
+PyObject *mxfp4_gemm(PyObject *const *a, Py_ssize_t) {                // packed, k, n, bias, x, x_scales, act, slope, out_type
+    const at::Tensor &packed = tensor(a[0], c10::kByte), &x = strided(a[4]);
+    tsx_mxfp4_gemm g{};
+    g.k = int32_t(integer(a[1]));
+    g.n = int32_t(integer(a[2]));
+    const Rows r(x);
+    const bool codes = a[5] != Py_None;
+    if (r.cols != (codes ? code_bytes(g.k) : int64_t(g.k)) || r.rows >= 1 << 28 || packed.get_device() != x.get_device()) throw Decline{};
+    g.m = int32_t(r.rows);
+    g.x_type = codes ? TSX_TYPE_MXFP4 : type_code(x.scalar_type());
+    g.x_stride = r.stride;
+    g.x_dev = x.const_data_ptr();
+    if (codes) {
+        const at::Tensor &scales = bytes(a[5]);
+        g.x_scales_stride = scale_rows(scales, bytes(a[4]), g.k).stride;
+        g.x_scales_dev = scales.const_data_ptr<uint8_t>();
+    } else if (g.x_type == TSX_TYPE_I8) {
+        throw Decline{};
+    }
+    g.bias_dev = f32_of(a[3], g.n);
+    g.act = int32_t(integer(a[6]));
+    g.slope = float(number(a[7]));
+    const long out_type = integer(a[8]);
+    if (out_type > TSX_TYPE_BF16 || (out_type < 0 && codes)) throw Decline{};
+    g.out_type = out_type < 0 ? g.x_type : int32_t(out_type);
+    g.out_stride = g.n;
+    g.packed_w_dev = packed.const_data_ptr();
+    at::TensorBase out;
+    launch([&] {
+        out = empty(with_last(x, g.n), float_type(g.out_type), x);
+        g.out_dev = out.mutable_data_ptr();
+        const size_t need = L.tsx_gemm_mxfp4_workspace_bytes(&g);
+        at::TensorBase workspace;
+        if (need) workspace = empty({int64_t(need)}, c10::kByte, x);
+        return L.tsx_gemm_mxfp4(&g, data<void>(workspace), need, stream());
+    });
+    return wrap(out);
+}
+
+PyObject *rms_norm(PyObject *const *a, Py_ssize_t) {                  // x, weight, epsilon, residual, to: 0 rows, 1 int8 tokens, 2 MXFP4
+    const at::Tensor &x = strided(a[0]);
+    tsx_rms_norm g{};
+    g.type = type_code(x.scalar_type());
+    if (g.type == TSX_TYPE_I8) throw Decline{};
+    const Rows r(x);
+    g.rows = r.rows;
+    g.cols = r.cols;
+    g.x_dev = x.const_data_ptr();
+    g.x_stride = r.stride;
+    g.weight_dev = f32_of(a[1], r.cols);
+    g.epsilon = float(number(a[2]));
+    const bool adds = a[3] != Py_None;
+    if (adds) {
+        const at::Tensor &residual = strided(a[3]);
+        if (residual.scalar_type() != x.scalar_type() || residual.sizes() != x.sizes()) throw Decline{};
+        g.residual_dev = residual.const_data_ptr();
+        g.residual_stride = Rows(residual).stride;
+    }
+    const long to = integer(a[4]);
+    at::TensorBase out, scales, sum;
+    launch([&] {
+        if (adds) {
+            sum = empty(x.sizes(), x.scalar_type(), x);
+            g.sum_dev = sum.mutable_data_ptr();
+            g.sum_stride = r.cols;
+        }
+        if (to == 0) {
+            out = empty(x.sizes(), x.scalar_type(), x);
+            return L.tsx_rms_norm_rows(&g, out.mutable_data_ptr(), r.cols, stream());
+        }
+        if (to == 1) {
+            out = empty(x.sizes(), c10::kChar, x);
+            scales = empty(x.sizes().slice(0, x.dim() - 1), c10::kFloat, x);
+            return L.tsx_rms_norm_tokens(&g, data<int8_t>(out), data<float>(scales), stream());
+        }
+        out = empty(with_last(x, code_bytes(r.cols)), c10::kByte, x);
+        scales = empty(with_last(x, blocks(r.cols)), c10::kByte, x);
+        return L.tsx_rms_norm_mxfp4(&g, data<uint8_t>(out), data<uint8_t>(scales), stream());
+    });
+    if (to == 0) return adds ? results(out, sum) : wrap(out);
+    return adds ? results(out, scales, sum) : results(out, scales);
+}
+
 // ---- module
 
 PyObject *bind(PyObject *, PyObject *args) {           // {entry point: address}, TsxError
@@ -850,6 +1003,7 @@ PyMethodDef methods[] = {
     TSX_METHOD(pooling2d, 6), TSX_METHOD(max_pooling2d_staged, 5), TSX_METHOD(conv2d_f32, 9), TSX_METHOD(depthwise_conv2d, 9),
     TSX_METHOD(inner_prod_f32, 3), TSX_METHOD(winograd, 10), TSX_METHOD(gemm_i8, 13), TSX_METHOD(conv_i8, 14), TSX_METHOD(conv_i8_staged, 12),
     TSX_METHOD(quantize_tokens, 1), TSX_METHOD(token_gemm, 10), TSX_METHOD(group_norm, 8),
+    TSX_METHOD(quantize_mxfp4, 1), TSX_METHOD(dequantize, 4), TSX_METHOD(mxfp4_gemm, 9), TSX_METHOD(rms_norm, 5),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tsx_native", "The host work of tennis_amd.capi's calls.", -1, methods, nullptr, nullptr, nullptr, nullptr};
