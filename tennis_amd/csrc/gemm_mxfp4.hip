@@ -23,9 +23,9 @@ constexpr int KSTEP = MX_STEP / 2;     // bytes of codes
 constexpr int FP4 = 4;                 // the instructions' number for this type
 
 // Packed weights: codes [K-step][fragment of 32 columns][half of the K-step][lane][16], as the 32x32x64 instruction takes them, behind
-// them scales [K-step][column][4].  Columns in whole groups of 128, K-steps in pairs; zeros behind n and k, whose scales are 2^-127.
+// them scales [K-step][column][4].  Columns in whole groups of 128, K-steps in whole chunks of every kernel, fours; zeros behind n and k, whose scales are 2^-127.
 int frags_of(int n) { return int(round_up(n, 128) / 32); }
-int ksteps_of(int k) { return int(round_up(ceil_div(k, MX_STEP), 2)); }
+int ksteps_of(int k) { return int(round_up(ceil_div(k, MX_STEP), 4)); }
 int64_t packed_codes(int k, int n) { return int64_t(ksteps_of(k)) * frags_of(n) * 2048; }
 
 struct MxGemmParams {
@@ -39,6 +39,7 @@ struct MxGemmParams {
     float slope;
     int act;
     int row_tiles, col_tiles, tiles_per_xcd;
+    bool streams;                      // outputs are more than the L2s hold: past them
 };
 
 __device__ __forceinline__ v8i operand(v4i v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
@@ -67,33 +68,45 @@ __device__ __forceinline__ void word_to_lds(const uint8_t *at, int8_t *lds) {
     __builtin_amdgcn_global_load_lds((global_void *)at, (lds_void *)lds, 4, 0, 0);
 }
 
+// A wavefront's reads of LDS are done and its requests but the last N here, then those of all wavefronts.  In one piece: in front of a barrier of its
+// own the compiler waits for every request.
+template <int N>
+__device__ __forceinline__ void barrier_but_for() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
+
 // A sum, taken from the accumulators here and not before: all of them taken at once would not fit the other registers.
 __device__ __forceinline__ float sum_of(float v) {
     asm volatile("" : "+v"(v));
     return v;
 }
 
-// WR x WC wavefronts, each with FR x FC fragments of 32 tokens x 32 columns; S chunks of KS K-steps in LDS, a K-step's scales behind its codes.
-template <int WR, int WC, int FR, int FC, int KS, int S, int OUT>
-__global__ __launch_bounds__(WR *WC * 64, WR * FR == 4 ? 3 : 1) void gemm_mxfp4_kernel(MxGemmParams p) {
-    constexpr int CHUNK = KS * KSTEP, PIECES = CHUNK / 16, WAVES = WR * WC, ROWS = 32 * WR * FR, COLS = 32 * WC * FC, HALVES = 2 * KS;
+// WR x WC wavefronts, each with FR x FC fragments of 32 tokens x 32 columns; S chunks of KS K-steps in LDS, scales behind their codes; KG such groups of
+// wavefronts, each with its part of every chunk's K-steps.
+//
+// Bound: 8192^3 260 us, 4.2 P operations/s, where the matrix cores are busy for 60 % of the cycles at 1.7 GHz, the clock that the card's power leaves
+// (the same instructions on random operands from registers, nothing else: 6.5 P, at 1.55 GHz).  Each multiplication takes 32 cycles of its SIMD; a
+// tile's epilogue and first chunk are 9 us of 67.  4 x 4 fragments on four wavefronts read a third less LDS and take 268 us, one wavefront a SIMD hides less.
+// Few tiles with a long K wait for one K-step after the other, 0.19 us each in tiles of 64; two groups of wavefronts halve that.
+template <int WR, int WC, int FR, int FC, int KS, int S, int KG, int OUT>
+__global__ __launch_bounds__(WR *WC *KG * 64, WR * FR == 4 && KG == 1 ? 3 : 1) void gemm_mxfp4_kernel(MxGemmParams p) {
+    constexpr int CHUNK = KS * KSTEP, PIECES = CHUNK / 16, WAVES = WR * WC * KG, ROWS = 32 * WR * FR, COLS = 32 * WC * FC, HALVES = 2 * KS / KG;
     constexpr int A_BYTES = ROWS * CHUNK, B_BYTES = COLS * CHUNK, A_LOADS = A_BYTES / 1024 / WAVES, B_LOADS = B_BYTES / 1024 / WAVES;
-    constexpr int A_WORDS = KS * ROWS / 64, S_LOADS = KS * (ROWS + COLS) / 64 / WAVES;      // requests of 64 words of scales
+    constexpr int A_WORDS = KS * ROWS / 64, WORDS = KS * (ROWS + COLS) / 64, S_LOADS = (WORDS + WAVES - 1) / WAVES;      // scales: by 64 words
     constexpr int SCALES = A_BYTES + B_BYTES, BUFFER = SCALES + KS * (ROWS + COLS) * 4, LOADS = A_LOADS + B_LOADS + S_LOADS;
-    static_assert(A_LOADS * 1024 * WAVES == A_BYTES && B_LOADS * 1024 * WAVES == B_BYTES && S_LOADS * 64 * WAVES == KS * (ROWS + COLS) && (S - 1) * LOADS < 64,
+    static_assert(4 % KS == 0, "the weights hold whole chunks");
+    static_assert(A_LOADS * 1024 * WAVES == A_BYTES && B_LOADS * 1024 * WAVES == B_BYTES && S >= 3 && (S - 1) * LOADS < 64,
                   "whole loads, counted in six bits");
     extern __shared__ __attribute__((aligned(16))) int8_t lds[];      // [S][BUFFER]
     __shared__ __attribute__((aligned(16))) float of_cols[COLS];      // biases, requested ahead of everything
     constexpr int THREADS = WAVES * 64;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int wave_r = wave / WC, wave_c = wave % WC;
+    const int in_group = wave % (WR * WC), k_group = wave / (WR * WC), wave_r = in_group / WC, wave_c = in_group % WC;
     // blockIdx % 8 is the XCD: each takes a run of consecutive tiles, which walk four row tiles before the next column tile
     const int tiles = p.row_tiles * p.col_tiles;
     const int t = int(blockIdx.x % 8) * p.tiles_per_xcd + int(blockIdx.x / 8);
     if (int(blockIdx.x / 8) >= p.tiles_per_xcd || t >= tiles) return;      // uniform, ahead of every barrier
-    const int group = t / (4 * p.col_tiles), in_group = t - group * 4 * p.col_tiles;
+    const int group = t / (4 * p.col_tiles), in_four = t - group * 4 * p.col_tiles;
     const int group_rows = min(4, p.row_tiles - 4 * group);
-    const int tile_c = in_group / group_rows, tile_r = 4 * group + in_group - tile_c * group_rows;
+    const int tile_c = in_four / group_rows, tile_r = 4 * group + in_four - tile_c * group_rows;
     const int row0 = tile_r * ROWS, frag0 = tile_c * (COLS / 32);
     constexpr int COL_TURNS = (COLS + THREADS - 1) / THREADS;
     float col_bias[COL_TURNS];
@@ -103,8 +116,8 @@ __global__ __launch_bounds__(WR *WC * 64, WR * FR == 4 ? 3 : 1) void gemm_mxfp4_
     // A row in LDS is its CHUNK bytes, its pieces of 16 XORed with bits of the row that make 16 rows cover all banks for one piece.  A
     // load instruction fills 1 KiB of such rows; rows beyond m are the last one again, never stored.  Pieces behind the end of a row are
     // its first one, against weights that are zero.  Scalar bases and 32-bit lane offsets.
-    const auto key_of = [](int row) { return (row >> (KS == 1 ? 2 : 1)) & (PIECES - 1); };
-    const int chunks = p.ksteps / KS;
+    const auto key_of = [](int row) { return (row >> (KS == 1 ? 2 : KS == 2 ? 1 : 0)) & (PIECES - 1); };
+    const int chunks = (p.x_steps + KS - 1) / KS;
     const uint8_t *const a_base = p.x + int64_t(row0) * p.x_pitch;
     unsigned a_off[A_LOADS], b_off[B_LOADS], s_off[S_LOADS];
     int a_piece[A_LOADS];
@@ -127,7 +140,7 @@ __global__ __launch_bounds__(WR *WC * 64, WR * FR == 4 ? 3 : 1) void gemm_mxfp4_
     int s_step[S_LOADS], s_last[S_LOADS];
     static_for<0, S_LOADS>([&](auto ic) {
         constexpr int i = decltype(ic)::value;
-        const int unit = wave * S_LOADS + i, of_w = unit - A_WORDS;
+        const int unit = min(wave * S_LOADS + i, WORDS - 1), of_w = unit - A_WORDS;      // more wavefronts than requests: the last one again
         const bool is_x = unit < A_WORDS;
         s_step[i] = is_x ? unit / (ROWS / 64) : of_w / (COLS / 64);
         s_base[i] = is_x ? p.x_scales + int64_t(row0) * p.scale_row : reinterpret_cast<const uint8_t *>(p.w_scales) + frag0 * 128;
@@ -137,20 +150,21 @@ __global__ __launch_bounds__(WR *WC * 64, WR * FR == 4 ? 3 : 1) void gemm_mxfp4_
                         : unsigned(min(of_w % (COLS / 64) * 64 + lane, (p.frags - frag0) * 32 - 1)) * 4u;
     });
     const int64_t b_step = int64_t(p.frags) * (KS * 2048);
-    auto fetch = [&](int chunk, int buf) __attribute__((always_inline)) {
+    // request i of LOADS of a chunk
+    auto request = [&](auto ic, int chunk, int buf) __attribute__((always_inline)) {
+        constexpr int i = decltype(ic)::value;
         const int c = min(chunk, chunks - 1);                // behind the last chunk: that one again, not read from LDS
         int8_t *const at = lds + buf * BUFFER;
-        const int8_t *const b = p.w + c * b_step;
-        static_for<0, A_LOADS>([&](auto ic) {
-            constexpr int i = decltype(ic)::value;
+        if constexpr (i < A_LOADS) {
             const int k = c * CHUNK + a_piece[i];
             to_lds(reinterpret_cast<const int8_t *>(a_base) + (a_off[i] + unsigned(k < p.k ? k : 0)), at + (wave * A_LOADS + i) * 1024);
-        });
-        static_for<0, B_LOADS>([&](auto ic) { constexpr int i = decltype(ic)::value; to_lds(b + b_off[i], at + A_BYTES + (wave * B_LOADS + i) * 1024); });
-        static_for<0, S_LOADS>([&](auto ic) {
-            constexpr int i = decltype(ic)::value;
-            word_to_lds(s_base[i] + min(c * KS + s_step[i], s_last[i]) * s_stride[i] + s_off[i], at + SCALES + (wave * S_LOADS + i) * 256);
-        });
+        } else if constexpr (i < A_LOADS + B_LOADS) {
+            constexpr int j = i - A_LOADS;
+            to_lds(p.w + c * b_step + b_off[j], at + A_BYTES + (wave * B_LOADS + j) * 1024);
+        } else {
+            constexpr int j = i - A_LOADS - B_LOADS;
+            word_to_lds(s_base[j] + min(c * KS + s_step[j], s_last[j]) * s_stride[j] + s_off[j], at + SCALES + min(wave * S_LOADS + j, WORDS - 1) * 256);
+        }
     };
 
     v16f acc[FR][FC];
@@ -161,81 +175,94 @@ __global__ __launch_bounds__(WR *WC * 64, WR * FR == 4 ? 3 : 1) void gemm_mxfp4_
     const int a_row = (wave_r * FR * 32 + lane % 32) * CHUNK, a_key = key_of(lane % 32);
     v4i a[2][FR], b[2][FC];
     int a_scale[2][FR], b_scale[2][FC];      // of a K-step: blocks l / 32 and 2 + l / 32 in bytes 0 and 2
-    auto read = [&](auto hc, int buf) __attribute__((always_inline)) {
-        constexpr int h = decltype(hc)::value, set = h % 2, step = h / 2;
+    // read i of a half's operands; the scales of a K-step come with its first half
+    constexpr int READS = 2 * (FR + FC);
+    auto read = [&](auto hc, auto ic, int buf) __attribute__((always_inline)) {
+        constexpr int h = decltype(hc)::value, i = decltype(ic)::value, set = h % 2;
+        const int step = k_group * (KS / KG) + h / 2;      // a K group's K-steps of a chunk lie together
         const int8_t *const at = lds + buf * BUFFER;
-        if constexpr (h % 2 == 0) {
-            static_for<0, FC>([&](auto fc) {
-                constexpr int f = decltype(fc)::value;
-                b_scale[step % 2][f] = *reinterpret_cast<const int *>(at + SCALES + (KS * ROWS + step * COLS + (wave_c * FC + f) * 32 + lane % 32) * 4);
-            });
-            static_for<0, FR>([&](auto ic) {
-                constexpr int i = decltype(ic)::value;
-                a_scale[step % 2][i] = *reinterpret_cast<const int *>(at + SCALES + (step * ROWS + (wave_r * FR + i) * 32 + lane % 32) * 4);
-            });
+        if constexpr (i < FC) {
+            b[set][i] = *reinterpret_cast<const v4i *>(at + A_BYTES + ((step * (COLS / 32) + wave_c * FC + i) * 2 + h % 2) * 1024 + lane * 16);
+        } else if constexpr (i < FC + FR) {
+            constexpr int f = i - FC;
+            a[set][f] = *reinterpret_cast<const v4i *>(at + a_row + f * 32 * CHUNK + ((4 * step + 2 * (h % 2) + lane / 32) ^ a_key) * 16);
+        } else if constexpr (h % 2 == 0 && i < 2 * FC + FR) {
+            constexpr int f = i - FC - FR;
+            b_scale[h / 2 % 2][f] = *reinterpret_cast<const int *>(at + SCALES + (KS * ROWS + step * COLS + (wave_c * FC + f) * 32 + lane % 32) * 4);
+        } else if constexpr (h % 2 == 0 && i < READS) {
+            constexpr int f = i - 2 * FC - FR;
+            a_scale[h / 2 % 2][f] = *reinterpret_cast<const int *>(at + SCALES + (step * ROWS + (wave_r * FR + f) * 32 + lane % 32) * 4);
         }
-        static_for<0, FC>([&](auto fc) {
-            constexpr int f = decltype(fc)::value;
-            b[set][f] = *reinterpret_cast<const v4i *>(at + A_BYTES + ((step * (COLS / 32) + wave_c * FC + f) * 2 + h % 2) * 1024 + lane * 16);
-        });
-        static_for<0, FR>([&](auto ic) {
-            constexpr int i = decltype(ic)::value;
-            a[set][i] = *reinterpret_cast<const v4i *>(at + a_row + i * 32 * CHUNK + ((2 * h + lane / 32) ^ a_key) * 16);
-        });
     };
-    static_for<0, S>([&](auto sc) { fetch(decltype(sc)::value, decltype(sc)::value); });     // behind the last chunk: that one again
-    wait_for_all_but<(S - 1) * LOADS>();
+    static_for<0, S - 1>([&](auto sc) { static_for<0, LOADS>([&](auto ic) { request(ic, decltype(sc)::value, decltype(sc)::value); }); });
+    wait_for_all_but<(S - 2) * LOADS>();
     static_for<0, COL_TURNS>([&](auto ic) {
         const int at = threadIdx.x + decltype(ic)::value * THREADS;
         if (COLS % THREADS == 0 || at < COLS) of_cols[at] = col_bias[decltype(ic)::value];
     });
     lds_barrier();
-    read(std::integral_constant<int, 0>{}, 0);
+    static_for<0, READS>([&](auto ic) { read(std::integral_constant<int, 0>{}, ic, 0); });
     const int upper = 8 * (lane / 32);
     int buf = 0, c = 0;
+    // A chunk.  Between its multiplications, one after each: the reads of the next half's operands, and the requests of the chunk S - 1 further on,
+    // into the buffer that the barrier of the chunk before freed.  Spread so, none of them keeps the matrix cores waiting for its turn to be issued.
     auto multiply = [&](auto fetching) __attribute__((always_inline)) {
         constexpr bool FETCHES = decltype(fetching)::value;
-        const int after = buf + 1 == S ? 0 : buf + 1;
+        const int after = buf + 1 == S ? 0 : buf + 1, before = buf == 0 ? S - 1 : buf - 1;
         static_for<0, HALVES>([&](auto hc) {
-            constexpr int h = decltype(hc)::value;
+            constexpr int h = decltype(hc)::value, SLOTS = FR * FC, FIRST = LOADS * h / HALVES, COUNT = LOADS * (h + 1) / HALVES - FIRST;
             int as[FR], bs[FC];
             static_for<0, FR>([&](auto ic) { as[decltype(ic)::value] = int(unsigned(a_scale[h / 2 % 2][decltype(ic)::value]) >> upper); });
             static_for<0, FC>([&](auto fc) { bs[decltype(fc)::value] = int(unsigned(b_scale[h / 2 % 2][decltype(fc)::value]) >> upper); });
-            if constexpr (h + 1 < HALVES) {
-                read(std::integral_constant<int, h + 1>{}, buf);
-            } else {
+            if constexpr (h + 1 == HALVES) {
                 // Every wavefront has its operands of this chunk in registers: its buffer is free behind the barrier, and the next
                 // chunk is there for all.  The rest of this chunk's arithmetic covers the first reads behind it.
-                wait_for_all_but<FETCHES ? (S - 2) * LOADS : 0>();
-                lds_barrier();
-                read(std::integral_constant<int, 0>{}, after);
-                if constexpr (FETCHES) fetch(c + S, buf);
+                barrier_but_for<FETCHES ? (S - 3) * LOADS + FIRST : 0>();
             }
-            static_for<0, FR * FC>([&](auto fc) {
-                constexpr int i = decltype(fc)::value / FC, f = decltype(fc)::value % FC;
-                acc[i][f] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(b[h % 2][f]), operand(a[h % 2][i]), acc[i][f], FP4, FP4, 2 * (h % 2), bs[f],
+            static_for<0, SLOTS>([&](auto fc) {
+                constexpr int f = decltype(fc)::value, i = f / FC, j = f % FC;
+                constexpr int R0 = READS * f / SLOTS, R1 = READS * (f + 1) / SLOTS, L0 = COUNT * f / SLOTS, L1 = COUNT * (f + 1) / SLOTS;
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(b[h % 2][j]), operand(a[h % 2][i]), acc[i][j], FP4, FP4, 2 * (h % 2), bs[j],
                                                                             2 * (h % 2), as[i]);
+                static_for<R0, R1>([&](auto rc) {
+                    if constexpr (h + 1 == HALVES) read(std::integral_constant<int, 0>{}, rc, after);
+                    else read(std::integral_constant<int, h + 1>{}, rc, buf);
+                });
+                if constexpr (FETCHES) static_for<FIRST + L0, FIRST + L1>([&](auto lc) { request(lc, c + S - 1, before); });
+                __builtin_amdgcn_sched_barrier(0);
             });
-            // reads and requests between the multiplications
-            static_for<0, FR * FC>([&](auto fc) {
-                if constexpr (FETCHES && h + 1 == HALVES) __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-            });
-            __builtin_amdgcn_sched_barrier(0);
         });
         buf = after;
     };
-    for (; c + S < chunks; ++c) multiply(std::true_type{});
-    for (; c < chunks; ++c) multiply(std::false_type{});      // the last S chunks are all on their way
-    // The chunks' LDS is free: nothing is on its way into it, and behind this barrier nobody reads it.  A wavefront's 32 tokens x 32 FC
-    // columns go through it, so that a store instruction writes whole cache lines (straight from the registers it would write 16 bytes of
-    // each of 64 runs).
+    for (; c + S - 1 < chunks; ++c) multiply(std::true_type{});
+    for (; c < chunks; ++c) multiply(std::false_type{});      // the last S - 1 chunks are all on their way
+    // The chunks' LDS is free: nothing is on its way into it, and behind this barrier nobody reads it.
     wait_for_all_but<0>();
     lds_barrier();
+    constexpr int SUMS = FR * FC * 4096;                     // of a wavefront's fragments
+    if constexpr (KG > 1) {                                  // the first group adds up all groups' sums, in their order
+        float *const sums = reinterpret_cast<float *>(lds) + lane;
+        const int mine = in_group * (SUMS / 4);
+        if (k_group > 0)
+            static_for<0, FR * FC>([&](auto fc) {
+                constexpr int f = decltype(fc)::value;
+                static_for<0, 16>([&](auto rc) { sums[(k_group - 1) * (WR * WC * SUMS / 4) + mine + f * 1024 + decltype(rc)::value * 64] = acc[f / FC][f % FC][decltype(rc)::value]; });
+            });
+        lds_barrier();
+        if (k_group > 0) return;
+        static_for<1, KG>([&](auto gc) {
+            static_for<0, FR * FC>([&](auto fc) {
+                constexpr int f = decltype(fc)::value;
+                static_for<0, 16>([&](auto rc) { acc[f / FC][f % FC][decltype(rc)::value] += sums[(decltype(gc)::value - 1) * (WR * WC * SUMS / 4) + mine + f * 1024 + decltype(rc)::value * 64]; });
+            });
+        });
+    }
+    // A wavefront's 32 tokens x 32 FC columns go through LDS, so that a store instruction writes whole cache lines (straight from the registers it would
+    // write 16 bytes of each of 64 runs).
     constexpr int SIZE = OUT == TSX_TYPE_F32 ? 4 : 2, ROW = FC * 32 * SIZE, PITCH = ROW + 16, IN_ROW = ROW / 16, AT_ONCE = 64 / IN_ROW, EACH = 16 / SIZE;
-    static_assert(WAVES * 32 * PITCH <= S * BUFFER, "room for all wavefronts");
-    int8_t *const mine = lds + wave * (32 * PITCH);
+    constexpr int BEHIND = (KG - 1) * WR * WC * SUMS;
+    static_assert(BEHIND + WR * WC * 32 * PITCH <= S * BUFFER, "room for all wavefronts");
+    int8_t *const mine = lds + BEHIND + in_group * (32 * PITCH);
     const int col = (frag0 + wave_c * FC) * 32 + lane % IN_ROW * EACH, left = p.n - col;      // where a lane stores
     static_for<0, FR>([&](auto ic) {
         constexpr int i = decltype(ic)::value;
@@ -265,22 +292,24 @@ __global__ __launch_bounds__(WR *WC * 64, WR * FR == 4 ? 3 : 1) void gemm_mxfp4_
             static_for<0, 4>([&](auto wc) { to.word[decltype(wc)::value] = got[decltype(wc)::value]; });
             char *const out = static_cast<char *>(p.out) + (int64_t(row) * p.out_stride + col) * SIZE;
             if (row < p.m) {
-                if (left >= EACH) to.store(out);
-                else if (left > 0) to.store_some(out, left);
+                if (left >= EACH) {
+                    if (p.streams) to.template store<true>(out);      // uniform
+                    else to.store(out);
+                } else if (left > 0) to.store_some(out, left);
             }
         });
         __builtin_amdgcn_sched_barrier(0);               // 32 tokens at a time: their values would fill the registers
     });
 }
 
-// ---- few tokens: a stream over the weights
+// ---- up to 16 tokens: a stream over the weights
 //
-// There the product reads 17 / 32 n k bytes of weights and does little with each.  A workgroup owns 16 output columns and its 8 wavefronts split K, every
-// eighth K-step each; a K-step of 16 columns is one 16-byte load a lane and a word of scales, AHEAD of them in flight from the first instruction
+// There the product reads 17 / 32 n k bytes of weights and does little with each.  A workgroup owns 16 output columns and its wavefronts split K, every
+// WAVES-th K-step each; a K-step of 16 columns is one 16-byte load a lane and a word of scales, AHEAD of them in flight from the first instruction
 // on.  X, the type of the rows: MXFP4, or floats, which a lane quantizes where it needs them, 32 values of one token, a block: nothing has to meet
-// for a block's scale, so there is no launch ahead of the product and no barrier in it before the partial sums meet in LDS.  MT: groups of 16 tokens.
+// for a block's scale, so there is no launch ahead of the product and no barrier in it before the partial sums meet in LDS.
 // 16x16x128 instruction: accumulator r of lane l is column 4 (l / 16) + r of token l % 16.
-constexpr int FEW_THREADS = 512, FEW_WAVES = FEW_THREADS / 64;
+constexpr int FEW = 16;
 
 struct FewTokens : MxGemmParams {
     const void *values;                // rows of floats
@@ -288,89 +317,76 @@ struct FewTokens : MxGemmParams {
     int cols;                          // values of such a row
 };
 
-template <int X, int MT, int AHEAD, int OUT>
-__global__ __launch_bounds__(FEW_THREADS) void gemm_mxfp4_few_kernel(FewTokens p) {
-    __shared__ float sums[FEW_WAVES][MT][4][64];
+template <int X, int WAVES, int AHEAD, int OUT>
+__global__ __launch_bounds__(WAVES * 64) void gemm_mxfp4_few_kernel(FewTokens p) {
+    __shared__ float sums[WAVES][4][64];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), block = lane / 16, row = lane % 16;
-    const int row0 = int(blockIdx.y) * 16 * MT, col16 = blockIdx.x;      // in columns of 16
+    const int col16 = blockIdx.x;      // in columns of 16
     const int8_t *const w = p.w + int64_t(col16 >> 1) * 2048 + (block >> 1) * 1024 + (16 * (col16 & 1) + row + 32 * (block & 1)) * 16;
     const int8_t *const ws = p.w_scales + (col16 * 16 + row) * 4;
     const int64_t w_step = int64_t(p.frags) * 2048, ws_step = int64_t(p.frags) * 128;
+    const int token = min(row, p.m - 1);
     v4i a[AHEAD];
     unsigned as[AHEAD];
     auto fetch = [&](int first) __attribute__((always_inline)) {
         static_for<0, AHEAD>([&](auto uc) {
             constexpr int u = decltype(uc)::value;
-            const int step = min(first + FEW_WAVES * u, p.ksteps - 1);
+            const int step = min(first + WAVES * u, p.x_steps - 1);
             a[u] = *reinterpret_cast<const v4i *>(w + step * w_step);
             as[u] = *reinterpret_cast<const unsigned *>(ws + step * ws_step);
         });
     };
     fetch(wave);
-    v4f acc[MT];
-    static_for<0, MT>([&](auto mc) { acc[decltype(mc)::value] = v4f{0.f, 0.f, 0.f, 0.f}; });
-    for (int first = wave; first < p.ksteps; first += FEW_WAVES * AHEAD) {
-        v4i b[AHEAD][MT];
-        unsigned bs[AHEAD][MT];
+    v4f acc = {0.f, 0.f, 0.f, 0.f};
+    for (int first = wave; first < p.x_steps; first += WAVES * AHEAD) {
+        v4i b[AHEAD];
+        unsigned bs[AHEAD];
         static_for<0, AHEAD>([&](auto uc) {
             constexpr int u = decltype(uc)::value;
-            const int step = min(first + FEW_WAVES * u, p.ksteps - 1);
-            static_for<0, MT>([&](auto mc) {
-                constexpr int i = decltype(mc)::value;
-                const int token = min(row0 + 16 * i + row, p.m - 1);
-                if constexpr (X == TSX_TYPE_MXFP4) {
-                    const int k = step * KSTEP + block * 16;
-                    b[u][i] = *reinterpret_cast<const v4i *>(p.x + token * p.x_pitch + (k < p.k ? k : 0));
-                    bs[u][i] = p.x_scales[token * p.scale_row + min(step, p.x_steps - 1) * p.scale_step + block];
-                } else {
-                    constexpr int SIZE = X == TSX_TYPE_F32 ? 4 : 2;
-                    typedef Run<X, 8> Values;
-                    const int k = step * MX_STEP + block * MX_BLOCK;
-                    const char *const x = static_cast<const char *>(p.values) + token * p.x_stride * SIZE;
-                    Values v[4];
-                    unsigned top = 0;
-                    if (p.cols >= 8)             // uniform
-                        static_for<0, 4>([&](auto pc) { constexpr int q = decltype(pc)::value; v[q].load(x + int64_t(min(k + 8 * q, p.cols - 8)) * SIZE); });
-                    if (k + MX_BLOCK > p.cols)   // the row's end, and blocks behind it
-                        static_for<0, 4>([&](auto pc) {
-                            constexpr int q = decltype(pc)::value;
-                            const int left = p.cols - k - 8 * q;
-                            if (left < 8) v[q].clear();
-                            if (left > 0 && left < 8) v[q].load_some(x + int64_t(k + 8 * q) * SIZE, left);
-                        });
-                    static_for<0, 4>([&](auto pc) { top = v[decltype(pc)::value].top(top); });
-                    bs[u][i] = mx_scale(top_value<X>(top));
-                    static_for<0, 4>([&](auto pc) { constexpr int q = decltype(pc)::value; b[u][i][q] = int(mx_codes<X>(v[q], bs[u][i])); });
-                }
-            });
+            const int step = min(first + WAVES * u, p.x_steps - 1);
+            if constexpr (X == TSX_TYPE_MXFP4) {
+                b[u] = *reinterpret_cast<const v4i *>(p.x + token * p.x_pitch + (step * KSTEP + block * 16));
+                bs[u] = p.x_scales[token * p.scale_row + step * p.scale_step + block];
+            } else {
+                constexpr int SIZE = X == TSX_TYPE_F32 ? 4 : 2;
+                typedef Run<X, 8> Values;
+                const int k = step * MX_STEP + block * MX_BLOCK;
+                const char *const x = static_cast<const char *>(p.values) + token * p.x_stride * SIZE;
+                Values v[4];
+                unsigned top = 0;
+                if (p.cols >= 8)             // uniform
+                    static_for<0, 4>([&](auto pc) { constexpr int q = decltype(pc)::value; v[q].load(x + int64_t(min(k + 8 * q, p.cols - 8)) * SIZE); });
+                if (k + MX_BLOCK > p.cols)   // the row's end, and blocks behind it
+                    static_for<0, 4>([&](auto pc) {
+                        constexpr int q = decltype(pc)::value;
+                        const int left = p.cols - k - 8 * q;
+                        if (left < 8) v[q].clear();
+                        if (left > 0 && left < 8) v[q].load_some(x + int64_t(k + 8 * q) * SIZE, left);
+                    });
+                static_for<0, 4>([&](auto pc) { top = v[decltype(pc)::value].top(top); });
+                bs[u] = mx_scale(top_value<X>(top));
+                static_for<0, 4>([&](auto pc) { constexpr int q = decltype(pc)::value; b[u][q] = int(mx_codes<X>(v[q], bs[u])); });
+            }
         });
         static_for<0, AHEAD>([&](auto uc) {
             constexpr int u = decltype(uc)::value;
-            if (first + FEW_WAVES * u < p.ksteps)            // uniform
-                static_for<0, MT>([&](auto mc) {
-                    constexpr int i = decltype(mc)::value;
-                    acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(a[u]), operand(b[u][i]), acc[i], FP4, FP4, 0, int(as[u] >> (8 * block)), 0, int(bs[u][i]));
-                });
+            if (first + WAVES * u < p.x_steps)               // uniform
+                acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(a[u]), operand(b[u]), acc, FP4, FP4, 0, int(as[u] >> (8 * block)), 0, int(bs[u]));
         });
-        if (first + FEW_WAVES * AHEAD < p.ksteps) fetch(first + FEW_WAVES * AHEAD);
+        if (first + WAVES * AHEAD < p.x_steps) fetch(first + WAVES * AHEAD);
     }
-    static_for<0, MT>([&](auto mc) {
-        constexpr int i = decltype(mc)::value;
-        static_for<0, 4>([&](auto rc) { sums[wave][i][decltype(rc)::value][lane] = acc[i][decltype(rc)::value]; });
-    });
+    static_for<0, 4>([&](auto rc) { sums[wave][decltype(rc)::value][lane] = acc[decltype(rc)::value]; });
     __syncthreads();
-    for (int at = threadIdx.x; at < 256 * MT; at += FEW_THREADS) {
-        const int in = at % 16, col = col16 * 16 + in, token = at / 16;
-        if (col >= p.n || row0 + token >= p.m) continue;
-        float v[1] = {0.f};
+    const int in = threadIdx.x % 16, col = col16 * 16 + in, to = threadIdx.x / 16;
+    if (to >= p.m || col >= p.n) return;
+    float v[1] = {0.f};
 #pragma unroll
-        for (int i = 0; i < FEW_WAVES; ++i) v[0] = __fadd_rn(v[0], sums[i][token / 16][in % 4][token % 16 + 16 * (in / 4)]);
-        if (p.bias) v[0] = __fadd_rn(v[0], p.bias[col]);
-        activate_tokens<OUT>(v, p.act, p.slope);
-        Run<OUT, 1> out;
-        out.set(v);
-        out.store(static_cast<char *>(p.out) + ((row0 + token) * p.out_stride + col) * (OUT == TSX_TYPE_F32 ? 4 : 2));
-    }
+    for (int i = 0; i < WAVES; ++i) v[0] = __fadd_rn(v[0], sums[i][in % 4][to + 16 * (in / 4)]);
+    if (p.bias) v[0] = __fadd_rn(v[0], p.bias[col]);
+    activate_tokens<OUT>(v, p.act, p.slope);
+    Run<OUT, 1> out;
+    out.set(v);
+    out.store(static_cast<char *>(p.out) + (to * p.out_stride + col) * (OUT == TSX_TYPE_F32 ? 4 : 2));
 }
 
 // codes and scales of weights [n][k] to the layout above
@@ -426,74 +442,82 @@ __global__ __launch_bounds__(256) void copy_mxfp4_kernel(const uint8_t *codes, i
     }
 }
 
-template <int WR, int WC, int FR, int FC, int KS, int S, int OUT>
+template <int WR, int WC, int FR, int FC, int KS, int S, int KG, int OUT>
 int launch_tile(MxGemmParams p, hipStream_t stream) {
     p.row_tiles = int(ceil_div(p.m, 32 * WR * FR));
     p.col_tiles = int(ceil_div(p.n, 32 * WC * FC));
     const int64_t per_xcd = ceil_div(int64_t(p.row_tiles) * p.col_tiles, 8);
-    TSX_REQUIRE(8 * per_xcd * WR * WC * 64 < int64_t(1) << 32, "gemm_mxfp4: %d x %d outputs are more than a launch holds", p.m, p.n);
+    TSX_REQUIRE(8 * per_xcd * WR * WC * KG * 64 < int64_t(1) << 32, "gemm_mxfp4: %d x %d outputs are more than a launch holds", p.m, p.n);
     p.tiles_per_xcd = int(per_xcd);
+    p.streams = int64_t(p.m) * p.n * int64_t(element_bytes(OUT)) > 32 << 20;
     constexpr int LDS = S * 32 * (WR * FR + WC * FC) * KS * (KSTEP + 4);
-    const auto kernel = gemm_mxfp4_kernel<WR, WC, FR, FC, KS, S, OUT>;
+    const auto kernel = gemm_mxfp4_kernel<WR, WC, FR, FC, KS, S, KG, OUT>;
     if (LDS > 64 * 1024) {
         const int rc = grant_lds(reinterpret_cast<const void *>(kernel), LDS);
         if (rc) return rc;
     }
-    hipLaunchKernelGGL(kernel, dim3(unsigned(8 * p.tiles_per_xcd)), dim3(WR * WC * 64), LDS, stream, p);
+    hipLaunchKernelGGL(kernel, dim3(unsigned(8 * p.tiles_per_xcd)), dim3(WR * WC * KG * 64), LDS, stream, p);
     TSX_LAUNCH_CHECK("gemm_mxfp4_kernel");
     return 0;
 }
 
-template <int X, int MT, int AHEAD, int OUT>
+template <int X, int WAVES, int AHEAD, int OUT>
 int launch_few(const FewTokens &p, hipStream_t stream) {
-    const dim3 grid(unsigned(ceil_div(p.n, 16)), unsigned(ceil_div(p.m, 16 * MT)));
-    hipLaunchKernelGGL((gemm_mxfp4_few_kernel<X, MT, AHEAD, OUT>), grid, dim3(FEW_THREADS), 0, stream, p);
+    hipLaunchKernelGGL((gemm_mxfp4_few_kernel<X, WAVES, AHEAD, OUT>), dim3(unsigned(ceil_div(p.n, 16))), dim3(WAVES * 64), 0, stream, p);
     TSX_LAUNCH_CHECK("gemm_mxfp4_few_kernel");
     return 0;
 }
 template <int X, int OUT>
 int few_of(const FewTokens &p, hipStream_t stream) {
-    if constexpr (X == TSX_TYPE_MXFP4)
-        if (p.m > 16) return launch_few<X, 2, 4, OUT>(p, stream);
-    return launch_few<X, 1, 4, OUT>(p, stream);      // rows of floats: 16 at most
+    // 16 wavefronts where K is long: each has four K-steps up to K = 8192, all of them on their way at once (of rows of fp32 the registers hold two)
+    if (p.x_steps > 32) return launch_few<X, 16, X == TSX_TYPE_F32 ? 2 : 4, OUT>(p, stream);
+    return launch_few<X, 8, 4, OUT>(p, stream);
 }
 template <int OUT>
-int few_tokens(const tsx_mxfp4_gemm *g, const MxGemmParams &q, bool quantizes, hipStream_t stream) {
+int few_tokens(const tsx_mxfp4_gemm *g, const MxGemmParams &q, hipStream_t stream) {
     FewTokens p{};
     static_cast<MxGemmParams &>(p) = q;
     p.values = g->x_dev;
     p.x_stride = g->m <= 1 ? 0 : g->x_stride;
     p.cols = g->k;
-    if (quantizes)
-        return g->x_type == TSX_TYPE_F32 ? few_of<TSX_TYPE_F32, OUT>(p, stream)
-               : g->x_type == TSX_TYPE_F16 ? few_of<TSX_TYPE_F16, OUT>(p, stream) : few_of<TSX_TYPE_BF16, OUT>(p, stream);
-    return few_of<TSX_TYPE_MXFP4, OUT>(p, stream);
+    return g->x_type == TSX_TYPE_F32    ? few_of<TSX_TYPE_F32, OUT>(p, stream)
+           : g->x_type == TSX_TYPE_F16  ? few_of<TSX_TYPE_F16, OUT>(p, stream)
+           : g->x_type == TSX_TYPE_BF16 ? few_of<TSX_TYPE_BF16, OUT>(p, stream) : few_of<TSX_TYPE_MXFP4, OUT>(p, stream);
 }
 
-constexpr int FEW_MOST = 1 << 14;      // rows of the kernel for few tokens: with more their groups of rows leave a launch's second axis
-
-enum class Kernel { few, tile_64, tile_128, tile_256 };
+// The kernel a call takes: up to 16 tokens the stream over the weights; else by an estimate of its time in us, fitted to products of 32 .. 8192 rows on 256 ..
+// 8192 columns and K of 256 .. 8192 (bf16 output).  r: tiles a CU, ks: K / 1024.  Tiles of 64 with K split over two groups of wavefronts take a CU
+// each, so they are for up to 256; those of 64 and 128 share CUs, so that their times go by r once they fill the card and by the length of K before; those
+// of 256 come in whole turns, which a card half full goes through faster.  Measured, in this order (us): 64 x 4096, K = 4096 6.7, 7.6, 12, 23; 256 x 4096,
+// K = 4096 7.2, 8.0, 12.3, 23.5; 512 x 4096, K = 4096 13.1, 10.4, 13.4, 23.7; 512 x 8192, K = 1024 14.1, 8.6, 7.3, 11.5; 2048 x 4096, K = 4096 50, 37.8, 30.5,
+// 29.4; 4096^3 97, 73, 56, 41; 4096 x 8192, K = 1024 103, 50, 32, 35; 1024 x 1024, K = 8192 11, 12.9, 20.9, 40.7; 8192^3 611, 522, 396, 278.
+enum class Kernel { few, tile_64_by_k, tile_64, tile_128, tile_256 };
 
 Kernel choose(int m, int n, int k) {
-    if (m <= 32) return Kernel::few;
-    if (int64_t(m) * n >= int64_t(2048) * 2048) return Kernel::tile_256;
-    if (int64_t(m) * n >= int64_t(1024) * 1024) return Kernel::tile_128;
-    return Kernel::tile_64;
+    if (m <= FEW) return Kernel::few;
+    const float ks = float(k) / 1024.f;
+    const auto rounds = [&](int side) { return float(ceil_div(m, side) * ceil_div(n, side)) / 256.f; };
+    const float r64 = rounds(64), r128 = rounds(128), r256 = rounds(256);
+    const float cost[] = {r64 <= 1.f ? 3.6f + ks * (0.72f + 0.15f * r64) : INFINITY, std::max(3.5f + 1.1f * ks, 3.f + r64 * (0.5f + 0.97f * ks)),
+                          std::max(4.f + 2.05f * ks, 3.f + 0.4f * ks + r128 * (0.75f + 2.97f * ks)),
+                          3.f + std::ceil(r256) * (7.7f + 7.65f * ks) * (0.5f + 0.5f * std::min(r256, 1.f))};
+    int best = 0;
+    for (int i = 1; i < 4; ++i)
+        if (cost[i] < cost[best]) best = i;
+    return Kernel(best + 1);
 }
 
 template <int OUT>
-int launch(const tsx_mxfp4_gemm *g, const MxGemmParams &p, bool quantizes, hipStream_t stream) {
-    if (quantizes) return few_tokens<OUT>(g, p, true, stream);
+int launch(const tsx_mxfp4_gemm *g, const MxGemmParams &p, hipStream_t stream) {
     // TSX_MXFP4_KERNEL: that kernel, by its place in the list above, for any call it can take (tests, measurements)
     const char *e = std::getenv("TSX_MXFP4_KERNEL");
-    const bool named = e && e[0] >= (p.m <= FEW_MOST ? '0' : '1') && e[0] <= '3';
-    switch (named ? Kernel(e[0] - '0') : choose(p.m, p.n, p.k)) {
-        case Kernel::few: return few_tokens<OUT>(g, p, false, stream);
-        case Kernel::tile_64: return launch_tile<2, 2, 1, 1, 2, 3, OUT>(p, stream);
-        case Kernel::tile_128: return launch_tile<2, 2, 2, 2, 1, 3, OUT>(p, stream);
-        default:
-            if constexpr (OUT == TSX_TYPE_F32) return launch_tile<2, 4, 4, 2, 1, 4, OUT>(p, stream);
-            else return launch_tile<2, 2, 4, 4, 1, 4, OUT>(p, stream);
+    const bool named = e && e[0] >= (p.m <= FEW ? '0' : '1') && e[0] <= '4' && p.x;
+    switch (named ? Kernel(e[0] - '0') : choose(p.m, p.n, 2 * p.k)) {
+        case Kernel::few: return few_tokens<OUT>(g, p, stream);
+        case Kernel::tile_64_by_k: return launch_tile<2, 2, 1, 1, 4, 3, 2, OUT>(p, stream);
+        case Kernel::tile_64: return launch_tile<2, 2, 1, 1, 2, 3, 1, OUT>(p, stream);
+        case Kernel::tile_128: return launch_tile<2, 2, 2, 2, 1, 3, 1, OUT>(p, stream);
+        default: return launch_tile<2, 4, 4, 2, 1, 4, 1, OUT>(p, stream);
     }
 }
 
@@ -514,7 +538,7 @@ int check(const tsx_mxfp4_gemm *g) {
 bool is_multiple(const void *at, size_t bytes) { return reinterpret_cast<uintptr_t>(at) % bytes == 0; }
 
 // Whether the product's workgroups quantize the rows themselves
-bool quantizes_itself(const tsx_mxfp4_gemm *g) { return g->x_type != TSX_TYPE_MXFP4 && g->m <= 16; }
+bool quantizes_itself(const tsx_mxfp4_gemm *g) { return g->x_type != TSX_TYPE_MXFP4 && g->m <= FEW; }
 
 // A tile's rows are reached by 32-bit offsets: 256 of them at 2^23.
 bool reads_in_place(const tsx_mxfp4_gemm *g) {
@@ -620,8 +644,8 @@ int tsx_gemm_mxfp4(const tsx_mxfp4_gemm *g, void *workspace_dev, size_t workspac
     p.ksteps = tsx::ksteps_of(g->k);
     p.act = g->act;
     p.slope = g->slope;
-    return g->out_type == TSX_TYPE_F32 ? tsx::launch<TSX_TYPE_F32>(g, p, quantizes, stream) : g->out_type == TSX_TYPE_F16 ? tsx::launch<TSX_TYPE_F16>(g, p, quantizes, stream)
-                                                                                                          : tsx::launch<TSX_TYPE_BF16>(g, p, quantizes, stream);
+    return g->out_type == TSX_TYPE_F32 ? tsx::launch<TSX_TYPE_F32>(g, p, stream) : g->out_type == TSX_TYPE_F16 ? tsx::launch<TSX_TYPE_F16>(g, p, stream)
+                                                                                                          : tsx::launch<TSX_TYPE_BF16>(g, p, stream);
 }
 
 }  // extern "C"

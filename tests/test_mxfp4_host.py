@@ -79,7 +79,7 @@ def test_product_refuses(capi):
 
 def test_weights_refuse(capi):
     L = capi.lib()
-    assert L.tsx_gemm_mxfp4_packed_weight_bytes(1, 1) == 2 * 4 * (2048 + 128)
+    assert L.tsx_gemm_mxfp4_packed_weight_bytes(1, 1) == 4 * 4 * (2048 + 128)
     assert L.tsx_gemm_mxfp4_packed_weight_bytes(0, 1) == 0 and L.tsx_gemm_mxfp4_packed_weight_bytes(1 << 21, 1) == 0
     good = dict(k=64, n=4, codes=AT, codes_stride=32, scales=AT, scales_stride=2, packed=AT, stream=None)
     for change, word in ((dict(k=0), "K = 0"), (dict(n=0), "0 columns"), (dict(k=1 << 21), "2^21"), (dict(n=1 << 24), "2^24"), (dict(codes_stride=31), "overlap"),
