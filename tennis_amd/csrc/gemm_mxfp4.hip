@@ -86,14 +86,19 @@ __device__ __forceinline__ float sum_of(float v) {
 // (the same instructions on random operands from registers, nothing else: 6.5 P, at 1.55 GHz).  Each multiplication takes 32 cycles of its SIMD; a
 // tile's epilogue and first chunk are 9 us of 67.  4 x 4 fragments on four wavefronts read a third less LDS and take 268 us, one wavefront a SIMD hides less.
 // Few tiles with a long K wait for one K-step after the other, 0.19 us each in tiles of 64; two groups of wavefronts halve that.
-template <int WR, int WC, int FR, int FC, int KS, int S, int KG, int OUT>
+//
+// Scales arrive by 64 words, each wavefront's share of a chunk, from rows or from words of K-steps; or (IN_ROWS false), from words of K-steps only, by 256,
+// one request for all tokens and one for all columns, a wavefront each: the fewer requests a CU has to issue, the less the multiplications wait (8192^3
+// 260 us with eight requests a chunk for scales, 240 with none).
+template <int WR, int WC, int FR, int FC, int KS, int S, int KG, bool IN_ROWS, int OUT>
 __global__ __launch_bounds__(WR *WC *KG * 64, WR * FR == 4 && KG == 1 ? 3 : 1) void gemm_mxfp4_kernel(MxGemmParams p) {
     constexpr int CHUNK = KS * KSTEP, PIECES = CHUNK / 16, WAVES = WR * WC * KG, ROWS = 32 * WR * FR, COLS = 32 * WC * FC, HALVES = 2 * KS / KG;
     constexpr int A_BYTES = ROWS * CHUNK, B_BYTES = COLS * CHUNK, A_LOADS = A_BYTES / 1024 / WAVES, B_LOADS = B_BYTES / 1024 / WAVES;
-    constexpr int A_WORDS = KS * ROWS / 64, WORDS = KS * (ROWS + COLS) / 64, S_LOADS = (WORDS + WAVES - 1) / WAVES;      // scales: by 64 words
+    constexpr int A_WORDS = KS * ROWS / 64, WORDS = KS * (ROWS + COLS) / 64, S_LOADS = IN_ROWS ? (WORDS + WAVES - 1) / WAVES : 0;
     constexpr int SCALES = A_BYTES + B_BYTES, BUFFER = SCALES + KS * (ROWS + COLS) * 4, LOADS = A_LOADS + B_LOADS + S_LOADS;
     static_assert(4 % KS == 0, "the weights hold whole chunks");
-    static_assert(A_LOADS * 1024 * WAVES == A_BYTES && B_LOADS * 1024 * WAVES == B_BYTES && S >= 3 && (S - 1) * LOADS < 64,
+    static_assert(IN_ROWS || (KS == 1 && ROWS == 256 && COLS == 256), "scales by 256 words");
+    static_assert(A_LOADS * 1024 * WAVES == A_BYTES && B_LOADS * 1024 * WAVES == B_BYTES && S >= 3 && (S - 1) * (LOADS + 1) < 64,
                   "whole loads, counted in six bits");
     extern __shared__ __attribute__((aligned(16))) int8_t lds[];      // [S][BUFFER]
     __shared__ __attribute__((aligned(16))) float of_cols[COLS];      // biases, requested ahead of everything
@@ -119,7 +124,7 @@ __global__ __launch_bounds__(WR *WC *KG * 64, WR * FR == 4 && KG == 1 ? 3 : 1) v
     const auto key_of = [](int row) { return (row >> (KS == 1 ? 2 : KS == 2 ? 1 : 0)) & (PIECES - 1); };
     const int chunks = (p.x_steps + KS - 1) / KS;
     const uint8_t *const a_base = p.x + int64_t(row0) * p.x_pitch;
-    unsigned a_off[A_LOADS], b_off[B_LOADS], s_off[S_LOADS];
+    unsigned a_off[A_LOADS], b_off[B_LOADS], s_off[S_LOADS + 1];
     int a_piece[A_LOADS];
     static_for<0, A_LOADS>([&](auto ic) {
         constexpr int i = decltype(ic)::value;
@@ -135,9 +140,9 @@ __global__ __launch_bounds__(WR *WC *KG * 64, WR * FR == 4 && KG == 1 ? 3 : 1) v
     });
     // Scales in LDS: [K-step of the chunk][row], then [K-step of the chunk][column].  A request's K-steps lie s_stride apart, the last of them is
     // s_last; selects, no branches: all requests of a chunk are one run of instructions.
-    const uint8_t *s_base[S_LOADS];
-    int64_t s_stride[S_LOADS];
-    int s_step[S_LOADS], s_last[S_LOADS];
+    const uint8_t *s_base[S_LOADS + 1];
+    int64_t s_stride[S_LOADS + 1];
+    int s_step[S_LOADS + 1], s_last[S_LOADS + 1];
     static_for<0, S_LOADS>([&](auto ic) {
         constexpr int i = decltype(ic)::value;
         const int unit = min(wave * S_LOADS + i, WORDS - 1), of_w = unit - A_WORDS;      // more wavefronts than requests: the last one again
@@ -149,6 +154,15 @@ __global__ __launch_bounds__(WR *WC *KG * 64, WR * FR == 4 && KG == 1 ? 3 : 1) v
         s_off[i] = is_x ? unsigned(min(unit % (ROWS / 64) * 64 + lane, p.m - 1 - row0)) * unsigned(p.scale_row)
                         : unsigned(min(of_w % (COLS / 64) * 64 + lane, (p.frags - frag0) * 32 - 1)) * 4u;
     });
+    const bool has_scales = !IN_ROWS && wave < 2;             // uniform: the wavefront that requests 256 words of x, or of w
+    if constexpr (!IN_ROWS) {
+        s_base[0] = wave == 0 ? p.x_scales + int64_t(row0) * 4 : reinterpret_cast<const uint8_t *>(p.w_scales) + frag0 * 128;
+        s_stride[0] = wave == 0 ? p.scale_step : int64_t(p.frags) * 128;
+        s_off[0] = wave == 0 ? lane * 16u : unsigned(min(lane * 4, (p.frags - frag0) * 32 - 4)) * 4u;      // words of x go up to whole tiles
+    }
+    auto request_scales = [&](int chunk, int buf) __attribute__((always_inline)) {
+        if (has_scales) to_lds(reinterpret_cast<const int8_t *>(s_base[0] + min(chunk, chunks - 1) * s_stride[0] + s_off[0]), lds + buf * BUFFER + SCALES + wave * 1024);
+    };
     const int64_t b_step = int64_t(p.frags) * (KS * 2048);
     // request i of LOADS of a chunk
     auto request = [&](auto ic, int chunk, int buf) __attribute__((always_inline)) {
@@ -194,8 +208,11 @@ __global__ __launch_bounds__(WR *WC *KG * 64, WR * FR == 4 && KG == 1 ? 3 : 1) v
             a_scale[h / 2 % 2][f] = *reinterpret_cast<const int *>(at + SCALES + (step * ROWS + (wave_r * FR + f) * 32 + lane % 32) * 4);
         }
     };
-    static_for<0, S - 1>([&](auto sc) { static_for<0, LOADS>([&](auto ic) { request(ic, decltype(sc)::value, decltype(sc)::value); }); });
-    wait_for_all_but<(S - 2) * LOADS>();
+    static_for<0, S - 1>([&](auto sc) {
+        request_scales(decltype(sc)::value, decltype(sc)::value);
+        static_for<0, LOADS>([&](auto ic) { request(ic, decltype(sc)::value, decltype(sc)::value); });
+    });
+    wait_for_all_but<(S - 2) * LOADS>();                     // of a wavefront that requested scales, too, that is behind its first chunk
     static_for<0, COL_TURNS>([&](auto ic) {
         const int at = threadIdx.x + decltype(ic)::value * THREADS;
         if (COLS % THREADS == 0 || at < COLS) of_cols[at] = col_bias[decltype(ic)::value];
@@ -214,6 +231,7 @@ __global__ __launch_bounds__(WR *WC *KG * 64, WR * FR == 4 && KG == 1 ? 3 : 1) v
             int as[FR], bs[FC];
             static_for<0, FR>([&](auto ic) { as[decltype(ic)::value] = int(unsigned(a_scale[h / 2 % 2][decltype(ic)::value]) >> upper); });
             static_for<0, FC>([&](auto fc) { bs[decltype(fc)::value] = int(unsigned(b_scale[h / 2 % 2][decltype(fc)::value]) >> upper); });
+            if constexpr (h == 0 && FETCHES) request_scales(c + S - 1, before);
             if constexpr (h + 1 == HALVES) {
                 // Every wavefront has its operands of this chunk in registers: its buffer is free behind the barrier, and the next
                 // chunk is there for all.  The rest of this chunk's arithmetic covers the first reads behind it.
@@ -354,15 +372,13 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_mxfp4_few_kernel(FewTokens p)
                 const char *const x = static_cast<const char *>(p.values) + token * p.x_stride * SIZE;
                 Values v[4];
                 unsigned top = 0;
-                if (p.cols >= 8)             // uniform
-                    static_for<0, 4>([&](auto pc) { constexpr int q = decltype(pc)::value; v[q].load(x + int64_t(min(k + 8 * q, p.cols - 8)) * SIZE); });
-                if (k + MX_BLOCK > p.cols)   // the row's end, and blocks behind it
-                    static_for<0, 4>([&](auto pc) {
-                        constexpr int q = decltype(pc)::value;
-                        const int left = p.cols - k - 8 * q;
-                        if (left < 8) v[q].clear();
-                        if (left > 0 && left < 8) v[q].load_some(x + int64_t(k + 8 * q) * SIZE, left);
-                    });
+                if (p.cols >= 8) {           // uniform
+                    static_for<0, 4>([&](auto pc) { load_piece<X>(v[decltype(pc)::value], x, k + 8 * decltype(pc)::value, p.cols); });
+                    if ((step + 1) * MX_STEP > p.cols) static_for<0, 4>([&](auto pc) { settle_piece<X>(v[decltype(pc)::value], k + 8 * decltype(pc)::value, p.cols); });
+                } else {
+                    static_for<0, 4>([&](auto pc) { v[decltype(pc)::value].clear(); });
+                    if (k == 0) v[0].load_some(x, p.cols);
+                }
                 static_for<0, 4>([&](auto pc) { top = v[decltype(pc)::value].top(top); });
                 bs[u] = mx_scale(top_value<X>(top));
                 static_for<0, 4>([&](auto pc) { constexpr int q = decltype(pc)::value; b[u][q] = int(mx_codes<X>(v[q], bs[u])); });
@@ -418,10 +434,10 @@ __global__ __launch_bounds__(256) void pack_mxfp4_kernel(const uint8_t *codes, i
     }
 }
 
-// MXFP4 rows of another length, stride or alignment than the kernels read: codes to whole K-steps at `pitch`, scales to words of K-steps
+// MXFP4 rows that a kernel does not read where they are: codes to whole K-steps (unless `to` is null), scales to words of K-steps
 __global__ __launch_bounds__(256) void copy_mxfp4_kernel(const uint8_t *codes, int64_t codes_stride, const uint8_t *scales, int64_t scales_stride, int bytes,
-                                                         int blocks, int64_t rows, int steps, uint8_t *to, uint8_t *to_scales) {
-    const int64_t pitch = int64_t(steps) * KSTEP, pieces = rows * steps * 4, words = rows * steps;
+                                                         int blocks, int64_t rows, int steps, uint8_t *to, uint8_t *to_scales, int64_t scale_step) {
+    const int64_t pitch = int64_t(steps) * KSTEP, pieces = to ? rows * steps * 4 : 0, words = rows * steps;
     for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < pieces + words; i += int64_t(gridDim.x) * 256) {
         if (i < pieces) {
             const int64_t row = i / (steps * 4);
@@ -437,12 +453,12 @@ __global__ __launch_bounds__(256) void copy_mxfp4_kernel(const uint8_t *codes, i
             unsigned v = 0;
             for (int b = 0; b < 4; ++b)
                 if (step * 4 + b < blocks) v |= unsigned(scales[row * scales_stride + step * 4 + b]) << (8 * b);
-            reinterpret_cast<unsigned *>(to_scales)[word] = v;
+            *reinterpret_cast<unsigned *>(to_scales + step * scale_step + row * 4) = v;
         }
     }
 }
 
-template <int WR, int WC, int FR, int FC, int KS, int S, int KG, int OUT>
+template <int WR, int WC, int FR, int FC, int KS, int S, int KG, bool IN_ROWS, int OUT>
 int launch_tile(MxGemmParams p, hipStream_t stream) {
     p.row_tiles = int(ceil_div(p.m, 32 * WR * FR));
     p.col_tiles = int(ceil_div(p.n, 32 * WC * FC));
@@ -451,7 +467,7 @@ int launch_tile(MxGemmParams p, hipStream_t stream) {
     p.tiles_per_xcd = int(per_xcd);
     p.streams = int64_t(p.m) * p.n * int64_t(element_bytes(OUT)) > 32 << 20;
     constexpr int LDS = S * 32 * (WR * FR + WC * FC) * KS * (KSTEP + 4);
-    const auto kernel = gemm_mxfp4_kernel<WR, WC, FR, FC, KS, S, KG, OUT>;
+    const auto kernel = gemm_mxfp4_kernel<WR, WC, FR, FC, KS, S, KG, IN_ROWS, OUT>;
     if (LDS > 64 * 1024) {
         const int rc = grant_lds(reinterpret_cast<const void *>(kernel), LDS);
         if (rc) return rc;
@@ -508,16 +524,13 @@ Kernel choose(int m, int n, int k) {
 }
 
 template <int OUT>
-int launch(const tsx_mxfp4_gemm *g, const MxGemmParams &p, hipStream_t stream) {
-    // TSX_MXFP4_KERNEL: that kernel, by its place in the list above, for any call it can take (tests, measurements)
-    const char *e = std::getenv("TSX_MXFP4_KERNEL");
-    const bool named = e && e[0] >= (p.m <= FEW ? '0' : '1') && e[0] <= '4' && p.x;
-    switch (named ? Kernel(e[0] - '0') : choose(p.m, p.n, 2 * p.k)) {
+int launch(Kernel kernel, const tsx_mxfp4_gemm *g, const MxGemmParams &p, hipStream_t stream) {
+    switch (kernel) {
         case Kernel::few: return few_tokens<OUT>(g, p, stream);
-        case Kernel::tile_64_by_k: return launch_tile<2, 2, 1, 1, 4, 3, 2, OUT>(p, stream);
-        case Kernel::tile_64: return launch_tile<2, 2, 1, 1, 2, 3, 1, OUT>(p, stream);
-        case Kernel::tile_128: return launch_tile<2, 2, 2, 2, 1, 3, 1, OUT>(p, stream);
-        default: return launch_tile<2, 4, 4, 2, 1, 4, 1, OUT>(p, stream);
+        case Kernel::tile_64_by_k: return launch_tile<2, 2, 1, 1, 4, 3, 2, true, OUT>(p, stream);
+        case Kernel::tile_64: return launch_tile<2, 2, 1, 1, 2, 3, 1, true, OUT>(p, stream);
+        case Kernel::tile_128: return launch_tile<2, 2, 2, 2, 1, 3, 1, true, OUT>(p, stream);
+        default: return launch_tile<2, 4, 4, 2, 1, 4, 1, false, OUT>(p, stream);
     }
 }
 
@@ -537,21 +550,31 @@ int check(const tsx_mxfp4_gemm *g) {
 
 bool is_multiple(const void *at, size_t bytes) { return reinterpret_cast<uintptr_t>(at) % bytes == 0; }
 
-// Whether the product's workgroups quantize the rows themselves
-bool quantizes_itself(const tsx_mxfp4_gemm *g) { return g->x_type != TSX_TYPE_MXFP4 && g->m <= FEW; }
-
 // A tile's rows are reached by 32-bit offsets: 256 of them at 2^23.
 bool reads_in_place(const tsx_mxfp4_gemm *g) {
     return g->x_type == TSX_TYPE_MXFP4 && g->k % MX_STEP == 0 && is_multiple(g->x_dev, 16) && is_multiple(g->x_scales_dev, 4) &&
            (g->m <= 1 || (g->x_stride % 16 == 0 && g->x_stride <= 1 << 23 && g->x_scales_stride % 4 == 0 && g->x_scales_stride <= 1 << 23));
 }
 
-// the workspace: codes [m][steps][64], scales [steps][m][4]
-int64_t steps_of(int k) { return ceil_div(k, MX_STEP); }
-size_t workspace_bytes(const tsx_mxfp4_gemm *g) {
-    if (g->m == 0 || reads_in_place(g) || quantizes_itself(g)) return 0;
-    return size_t(g->m) * steps_of(g->k) * (KSTEP + 4);
-}
+// What a call does: its kernel, and what the workspace holds, codes [m][steps][64] and scales [steps][m in whole tiles of 256][4].
+struct Plan {
+    Kernel kernel;
+    bool codes, scales;
+    int64_t steps, code_bytes, words;      // words: of a K-step's scales
+    explicit Plan(const tsx_mxfp4_gemm *g) {
+        kernel = choose(g->m, g->n, g->k);
+        // TSX_MXFP4_KERNEL: that kernel, by its place in the list above, for any call it can take (tests, measurements)
+        const char *e = std::getenv("TSX_MXFP4_KERNEL");
+        if (e && e[0] >= (g->m <= FEW ? '0' : '1') && e[0] <= '4') kernel = Kernel(e[0] - '0');
+        const bool in_place = reads_in_place(g) || (kernel == Kernel::few && g->x_type != TSX_TYPE_MXFP4);
+        codes = g->m > 0 && !in_place;
+        scales = codes || (g->m > 0 && kernel == Kernel::tile_256);      // which reads words of K-steps
+        steps = ceil_div(g->k, MX_STEP);
+        code_bytes = codes ? g->m * steps * KSTEP : 0;
+        words = round_up(g->m, 256);
+    }
+    size_t workspace_bytes() const { return size_t(code_bytes) + (scales ? size_t(words) * steps * 4 : 0); }
+};
 
 int check_weights(int32_t k, int32_t n) {
     TSX_REQUIRE(k > 0 && n > 0 && k < 1 << 21 && n < 1 << 24, "gemm_mxfp4: weights of %d columns, K = %d (below 2^24 and 2^21)", n, k);
@@ -585,7 +608,7 @@ int tsx_gemm_mxfp4_pack_weights(int32_t k, int32_t n, const uint8_t *codes_dev, 
 
 size_t tsx_gemm_mxfp4_workspace_bytes(const tsx_mxfp4_gemm *g) {
     if (tsx::check(g)) return 0;
-    return tsx::workspace_bytes(g);
+    return tsx::Plan(g).workspace_bytes();
 }
 
 int tsx_gemm_mxfp4(const tsx_mxfp4_gemm *g, void *workspace_dev, size_t workspace_bytes, void *stream_) {
@@ -597,7 +620,8 @@ int tsx_gemm_mxfp4(const tsx_mxfp4_gemm *g, void *workspace_dev, size_t workspac
     TSX_REQUIRE(tsx::is_multiple(g->packed_w_dev, 16), "gemm_mxfp4: packed weights must be 16-byte aligned");
     TSX_REQUIRE((codes || tsx::is_multiple(g->x_dev, tsx::element_bytes(g->x_type))) && tsx::is_multiple(g->out_dev, tsx::element_bytes(g->out_type)) &&
                     tsx::is_multiple(g->bias_dev, 4), "gemm_mxfp4: pointer is no multiple of its elements");
-    const size_t need = tsx::workspace_bytes(g);
+    const tsx::Plan plan(g);
+    const size_t need = plan.workspace_bytes();
     if (need) {
         if (!workspace_dev || workspace_bytes < need)
             return tsx::fail(TSX_E_WORKSPACE, "gemm_mxfp4: workspace %zu < %zu bytes", workspace_dev ? workspace_bytes : size_t(0), need);
@@ -605,33 +629,25 @@ int tsx_gemm_mxfp4(const tsx_mxfp4_gemm *g, void *workspace_dev, size_t workspac
     }
     hipStream_t stream = tsx::as_stream(stream_);
     tsx::MxGemmParams p{};
-    const int steps = int(tsx::steps_of(g->k));
+    const int steps = int(plan.steps);
     p.x_steps = steps;
     p.k = steps * tsx::KSTEP;
-    const bool quantizes = tsx::quantizes_itself(g);
-    if (need) {
-        uint8_t *const to = static_cast<uint8_t *>(workspace_dev), *const to_scales = to + int64_t(g->m) * p.k;
-        p.x = to;
-        p.x_scales = to_scales;
-        p.x_pitch = p.k;
-        p.scale_row = 4;
-        p.scale_step = int64_t(g->m) * 4;
-        if (codes) {
-            const int64_t units = int64_t(g->m) * steps * 5, blocks = tsx::ceil_div(units, 256);
-            hipLaunchKernelGGL(tsx::copy_mxfp4_kernel, dim3(unsigned(std::min<int64_t>(blocks, 1 << 16))), dim3(256), 0, stream, static_cast<const uint8_t *>(g->x_dev),
-                               g->x_stride, g->x_scales_dev, g->x_scales_stride, (g->k + 1) / 2, (g->k + 31) / 32, int64_t(g->m), steps, to, to_scales);
-            TSX_LAUNCH_CHECK("copy_mxfp4_kernel");
-        } else {
-            rc = tsx::quantize_mxfp4_rows(g->m, g->k, steps * tsx::MX_STEP, g->x_dev, g->x_type, g->x_stride,
-                                          tsx::MxRows{to, to_scales, p.x_pitch, p.scale_row, p.scale_step}, stream);
-            if (rc) return rc;
-        }
-    } else if (!quantizes) {
-        p.x = static_cast<const uint8_t *>(g->x_dev);
-        p.x_scales = g->x_scales_dev;
-        p.x_pitch = g->m <= 1 ? 0 : g->x_stride;
-        p.scale_row = g->m <= 1 ? 0 : g->x_scales_stride;
-        p.scale_step = 4;
+    uint8_t *const to = static_cast<uint8_t *>(workspace_dev), *const to_scales = to + plan.code_bytes;
+    p.x = plan.codes ? to : static_cast<const uint8_t *>(g->x_dev);
+    p.x_pitch = plan.codes ? p.k : g->m <= 1 ? 0 : g->x_stride;
+    p.x_scales = plan.scales ? to_scales : g->x_scales_dev;
+    p.scale_row = plan.scales ? 4 : g->m <= 1 ? 0 : g->x_scales_stride;
+    p.scale_step = plan.scales ? plan.words * 4 : 4;
+    if (plan.scales && !codes) {
+        rc = tsx::quantize_mxfp4_rows(g->m, g->k, steps * tsx::MX_STEP, g->x_dev, g->x_type, g->x_stride,
+                                      tsx::MxRows{to, to_scales, p.x_pitch, p.scale_row, p.scale_step}, stream);
+        if (rc) return rc;
+    } else if (plan.scales) {
+        const int64_t units = int64_t(g->m) * steps * (plan.codes ? 5 : 1), blocks = tsx::ceil_div(units, 256);
+        hipLaunchKernelGGL(tsx::copy_mxfp4_kernel, dim3(unsigned(std::min<int64_t>(blocks, 1 << 16))), dim3(256), 0, stream, static_cast<const uint8_t *>(g->x_dev),
+                           g->x_stride, g->x_scales_dev, g->x_scales_stride, (g->k + 1) / 2, (g->k + 31) / 32, int64_t(g->m), steps, plan.codes ? to : nullptr, to_scales,
+                           p.scale_step);
+        TSX_LAUNCH_CHECK("copy_mxfp4_kernel");
     }
     p.w = static_cast<const int8_t *>(g->packed_w_dev);
     p.w_scales = p.w + tsx::packed_codes(g->k, g->n);
@@ -644,8 +660,8 @@ int tsx_gemm_mxfp4(const tsx_mxfp4_gemm *g, void *workspace_dev, size_t workspac
     p.ksteps = tsx::ksteps_of(g->k);
     p.act = g->act;
     p.slope = g->slope;
-    return g->out_type == TSX_TYPE_F32 ? tsx::launch<TSX_TYPE_F32>(g, p, stream) : g->out_type == TSX_TYPE_F16 ? tsx::launch<TSX_TYPE_F16>(g, p, stream)
-                                                                                                          : tsx::launch<TSX_TYPE_BF16>(g, p, stream);
+    return g->out_type == TSX_TYPE_F32 ? tsx::launch<TSX_TYPE_F32>(plan.kernel, g, p, stream) : g->out_type == TSX_TYPE_F16 ? tsx::launch<TSX_TYPE_F16>(plan.kernel, g, p, stream)
+                                                                                                          : tsx::launch<TSX_TYPE_BF16>(plan.kernel, g, p, stream);
 }
 
 }  // extern "C"

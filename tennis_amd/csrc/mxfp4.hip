@@ -27,7 +27,6 @@ __global__ __launch_bounds__(THREADS) void quantize_mxfp4_kernel(ToMxParams p) {
     constexpr int SIZE = TYPE == TSX_TYPE_F32 ? 4 : 2;
     typedef Run<TYPE, PIECE> Values;
     const unsigned first = blockIdx.x * (THREADS * P) + threadIdx.x;
-    const int whole = p.cols / PIECE;
     Values v[P];
     int64_t row[P];
     int piece[P];
@@ -37,12 +36,16 @@ __global__ __launch_bounds__(THREADS) void quantize_mxfp4_kernel(ToMxParams p) {
         row[i] = r;
         piece[i] = int(at - r * p.pieces.d);
         const char *const x = static_cast<const char *>(p.x) + row[i] * p.x_stride * SIZE;
-        if (!TAILS || whole) v[i].load(x + int64_t(TAILS ? min(piece[i], whole - 1) : piece[i]) * (PIECE * SIZE));       // uniform
-        if (TAILS && piece[i] >= whole) {
+        if (!TAILS) {
+            v[i].load(x + int64_t(piece[i]) * (PIECE * SIZE));
+        } else if (p.cols >= PIECE) {      // uniform
+            load_piece<TYPE>(v[i], x, piece[i] * PIECE, p.cols);
+        } else {
             v[i].clear();
-            if (piece[i] * PIECE < p.cols) v[i].load_some(x + int64_t(piece[i]) * (PIECE * SIZE), p.cols - piece[i] * PIECE);
+            if (piece[i] == 0) v[i].load_some(x, p.cols);
         }
     });
+    if (TAILS && p.cols >= PIECE) static_for<0, P>([&](auto ic) { settle_piece<TYPE>(v[decltype(ic)::value], piece[decltype(ic)::value] * PIECE, p.cols); });
     static_for<0, P>([&](auto ic) {
         constexpr int i = decltype(ic)::value;
         const unsigned top = over_lanes(v[i].top(0), 2, [](unsigned a, unsigned b) { return Values::template larger<TYPE>(a, b); });

@@ -43,6 +43,30 @@ __device__ __forceinline__ unsigned mx_scale(float top) {
 }
 __device__ __forceinline__ float mx_factor(unsigned scale) { return __builtin_bit_cast(float, scale << 23); }
 
+// The piece of eight values that begins at value `at` of a row of at least eight: what is left of the row, behind it zeros.  load: the eight values
+// there, or the row's last eight, a request like any other; then, where all requests are out, settle.
+template <int TYPE>
+__device__ __forceinline__ void load_piece(Run<TYPE, 8> &v, const char *row, int at, int cols) {
+    v.load(row + int64_t(min(at, cols - 8)) * (TYPE == TSX_TYPE_F32 ? 4 : 2));
+}
+template <int TYPE>
+__device__ __forceinline__ void settle_piece(Run<TYPE, 8> &v, int at, int cols) {
+    const int over = at + 8 - cols;                // of the row's last eight, those that come first belong to the piece before
+    if (over <= 0) return;
+    if (over >= 8) {
+        v.clear();
+        return;
+    }
+    constexpr int W = Run<TYPE, 8>::WORDS, PER = 8 / W;
+    static_for<0, 3>([&](auto bc) {
+        constexpr int by = 4 >> decltype(bc)::value, words = by / PER;
+        if (over & by) {
+            if constexpr (words > 0) static_for<0, W>([&](auto wc) { constexpr int w = decltype(wc)::value; v.word[w] = w + words < W ? v.word[(w + words) % W] : 0u; });
+            else static_for<0, W>([&](auto wc) { constexpr int w = decltype(wc)::value; v.word[w] = __builtin_amdgcn_alignbit(w + 1 < W ? v.word[(w + 1) % W] : 0u, v.word[w], 16); });
+        }
+    });
+}
+
 // eight values to four bytes of codes
 template <int TYPE>
 __device__ __forceinline__ unsigned mx_codes(const Run<TYPE, 8> &v, unsigned scale) {

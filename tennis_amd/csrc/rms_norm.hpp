@@ -35,8 +35,8 @@ int rms_norm_mxfp4(const RmsNormParams &p, int type, hipStream_t stream);
 constexpr float NORM_LEAST = 0x1p-120f, NORM_DOWN = 0x1p-80f, NORM_UP = 0x1p105f;
 
 template <int TYPE, int TO, int T, int P, bool HELD>
-__global__ __launch_bounds__(T < 256 ? 256 : T) void rms_norm_kernel(RmsNormParams p) {
-    constexpr int PIECE = 8, THREADS = T < 256 ? 256 : T, ROWS = THREADS / T, SIZE = TYPE == TSX_TYPE_F32 ? 4 : 2, WAVES = T / 64;
+__global__ __launch_bounds__(T <= 64 ? 256 : T) void rms_norm_kernel(RmsNormParams p) {
+    constexpr int PIECE = 8, THREADS = T <= 64 ? 256 : T, ROWS = THREADS / T, SIZE = TYPE == TSX_TYPE_F32 ? 4 : 2, WAVES = T / 64;
     constexpr int LG = lg_of(T < 64 ? T : 64);
     typedef Run<TYPE, PIECE> Values;
     typedef Run<TSX_TYPE_F32, PIECE> Weights;
@@ -46,59 +46,61 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rms_norm_kernel(RmsNormPara
     const int turns = HELD ? 1 : (pieces + T * P - 1) / (T * P);
     for (int64_t row0 = int64_t(blockIdx.x) * ROWS; row0 < p.rows; row0 += int64_t(gridDim.x) * ROWS) {
         const int64_t row = row0 + tid / T;
-        const bool there = row < p.rows;      // a row's threads agree; only T <= 64 has rows beyond the last one, which are that one again
+        const bool there = row < p.rows;      // a row's threads agree; only T <= 64 has several rows, and some beyond the last one, which are that one again
         const int64_t at = there ? row : p.rows - 1;
         const char *const x = static_cast<const char *>(p.x) + at * p.x_stride * SIZE;
         const char *const residual = static_cast<const char *>(p.residual) + at * p.residual_stride * SIZE;
         char *const sum = static_cast<char *>(p.sum) + at * p.sum_stride * SIZE;
         Values h[P];
         Weights w[P];
-        // P pieces of a row of values; all requests at once, none behind a branch, where it would be waited for: what lies behind the last whole piece is that
-        // piece again, and then zeros, or the values that are left there
+        // P pieces of a row of values: all requests of a turn first, none behind a branch, where it would be waited for; then what lies behind the row's end
+        // becomes zeros
         auto load = [&](auto &v, const char *from, int first) __attribute__((always_inline)) {
-            typedef std::remove_reference_t<decltype(v[0])> Piece;
-            constexpr int BYTES = Piece::BYTES;
-            if (whole)       // uniform
-                static_for<0, P>([&](auto ic) { v[decltype(ic)::value].load(from + int64_t(min(first + t + decltype(ic)::value * T, whole - 1)) * BYTES); });
-            if (in_last || pieces < turns * T * P) {       // uniform
-                Piece last;
-                last.clear();
-                if (in_last) last.load_some(from + int64_t(whole) * BYTES, in_last);
+            static_for<0, P>([&](auto ic) {
+                constexpr int i = decltype(ic)::value;
+                const int piece = first + t + i * T;
+                if (whole) {       // uniform
+                    load_piece(v[i], from, piece * PIECE, p.cols);
+                } else {
+                    v[i].clear();
+                    if (piece == 0) v[i].load_some(from, p.cols);
+                }
+            });
+        };
+        auto settle = [&](auto &v, int first) __attribute__((always_inline)) {
+            if (whole)
                 static_for<0, P>([&](auto ic) {
                     constexpr int i = decltype(ic)::value;
-                    const int piece = first + t + i * T;
-                    if (piece >= whole) v[i].clear();
-                    if (piece == whole) v[i] = last;
+                    if (first + (i + 1) * T > whole) settle_piece(v[i], (first + t + i * T) * PIECE, p.cols);       // uniform: where the row's end can be
                 });
-            }
         };
         auto store = [&](const Values &v, char *to, int piece) __attribute__((always_inline)) {
             if (!there || piece >= pieces) return;
             if (piece < whole) v.store(to + int64_t(piece) * (PIECE * SIZE));
             else v.store_some(to + int64_t(piece) * (PIECE * SIZE), in_last);
         };
-        auto fetch_weight = [&](int first) __attribute__((always_inline)) {
-            if (p.weight) load(w, reinterpret_cast<const char *>(p.weight), first);
-            else static_for<0, P>([&](auto ic) { static_for<0, PIECE>([&](auto ec) { w[decltype(ic)::value].word[decltype(ec)::value] = 0x3f800000u; }); });
-        };
-        // h of a turn; again: as it was kept
-        auto fetch = [&](int first, bool again) __attribute__((always_inline)) {
-            if (again && p.sum) {
-                load(h, sum, first);
-            } else {
-                load(h, x, first);
-                if (p.residual) {
-                    Values r[P];
-                    load(r, residual, first);
-                    static_for<0, P>([&](auto ic) {
-                        constexpr int i = decltype(ic)::value;
-                        float v[PIECE];
-                        static_for<0, PIECE>([&](auto ec) { constexpr int e = decltype(ec)::value; v[e] = __fadd_rn(h[i].template get<e>(), r[i].template get<e>()); });
-                        h[i].set(v);
-                    });
-                }
-                if (p.sum) static_for<0, P>([&](auto ic) { store(h[decltype(ic)::value], sum, first + t + decltype(ic)::value * T); });
+        // h of a turn, and the weights where they are wanted; again: h as it was kept
+        auto fetch = [&](int first, bool again, bool weights) __attribute__((always_inline)) {
+            const bool adds = p.residual && !(again && p.sum);       // uniform, as all conditions here
+            Values r[P];
+            load(h, again && p.sum ? sum : x, first);
+            if (adds) load(r, residual, first);
+            if (weights) {
+                if (p.weight) load(w, reinterpret_cast<const char *>(p.weight), first);
+                else static_for<0, P>([&](auto ic) { static_for<0, PIECE>([&](auto ec) { w[decltype(ic)::value].word[decltype(ec)::value] = 0x3f800000u; }); });
             }
+            settle(h, first);
+            if (adds) {
+                settle(r, first);
+                static_for<0, P>([&](auto ic) {
+                    constexpr int i = decltype(ic)::value;
+                    float v[PIECE];
+                    static_for<0, PIECE>([&](auto ec) { constexpr int e = decltype(ec)::value; v[e] = __fadd_rn(h[i].template get<e>(), r[i].template get<e>()); });
+                    h[i].set(v);
+                });
+            }
+            if (p.sum && !again) static_for<0, P>([&](auto ic) { store(h[decltype(ic)::value], sum, first + t + decltype(ic)::value * T); });
+            if (weights && p.weight) settle(w, first);
         };
         // the sum of (h lift)^2 and the largest |h lift w| over the row, in all its threads
         float squares, top;
@@ -107,8 +109,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rms_norm_kernel(RmsNormPara
             double long_sum = 0;                  // over turns
             unsigned most = 0;                    // magnitudes' bits sort as they do, infinities and NaN last
             for (int turn = 0; turn < turns; ++turn) {
-                if (!HELD || !again) fetch(turn * T * P, again);
-                if (TO == NORM_TOKENS && (!HELD || !again)) fetch_weight(turn * T * P);
+                if (!HELD || !again) fetch(turn * T * P, again, HELD || TO == NORM_TOKENS);
                 float s[2] = {0.f, 0.f};
                 static_for<0, P>([&](auto ic) {
                     constexpr int i = decltype(ic)::value;
@@ -136,7 +137,6 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rms_norm_kernel(RmsNormPara
             }
             top = __builtin_bit_cast(float, most);
         };
-        if (TO != NORM_TOKENS && HELD) fetch_weight(0);
         statistics(std::false_type{}, 1.f, false);
         float mean = __builtin_fmaf(squares, p.inv_cols, p.epsilon), lift = 1.f;
         if (!(mean >= NORM_LEAST && mean < __builtin_inff())) {       // a row's threads agree
@@ -150,7 +150,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rms_norm_kernel(RmsNormPara
             static_cast<float *>(p.scales)[row] = top < __builtin_inff() ? __fdiv_rn(__fmul_rn(top, r), 127.f) : __builtin_nanf("");
         char *const out = static_cast<char *>(p.out) + at * p.out_stride * (TO == NORM_ROWS ? SIZE : 1);
         for (int turn = 0; turn < turns; ++turn) {
-            if (!HELD) fetch(turn * T * P, true), fetch_weight(turn * T * P);
+            if (!HELD) fetch(turn * T * P, true, true);
             static_for<0, P>([&](auto ic) {
                 constexpr int i = decltype(ic)::value;
                 const int piece = turn * T * P + t + i * T;
@@ -195,7 +195,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rms_norm_kernel(RmsNormPara
 
 template <int TYPE, int TO, int T, int P, bool HELD>
 int launch_rms_norm(const RmsNormParams &p, hipStream_t stream) {
-    constexpr int THREADS = T < 256 ? 256 : T, ROWS = THREADS / T;
+    constexpr int THREADS = T <= 64 ? 256 : T, ROWS = THREADS / T;
     const int64_t blocks = ceil_div(p.rows, ROWS), most = int64_t(1) << 20;       // beyond that a workgroup takes several rows
     hipLaunchKernelGGL((rms_norm_kernel<TYPE, TO, T, P, HELD>), dim3(unsigned(blocks < most ? blocks : most)), dim3(THREADS), 0, stream, p);
     TSX_LAUNCH_CHECK("rms_norm_kernel");
@@ -204,19 +204,20 @@ int launch_rms_norm(const RmsNormParams &p, hipStream_t stream) {
 
 template <int TYPE, int TO>
 int rms_norm_type(const RmsNormParams &p, hipStream_t stream) {
-    // Several rows a wavefront where they are short, a wavefront a row, with no barrier, while there are rows for all CUs; more threads a
-    // row where there are few rows or it is long.
+    // One piece of eight values a thread where that makes a workgroup, two or three of a longer row: more of them leave a CU too few threads (bf16 with a
+    // residual, us: 2048 x 2048 256 threads a row 7.5, 128 7.9, 64 8.9; 5000 x 2050 128 threads with three pieces each 16.7, 64 with five 18.4, 256 with two
+    // 16.9; 8192 x 4096 256 threads 48, 64 55; 2000 x 8192 512 threads 27, 256 28).  Rows of two pieces a lane stay in a wavefront, with no barrier (8192 x
+    // 1000: 11.7, 256 threads 15.9), several short ones to each.  512 threads for rows of up to 4096 while there are few (1 x 4096 3.0, 256 threads 3.2).
     const int64_t pieces = ceil_div(p.cols, 8);
     if (pieces <= 4) return launch_rms_norm<TYPE, TO, 4, 1, true>(p, stream);
     if (pieces <= 16) return launch_rms_norm<TYPE, TO, 16, 1, true>(p, stream);
     if (pieces <= 64) return launch_rms_norm<TYPE, TO, 64, 1, true>(p, stream);
-    if (p.rows >= 512 || pieces <= 128) {
-        if (pieces <= 128) return launch_rms_norm<TYPE, TO, 64, 2, true>(p, stream);
-        if (pieces <= 256) return launch_rms_norm<TYPE, TO, 64, 4, true>(p, stream);
-    }
+    if (pieces <= 128) return launch_rms_norm<TYPE, TO, 64, 2, true>(p, stream);
     if (pieces <= 256) return launch_rms_norm<TYPE, TO, 256, 1, true>(p, stream);
+    if (pieces <= 384) return launch_rms_norm<TYPE, TO, 128, 3, true>(p, stream);
+    if (pieces <= 512 && p.rows < 2048) return launch_rms_norm<TYPE, TO, 512, 1, true>(p, stream);
     if (pieces <= 512) return launch_rms_norm<TYPE, TO, 256, 2, true>(p, stream);
-    if (pieces <= 1024) return launch_rms_norm<TYPE, TO, 256, 4, true>(p, stream);
+    if (pieces <= 1024) return launch_rms_norm<TYPE, TO, 512, 2, true>(p, stream);
     if (pieces <= 2048) return launch_rms_norm<TYPE, TO, 1024, 2, true>(p, stream);
     return launch_rms_norm<TYPE, TO, 1024, 2, false>(p, stream);
 }
