@@ -86,19 +86,14 @@ __device__ __forceinline__ float sum_of(float v) {
 // (the same instructions on random operands from registers, nothing else: 6.5 P, at 1.55 GHz).  Each multiplication takes 32 cycles of its SIMD; a
 // tile's epilogue and first chunk are 9 us of 67.  4 x 4 fragments on four wavefronts read a third less LDS and take 268 us, one wavefront a SIMD hides less.
 // Few tiles with a long K wait for one K-step after the other, 0.19 us each in tiles of 64; two groups of wavefronts halve that.
-//
-// Scales arrive by 64 words, each wavefront's share of a chunk, from rows or from words of K-steps; or (IN_ROWS false), from words of K-steps only, by 256,
-// one request for all tokens and one for all columns, a wavefront each: the fewer requests a CU has to issue, the less the multiplications wait (8192^3
-// 260 us with eight requests a chunk for scales, 240 with none).
-template <int WR, int WC, int FR, int FC, int KS, int S, int KG, bool IN_ROWS, int OUT>
+template <int WR, int WC, int FR, int FC, int KS, int S, int KG, int OUT>
 __global__ __launch_bounds__(WR *WC *KG * 64, WR * FR == 4 && KG == 1 ? 3 : 1) void gemm_mxfp4_kernel(MxGemmParams p) {
     constexpr int CHUNK = KS * KSTEP, PIECES = CHUNK / 16, WAVES = WR * WC * KG, ROWS = 32 * WR * FR, COLS = 32 * WC * FC, HALVES = 2 * KS / KG;
     constexpr int A_BYTES = ROWS * CHUNK, B_BYTES = COLS * CHUNK, A_LOADS = A_BYTES / 1024 / WAVES, B_LOADS = B_BYTES / 1024 / WAVES;
-    constexpr int A_WORDS = KS * ROWS / 64, WORDS = KS * (ROWS + COLS) / 64, S_LOADS = IN_ROWS ? (WORDS + WAVES - 1) / WAVES : 0;
+    constexpr int A_WORDS = KS * ROWS / 64, WORDS = KS * (ROWS + COLS) / 64, S_LOADS = (WORDS + WAVES - 1) / WAVES;      // scales: by 64 words
     constexpr int SCALES = A_BYTES + B_BYTES, BUFFER = SCALES + KS * (ROWS + COLS) * 4, LOADS = A_LOADS + B_LOADS + S_LOADS;
     static_assert(4 % KS == 0, "the weights hold whole chunks");
-    static_assert(IN_ROWS || (KS == 1 && ROWS == 256 && COLS == 256), "scales by 256 words");
-    static_assert(A_LOADS * 1024 * WAVES == A_BYTES && B_LOADS * 1024 * WAVES == B_BYTES && S >= 3 && (S - 1) * (LOADS + 1) < 64,
+    static_assert(A_LOADS * 1024 * WAVES == A_BYTES && B_LOADS * 1024 * WAVES == B_BYTES && S >= 3 && (S - 1) * LOADS < 64,
                   "whole loads, counted in six bits");
     extern __shared__ __attribute__((aligned(16))) int8_t lds[];      // [S][BUFFER]
     __shared__ __attribute__((aligned(16))) float of_cols[COLS];      // biases, requested ahead of everything
@@ -124,7 +119,7 @@ __global__ __launch_bounds__(WR *WC *KG * 64, WR * FR == 4 && KG == 1 ? 3 : 1) v
     const auto key_of = [](int row) { return (row >> (KS == 1 ? 2 : KS == 2 ? 1 : 0)) & (PIECES - 1); };
     const int chunks = (p.x_steps + KS - 1) / KS;
     const uint8_t *const a_base = p.x + int64_t(row0) * p.x_pitch;
-    unsigned a_off[A_LOADS], b_off[B_LOADS], s_off[S_LOADS + 1];
+    unsigned a_off[A_LOADS], b_off[B_LOADS], s_off[S_LOADS];
     int a_piece[A_LOADS];
     static_for<0, A_LOADS>([&](auto ic) {
         constexpr int i = decltype(ic)::value;
@@ -140,9 +135,9 @@ __global__ __launch_bounds__(WR *WC *KG * 64, WR * FR == 4 && KG == 1 ? 3 : 1) v
     });
     // Scales in LDS: [K-step of the chunk][row], then [K-step of the chunk][column].  A request's K-steps lie s_stride apart, the last of them is
     // s_last; selects, no branches: all requests of a chunk are one run of instructions.
-    const uint8_t *s_base[S_LOADS + 1];
-    int64_t s_stride[S_LOADS + 1];
-    int s_step[S_LOADS + 1], s_last[S_LOADS + 1];
+    const uint8_t *s_base[S_LOADS];
+    int64_t s_stride[S_LOADS];
+    int s_step[S_LOADS], s_last[S_LOADS];
     static_for<0, S_LOADS>([&](auto ic) {
         constexpr int i = decltype(ic)::value;
         const int unit = min(wave * S_LOADS + i, WORDS - 1), of_w = unit - A_WORDS;      // more wavefronts than requests: the last one again
@@ -154,15 +149,6 @@ __global__ __launch_bounds__(WR *WC *KG * 64, WR * FR == 4 && KG == 1 ? 3 : 1) v
         s_off[i] = is_x ? unsigned(min(unit % (ROWS / 64) * 64 + lane, p.m - 1 - row0)) * unsigned(p.scale_row)
                         : unsigned(min(of_w % (COLS / 64) * 64 + lane, (p.frags - frag0) * 32 - 1)) * 4u;
     });
-    const bool has_scales = !IN_ROWS && wave < 2;             // uniform: the wavefront that requests 256 words of x, or of w
-    if constexpr (!IN_ROWS) {
-        s_base[0] = wave == 0 ? p.x_scales + int64_t(row0) * 4 : reinterpret_cast<const uint8_t *>(p.w_scales) + frag0 * 128;
-        s_stride[0] = wave == 0 ? p.scale_step : int64_t(p.frags) * 128;
-        s_off[0] = wave == 0 ? lane * 16u : unsigned(min(lane * 4, (p.frags - frag0) * 32 - 4)) * 4u;      // words of x go up to whole tiles
-    }
-    auto request_scales = [&](int chunk, int buf) __attribute__((always_inline)) {
-        if (has_scales) to_lds(reinterpret_cast<const int8_t *>(s_base[0] + min(chunk, chunks - 1) * s_stride[0] + s_off[0]), lds + buf * BUFFER + SCALES + wave * 1024);
-    };
     const int64_t b_step = int64_t(p.frags) * (KS * 2048);
     // request i of LOADS of a chunk
     auto request = [&](auto ic, int chunk, int buf) __attribute__((always_inline)) {
@@ -208,11 +194,8 @@ __global__ __launch_bounds__(WR *WC *KG * 64, WR * FR == 4 && KG == 1 ? 3 : 1) v
             a_scale[h / 2 % 2][f] = *reinterpret_cast<const int *>(at + SCALES + (step * ROWS + (wave_r * FR + f) * 32 + lane % 32) * 4);
         }
     };
-    static_for<0, S - 1>([&](auto sc) {
-        request_scales(decltype(sc)::value, decltype(sc)::value);
-        static_for<0, LOADS>([&](auto ic) { request(ic, decltype(sc)::value, decltype(sc)::value); });
-    });
-    wait_for_all_but<(S - 2) * LOADS>();                     // of a wavefront that requested scales, too, that is behind its first chunk
+    static_for<0, S - 1>([&](auto sc) { static_for<0, LOADS>([&](auto ic) { request(ic, decltype(sc)::value, decltype(sc)::value); }); });
+    wait_for_all_but<(S - 2) * LOADS>();
     static_for<0, COL_TURNS>([&](auto ic) {
         const int at = threadIdx.x + decltype(ic)::value * THREADS;
         if (COLS % THREADS == 0 || at < COLS) of_cols[at] = col_bias[decltype(ic)::value];
@@ -231,7 +214,6 @@ __global__ __launch_bounds__(WR *WC *KG * 64, WR * FR == 4 && KG == 1 ? 3 : 1) v
             int as[FR], bs[FC];
             static_for<0, FR>([&](auto ic) { as[decltype(ic)::value] = int(unsigned(a_scale[h / 2 % 2][decltype(ic)::value]) >> upper); });
             static_for<0, FC>([&](auto fc) { bs[decltype(fc)::value] = int(unsigned(b_scale[h / 2 % 2][decltype(fc)::value]) >> upper); });
-            if constexpr (h == 0 && FETCHES) request_scales(c + S - 1, before);
             if constexpr (h + 1 == HALVES) {
                 // Every wavefront has its operands of this chunk in registers: its buffer is free behind the barrier, and the next
                 // chunk is there for all.  The rest of this chunk's arithmetic covers the first reads behind it.
@@ -327,7 +309,7 @@ __global__ __launch_bounds__(WR *WC *KG * 64, WR * FR == 4 && KG == 1 ? 3 : 1) v
 // on.  X, the type of the rows: MXFP4, or floats, which a lane quantizes where it needs them, 32 values of one token, a block: nothing has to meet
 // for a block's scale, so there is no launch ahead of the product and no barrier in it before the partial sums meet in LDS.
 // 16x16x128 instruction: accumulator r of lane l is column 4 (l / 16) + r of token l % 16.
-constexpr int FEW = 16;
+constexpr int FEW = 16, FEW_MOST = 1 << 14;      // more would leave a launch's second axis
 
 struct FewTokens : MxGemmParams {
     const void *values;                // rows of floats
@@ -339,11 +321,13 @@ template <int X, int WAVES, int AHEAD, int OUT>
 __global__ __launch_bounds__(WAVES * 64) void gemm_mxfp4_few_kernel(FewTokens p) {
     __shared__ float sums[WAVES][4][64];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), block = lane / 16, row = lane % 16;
-    const int col16 = blockIdx.x;      // in columns of 16
+    // blockIdx % 8 is the XCD: each takes a run of columns, so that no two L2s have parts of an output's cache line
+    const int col16 = int(blockIdx.x % 8) * p.tiles_per_xcd + int(blockIdx.x / 8), row0 = int(blockIdx.y) * FEW;      // in columns of 16
+    if (16 * col16 >= p.n) return;
     const int8_t *const w = p.w + int64_t(col16 >> 1) * 2048 + (block >> 1) * 1024 + (16 * (col16 & 1) + row + 32 * (block & 1)) * 16;
     const int8_t *const ws = p.w_scales + (col16 * 16 + row) * 4;
     const int64_t w_step = int64_t(p.frags) * 2048, ws_step = int64_t(p.frags) * 128;
-    const int token = min(row, p.m - 1);
+    const int token = min(row0 + row, p.m - 1);
     v4i a[AHEAD];
     unsigned as[AHEAD];
     auto fetch = [&](int first) __attribute__((always_inline)) {
@@ -394,7 +378,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_mxfp4_few_kernel(FewTokens p)
     static_for<0, 4>([&](auto rc) { sums[wave][decltype(rc)::value][lane] = acc[decltype(rc)::value]; });
     __syncthreads();
     const int in = threadIdx.x % 16, col = col16 * 16 + in, to = threadIdx.x / 16;
-    if (to >= p.m || col >= p.n) return;
+    if (to >= FEW || row0 + to >= p.m || col >= p.n) return;
     float v[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < WAVES; ++i) v[0] = __fadd_rn(v[0], sums[i][in % 4][to + 16 * (in / 4)]);
@@ -402,7 +386,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_mxfp4_few_kernel(FewTokens p)
     activate_tokens<OUT>(v, p.act, p.slope);
     Run<OUT, 1> out;
     out.set(v);
-    out.store(static_cast<char *>(p.out) + (to * p.out_stride + col) * (OUT == TSX_TYPE_F32 ? 4 : 2));
+    out.store(static_cast<char *>(p.out) + ((row0 + to) * p.out_stride + col) * (OUT == TSX_TYPE_F32 ? 4 : 2));
 }
 
 // codes and scales of weights [n][k] to the layout above
@@ -434,10 +418,10 @@ __global__ __launch_bounds__(256) void pack_mxfp4_kernel(const uint8_t *codes, i
     }
 }
 
-// MXFP4 rows that a kernel does not read where they are: codes to whole K-steps (unless `to` is null), scales to words of K-steps
+// MXFP4 rows of another length, stride or alignment than the kernels read: codes to whole K-steps, scales to words of K-steps
 __global__ __launch_bounds__(256) void copy_mxfp4_kernel(const uint8_t *codes, int64_t codes_stride, const uint8_t *scales, int64_t scales_stride, int bytes,
-                                                         int blocks, int64_t rows, int steps, uint8_t *to, uint8_t *to_scales, int64_t scale_step) {
-    const int64_t pitch = int64_t(steps) * KSTEP, pieces = to ? rows * steps * 4 : 0, words = rows * steps;
+                                                         int blocks, int64_t rows, int steps, uint8_t *to, uint8_t *to_scales) {
+    const int64_t pitch = int64_t(steps) * KSTEP, pieces = rows * steps * 4, words = rows * steps;
     for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < pieces + words; i += int64_t(gridDim.x) * 256) {
         if (i < pieces) {
             const int64_t row = i / (steps * 4);
@@ -453,12 +437,12 @@ __global__ __launch_bounds__(256) void copy_mxfp4_kernel(const uint8_t *codes, i
             unsigned v = 0;
             for (int b = 0; b < 4; ++b)
                 if (step * 4 + b < blocks) v |= unsigned(scales[row * scales_stride + step * 4 + b]) << (8 * b);
-            *reinterpret_cast<unsigned *>(to_scales + step * scale_step + row * 4) = v;
+            reinterpret_cast<unsigned *>(to_scales)[word] = v;
         }
     }
 }
 
-template <int WR, int WC, int FR, int FC, int KS, int S, int KG, bool IN_ROWS, int OUT>
+template <int WR, int WC, int FR, int FC, int KS, int S, int KG, int OUT>
 int launch_tile(MxGemmParams p, hipStream_t stream) {
     p.row_tiles = int(ceil_div(p.m, 32 * WR * FR));
     p.col_tiles = int(ceil_div(p.n, 32 * WC * FC));
@@ -467,7 +451,7 @@ int launch_tile(MxGemmParams p, hipStream_t stream) {
     p.tiles_per_xcd = int(per_xcd);
     p.streams = int64_t(p.m) * p.n * int64_t(element_bytes(OUT)) > 32 << 20;
     constexpr int LDS = S * 32 * (WR * FR + WC * FC) * KS * (KSTEP + 4);
-    const auto kernel = gemm_mxfp4_kernel<WR, WC, FR, FC, KS, S, KG, IN_ROWS, OUT>;
+    const auto kernel = gemm_mxfp4_kernel<WR, WC, FR, FC, KS, S, KG, OUT>;
     if (LDS > 64 * 1024) {
         const int rc = grant_lds(reinterpret_cast<const void *>(kernel), LDS);
         if (rc) return rc;
@@ -478,8 +462,9 @@ int launch_tile(MxGemmParams p, hipStream_t stream) {
 }
 
 template <int X, int WAVES, int AHEAD, int OUT>
-int launch_few(const FewTokens &p, hipStream_t stream) {
-    hipLaunchKernelGGL((gemm_mxfp4_few_kernel<X, WAVES, AHEAD, OUT>), dim3(unsigned(ceil_div(p.n, 16))), dim3(WAVES * 64), 0, stream, p);
+int launch_few(FewTokens p, hipStream_t stream) {
+    p.tiles_per_xcd = int(ceil_div(p.n, 128));
+    hipLaunchKernelGGL((gemm_mxfp4_few_kernel<X, WAVES, AHEAD, OUT>), dim3(unsigned(8 * p.tiles_per_xcd), unsigned(ceil_div(p.m, FEW))), dim3(WAVES * 64), 0, stream, p);
     TSX_LAUNCH_CHECK("gemm_mxfp4_few_kernel");
     return 0;
 }
@@ -527,10 +512,10 @@ template <int OUT>
 int launch(Kernel kernel, const tsx_mxfp4_gemm *g, const MxGemmParams &p, hipStream_t stream) {
     switch (kernel) {
         case Kernel::few: return few_tokens<OUT>(g, p, stream);
-        case Kernel::tile_64_by_k: return launch_tile<2, 2, 1, 1, 4, 3, 2, true, OUT>(p, stream);
-        case Kernel::tile_64: return launch_tile<2, 2, 1, 1, 2, 3, 1, true, OUT>(p, stream);
-        case Kernel::tile_128: return launch_tile<2, 2, 2, 2, 1, 3, 1, true, OUT>(p, stream);
-        default: return launch_tile<2, 4, 4, 2, 1, 4, 1, false, OUT>(p, stream);
+        case Kernel::tile_64_by_k: return launch_tile<2, 2, 1, 1, 4, 3, 2, OUT>(p, stream);
+        case Kernel::tile_64: return launch_tile<2, 2, 1, 1, 2, 3, 1, OUT>(p, stream);
+        case Kernel::tile_128: return launch_tile<2, 2, 2, 2, 1, 3, 1, OUT>(p, stream);
+        default: return launch_tile<2, 4, 4, 2, 1, 3, 1, OUT>(p, stream);
     }
 }
 
@@ -556,24 +541,22 @@ bool reads_in_place(const tsx_mxfp4_gemm *g) {
            (g->m <= 1 || (g->x_stride % 16 == 0 && g->x_stride <= 1 << 23 && g->x_scales_stride % 4 == 0 && g->x_scales_stride <= 1 << 23));
 }
 
-// What a call does: its kernel, and what the workspace holds, codes [m][steps][64] and scales [steps][m in whole tiles of 256][4].
+// What a call does: its kernel, and whether the workspace holds its rows, codes [m][steps][64] and scales [steps][m][4].
 struct Plan {
     Kernel kernel;
-    bool codes, scales;
-    int64_t steps, code_bytes, words;      // words: of a K-step's scales
+    bool copies;
+    int64_t steps, code_bytes, word_bytes;      // word_bytes: of a K-step's scales
     explicit Plan(const tsx_mxfp4_gemm *g) {
         kernel = choose(g->m, g->n, g->k);
         // TSX_MXFP4_KERNEL: that kernel, by its place in the list above, for any call it can take (tests, measurements)
         const char *e = std::getenv("TSX_MXFP4_KERNEL");
-        if (e && e[0] >= (g->m <= FEW ? '0' : '1') && e[0] <= '4') kernel = Kernel(e[0] - '0');
-        const bool in_place = reads_in_place(g) || (kernel == Kernel::few && g->x_type != TSX_TYPE_MXFP4);
-        codes = g->m > 0 && !in_place;
-        scales = codes || (g->m > 0 && kernel == Kernel::tile_256);      // which reads words of K-steps
+        if (e && e[0] >= (g->m <= FEW_MOST ? '0' : '1') && e[0] <= '4') kernel = Kernel(e[0] - '0');
+        copies = g->m > 0 && !reads_in_place(g) && (kernel != Kernel::few || g->x_type == TSX_TYPE_MXFP4);
         steps = ceil_div(g->k, MX_STEP);
-        code_bytes = codes ? g->m * steps * KSTEP : 0;
-        words = round_up(g->m, 256);
+        code_bytes = g->m * steps * KSTEP;
+        word_bytes = int64_t(g->m) * 4;
     }
-    size_t workspace_bytes() const { return size_t(code_bytes) + (scales ? size_t(words) * steps * 4 : 0); }
+    size_t workspace_bytes() const { return copies ? size_t(code_bytes + word_bytes * steps) : 0; }
 };
 
 int check_weights(int32_t k, int32_t n) {
@@ -632,22 +615,29 @@ int tsx_gemm_mxfp4(const tsx_mxfp4_gemm *g, void *workspace_dev, size_t workspac
     const int steps = int(plan.steps);
     p.x_steps = steps;
     p.k = steps * tsx::KSTEP;
-    uint8_t *const to = static_cast<uint8_t *>(workspace_dev), *const to_scales = to + plan.code_bytes;
-    p.x = plan.codes ? to : static_cast<const uint8_t *>(g->x_dev);
-    p.x_pitch = plan.codes ? p.k : g->m <= 1 ? 0 : g->x_stride;
-    p.x_scales = plan.scales ? to_scales : g->x_scales_dev;
-    p.scale_row = plan.scales ? 4 : g->m <= 1 ? 0 : g->x_scales_stride;
-    p.scale_step = plan.scales ? plan.words * 4 : 4;
-    if (plan.scales && !codes) {
-        rc = tsx::quantize_mxfp4_rows(g->m, g->k, steps * tsx::MX_STEP, g->x_dev, g->x_type, g->x_stride,
-                                      tsx::MxRows{to, to_scales, p.x_pitch, p.scale_row, p.scale_step}, stream);
-        if (rc) return rc;
-    } else if (plan.scales) {
-        const int64_t units = int64_t(g->m) * steps * (plan.codes ? 5 : 1), blocks = tsx::ceil_div(units, 256);
-        hipLaunchKernelGGL(tsx::copy_mxfp4_kernel, dim3(unsigned(std::min<int64_t>(blocks, 1 << 16))), dim3(256), 0, stream, static_cast<const uint8_t *>(g->x_dev),
-                           g->x_stride, g->x_scales_dev, g->x_scales_stride, (g->k + 1) / 2, (g->k + 31) / 32, int64_t(g->m), steps, plan.codes ? to : nullptr, to_scales,
-                           p.scale_step);
-        TSX_LAUNCH_CHECK("copy_mxfp4_kernel");
+    if (plan.copies) {
+        uint8_t *const to = static_cast<uint8_t *>(workspace_dev), *const to_scales = to + plan.code_bytes;
+        p.x = to;
+        p.x_scales = to_scales;
+        p.x_pitch = p.k;
+        p.scale_row = 4;
+        p.scale_step = plan.word_bytes;
+        if (codes) {
+            const int64_t units = int64_t(g->m) * steps * 5, blocks = tsx::ceil_div(units, 256);
+            hipLaunchKernelGGL(tsx::copy_mxfp4_kernel, dim3(unsigned(std::min<int64_t>(blocks, 1 << 16))), dim3(256), 0, stream, static_cast<const uint8_t *>(g->x_dev),
+                               g->x_stride, g->x_scales_dev, g->x_scales_stride, (g->k + 1) / 2, (g->k + 31) / 32, int64_t(g->m), steps, to, to_scales);
+            TSX_LAUNCH_CHECK("copy_mxfp4_kernel");
+        } else {
+            rc = tsx::quantize_mxfp4_rows(g->m, g->k, steps * tsx::MX_STEP, g->x_dev, g->x_type, g->x_stride,
+                                          tsx::MxRows{to, to_scales, p.x_pitch, p.scale_row, p.scale_step}, stream);
+            if (rc) return rc;
+        }
+    } else if (codes) {
+        p.x = static_cast<const uint8_t *>(g->x_dev);
+        p.x_scales = g->x_scales_dev;
+        p.x_pitch = g->m <= 1 ? 0 : g->x_stride;
+        p.scale_row = g->m <= 1 ? 0 : g->x_scales_stride;
+        p.scale_step = 4;
     }
     p.w = static_cast<const int8_t *>(g->packed_w_dev);
     p.w_scales = p.w + tsx::packed_codes(g->k, g->n);

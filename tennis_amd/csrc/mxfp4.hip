@@ -2,7 +2,8 @@
 //
 // Bound: HBM, the values' bytes and 17 / 32 of a byte each.  A lane holds pieces of eight values; four neighbouring lanes hold a block, find
 // its largest magnitude by two lane exchanges, and each leaves four bytes of codes.  Pieces of all rows are numbered through, so that short
-// rows and long ones fill the card alike; nothing but the four lanes of a block has to meet.
+// rows and long ones fill the card alike; nothing but the four lanes of a block has to meet.  One piece a lane: two, four and eight are no faster (bf16
+// to codes, us: 8192 x 8192 30.1, 30.0, 31.3, 32.9; 4096 x 4096 8.1, 8.3, 8.8, 9.0).  8192 x 8192 is 5.6 TB/s, a copy of 1 GiB 5.1.
 #include <algorithm>
 
 #include "mxfp4.hpp"
@@ -22,41 +23,31 @@ struct ToMxParams {
 };
 
 // TAILS: rows end inside a piece, or pieces behind their ends are written
-template <int TYPE, int P, bool TAILS>
+template <int TYPE, bool TAILS>
 __global__ __launch_bounds__(THREADS) void quantize_mxfp4_kernel(ToMxParams p) {
     constexpr int SIZE = TYPE == TSX_TYPE_F32 ? 4 : 2;
     typedef Run<TYPE, PIECE> Values;
-    const unsigned first = blockIdx.x * (THREADS * P) + threadIdx.x;
-    Values v[P];
-    int64_t row[P];
-    int piece[P];
-    static_for<0, P>([&](auto ic) {
-        constexpr int i = decltype(ic)::value;
-        const unsigned at = min(first + i * THREADS, p.total - 1), r = p.pieces.quotient(at);
-        row[i] = r;
-        piece[i] = int(at - r * p.pieces.d);
-        const char *const x = static_cast<const char *>(p.x) + row[i] * p.x_stride * SIZE;
-        if (!TAILS) {
-            v[i].load(x + int64_t(piece[i]) * (PIECE * SIZE));
-        } else if (p.cols >= PIECE) {      // uniform
-            load_piece<TYPE>(v[i], x, piece[i] * PIECE, p.cols);
-        } else {
-            v[i].clear();
-            if (piece[i] == 0) v[i].load_some(x, p.cols);
-        }
-    });
-    if (TAILS && p.cols >= PIECE) static_for<0, P>([&](auto ic) { settle_piece<TYPE>(v[decltype(ic)::value], piece[decltype(ic)::value] * PIECE, p.cols); });
-    static_for<0, P>([&](auto ic) {
-        constexpr int i = decltype(ic)::value;
-        const unsigned top = over_lanes(v[i].top(0), 2, [](unsigned a, unsigned b) { return Values::template larger<TYPE>(a, b); });
-        const unsigned scale = mx_scale(top_value<TYPE>(top));
-        const unsigned codes = mx_codes<TYPE>(v[i], scale);
-        if (first + i * THREADS >= p.total) return;
-        const int left = p.cols_out - piece[i] * PIECE;
-        if (!TAILS || left > 0) store_codes(p.to.codes + row[i] * p.to.codes_stride + int64_t(piece[i]) * (PIECE / 2), codes, TAILS ? left : PIECE);
-        const int block = piece[i] / 4;
-        if (piece[i] % 4 == 0) p.to.scales[row[i] * p.to.scale_row + (block >> 2) * p.to.scale_group + (block & 3)] = uint8_t(scale);
-    });
+    const unsigned id = blockIdx.x * THREADS + threadIdx.x, at = min(id, p.total - 1), r = p.pieces.quotient(at);      // a block's lanes agree on whether they are there
+    const int64_t row = r;
+    const int piece = int(at - r * p.pieces.d);
+    const char *const x = static_cast<const char *>(p.x) + row * p.x_stride * SIZE;
+    Values v;
+    if (!TAILS) {
+        v.load(x + int64_t(piece) * (PIECE * SIZE));
+    } else if (p.cols >= PIECE) {      // uniform
+        load_piece<TYPE>(v, x, piece * PIECE, p.cols);
+        settle_piece<TYPE>(v, piece * PIECE, p.cols);
+    } else {
+        v.clear();
+        if (piece == 0) v.load_some(x, p.cols);
+    }
+    const unsigned top = over_lanes(v.top(0), 2, [](unsigned a, unsigned b) { return Values::template larger<TYPE>(a, b); });
+    const unsigned scale = mx_scale(top_value<TYPE>(top)), codes = mx_codes<TYPE>(v, scale);
+    if (id >= p.total) return;
+    const int left = p.cols_out - piece * PIECE;
+    if (!TAILS || left > 0) store_codes(p.to.codes + row * p.to.codes_stride + int64_t(piece) * (PIECE / 2), codes, TAILS ? left : PIECE);
+    const int block = piece / 4;
+    if (piece % 4 == 0) p.to.scales[row * p.to.scale_row + (block >> 2) * p.to.scale_group + (block & 3)] = uint8_t(scale);
 }
 
 struct FromParams {
@@ -68,57 +59,47 @@ struct FromParams {
     int cols;
 };
 
-// MX: MXFP4 rows, otherwise int8 tokens.  A lane writes pieces of eight values.
-template <int TYPE, int P, bool MX>
+// MX: MXFP4 rows, otherwise int8 tokens
+template <int TYPE, bool MX>
 __global__ __launch_bounds__(THREADS) void dequantize_kernel(FromParams p) {
-    constexpr int SIZE = TYPE == TSX_TYPE_F32 ? 4 : 2;
-    typedef Run<TYPE, PIECE> Values;
-    const unsigned first = blockIdx.x * (THREADS * P) + threadIdx.x;
-    v2u word[P];
-    unsigned scale[P];
-    int64_t row[P];
-    int piece[P];
-    static_for<0, P>([&](auto ic) {
-        constexpr int i = decltype(ic)::value, BYTES = MX ? PIECE / 2 : PIECE;
-        const unsigned at = min(first + i * THREADS, p.total - 1), r = p.pieces.quotient(at);
-        row[i] = r;
-        piece[i] = int(at - r * p.pieces.d);
-        const uint8_t *const codes = p.codes + row[i] * p.codes_stride + int64_t(piece[i]) * BYTES;
-        const int bytes = MX ? (p.cols + 1) / 2 - piece[i] * BYTES : p.cols - piece[i] * BYTES;
-        if (bytes >= BYTES) {
-            if constexpr (MX) word[i][0] = *reinterpret_cast<const u_any *>(codes);
-            else word[i] = *reinterpret_cast<const v2u_any *>(codes);
-        } else {
-            word[i] = v2u{0, 0};
-            static_for<0, BYTES - 1>([&](auto bc) {
-                constexpr int b = decltype(bc)::value;
-                if (b < bytes) word[i][b / 4] |= unsigned(codes[b]) << (8 * (b % 4));
-            });
-        }
-        if constexpr (MX) scale[i] = p.scales[row[i] * p.scales_stride + piece[i] / 4];
-        else scale[i] = reinterpret_cast<const unsigned *>(p.scales)[row[i]];
-    });
-    static_for<0, P>([&](auto ic) {
-        constexpr int i = decltype(ic)::value;
-        Values v;
-        if constexpr (MX) {
-            v = mx_values<TYPE>(word[i][0], scale[i]);
-        } else {
-            float f[PIECE];
-            static_for<0, PIECE>([&](auto ec) {
-                constexpr int e = decltype(ec)::value;
-                unsigned product = __builtin_bit_cast(unsigned, __fmul_rn(float(int(word[i][e / 4] << (24 - 8 * (e % 4))) >> 24), __builtin_bit_cast(float, scale[i])));
-                if constexpr (TYPE == TSX_TYPE_F16) renew(product);      // else the product and its conversion become one instruction with one rounding
-                f[e] = __builtin_bit_cast(float, product);
-            });
-            v.set(f);
-        }
-        if (first + i * THREADS >= p.total) return;
-        char *const out = static_cast<char *>(p.out) + (row[i] * p.out_stride + int64_t(piece[i]) * PIECE) * SIZE;
-        const int left = p.cols - piece[i] * PIECE;
-        if (left >= PIECE) v.store(out);
-        else v.store_some(out, left);
-    });
+    constexpr int SIZE = TYPE == TSX_TYPE_F32 ? 4 : 2, BYTES = MX ? PIECE / 2 : PIECE;
+    const unsigned id = blockIdx.x * THREADS + threadIdx.x;
+    if (id >= p.total) return;
+    const unsigned r = p.pieces.quotient(id);
+    const int64_t row = r;
+    const int piece = int(id - r * p.pieces.d);
+    const uint8_t *const codes = p.codes + row * p.codes_stride + int64_t(piece) * BYTES;
+    const int bytes = (MX ? (p.cols + 1) / 2 : p.cols) - piece * BYTES;
+    unsigned scale;
+    if constexpr (MX) scale = p.scales[row * p.scales_stride + piece / 4];
+    else scale = reinterpret_cast<const unsigned *>(p.scales)[row];
+    v2u word = {0, 0};
+    if (bytes >= BYTES) {
+        if constexpr (MX) word[0] = *reinterpret_cast<const u_any *>(codes);
+        else word = *reinterpret_cast<const v2u_any *>(codes);
+    } else {
+        static_for<0, BYTES - 1>([&](auto bc) {
+            constexpr int b = decltype(bc)::value;
+            if (b < bytes) word[b / 4] |= unsigned(codes[b]) << (8 * (b % 4));
+        });
+    }
+    Run<TYPE, PIECE> v;
+    if constexpr (MX) {
+        v = mx_values<TYPE>(word[0], scale);
+    } else {
+        float f[PIECE];
+        static_for<0, PIECE>([&](auto ec) {
+            constexpr int e = decltype(ec)::value;
+            unsigned product = __builtin_bit_cast(unsigned, __fmul_rn(float(int(word[e / 4] << (24 - 8 * (e % 4))) >> 24), __builtin_bit_cast(float, scale)));
+            if constexpr (TYPE == TSX_TYPE_F16) renew(product);      // else the product and its conversion become one instruction with one rounding
+            f[e] = __builtin_bit_cast(float, product);
+        });
+        v.set(f);
+    }
+    char *const out = static_cast<char *>(p.out) + (row * p.out_stride + int64_t(piece) * PIECE) * SIZE;
+    const int left = p.cols - piece * PIECE;
+    if (left >= PIECE) v.store(out);
+    else v.store_some(out, left);
 }
 
 // Pieces are counted in 31 bits: rows in runs of as many as that holds.  launch(first row, rows)
@@ -130,9 +111,6 @@ int in_runs(int64_t rows, int64_t pieces, F &&launch) {
     return 0;
 }
 
-// Four pieces a lane where that still gives every CU its 2048 lanes, so that a lane has four requests on their way; else one
-constexpr int64_t MANY = 4 * 256 * 2048;
-
 template <int TYPE>
 int to_mx(int64_t rows, int cols, int cols_out, const void *x, int64_t x_stride, const MxRows &to, hipStream_t stream) {
     const int64_t pieces = ceil_div(cols_out, MX_BLOCK) * (MX_BLOCK / PIECE);
@@ -143,13 +121,9 @@ int to_mx(int64_t rows, int cols, int cols_out, const void *x, int64_t x_stride,
         part.scales += at * to.scale_row;
         const ToMxParams p{static_cast<const char *>(x) + at * x_stride * int64_t(element_bytes(TYPE)), part, Divider(pieces), x_stride, unsigned(total), cols, cols_out};
         const bool tails = cols % MX_BLOCK != 0 || cols_out != cols;
-        const auto start = [&](auto kernel, int per) {
-            hipLaunchKernelGGL(kernel, dim3(unsigned(ceil_div(total, THREADS * per))), dim3(THREADS), 0, stream, p);
-            TSX_LAUNCH_CHECK("quantize_mxfp4_kernel");
-            return 0;
-        };
-        if (total >= MANY) return tails ? start(quantize_mxfp4_kernel<TYPE, 4, true>, 4) : start(quantize_mxfp4_kernel<TYPE, 4, false>, 4);
-        return tails ? start(quantize_mxfp4_kernel<TYPE, 1, true>, 1) : start(quantize_mxfp4_kernel<TYPE, 1, false>, 1);
+        hipLaunchKernelGGL((tails ? quantize_mxfp4_kernel<TYPE, true> : quantize_mxfp4_kernel<TYPE, false>), dim3(unsigned(ceil_div(total, THREADS))), dim3(THREADS), 0, stream, p);
+        TSX_LAUNCH_CHECK("quantize_mxfp4_kernel");
+        return 0;
     });
 }
 
@@ -162,9 +136,7 @@ int from(int64_t rows, int cols, const void *codes, int64_t codes_stride, const 
         const FromParams p{static_cast<const uint8_t *>(codes) + at * codes_stride, static_cast<const uint8_t *>(scales) + at * (MX ? scales_stride : 4),
                            static_cast<char *>(out) + at * out_stride * int64_t(element_bytes(TYPE)), Divider(pieces), codes_stride, scales_stride, out_stride,
                            unsigned(total), cols};
-        const int per = total >= MANY ? 4 : 1;
-        const auto kernel = per == 4 ? dequantize_kernel<TYPE, 4, MX> : dequantize_kernel<TYPE, 1, MX>;
-        hipLaunchKernelGGL(kernel, dim3(unsigned(ceil_div(total, THREADS * per))), dim3(THREADS), 0, stream, p);
+        hipLaunchKernelGGL((dequantize_kernel<TYPE, MX>), dim3(unsigned(ceil_div(total, THREADS))), dim3(THREADS), 0, stream, p);
         TSX_LAUNCH_CHECK("dequantize_kernel");
         return 0;
     });

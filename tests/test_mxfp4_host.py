@@ -57,10 +57,10 @@ def gemm(capi, **change):
 
 def test_product_refuses(capi):
     L = capi.lib()
-    assert L.tsx_gemm_mxfp4_workspace_bytes(ctypes.byref(gemm(capi, m=100))) == 100 * 128 + 256 * 8
+    assert L.tsx_gemm_mxfp4_workspace_bytes(ctypes.byref(gemm(capi, m=100))) == 100 * (128 + 8)
     codes = dict(x_type=4, x_stride=128, x_scales_dev=AT)
     assert L.tsx_gemm_mxfp4_workspace_bytes(ctypes.byref(gemm(capi, m=100, **codes))) == 0
-    assert L.tsx_gemm_mxfp4_workspace_bytes(ctypes.byref(gemm(capi, m=100, **dict(codes, x_dev=AT + 1)))) == 100 * 128 + 256 * 8
+    assert L.tsx_gemm_mxfp4_workspace_bytes(ctypes.byref(gemm(capi, m=100, **dict(codes, x_dev=AT + 1)))) == 100 * (128 + 8)
     assert L.tsx_gemm_mxfp4(ctypes.byref(gemm(capi, m=0)), None, 0, None) == 0
     for change, word in ((dict(m=-1), "extents"), (dict(n=0), "extents"), (dict(k=0), "extents"), (dict(m=1 << 28), "2^28"), (dict(n=1 << 24, out_stride=1 << 24), "2^24"),
                          (dict(k=1 << 21, x_stride=1 << 21), "2^21"), (dict(x_type=3), "element type"), (dict(x_type=5), "element type"), (dict(out_type=3), "output type"),
