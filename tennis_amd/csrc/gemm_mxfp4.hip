@@ -302,14 +302,15 @@ __global__ __launch_bounds__(WR *WC *KG * 64, WR * FR == 4 && KG == 1 ? 3 : 1) v
     });
 }
 
-// ---- up to 16 tokens: a stream over the weights
+// ---- few tokens: a stream over the weights
 //
-// There the product reads 17 / 32 n k bytes of weights and does little with each.  A workgroup owns 16 output columns and its wavefronts split K, every
-// WAVES-th K-step each; a K-step of 16 columns is one 16-byte load a lane and a word of scales, AHEAD of them in flight from the first instruction
-// on.  X, the type of the rows: MXFP4, or floats, which a lane quantizes where it needs them, 32 values of one token, a block: nothing has to meet
-// for a block's scale, so there is no launch ahead of the product and no barrier in it before the partial sums meet in LDS.
-// 16x16x128 instruction: accumulator r of lane l is column 4 (l / 16) + r of token l % 16.
-constexpr int FEW = 16, FEW_MOST = 1 << 14;      // more would leave a launch's second axis
+// There the product reads 17 / 32 n k bytes of weights and does little with each.  A workgroup owns 16 output columns of 16 tokens and its wavefronts split K,
+// every WAVES-th K-step each; a K-step of 16 columns is one 16-byte load a lane and a word of scales, AHEAD of them in flight from the first instruction
+// on.  X, the type of the rows: MXFP4, or floats, which a wavefront quantizes where it needs them: a K-step of 16 rows is four requests of whole cache lines,
+// eight values a lane, four lanes a block, and its codes change lanes through the wavefront's own LDS.  Nothing there has to meet another wavefront, so
+// there is no launch ahead of the product and no barrier in it before the partial sums meet.  16x16x128 instruction: accumulator r of lane l is
+// column 4 (l / 16) + r of token l % 16.
+constexpr int FEW = 16, FEW_MOST = 1 << 14;      // more rows would leave a launch's second axis
 
 struct FewTokens : MxGemmParams {
     const void *values;                // rows of floats
@@ -317,17 +318,35 @@ struct FewTokens : MxGemmParams {
     int cols;                          // values of such a row
 };
 
-template <int X, int WAVES, int AHEAD, int OUT>
+// What a wavefront writes to its own LDS it reads in that order, without a wait: the compiler is not to change it.
+__device__ __forceinline__ void wavefront_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local"); }
+template <int N>
+__device__ __forceinline__ void put(const Run<N, 8> &v, char *at) {
+    static_for<0, Run<N, 8>::WORDS / 4>([&](auto wc) { constexpr int w = 4 * decltype(wc)::value; reinterpret_cast<v4u *>(at)[w / 4] = v4u{v.word[w], v.word[w + 1], v.word[w + 2], v.word[w + 3]}; });
+}
+template <int N>
+__device__ __forceinline__ void get(Run<N, 8> &v, const char *at) {
+    static_for<0, Run<N, 8>::WORDS / 4>([&](auto wc) {
+        constexpr int w = 4 * decltype(wc)::value;
+        const v4u q = reinterpret_cast<const v4u *>(at)[w / 4];
+        static_for<0, 4>([&](auto jc) { v.word[w + decltype(jc)::value] = q[decltype(jc)::value]; });
+    });
+}
+
+// G: of a workgroup's rows of floats, in fours, those that are there: one, or all
+template <int X, int G, int WAVES, int AHEAD, int OUT>
 __global__ __launch_bounds__(WAVES * 64) void gemm_mxfp4_few_kernel(FewTokens p) {
-    __shared__ float sums[WAVES][4][64];
+    constexpr bool FLOATS = X != TSX_TYPE_MXFP4;
+    // of a wavefront in LDS: a K-step, codes and scales of four rows or values of 16; then its sums [4][64]
+    constexpr int OWN = !FLOATS || G == 1 ? 1024 : 16 * MX_STEP * (X == TSX_TYPE_F32 ? 4 : 2);
+    __shared__ __attribute__((aligned(16))) char lds[WAVES * OWN];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), block = lane / 16, row = lane % 16;
     // blockIdx % 8 is the XCD: each takes a run of columns, so that no two L2s have parts of an output's cache line
     const int col16 = int(blockIdx.x % 8) * p.tiles_per_xcd + int(blockIdx.x / 8), row0 = int(blockIdx.y) * FEW;      // in columns of 16
-    if (16 * col16 >= p.n) return;
+    if (16 * col16 >= p.n) return;                           // uniform, ahead of the barriers
     const int8_t *const w = p.w + int64_t(col16 >> 1) * 2048 + (block >> 1) * 1024 + (16 * (col16 & 1) + row + 32 * (block & 1)) * 16;
     const int8_t *const ws = p.w_scales + (col16 * 16 + row) * 4;
     const int64_t w_step = int64_t(p.frags) * 2048, ws_step = int64_t(p.frags) * 128;
-    const int token = min(row0 + row, p.m - 1);
     v4i a[AHEAD];
     unsigned as[AHEAD];
     auto fetch = [&](int first) __attribute__((always_inline)) {
@@ -339,35 +358,67 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_mxfp4_few_kernel(FewTokens p)
         });
     };
     fetch(wave);
+    char *const mine = lds + wave * OWN;
     v4f acc = {0.f, 0.f, 0.f, 0.f};
     for (int first = wave; first < p.x_steps; first += WAVES * AHEAD) {
         v4i b[AHEAD];
         unsigned bs[AHEAD];
-        static_for<0, AHEAD>([&](auto uc) {
-            constexpr int u = decltype(uc)::value;
-            const int step = min(first + WAVES * u, p.x_steps - 1);
-            if constexpr (X == TSX_TYPE_MXFP4) {
+        if constexpr (FLOATS) {
+            constexpr int SIZE = X == TSX_TYPE_F32 ? 4 : 2;
+            typedef Run<X, 8> Values;
+            Values v[G][AHEAD];
+            static_for<0, G * AHEAD>([&](auto ic) {          // all requests at once; here `row` counts a K-step's pieces, `block` rows
+                constexpr int i = decltype(ic)::value / AHEAD, u = decltype(ic)::value % AHEAD;
+                const char *const x = static_cast<const char *>(p.values) + min(row0 + 4 * i + block, p.m - 1) * p.x_stride * SIZE;
+                const int k = min(first + WAVES * u, p.x_steps - 1) * MX_STEP + 8 * row;
+                if (p.cols >= 8) {                           // uniform
+                    load_piece<X>(v[i][u], x, k, p.cols);
+                } else {
+                    v[i][u].clear();
+                    if (k == 0) v[i][u].load_some(x, p.cols);
+                }
+            });
+            static_for<0, G * AHEAD>([&](auto ic) {
+                constexpr int i = decltype(ic)::value / AHEAD, u = decltype(ic)::value % AHEAD;
+                const int step = min(first + WAVES * u, p.x_steps - 1);
+                if ((step + 1) * MX_STEP > p.cols && p.cols >= 8) settle_piece<X>(v[i][u], step * MX_STEP + 8 * row, p.cols);      // uniform
+            });
+            const auto larger = [](unsigned one, unsigned other) { return Values::template larger<X>(one, other); };
+            static_for<0, AHEAD>([&](auto uc) {
+                constexpr int u = decltype(uc)::value;
+                if (u > 0 && first + WAVES * u >= p.x_steps) return;      // uniform
+                if constexpr (G == 1) {                      // four lanes a block, before its codes change lanes
+                    const unsigned scale = mx_scale(top_value<X>(over_lanes(v[0][u].top(0), 2, larger)));
+                    *reinterpret_cast<unsigned *>(mine + block * KSTEP + 4 * row) = mx_codes<X>(v[0][u], scale);
+                    if (row % 4 == 0) mine[4 * KSTEP + block * 4 + row / 4] = char(scale);
+                    wavefront_order();
+                    b[u] = *reinterpret_cast<const v4i *>(mine + row % 4 * KSTEP + block * 16);
+                    bs[u] = static_cast<unsigned char>(mine[4 * KSTEP + row % 4 * 4 + block]);
+                } else {                                     // values change lanes; a piece's place is XORed with its row, so that 16 rows cover all banks
+                    constexpr int PIECE = 8 * SIZE;
+                    static_for<0, 4>([&](auto ic) {
+                        constexpr int i = decltype(ic)::value;
+                        put(v[i][u], mine + ((4 * i + block) * 16 + (row ^ (4 * i + block))) * PIECE);
+                    });
+                    wavefront_order();
+                    Values own[4];
+                    unsigned top = 0;
+                    static_for<0, 4>([&](auto qc) { constexpr int q = decltype(qc)::value; get(own[q], mine + (row * 16 + ((4 * block + q) ^ row)) * PIECE); });
+                    static_for<0, 4>([&](auto qc) { top = own[decltype(qc)::value].top(top); });
+                    bs[u] = mx_scale(top_value<X>(top));
+                    static_for<0, 4>([&](auto qc) { constexpr int q = decltype(qc)::value; b[u][q] = int(mx_codes<X>(own[q], bs[u])); });
+                }
+                wavefront_order();
+            });
+        } else {
+            const int token = min(row0 + row, p.m - 1);
+            static_for<0, AHEAD>([&](auto uc) {
+                constexpr int u = decltype(uc)::value;
+                const int step = min(first + WAVES * u, p.x_steps - 1);
                 b[u] = *reinterpret_cast<const v4i *>(p.x + token * p.x_pitch + (step * KSTEP + block * 16));
                 bs[u] = p.x_scales[token * p.scale_row + step * p.scale_step + block];
-            } else {
-                constexpr int SIZE = X == TSX_TYPE_F32 ? 4 : 2;
-                typedef Run<X, 8> Values;
-                const int k = step * MX_STEP + block * MX_BLOCK;
-                const char *const x = static_cast<const char *>(p.values) + token * p.x_stride * SIZE;
-                Values v[4];
-                unsigned top = 0;
-                if (p.cols >= 8) {           // uniform
-                    static_for<0, 4>([&](auto pc) { load_piece<X>(v[decltype(pc)::value], x, k + 8 * decltype(pc)::value, p.cols); });
-                    if ((step + 1) * MX_STEP > p.cols) static_for<0, 4>([&](auto pc) { settle_piece<X>(v[decltype(pc)::value], k + 8 * decltype(pc)::value, p.cols); });
-                } else {
-                    static_for<0, 4>([&](auto pc) { v[decltype(pc)::value].clear(); });
-                    if (k == 0) v[0].load_some(x, p.cols);
-                }
-                static_for<0, 4>([&](auto pc) { top = v[decltype(pc)::value].top(top); });
-                bs[u] = mx_scale(top_value<X>(top));
-                static_for<0, 4>([&](auto pc) { constexpr int q = decltype(pc)::value; b[u][q] = int(mx_codes<X>(v[q], bs[u])); });
-            }
-        });
+            });
+        }
         static_for<0, AHEAD>([&](auto uc) {
             constexpr int u = decltype(uc)::value;
             if (first + WAVES * u < p.x_steps)               // uniform
@@ -375,13 +426,13 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_mxfp4_few_kernel(FewTokens p)
         });
         if (first + WAVES * AHEAD < p.x_steps) fetch(first + WAVES * AHEAD);
     }
-    static_for<0, 4>([&](auto rc) { sums[wave][decltype(rc)::value][lane] = acc[decltype(rc)::value]; });
+    static_for<0, 4>([&](auto rc) { reinterpret_cast<float *>(mine)[decltype(rc)::value * 64 + lane] = acc[decltype(rc)::value]; });
     __syncthreads();
     const int in = threadIdx.x % 16, col = col16 * 16 + in, to = threadIdx.x / 16;
     if (to >= FEW || row0 + to >= p.m || col >= p.n) return;
     float v[1] = {0.f};
 #pragma unroll
-    for (int i = 0; i < WAVES; ++i) v[0] = __fadd_rn(v[0], sums[i][in % 4][to + 16 * (in / 4)]);
+    for (int i = 0; i < WAVES; ++i) v[0] = __fadd_rn(v[0], reinterpret_cast<const float *>(lds + i * OWN)[in % 4 * 64 + to + 16 * (in / 4)]);
     if (p.bias) v[0] = __fadd_rn(v[0], p.bias[col]);
     activate_tokens<OUT>(v, p.act, p.slope);
     Run<OUT, 1> out;
@@ -461,18 +512,19 @@ int launch_tile(MxGemmParams p, hipStream_t stream) {
     return 0;
 }
 
-template <int X, int WAVES, int AHEAD, int OUT>
+template <int X, int G, int WAVES, int AHEAD, int OUT>
 int launch_few(FewTokens p, hipStream_t stream) {
     p.tiles_per_xcd = int(ceil_div(p.n, 128));
-    hipLaunchKernelGGL((gemm_mxfp4_few_kernel<X, WAVES, AHEAD, OUT>), dim3(unsigned(8 * p.tiles_per_xcd), unsigned(ceil_div(p.m, FEW))), dim3(WAVES * 64), 0, stream, p);
+    hipLaunchKernelGGL((gemm_mxfp4_few_kernel<X, G, WAVES, AHEAD, OUT>), dim3(unsigned(8 * p.tiles_per_xcd), unsigned(ceil_div(p.m, FEW))), dim3(WAVES * 64), 0, stream, p);
     TSX_LAUNCH_CHECK("gemm_mxfp4_few_kernel");
     return 0;
 }
 template <int X, int OUT>
 int few_of(const FewTokens &p, hipStream_t stream) {
-    // 16 wavefronts where K is long: each has four K-steps up to K = 8192, all of them on their way at once (of rows of fp32 the registers hold two)
-    if (p.x_steps > 32) return launch_few<X, 16, X == TSX_TYPE_F32 ? 2 : 4, OUT>(p, stream);
-    return launch_few<X, 8, 4, OUT>(p, stream);
+    // 16 wavefronts where K is long and the registers allow it: each has four K-steps up to K = 8192, all of them on their way at once
+    if constexpr (X != TSX_TYPE_MXFP4)
+        if (p.m > 4) return launch_few<X, 4, 8, X == TSX_TYPE_F32 ? 2 : 4, OUT>(p, stream);
+    return p.x_steps > 32 ? launch_few<X, 1, 16, 4, OUT>(p, stream) : launch_few<X, 1, 8, 4, OUT>(p, stream);
 }
 template <int OUT>
 int few_tokens(const tsx_mxfp4_gemm *g, const MxGemmParams &q, hipStream_t stream) {
@@ -486,25 +538,34 @@ int few_tokens(const tsx_mxfp4_gemm *g, const MxGemmParams &q, hipStream_t strea
            : g->x_type == TSX_TYPE_BF16 ? few_of<TSX_TYPE_BF16, OUT>(p, stream) : few_of<TSX_TYPE_MXFP4, OUT>(p, stream);
 }
 
-// The kernel a call takes: up to 16 tokens the stream over the weights; else by an estimate of its time in us, fitted to products of 32 .. 8192 rows on 256 ..
-// 8192 columns and K of 256 .. 8192 (bf16 output).  r: tiles a CU, ks: K / 1024.  Tiles of 64 with K split over two groups of wavefronts take a CU
-// each, so they are for up to 256; those of 64 and 128 share CUs, so that their times go by r once they fill the card and by the length of K before; those
-// of 256 come in whole turns, which a card half full goes through faster.  Measured, in this order (us): 64 x 4096, K = 4096 6.7, 7.6, 12, 23; 256 x 4096,
-// K = 4096 7.2, 8.0, 12.3, 23.5; 512 x 4096, K = 4096 13.1, 10.4, 13.4, 23.7; 512 x 8192, K = 1024 14.1, 8.6, 7.3, 11.5; 2048 x 4096, K = 4096 50, 37.8, 30.5,
-// 29.4; 4096^3 97, 73, 56, 41; 4096 x 8192, K = 1024 103, 50, 32, 35; 1024 x 1024, K = 8192 11, 12.9, 20.9, 40.7; 8192^3 611, 522, 396, 278.
+// The kernel a call takes, by an estimate of its time in us, fitted to products of 16 .. 8192 rows on 256 .. 8192 columns and K of 256 .. 8192 (bf16).
+// r: workgroups or tiles a CU, ks: K / 1024.  MXFP4 rows: up to 16 the stream over the weights, else tiles.  Those of 64 with K split over two groups of
+// wavefronts take a CU each, so they are for up to 256; those of 64 and 128 share CUs, so that their times go by r once they fill the card and by the length
+// of K before; those of 256 come in whole turns, which a card half full goes through faster.  Measured, in this order (us): 64 x 4096, K = 4096 6.7, 7.6, 12,
+// 23; 256 x 4096, K = 4096 7.2, 8.0, 12.3, 23.5; 512 x 4096, K = 4096 13.1, 10.4, 13.4, 23.7; 512 x 8192, K = 1024 14.1, 8.6, 7.3, 11.5; 2048 x 4096, K = 4096
+// 50, 37.8, 30.5, 29.4; 4096^3 97, 73, 56, 41; 4096 x 8192, K = 1024 103, 50, 32, 35; 1024 x 1024, K = 8192 11, 12.9, 20.9, 40.7; 8192^3 611, 522, 396, 278.
+// Rows of floats: the stream, which quantizes them itself, against tiles behind a launch that does, 3 us and the rows' bytes.  The stream is a workgroup a CU
+// at a time (of up to four rows, several, and always it); the stream and what tiles took with their launch: 64 x 1024, K = 1024 4.6 and 7.4, 128 x 1024 7.6
+// and 7.5; 256 x 256, K = 256 4.0 and 7.2; 128 x 300, K = 4096 5.8 and 9.2; 16 x 8192, K = 8192 15.5 and 12.6.
 enum class Kernel { few, tile_64_by_k, tile_64, tile_128, tile_256 };
 
-Kernel choose(int m, int n, int k) {
-    if (m <= FEW) return Kernel::few;
+Kernel choose(const tsx_mxfp4_gemm *g) {
+    const int m = g->m, n = g->n, k = g->k;
+    const bool floats = g->x_type != TSX_TYPE_MXFP4;
+    if (m <= (floats ? 4 : FEW)) return Kernel::few;
     const float ks = float(k) / 1024.f;
-    const auto rounds = [&](int side) { return float(ceil_div(m, side) * ceil_div(n, side)) / 256.f; };
-    const float r64 = rounds(64), r128 = rounds(128), r256 = rounds(256);
+    const auto rounds = [&](int rows, int cols) { return float(ceil_div(m, rows) * ceil_div(n, cols)) / 256.f; };
+    const float r16 = rounds(FEW, 16), r64 = rounds(64, 64), r128 = rounds(128, 128), r256 = rounds(256, 256);
     const float cost[] = {r64 <= 1.f ? 3.6f + ks * (0.72f + 0.15f * r64) : INFINITY, std::max(3.5f + 1.1f * ks, 3.f + r64 * (0.5f + 0.97f * ks)),
                           std::max(4.f + 2.05f * ks, 3.f + 0.4f * ks + r128 * (0.75f + 2.97f * ks)),
                           3.f + std::ceil(r256) * (7.7f + 7.65f * ks) * (0.5f + 0.5f * std::min(r256, 1.f))};
     int best = 0;
     for (int i = 1; i < 4; ++i)
         if (cost[i] < cost[best]) best = i;
+    if (floats && m <= FEW_MOST) {
+        const float few = 1.2f + std::ceil(r16) * (2.4f + 0.55f * ks + (k % MX_STEP ? 1.2f : 0.f));
+        if (few < cost[best] + 3.f + float(m) * float(k) * 5e-7f) return Kernel::few;
+    }
     return Kernel(best + 1);
 }
 
@@ -547,7 +608,7 @@ struct Plan {
     bool copies;
     int64_t steps, code_bytes, word_bytes;      // word_bytes: of a K-step's scales
     explicit Plan(const tsx_mxfp4_gemm *g) {
-        kernel = choose(g->m, g->n, g->k);
+        kernel = choose(g);
         // TSX_MXFP4_KERNEL: that kernel, by its place in the list above, for any call it can take (tests, measurements)
         const char *e = std::getenv("TSX_MXFP4_KERNEL");
         if (e && e[0] >= (g->m <= FEW_MOST ? '0' : '1') && e[0] <= '4') kernel = Kernel(e[0] - '0');

@@ -57,7 +57,9 @@ def gemm(capi, **change):
 
 def test_product_refuses(capi):
     L = capi.lib()
-    assert L.tsx_gemm_mxfp4_workspace_bytes(ctypes.byref(gemm(capi, m=100))) == 100 * (128 + 8)
+    many = dict(m=1000, n=1000, out_stride=1000)
+    assert L.tsx_gemm_mxfp4_workspace_bytes(ctypes.byref(gemm(capi, **many))) == 1000 * (128 + 8)
+    assert L.tsx_gemm_mxfp4_workspace_bytes(ctypes.byref(gemm(capi, m=100))) == 0      # the product quantizes few rows itself
     codes = dict(x_type=4, x_stride=128, x_scales_dev=AT)
     assert L.tsx_gemm_mxfp4_workspace_bytes(ctypes.byref(gemm(capi, m=100, **codes))) == 0
     assert L.tsx_gemm_mxfp4_workspace_bytes(ctypes.byref(gemm(capi, m=100, **dict(codes, x_dev=AT + 1)))) == 100 * (128 + 8)
@@ -70,7 +72,7 @@ def test_product_refuses(capi):
                          (dict(out_dev=AT + 1), "multiple"), (dict(bias_dev=AT + 2), "multiple")):
         refused(capi, L.tsx_gemm_mxfp4, (ctypes.byref(gemm(capi, **change)), AT, 1 << 30, None), word)
     assert L.tsx_gemm_mxfp4(None, AT, 1 << 30, None) == -1
-    g = gemm(capi, m=100)
+    g = gemm(capi, **many)
     assert L.tsx_gemm_mxfp4(ctypes.byref(g), AT, 16, None) == -2 and "workspace" in said(capi)
     assert L.tsx_gemm_mxfp4(ctypes.byref(g), None, 1 << 30, None) == -2
     assert L.tsx_gemm_mxfp4(ctypes.byref(g), AT + 4, 1 << 30, None) == -1 and "aligned" in said(capi)
