@@ -39,7 +39,7 @@ struct MxGemmParams {
     float slope;
     int act;
     int row_tiles, col_tiles, tiles_per_xcd;
-    bool streams;                      // outputs are more than the L2s hold: past them
+    bool streams;                      // outputs go past the caches
 };
 
 __device__ __forceinline__ v8i operand(v4i v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
@@ -260,45 +260,46 @@ __global__ __launch_bounds__(WR *WC *KG * 64, WR * FR == 4 && KG == 1 ? 3 : 1) v
     // A wavefront's 32 tokens x 32 FC columns go through LDS, so that a store instruction writes whole cache lines (straight from the registers it would
     // write 16 bytes of each of 64 runs).
     constexpr int SIZE = OUT == TSX_TYPE_F32 ? 4 : 2, ROW = FC * 32 * SIZE, PITCH = ROW + 16, IN_ROW = ROW / 16, AT_ONCE = 64 / IN_ROW, EACH = 16 / SIZE;
-    constexpr int BEHIND = (KG - 1) * WR * WC * SUMS;
-    static_assert(BEHIND + WR * WC * 32 * PITCH <= S * BUFFER, "room for all wavefronts");
-    int8_t *const mine = lds + BEHIND + in_group * (32 * PITCH);
+    constexpr int BEHIND = (KG - 1) * WR * WC * SUMS, AREAS = FR > 1 && BEHIND + WR * WC * 64 * PITCH <= S * BUFFER ? 2 : 1;      // 32 tokens on their way out while the next are computed, where there is room
+    static_assert(BEHIND + WR * WC * AREAS * 32 * PITCH <= S * BUFFER, "room for all wavefronts");
+    int8_t *const mine = lds + BEHIND + in_group * (AREAS * 32 * PITCH);
     const int col = (frag0 + wave_c * FC) * 32 + lane % IN_ROW * EACH, left = p.n - col;      // where a lane stores
-    static_for<0, FR>([&](auto ic) {
-        constexpr int i = decltype(ic)::value;
-        const int in_tile = (wave_r * FR + i) * 32;
-        float v[FC][16];
-        static_for<0, FC>([&](auto fc) {
-            constexpr int f = decltype(fc)::value;
-            static_for<0, 4>([&](auto gc) {
-                constexpr int g = decltype(gc)::value;
-                const v4f bias = *reinterpret_cast<const v4f *>(of_cols + (wave_c * FC + f) * 32 + 8 * g + 4 * (lane / 32));
-                static_for<0, 4>([&](auto jc) { constexpr int j = decltype(jc)::value; v[f][4 * g + j] = __fadd_rn(sum_of(acc[i][f][4 * g + j]), bias[j]); });
+    const bool inside = row0 + ROWS <= p.m && frag0 * 32 + COLS <= p.n;      // no test of rows and columns then: 4096 x 4096, K = 256 11.3 -> 9.9 us
+    by_act(p.act, [&](auto act) __attribute__((always_inline)) {
+        static_for<0, FR>([&](auto ic) {
+            constexpr int i = decltype(ic)::value;
+            const int in_tile = (wave_r * FR + i) * 32;
+            int8_t *const area = mine + i % AREAS * (32 * PITCH);
+            static_for<0, FC>([&](auto fc) {
+                constexpr int f = decltype(fc)::value;
+                float v[16];
+                static_for<0, 4>([&](auto gc) {
+                    constexpr int g = decltype(gc)::value;
+                    const v4f bias = *reinterpret_cast<const v4f *>(of_cols + (wave_c * FC + f) * 32 + 8 * g + 4 * (lane / 32));
+                    static_for<0, 4>([&](auto jc) { constexpr int j = decltype(jc)::value; v[4 * g + j] = __fadd_rn(acc[i][f][4 * g + j], bias[j]); });
+                });
+                activate_as<OUT, decltype(act)::value>(v, p.slope);
+                const Run<OUT, 16> to = fragment_values<OUT>(v);
+                v4u *const at = reinterpret_cast<v4u *>(area + lane % 32 * PITCH + (f * 32 + 16 * (lane / 32)) * SIZE);
+                static_for<0, SIZE>([&](auto wc) { constexpr int w = 4 * decltype(wc)::value; at[w / 4] = v4u{to.word[w], to.word[w + 1], to.word[w + 2], to.word[w + 3]}; });
+            });
+            static_for<0, 32 / AT_ONCE>([&](auto kc) {
+                const int r = decltype(kc)::value * AT_ONCE + lane / IN_ROW, row = row0 + in_tile + r;
+                Run<OUT, EACH> to;
+                const v4u got = *reinterpret_cast<const v4u *>(area + r * PITCH + lane % IN_ROW * 16);
+                static_for<0, 4>([&](auto wc) { to.word[decltype(wc)::value] = got[decltype(wc)::value]; });
+                char *const out = static_cast<char *>(p.out) + (int64_t(row) * p.out_stride + col) * SIZE;
+                if (inside && p.streams) {                   // uniform
+                    asm volatile("; past the caches");       // keeps the two stores from becoming one
+                    to.template store<true>(out);
+                } else if (inside) {
+                    to.store(out);
+                } else if (row < p.m) {
+                    if (left >= EACH) to.store(out);
+                    else if (left > 0) to.store_some(out, left);
+                }
             });
         });
-        by_act(p.act, [&](auto act) __attribute__((always_inline)) {
-            static_for<0, FC>([&](auto fc) { activate_as<OUT, decltype(act)::value>(v[decltype(fc)::value], p.slope); });
-        });
-        static_for<0, FC>([&](auto fc) {
-            constexpr int f = decltype(fc)::value;
-            const Run<OUT, 16> to = fragment_values<OUT>(v[f]);
-            v4u *const at = reinterpret_cast<v4u *>(mine + lane % 32 * PITCH + (f * 32 + 16 * (lane / 32)) * SIZE);
-            static_for<0, SIZE>([&](auto wc) { constexpr int w = 4 * decltype(wc)::value; at[w / 4] = v4u{to.word[w], to.word[w + 1], to.word[w + 2], to.word[w + 3]}; });
-        });
-        static_for<0, 32 / AT_ONCE>([&](auto kc) {
-            const int r = decltype(kc)::value * AT_ONCE + lane / IN_ROW, row = row0 + in_tile + r;
-            Run<OUT, EACH> to;
-            const v4u got = *reinterpret_cast<const v4u *>(mine + r * PITCH + lane % IN_ROW * 16);
-            static_for<0, 4>([&](auto wc) { to.word[decltype(wc)::value] = got[decltype(wc)::value]; });
-            char *const out = static_cast<char *>(p.out) + (int64_t(row) * p.out_stride + col) * SIZE;
-            if (row < p.m) {
-                if (left >= EACH) {
-                    if (p.streams) to.template store<true>(out);      // uniform
-                    else to.store(out);
-                } else if (left > 0) to.store_some(out, left);
-            }
-        });
-        __builtin_amdgcn_sched_barrier(0);               // 32 tokens at a time: their values would fill the registers
     });
 }
 
@@ -500,7 +501,9 @@ int launch_tile(MxGemmParams p, hipStream_t stream) {
     const int64_t per_xcd = ceil_div(int64_t(p.row_tiles) * p.col_tiles, 8);
     TSX_REQUIRE(8 * per_xcd * WR * WC * KG * 64 < int64_t(1) << 32, "gemm_mxfp4: %d x %d outputs are more than a launch holds", p.m, p.n);
     p.tiles_per_xcd = int(per_xcd);
-    p.streams = int64_t(p.m) * p.n * int64_t(element_bytes(OUT)) > 32 << 20;
+    // Outputs of more than 64 MiB go past the caches: what reads them next finds little there, and the product ends sooner.  The product and a norm of its
+    // outputs, with and without (us): 33 MB 32.8 and 31.1, 67 MB 51.7 and 51.2, 134 MB 336 and 357.
+    p.streams = int64_t(p.m) * p.n * int64_t(element_bytes(OUT)) > 64 << 20;
     constexpr int LDS = S * 32 * (WR * FR + WC * FC) * KS * (KSTEP + 4);
     const auto kernel = gemm_mxfp4_kernel<WR, WC, FR, FC, KS, S, KG, OUT>;
     if (LDS > 64 * 1024) {
