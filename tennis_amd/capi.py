@@ -873,7 +873,9 @@ def quantize_mxfp4(x):
 def dequantize_mxfp4(codes, scales, k=None, dtype=torch.float32):
     """tsx_dequantize_mxfp4: the values [..., k] in dtype (fp32, fp16 or bf16) of codes and scales as quantize_mxfp4 gives them; k, by default two
     values for each byte, says where it is odd."""
-    out = _native().dequantize(codes, scales, 0 if k is None else k, _TYPES.get(dtype, 3))
+    if k is not None and k < 1:
+        raise TsxError("dequantize_mxfp4: rows of %s values" % k)
+    out = _native().dequantize(codes, scales, k or 0, _TYPES.get(dtype, 3))
     if out is not NotImplemented:
         return out
     kind = _float_dtype("dequantize_mxfp4", dtype)

@@ -294,6 +294,39 @@ def test_product_of_special_rows(torch, capi, monkeypatch, kernel):
         assert (got[5][~nan[5]] == 0).all()
 
 
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("m,n,k", [(3, 40, 200), (16, 300, 1500), (60, 64, 256), (300, 2000, 640)])
+def test_product_of_floats_beside_bad_rows(torch, capi, name, m, n, k):
+    """Infinities and NaN in rows that the call quantizes: those rows are not numbers, the others what they are alone."""
+    torch.manual_seed(m)
+    layer = capi.TokenGemmMxfp4.from_float(torch.randn((n, k), device="cuda"), torch.randn(n, device="cuda"))
+    x = torch.randn((m, k)).to(dtype(torch, name))
+    good = x.clone()
+    bad = sorted({0, m - 1, m // 2})
+    for row, (at, value) in zip(bad, ((0, math.inf), (k - 1, math.nan), (k // 2, -math.inf))):
+        x[row, at], good[row] = value, 0.0
+    got, want = layer(x.cuda()).cpu(), layer(good.cuda()).cpu()
+    for row in range(m):
+        assert torch.isnan(got[row]).all() if row in bad else torch.equal(got[row], want[row]), row
+
+
+@pytest.mark.parametrize("name", TYPES)
+def test_two_streams_at_once(torch, capi, name):
+    """One layer, calls in turn on two streams that nothing orders: each with a workspace of its own."""
+    layer = capi.TokenGemmMxfp4.from_float(torch.randn((3000, 520), device="cuda"))
+    inputs = [torch.randn((m, 520), device="cuda").to(dtype(torch, name)) for m in (700, 650)]
+    want = [layer(x) for x in inputs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(layer(inputs[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i in range(2) for y in got[i])
+
+
 def test_product_of_strided_rows(torch, capi):
     """Rows and scales at strides of their own, aligned and not, read in place and copied."""
     rng = np.random.default_rng(9)
@@ -377,3 +410,24 @@ def test_long_rows(torch, capi):
     assert torch.equal(codes[-2:], ec) and torch.equal(scales[-2:], es) and not codes[:-2].any()
     back = capi.dequantize_mxfp4(codes, scales, dtype=torch.bfloat16)
     assert torch.equal(back[-2:], capi.dequantize_mxfp4(ec, es, dtype=torch.bfloat16)) and not back[:-2].any()
+
+
+def test_python_calls_refuse(torch, capi):
+    """What the calls say about operands that do not fit each other."""
+    codes, scales = capi.quantize_mxfp4(torch.randn((6, 70), device="cuda"))
+    layer = capi.TokenGemmMxfp4(codes, scales, k=70)
+    x = torch.randn((4, 70), device="cuda")
+    xc, xs = capi.quantize_mxfp4(x)
+    for call, word in ((lambda: capi.dequantize_mxfp4(codes, scales, k=72), "shape"), (lambda: capi.dequantize_mxfp4(codes, scales[:, :2]), "shape"),
+                       (lambda: capi.dequantize_mxfp4(codes[:5], scales), "shape"), (lambda: capi.dequantize_mxfp4(codes, scales.float()), "float32"),
+                       (lambda: capi.TokenGemmMxfp4(codes, scales, k=64), "shape"), (lambda: capi.TokenGemmMxfp4(codes[0], scales[0]), "shape"),
+                       (lambda: capi.TokenGemmMxfp4(codes, scales, bias=torch.zeros(5, device="cuda")), "values"), (lambda: layer(x[:, :69]), "weights of 70"),
+                       (lambda: layer(xc), "come with their scales"), (lambda: layer(x, x_scales=xs), "come with their scales"), (lambda: layer(xc, x_scales=xs[:, :2]), "shape"),
+                       (lambda: layer(xc, x_scales=xs[:3]), "shape"), (lambda: layer(x, act="mish"), "activation"), (lambda: layer(x, out_dtype=torch.int8), "output type"),
+                       (lambda: layer(x.double()), "float64"), (lambda: capi.quantize_mxfp4(x.to(torch.int8)), "int8"), (lambda: capi.quantize_mxfp4(x[:, :0]), "shape"),
+                       (lambda: capi.rms_norm(x, torch.ones(69, device="cuda")), "values"), (lambda: capi.rms_norm(x, residual=x.half()), "float16"),
+                       (lambda: capi.rms_norm(x, residual=x[:3]), "residual of shape"), (lambda: capi.rms_norm(x, epsilon=-1.0), "epsilon"),
+                       (lambda: capi.rms_norm_tokens(x[:, :0]), "shape"), (lambda: capi.dequantize_tokens(x.to(torch.int8), x[:3, 0]), "values"),
+                       (lambda: capi.dequantize_tokens(x.to(torch.int8), None), "scales")):
+        with pytest.raises(capi.TsxError, match=word):
+            call()

@@ -123,5 +123,8 @@ def test_python_calls_refuse(capi):
                  lambda: capi.dequantize_tokens(x.to(torch.int8), x[:, 0])):
         with pytest.raises(capi.TsxError, match="device tensor"):
             call()
+    for k in (0, -1):
+        with pytest.raises(capi.TsxError, match="values"):
+            capi.dequantize_mxfp4(b, b[:, :2], k=k)
     with pytest.raises(capi.TsxError, match="output type"):
         capi.dequantize_mxfp4(b, b[:, :2], dtype=torch.int8)
