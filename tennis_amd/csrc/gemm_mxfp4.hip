@@ -379,15 +379,12 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_mxfp4_few_kernel(FewTokens p)
                     if (k == 0) v[i][u].load_some(x, p.cols);
                 }
             });
-            static_for<0, G * AHEAD>([&](auto ic) {
-                constexpr int i = decltype(ic)::value / AHEAD, u = decltype(ic)::value % AHEAD;
-                const int step = min(first + WAVES * u, p.x_steps - 1);
-                if ((step + 1) * MX_STEP > p.cols && p.cols >= 8) settle_piece<X>(v[i][u], step * MX_STEP + 8 * row, p.cols);      // uniform
-            });
             const auto larger = [](unsigned one, unsigned other) { return Values::template larger<X>(one, other); };
             static_for<0, AHEAD>([&](auto uc) {
                 constexpr int u = decltype(uc)::value;
-                if (u > 0 && first + WAVES * u >= p.x_steps) return;      // uniform
+                const int step = first + WAVES * u;
+                if (u > 0 && step >= p.x_steps) return;      // uniform
+                if ((step + 1) * MX_STEP > p.cols && p.cols >= 8) static_for<0, G>([&](auto ic) { settle_piece<X>(v[decltype(ic)::value][u], step * MX_STEP + 8 * row, p.cols); });
                 if constexpr (G == 1) {                      // four lanes a block, before its codes change lanes
                     const unsigned scale = mx_scale(top_value<X>(over_lanes(v[0][u].top(0), 2, larger)));
                     *reinterpret_cast<unsigned *>(mine + block * KSTEP + 4 * row) = mx_codes<X>(v[0][u], scale);
@@ -548,8 +545,8 @@ int few_tokens(const tsx_mxfp4_gemm *g, const MxGemmParams &q, hipStream_t strea
 // 23; 256 x 4096, K = 4096 7.2, 8.0, 12.3, 23.5; 512 x 4096, K = 4096 13.1, 10.4, 13.4, 23.7; 512 x 8192, K = 1024 14.1, 8.6, 7.3, 11.5; 2048 x 4096, K = 4096
 // 50, 37.8, 30.5, 29.4; 4096^3 97, 73, 56, 41; 4096 x 8192, K = 1024 103, 50, 32, 35; 1024 x 1024, K = 8192 11, 12.9, 20.9, 40.7; 8192^3 611, 522, 396, 278.
 // Rows of floats: the stream, which quantizes them itself, against tiles behind a launch that does, 3 us and the rows' bytes.  The stream is a workgroup a CU
-// at a time (of up to four rows, several, and always it); the stream and what tiles took with their launch: 64 x 1024, K = 1024 4.6 and 7.4, 128 x 1024 7.6
-// and 7.5; 256 x 256, K = 256 4.0 and 7.2; 128 x 300, K = 4096 5.8 and 9.2; 16 x 8192, K = 8192 15.5 and 12.6.
+// at a time (of up to four rows, several, and always it); the stream and what tiles took with their launch: 64 x 1024, K = 1024 4.3 and 7.4, 128 x 1024 7.0
+// and 7.5; 256 x 256, K = 256 4.0 and 7.2; 128 x 300, K = 4096 5.8 and 9.2; 32 x 4096, K = 300 6.5 and 7.7; 16 x 8192, K = 8192 15.7 and 12.4.
 enum class Kernel { few, tile_64_by_k, tile_64, tile_128, tile_256 };
 
 Kernel choose(const tsx_mxfp4_gemm *g) {
@@ -566,7 +563,7 @@ Kernel choose(const tsx_mxfp4_gemm *g) {
     for (int i = 1; i < 4; ++i)
         if (cost[i] < cost[best]) best = i;
     if (floats && m <= FEW_MOST) {
-        const float few = 1.2f + std::ceil(r16) * (2.4f + 0.55f * ks + (k % MX_STEP ? 1.2f : 0.f));
+        const float few = 1.2f + std::ceil(r16) * (2.4f + 0.55f * ks);
         if (few < cost[best] + 3.f + float(m) * float(k) * 5e-7f) return Kernel::few;
     }
     return Kernel(best + 1);

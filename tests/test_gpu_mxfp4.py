@@ -356,6 +356,21 @@ def test_product_of_strided_rows(torch, capi):
     assert torch.equal(other.packed, layer.packed)
 
 
+@pytest.mark.parametrize("m,n,k,name", [(8300, 4099, 96, "bf16"), (4096, 8192, 130, "f16"), (5000, 4096, 256, "f32"), (70000, 130, 64, "bf16")])
+def test_large_outputs(torch, capi, m, n, k, name):
+    """Many tiles, inside and across the edges, outputs of more than the caches hold: exact sums again."""
+    rng = np.random.default_rng(k)
+    wc, ws = random_rows(rng, n, k)
+    xc, xs = random_rows(rng, m, k)
+    layer = capi.TokenGemmMxfp4(*device(torch, wc, ws), k=k)
+    codes, scales = device(torch, xc, xs)
+    bias = torch.randint(-8, 8, (n,)).float().cuda()
+    layer.bias = bias
+    x, w = (torch.from_numpy(values64(*v)).cuda() for v in ((xc, xs), (wc, ws)))
+    want = ((x @ w.t().contiguous()) + bias.double()).clamp(min=0.0).float().to(dtype(torch, name))
+    assert torch.equal(layer(codes, x_scales=scales, act="relu", out_dtype=dtype(torch, name)), want)
+
+
 def test_product_leaves_its_inputs_and_repeats(torch, capi):
     """The same bits from call to call, inputs as they were."""
     x = torch.randn((100, 1000), device="cuda").bfloat16()
