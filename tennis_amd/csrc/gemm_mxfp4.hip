@@ -73,12 +73,6 @@ __device__ __forceinline__ void word_to_lds(const uint8_t *at, int8_t *lds) {
 template <int N>
 __device__ __forceinline__ void barrier_but_for() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
 
-// A sum, taken from the accumulators here and not before: all of them taken at once would not fit the other registers.
-__device__ __forceinline__ float sum_of(float v) {
-    asm volatile("" : "+v"(v));
-    return v;
-}
-
 // WR x WC wavefronts, each with FR x FC fragments of 32 tokens x 32 columns; S chunks of KS K-steps in LDS, scales behind their codes; KG such groups of
 // wavefronts, each with its part of every chunk's K-steps.
 //
@@ -92,12 +86,11 @@ __global__ __launch_bounds__(WR *WC *KG * 64, WR * FR == 4 && KG == 1 ? 3 : 1) v
     constexpr int A_BYTES = ROWS * CHUNK, B_BYTES = COLS * CHUNK, A_LOADS = A_BYTES / 1024 / WAVES, B_LOADS = B_BYTES / 1024 / WAVES;
     constexpr int A_WORDS = KS * ROWS / 64, WORDS = KS * (ROWS + COLS) / 64, S_LOADS = (WORDS + WAVES - 1) / WAVES;      // scales: by 64 words
     constexpr int SCALES = A_BYTES + B_BYTES, BUFFER = SCALES + KS * (ROWS + COLS) * 4, LOADS = A_LOADS + B_LOADS + S_LOADS;
-    static_assert(4 % KS == 0, "the weights hold whole chunks");
+    static_assert(4 % KS == 0 && S % 2 == 1, "the weights hold whole chunks; an even number of chunks in front of the last S of an odd number");
     static_assert(A_LOADS * 1024 * WAVES == A_BYTES && B_LOADS * 1024 * WAVES == B_BYTES && S >= 3 && (S - 1) * LOADS < 64,
                   "whole loads, counted in six bits");
     extern __shared__ __attribute__((aligned(16))) int8_t lds[];      // [S][BUFFER]
     __shared__ __attribute__((aligned(16))) float of_cols[COLS];      // biases, requested ahead of everything
-    constexpr int THREADS = WAVES * 64;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int in_group = wave % (WR * WC), k_group = wave / (WR * WC), wave_r = in_group / WC, wave_c = in_group % WC;
     // blockIdx % 8 is the XCD: each takes a run of consecutive tiles, which walk four row tiles before the next column tile
@@ -108,10 +101,12 @@ __global__ __launch_bounds__(WR *WC *KG * 64, WR * FR == 4 && KG == 1 ? 3 : 1) v
     const int group_rows = min(4, p.row_tiles - 4 * group);
     const int tile_c = in_four / group_rows, tile_r = 4 * group + in_four - tile_c * group_rows;
     const int row0 = tile_r * ROWS, frag0 = tile_c * (COLS / 32);
-    constexpr int COL_TURNS = (COLS + THREADS - 1) / THREADS;
-    float col_bias[COL_TURNS];
-    static_for<0, COL_TURNS>([&](auto ic) { col_bias[decltype(ic)::value] = -0.f; });      // changes no sum
-    if (p.bias) static_for<0, COL_TURNS>([&](auto ic) { col_bias[decltype(ic)::value] = p.bias[min(frag0 * 32 + int(threadIdx.x) + decltype(ic)::value * THREADS, p.n - 1)]; });
+    static_assert(COLS / 64 <= WAVES, "biases in one request a wavefront");
+    if (wave < COLS / 64) {                                  // uniform, as the next
+        const int first = wave * 64;
+        if (p.bias) word_to_lds(reinterpret_cast<const uint8_t *>(p.bias + min(frag0 * 32 + first + lane, p.n - 1)), reinterpret_cast<int8_t *>(of_cols + first));
+        else of_cols[first + lane] = -0.f;                   // changes no sum
+    }
 
     // A row in LDS is its CHUNK bytes, its pieces of 16 XORed with bits of the row that make 16 rows cover all banks for one piece.  A
     // load instruction fills 1 KiB of such rows; rows beyond m are the last one again, never stored.  Pieces behind the end of a row are
@@ -172,70 +167,132 @@ __global__ __launch_bounds__(WR *WC *KG * 64, WR * FR == 4 && KG == 1 ? 3 : 1) v
         constexpr int f = decltype(fc)::value;
         static_for<0, 16>([&](auto rc) { acc[f / FC][f % FC][decltype(rc)::value] = 0.f; });
     });
-    const int a_row = (wave_r * FR * 32 + lane % 32) * CHUNK, a_key = key_of(lane % 32);
-    v4i a[2][FR], b[2][FC];
-    int a_scale[2][FR], b_scale[2][FC];      // of a K-step: blocks l / 32 and 2 + l / 32 in bytes 0 and 2
-    // read i of a half's operands; the scales of a K-step come with its first half
-    constexpr int READS = 2 * (FR + FC);
-    auto read = [&](auto hc, auto ic, int buf) __attribute__((always_inline)) {
-        constexpr int h = decltype(hc)::value, i = decltype(ic)::value, set = h % 2;
-        const int step = k_group * (KS / KG) + h / 2;      // a K group's K-steps of a chunk lie together
-        const int8_t *const at = lds + buf * BUFFER;
-        if constexpr (i < FC) {
-            b[set][i] = *reinterpret_cast<const v4i *>(at + A_BYTES + ((step * (COLS / 32) + wave_c * FC + i) * 2 + h % 2) * 1024 + lane * 16);
-        } else if constexpr (i < FC + FR) {
-            constexpr int f = i - FC;
-            a[set][f] = *reinterpret_cast<const v4i *>(at + a_row + f * 32 * CHUNK + ((4 * step + 2 * (h % 2) + lane / 32) ^ a_key) * 16);
-        } else if constexpr (h % 2 == 0 && i < 2 * FC + FR) {
-            constexpr int f = i - FC - FR;
-            b_scale[h / 2 % 2][f] = *reinterpret_cast<const int *>(at + SCALES + (KS * ROWS + step * COLS + (wave_c * FC + f) * 32 + lane % 32) * 4);
-        } else if constexpr (h % 2 == 0 && i < READS) {
-            constexpr int f = i - 2 * FC - FR;
-            a_scale[h / 2 % 2][f] = *reinterpret_cast<const int *>(at + SCALES + (step * ROWS + (wave_r * FR + f) * 32 + lane % 32) * 4);
-        }
-    };
-    static_for<0, S - 1>([&](auto sc) { static_for<0, LOADS>([&](auto ic) { request(ic, decltype(sc)::value, decltype(sc)::value); }); });
-    wait_for_all_but<(S - 2) * LOADS>();
-    static_for<0, COL_TURNS>([&](auto ic) {
-        const int at = threadIdx.x + decltype(ic)::value * THREADS;
-        if (COLS % THREADS == 0 || at < COLS) of_cols[at] = col_bias[decltype(ic)::value];
-    });
-    lds_barrier();
-    static_for<0, READS>([&](auto ic) { read(std::integral_constant<int, 0>{}, ic, 0); });
-    const int upper = 8 * (lane / 32);
+    const int a_row = (wave_r * FR * 32 + lane % 32) * CHUNK, a_key = key_of(lane % 32), upper = 8 * (lane / 32);
     int buf = 0, c = 0;
-    // A chunk.  Between its multiplications, one after each: the reads of the next half's operands, and the requests of the chunk S - 1 further on,
-    // into the buffer that the barrier of the chunk before freed.  Spread so, none of them keeps the matrix cores waiting for its turn to be issued.
-    auto multiply = [&](auto fetching) __attribute__((always_inline)) {
-        constexpr bool FETCHES = decltype(fetching)::value;
-        const int after = buf + 1 == S ? 0 : buf + 1, before = buf == 0 ? S - 1 : buf - 1;
-        static_for<0, HALVES>([&](auto hc) {
-            constexpr int h = decltype(hc)::value, SLOTS = FR * FC, FIRST = LOADS * h / HALVES, COUNT = LOADS * (h + 1) / HALVES - FIRST;
-            int as[FR], bs[FC];
-            static_for<0, FR>([&](auto ic) { as[decltype(ic)::value] = int(unsigned(a_scale[h / 2 % 2][decltype(ic)::value]) >> upper); });
-            static_for<0, FC>([&](auto fc) { bs[decltype(fc)::value] = int(unsigned(b_scale[h / 2 % 2][decltype(fc)::value]) >> upper); });
-            if constexpr (h + 1 == HALVES) {
-                // Every wavefront has its operands of this chunk in registers: its buffer is free behind the barrier, and the next
-                // chunk is there for all.  The rest of this chunk's arithmetic covers the first reads behind it.
-                barrier_but_for<FETCHES ? (S - 3) * LOADS + FIRST : 0>();
+    // Few fragments: a chunk's operands are read all at once, a chunk ahead of its multiplications, so that these wait for nothing else in between (1024 x
+    // 4096, K = 8192 in tiles of 128 31 -> 25 us).  Many: half a K-step ahead, which the registers hold without moving sums (8192^3 255 us, a chunk ahead 278).
+    if constexpr (FR * FC <= 4) {
+        constexpr int STEPS = KS / KG;                           // K-steps of a chunk that are this wavefront's; they lie together
+        v4i a[2][HALVES][FR], b[2][HALVES][FC];
+        int a_scale[2][STEPS][FR], b_scale[2][STEPS][FC];        // of a K-step: blocks l / 32 and 2 + l / 32 in bytes 0 and 2, once shifted
+        constexpr int PER_HALF = FR + FC, READS = HALVES * PER_HALF + STEPS * PER_HALF;
+        auto read = [&](auto sc, auto ic, int buf) __attribute__((always_inline)) {
+            constexpr int set = decltype(sc)::value, n = decltype(ic)::value;
+            const int8_t *const at = lds + buf * BUFFER;
+            if constexpr (n < HALVES * PER_HALF) {
+                constexpr int h = n / PER_HALF, i = n % PER_HALF;
+                const int step = k_group * STEPS + h / 2;
+                if constexpr (i < FC) b[set][h][i] = *reinterpret_cast<const v4i *>(at + A_BYTES + ((step * (COLS / 32) + wave_c * FC + i) * 2 + h % 2) * 1024 + lane * 16);
+                else a[set][h][i - FC] = *reinterpret_cast<const v4i *>(at + a_row + (i - FC) * 32 * CHUNK + ((4 * step + 2 * (h % 2) + lane / 32) ^ a_key) * 16);
+            } else {
+                constexpr int u = (n - HALVES * PER_HALF) / PER_HALF, i = n % PER_HALF;
+                const int step = k_group * STEPS + u;
+                if constexpr (i < FC) b_scale[set][u][i] = *reinterpret_cast<const int *>(at + SCALES + (KS * ROWS + step * COLS + (wave_c * FC + i) * 32 + lane % 32) * 4);
+                else a_scale[set][u][i - FC] = *reinterpret_cast<const int *>(at + SCALES + (step * ROWS + (wave_r * FR + i - FC) * 32 + lane % 32) * 4);
             }
+        };
+        static_for<0, S>([&](auto sc) { static_for<0, LOADS>([&](auto ic) { request(ic, decltype(sc)::value, decltype(sc)::value); }); });
+        barrier_but_for<(S - 1) * LOADS>();
+        // Which registers a chunk has goes by how many are left, so that the last ones are known to the code.
+        if (chunks % 2) static_for<0, READS>([&](auto ic) { read(std::integral_constant<int, 0>{}, ic, 0); });
+        else static_for<0, READS>([&](auto ic) { read(std::integral_constant<int, 1>{}, ic, 0); });
+        // Between the multiplications of a chunk, one after each: the reads of the next chunk's operands, and the requests of the chunk S further on, into the
+        // buffer that this chunk's operands came from.  Spread so, none of them keeps the matrix cores waiting for its turn to be issued.
+        auto multiply = [&](auto sc, auto left) __attribute__((always_inline)) {
+            constexpr int set = decltype(sc)::value, LEFT = decltype(left)::value, SLOTS = HALVES * FR * FC;      // LEFT: chunks from this one on; above S, more than S
+            constexpr bool FETCHES = LEFT > S;
+            const int after = buf + 1 == S ? 0 : buf + 1;
+            // The next chunk is there for all behind the barrier, and every wavefront has this chunk's operands.
+            if constexpr (LEFT > 1) barrier_but_for<(LEFT > S ? S - 2 : LEFT - 2) * LOADS>();
+            int as[STEPS][FR], bs[STEPS][FC];
+            static_for<0, STEPS>([&](auto uc) {
+                constexpr int u = decltype(uc)::value;
+                static_for<0, FR>([&](auto ic) { as[u][decltype(ic)::value] = int(unsigned(a_scale[set][u][decltype(ic)::value]) >> upper); });
+                static_for<0, FC>([&](auto fc) { bs[u][decltype(fc)::value] = int(unsigned(b_scale[set][u][decltype(fc)::value]) >> upper); });
+            });
             static_for<0, SLOTS>([&](auto fc) {
-                constexpr int f = decltype(fc)::value, i = f / FC, j = f % FC;
-                constexpr int R0 = READS * f / SLOTS, R1 = READS * (f + 1) / SLOTS, L0 = COUNT * f / SLOTS, L1 = COUNT * (f + 1) / SLOTS;
-                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(b[h % 2][j]), operand(a[h % 2][i]), acc[i][j], FP4, FP4, 2 * (h % 2), bs[j],
-                                                                            2 * (h % 2), as[i]);
-                static_for<R0, R1>([&](auto rc) {
-                    if constexpr (h + 1 == HALVES) read(std::integral_constant<int, 0>{}, rc, after);
-                    else read(std::integral_constant<int, h + 1>{}, rc, buf);
-                });
-                if constexpr (FETCHES) static_for<FIRST + L0, FIRST + L1>([&](auto lc) { request(lc, c + S - 1, before); });
+                constexpr int f = decltype(fc)::value, h = f / (FR * FC), i = f / FC % FR, j = f % FC;
+                constexpr int R0 = READS * f / SLOTS, R1 = READS * (f + 1) / SLOTS, L0 = LOADS * f / SLOTS, L1 = LOADS * (f + 1) / SLOTS;
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(b[set][h][j]), operand(a[set][h][i]), acc[i][j], FP4, FP4, 2 * (h % 2), bs[h / 2][j],
+                                                                            2 * (h % 2), as[h / 2][i]);
+                if constexpr (LEFT > 1) static_for<R0, R1>([&](auto rc) { read(std::integral_constant<int, 1 - set>{}, rc, after); });
+                if constexpr (FETCHES) static_for<L0, L1>([&](auto lc) { request(lc, c + S, buf); });
                 __builtin_amdgcn_sched_barrier(0);
             });
+            buf = after;
+            ++c;
+        };
+        const std::integral_constant<int, 0> first;
+        const std::integral_constant<int, 1> second;
+        const std::integral_constant<int, S + 1> more;
+        if (chunks > S && chunks % 2 == 0) multiply(second, more);
+        while (chunks - c > S + 1) {
+            multiply(first, more);
+            multiply(second, more);
+        }
+        static_for<0, S>([&](auto rc) {                          // the last S chunks are all on their way
+            constexpr int LEFT = S - decltype(rc)::value;
+            if (chunks - c >= LEFT) multiply(std::integral_constant<int, (LEFT - 1) % 2>{}, std::integral_constant<int, LEFT>{});
         });
-        buf = after;
-    };
-    for (; c + S - 1 < chunks; ++c) multiply(std::true_type{});
-    for (; c < chunks; ++c) multiply(std::false_type{});      // the last S - 1 chunks are all on their way
+    } else {
+        v4i a[2][FR], b[2][FC];
+        int a_scale[2][FR], b_scale[2][FC];      // of a K-step: blocks l / 32 and 2 + l / 32 in bytes 0 and 2
+        // read i of a half's operands; the scales of a K-step come with its first half
+        constexpr int READS = 2 * (FR + FC);
+        auto read = [&](auto hc, auto ic, int buf) __attribute__((always_inline)) {
+            constexpr int h = decltype(hc)::value, i = decltype(ic)::value, set = h % 2;
+            const int step = k_group * (KS / KG) + h / 2;      // a K group's K-steps of a chunk lie together
+            const int8_t *const at = lds + buf * BUFFER;
+            if constexpr (i < FC) {
+                b[set][i] = *reinterpret_cast<const v4i *>(at + A_BYTES + ((step * (COLS / 32) + wave_c * FC + i) * 2 + h % 2) * 1024 + lane * 16);
+            } else if constexpr (i < FC + FR) {
+                constexpr int f = i - FC;
+                a[set][f] = *reinterpret_cast<const v4i *>(at + a_row + f * 32 * CHUNK + ((4 * step + 2 * (h % 2) + lane / 32) ^ a_key) * 16);
+            } else if constexpr (h % 2 == 0 && i < 2 * FC + FR) {
+                constexpr int f = i - FC - FR;
+                b_scale[h / 2 % 2][f] = *reinterpret_cast<const int *>(at + SCALES + (KS * ROWS + step * COLS + (wave_c * FC + f) * 32 + lane % 32) * 4);
+            } else if constexpr (h % 2 == 0 && i < READS) {
+                constexpr int f = i - 2 * FC - FR;
+                a_scale[h / 2 % 2][f] = *reinterpret_cast<const int *>(at + SCALES + (step * ROWS + (wave_r * FR + f) * 32 + lane % 32) * 4);
+            }
+        };
+        static_for<0, S - 1>([&](auto sc) { static_for<0, LOADS>([&](auto ic) { request(ic, decltype(sc)::value, decltype(sc)::value); }); });
+        wait_for_all_but<(S - 2) * LOADS>();
+        lds_barrier();
+        static_for<0, READS>([&](auto ic) { read(std::integral_constant<int, 0>{}, ic, 0); });
+        // A chunk.  Between its multiplications, one after each: the reads of the next half's operands, and the requests of the chunk S - 1 further on,
+        // into the buffer that the barrier of the chunk before freed.  Spread so, none of them keeps the matrix cores waiting for its turn to be issued.
+        auto multiply = [&](auto fetching) __attribute__((always_inline)) {
+            constexpr bool FETCHES = decltype(fetching)::value;
+            const int after = buf + 1 == S ? 0 : buf + 1, before = buf == 0 ? S - 1 : buf - 1;
+            static_for<0, HALVES>([&](auto hc) {
+                constexpr int h = decltype(hc)::value, SLOTS = FR * FC, FIRST = LOADS * h / HALVES, COUNT = LOADS * (h + 1) / HALVES - FIRST;
+                int as[FR], bs[FC];
+                static_for<0, FR>([&](auto ic) { as[decltype(ic)::value] = int(unsigned(a_scale[h / 2 % 2][decltype(ic)::value]) >> upper); });
+                static_for<0, FC>([&](auto fc) { bs[decltype(fc)::value] = int(unsigned(b_scale[h / 2 % 2][decltype(fc)::value]) >> upper); });
+                if constexpr (h + 1 == HALVES) {
+                    // Every wavefront has its operands of this chunk in registers: its buffer is free behind the barrier, and the next
+                    // chunk is there for all.  The rest of this chunk's arithmetic covers the first reads behind it.
+                    barrier_but_for<FETCHES ? (S - 3) * LOADS + FIRST : 0>();
+                }
+                static_for<0, SLOTS>([&](auto fc) {
+                    constexpr int f = decltype(fc)::value, i = f / FC, j = f % FC;
+                    constexpr int R0 = READS * f / SLOTS, R1 = READS * (f + 1) / SLOTS, L0 = COUNT * f / SLOTS, L1 = COUNT * (f + 1) / SLOTS;
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(b[h % 2][j]), operand(a[h % 2][i]), acc[i][j], FP4, FP4, 2 * (h % 2), bs[j],
+                                                                                2 * (h % 2), as[i]);
+                    static_for<R0, R1>([&](auto rc) {
+                        if constexpr (h + 1 == HALVES) read(std::integral_constant<int, 0>{}, rc, after);
+                        else read(std::integral_constant<int, h + 1>{}, rc, buf);
+                    });
+                    if constexpr (FETCHES) static_for<FIRST + L0, FIRST + L1>([&](auto lc) { request(lc, c + S - 1, before); });
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+            });
+            buf = after;
+        };
+        for (; c + S - 1 < chunks; ++c) multiply(std::true_type{});
+        for (; c < chunks; ++c) multiply(std::false_type{});      // the last S - 1 chunks are all on their way
+    }
     // The chunks' LDS is free: nothing is on its way into it, and behind this barrier nobody reads it.
     wait_for_all_but<0>();
     lds_barrier();
@@ -491,6 +548,20 @@ __global__ __launch_bounds__(256) void copy_mxfp4_kernel(const uint8_t *codes, i
     }
 }
 
+// Rows of scales, whole words at multiples of 4, to words of K-steps: a lane has four words of a row
+__global__ __launch_bounds__(256) void turn_scales_kernel(const uint8_t *scales, int64_t stride, int64_t rows, int steps, unsigned *to) {
+    const int64_t row = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    const int first = int(blockIdx.y) * 4;
+    if (row >= rows) return;
+    const unsigned *const from = reinterpret_cast<const unsigned *>(scales + row * stride) + first;
+    unsigned word[4];
+    static_for<0, 4>([&](auto uc) { constexpr int u = decltype(uc)::value; word[u] = from[min(u, steps - 1 - first)]; });
+    static_for<0, 4>([&](auto uc) {
+        constexpr int u = decltype(uc)::value;
+        if (first + u < steps) to[int64_t(first + u) * rows + row] = word[u];
+    });
+}
+
 template <int WR, int WC, int FR, int FC, int KS, int S, int KG, int OUT>
 int launch_tile(MxGemmParams p, hipStream_t stream) {
     p.row_tiles = int(ceil_div(p.m, 32 * WR * FR));
@@ -541,9 +612,9 @@ int few_tokens(const tsx_mxfp4_gemm *g, const MxGemmParams &q, hipStream_t strea
 // The kernel a call takes, by an estimate of its time in us, fitted to products of 16 .. 8192 rows on 256 .. 8192 columns and K of 256 .. 8192 (bf16).
 // r: workgroups or tiles a CU, ks: K / 1024.  MXFP4 rows: up to 16 the stream over the weights, else tiles.  Those of 64 with K split over two groups of
 // wavefronts take a CU each, so they are for up to 256; those of 64 and 128 share CUs, so that their times go by r once they fill the card and by the length
-// of K before; those of 256 come in whole turns, which a card half full goes through faster.  Measured, in this order (us): 64 x 4096, K = 4096 6.7, 7.6, 12,
-// 23; 256 x 4096, K = 4096 7.2, 8.0, 12.3, 23.5; 512 x 4096, K = 4096 13.1, 10.4, 13.4, 23.7; 512 x 8192, K = 1024 14.1, 8.6, 7.3, 11.5; 2048 x 4096, K = 4096
-// 50, 37.8, 30.5, 29.4; 4096^3 97, 73, 56, 41; 4096 x 8192, K = 1024 103, 50, 32, 35; 1024 x 1024, K = 8192 11, 12.9, 20.9, 40.7; 8192^3 611, 522, 396, 278.
+// of K before; those of 256 come in whole turns, which a card half full goes through faster.  Measured, in this order (us): 64 x 4096, K = 4096 6.4, 6.8, 11.1,
+// 23.5; 256 x 4096, K = 4096 7.0, 7.1, 11.1, 23.5; 512 x 4096, K = 4096 12.7, 10.4, 12.8, 23.6; 512 x 8192, K = 1024 14, 7.9, 6.7, 11.2; 2048 x 4096, K =
+// 4096 46, 36, 30, 31; 4096^3 91, 70, 48, 42; 4096 x 8192, K = 1024 101, 46, 33, 38; 1024 x 1024, K = 8192 10, 11, 21, 42; 8192^3 588, 530, 326, 267.
 // Rows of floats: the stream, which quantizes them itself, against tiles behind a launch that does, 3 us and the rows' bytes.  The stream is a workgroup a CU
 // at a time (of up to four rows, several, and always it); the stream and what tiles took with their launch: 64 x 1024, K = 1024 4.3 and 7.4, 128 x 1024 7.0
 // and 7.5; 256 x 256, K = 256 4.0 and 7.2; 128 x 300, K = 4096 5.8 and 9.2; 32 x 4096, K = 300 6.5 and 7.7; 16 x 8192, K = 8192 15.7 and 12.4.
@@ -556,8 +627,8 @@ Kernel choose(const tsx_mxfp4_gemm *g) {
     const float ks = float(k) / 1024.f;
     const auto rounds = [&](int rows, int cols) { return float(ceil_div(m, rows) * ceil_div(n, cols)) / 256.f; };
     const float r16 = rounds(FEW, 16), r64 = rounds(64, 64), r128 = rounds(128, 128), r256 = rounds(256, 256);
-    const float cost[] = {r64 <= 1.f ? 3.6f + ks * (0.72f + 0.15f * r64) : INFINITY, std::max(3.5f + 1.1f * ks, 3.f + r64 * (0.5f + 0.97f * ks)),
-                          std::max(4.f + 2.05f * ks, 3.f + 0.4f * ks + r128 * (0.75f + 2.97f * ks)),
+    const float cost[] = {r64 <= 1.f ? 3.6f + ks * (0.72f + 0.15f * r64) : INFINITY, std::max(3.4f + 0.88f * ks, 2.8f + r64 * (0.42f + 0.97f * ks)),
+                          std::max(3.7f + 1.82f * ks, 3.f + 0.4f * ks + r128 * (0.75f + 2.6f * ks)),
                           3.f + std::ceil(r256) * (7.7f + 7.65f * ks) * (0.5f + 0.5f * std::min(r256, 1.f))};
     int best = 0;
     for (int i = 1; i < 4; ++i)
@@ -602,22 +673,27 @@ bool reads_in_place(const tsx_mxfp4_gemm *g) {
            (g->m <= 1 || (g->x_stride % 16 == 0 && g->x_stride <= 1 << 23 && g->x_scales_stride % 4 == 0 && g->x_scales_stride <= 1 << 23));
 }
 
-// What a call does: its kernel, and whether the workspace holds its rows, codes [m][steps][64] and scales [steps][m][4].
+// What a call does: its kernel, and whether the workspace holds its rows, codes [m][steps][64] and scales [steps][m][4], or such scales alone.
 struct Plan {
     Kernel kernel;
-    bool copies;
+    bool copies, turns;
     int64_t steps, code_bytes, word_bytes;      // word_bytes: of a K-step's scales
     explicit Plan(const tsx_mxfp4_gemm *g) {
         kernel = choose(g);
         // TSX_MXFP4_KERNEL: that kernel, by its place in the list above, for any call it can take (tests, measurements)
         const char *e = std::getenv("TSX_MXFP4_KERNEL");
         if (e && e[0] >= (g->m <= FEW_MOST ? '0' : '1') && e[0] <= '4') kernel = Kernel(e[0] - '0');
-        copies = g->m > 0 && !reads_in_place(g) && (kernel != Kernel::few || g->x_type == TSX_TYPE_MXFP4);
         steps = ceil_div(g->k, MX_STEP);
-        code_bytes = g->m * steps * KSTEP;
+        copies = g->m > 0 && !reads_in_place(g) && (kernel != Kernel::few || g->x_type == TSX_TYPE_MXFP4);
+        // Rows of scales cost a tile a request of 64 cache lines where words of K-steps are four: 0.09 us a K-step in tiles of 128, 0.15 in those of 256.
+        // A launch that turns them is worth 4 us of that (8192^3 291 us without, 2048 x 4096, K = 4096 30).
+        const int side = kernel == Kernel::tile_256 ? 256 : 128;
+        const float tiles = std::max(1.f, float(ceil_div(g->m, side) * ceil_div(g->n, side)) / 256.f);
+        turns = g->m > 0 && !copies && kernel >= Kernel::tile_128 && float(steps) * tiles * (side == 256 ? 0.15f : 0.09f) > 4.f;
+        code_bytes = copies ? g->m * steps * KSTEP : 0;
         word_bytes = int64_t(g->m) * 4;
     }
-    size_t workspace_bytes() const { return copies ? size_t(code_bytes + word_bytes * steps) : 0; }
+    size_t workspace_bytes() const { return copies || turns ? size_t(code_bytes + word_bytes * steps) : 0; }
 };
 
 int check_weights(int32_t k, int32_t n) {
@@ -699,6 +775,14 @@ int tsx_gemm_mxfp4(const tsx_mxfp4_gemm *g, void *workspace_dev, size_t workspac
         p.x_pitch = g->m <= 1 ? 0 : g->x_stride;
         p.scale_row = g->m <= 1 ? 0 : g->x_scales_stride;
         p.scale_step = 4;
+        if (plan.turns) {
+            hipLaunchKernelGGL(tsx::turn_scales_kernel, dim3(unsigned(tsx::ceil_div(g->m, 256)), unsigned(tsx::ceil_div(steps, 4))), dim3(256), 0, stream,
+                               g->x_scales_dev, p.scale_row, int64_t(g->m), steps, static_cast<unsigned *>(workspace_dev));
+            TSX_LAUNCH_CHECK("turn_scales_kernel");
+            p.x_scales = static_cast<const uint8_t *>(workspace_dev);
+            p.scale_row = 4;
+            p.scale_step = plan.word_bytes;
+        }
     }
     p.w = static_cast<const int8_t *>(g->packed_w_dev);
     p.w_scales = p.w + tsx::packed_codes(g->k, g->n);

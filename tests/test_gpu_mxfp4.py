@@ -356,6 +356,26 @@ def test_product_of_strided_rows(torch, capi):
     assert torch.equal(other.packed, layer.packed)
 
 
+@pytest.mark.parametrize("kernel,m,n,k", [("3", 1, 40, 5888), ("3", 130, 140, 6016), ("3", 300, 129, 6144), ("4", 3, 300, 4096), ("4", 257, 130, 3584), ("4", 300, 513, 4480),
+                                          (None, 2048, 4096, 4352)])
+def test_product_of_long_rows_with_scales_apart(torch, capi, monkeypatch, kernel, m, n, k):
+    """Scales of long rows, which are turned first: exact sums, from rows at strides of their own too, of which nothing behind the scales is used."""
+    if kernel:
+        monkeypatch.setenv("TSX_MXFP4_KERNEL", kernel)
+    rng = np.random.default_rng(m + k)
+    xc, xs = random_rows(rng, m, k, scales=(126, 128))
+    wc, ws = random_rows(rng, n, k, scales=(126, 128))      # values of at most 6, in steps of 1/4
+    assert k * 36 * 16 < 2 ** 24
+    layer = capi.TokenGemmMxfp4(*device(torch, wc, ws))
+    codes, scales = device(torch, xc, xs)
+    x, w = (torch.from_numpy(values64(*v)).cuda() for v in ((xc, xs), (wc, ws)))
+    want = (x @ w.t().contiguous()).float()
+    assert torch.equal(layer(codes, x_scales=scales), want)
+    room = torch.full((m + 1, k // 32 + 12), 255, dtype=torch.uint8, device="cuda")
+    room[:m, 4:4 + k // 32] = scales
+    assert torch.equal(layer(codes, x_scales=room[:m, 4:4 + k // 32]), want)
+
+
 @pytest.mark.parametrize("m,n,k,name", [(8300, 4099, 96, "bf16"), (4096, 8192, 130, "f16"), (5000, 4096, 256, "f32"), (70000, 130, 64, "bf16")])
 def test_large_outputs(torch, capi, m, n, k, name):
     """Many tiles, inside and across the edges, outputs of more than the caches hold: exact sums again."""
