@@ -154,10 +154,14 @@ __global__ __launch_bounds__(T <= 64 ? 256 : T) void rms_norm_kernel(RmsNormPara
             static_for<0, P>([&](auto ic) {
                 constexpr int i = decltype(ic)::value;
                 const int piece = turn * T * P + t + i * T;
-                float y[PIECE];
-                static_for<0, PIECE>([&](auto ec) { constexpr int e = decltype(ec)::value; y[e] = __fmul_rn(__fmul_rn(h[i].template get<e>(), lift), w[i].template get<e>()); });
+                float y[PIECE];                   // of int8 tokens: y / r
+                static_for<0, PIECE>([&](auto ec) {
+                    constexpr int e = decltype(ec)::value;
+                    y[e] = __fmul_rn(h[i].template get<e>(), lift);
+                    if constexpr (TO != NORM_TOKENS) y[e] = __fmul_rn(y[e], r);      // ahead of the weight: h w may leave fp32 where y does not
+                    y[e] = __fmul_rn(y[e], w[i].template get<e>());
+                });
                 if constexpr (TO == NORM_ROWS) {
-                    static_for<0, PIECE>([&](auto ec) { constexpr int e = decltype(ec)::value; y[e] = __fmul_rn(y[e], r); });
                     Values v;
                     v.set(y);
                     store(v, out, piece);
@@ -177,7 +181,6 @@ __global__ __launch_bounds__(T <= 64 ? 256 : T) void rms_norm_kernel(RmsNormPara
                         });
                     }
                 } else {
-                    static_for<0, PIECE>([&](auto ec) { constexpr int e = decltype(ec)::value; y[e] = __fmul_rn(y[e], r); });
                     Weights v;
                     v.set(y);
                     // a block's four lanes: pieces behind the row's end are zeros, but for r: NaN and infinities have to come from the row itself

@@ -177,6 +177,21 @@ def test_sizes_that_leave_fp32_when_squared(torch, capi, name, k):
         check_mxfp4(torch, capi, x, None, None, epsilon)
 
 
+@pytest.mark.parametrize("k", [24, 700, 5000, 17000])
+def test_weights_that_leave_fp32_times_the_row(torch, capi, k):
+    """Rows and weights whose products are beyond fp32 or below its normal numbers, where the norm itself is not."""
+    rng = np.random.default_rng(k)
+    x = torch.from_numpy(rng.standard_normal((3, k)) * np.array([[1e15], [1e-17], [1.0]])).float()
+    x[1, ::2] *= 1e-19
+    for size in (1e25, 1e-9):
+        w = torch.from_numpy(size * (1.0 + 0.3 * rng.standard_normal(k))).float()
+        for name in ("f32", "bf16"):
+            check_rows(torch, capi, x.to(dtype(torch, name)), None, w, name, 0.0)
+        check_mxfp4(torch, capi, x, None, w, 0.0)
+    q, scales = capi.rms_norm_tokens(x.cuda(), torch.full((k,), 1e25, device="cuda"))
+    assert torch.isnan(scales).tolist() == [True, False, False]
+
+
 @pytest.mark.parametrize("name", TYPES)
 @pytest.mark.parametrize("k", [6, 100, 1000, 9000, 17000])
 def test_rows_of_infinities_and_zeros(torch, capi, name, k):
