@@ -495,9 +495,25 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_mxfp4_few_kernel(FewTokens p)
     out.store(static_cast<char *>(p.out) + ((row0 + to) * p.out_stride + col) * (OUT == TSX_TYPE_F32 ? 4 : 2));
 }
 
+// 16 bytes of a row's codes from byte `at` on, zeros behind its end, and for what stands behind an odd number of values in its last byte
+__device__ __forceinline__ v4i row_codes(const uint8_t *row, int64_t at, int k) {
+    const int left = int(min(k - 2 * at, int64_t(32)));      // values
+    if (left == 32) return __builtin_bit_cast(v4i, v4u(*reinterpret_cast<const v4u_any *>(row + at)));
+    unsigned word[4];
+    static_for<0, 4>([&](auto wc) {
+        constexpr int w = decltype(wc)::value;
+        word[w] = 0;
+        static_for<0, 4>([&](auto bc) {
+            constexpr int b = 4 * w + decltype(bc)::value;
+            if (2 * b < left) word[w] |= unsigned(row[at + b] & (2 * b + 1 < left ? 0xff : 0x0f)) << (8 * (b % 4));
+        });
+    });
+    return v4i{int(word[0]), int(word[1]), int(word[2]), int(word[3])};
+}
+
 // codes and scales of weights [n][k] to the layout above
 __global__ __launch_bounds__(256) void pack_mxfp4_kernel(const uint8_t *codes, int64_t codes_stride, const uint8_t *scales, int64_t scales_stride, int n,
-                                                         int bytes, int blocks, int frags, int64_t pieces, int64_t words, int8_t *packed) {
+                                                         int k, int blocks, int frags, int64_t pieces, int64_t words, int8_t *packed) {
     for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < pieces + words; i += int64_t(gridDim.x) * 256) {
         if (i < pieces) {
             const int lane = int(i % 64);
@@ -506,12 +522,7 @@ __global__ __launch_bounds__(256) void pack_mxfp4_kernel(const uint8_t *codes, i
             const int col = frag * 32 + lane % 32;
             const int64_t at = step * KSTEP + (2 * half + lane / 32) * 16;
             v4i v = {0, 0, 0, 0};
-            if (col < n) {
-                const uint8_t *const from = codes + col * codes_stride + at;
-                if (at + 16 <= bytes) v = __builtin_bit_cast(v4i, v4u(*reinterpret_cast<const v4u_any *>(from)));
-                else
-                    for (int b = 0; b < 16 && at + b < bytes; ++b) v[b / 4] |= int(unsigned(from[b]) << (8 * (b % 4)));
-            }
+            if (col < n) v = row_codes(codes + col * codes_stride, at, k);
             reinterpret_cast<v4i *>(packed)[i] = v;
         } else {
             const int64_t word = i - pieces, step = word / (frags * 32);
@@ -525,19 +536,14 @@ __global__ __launch_bounds__(256) void pack_mxfp4_kernel(const uint8_t *codes, i
 }
 
 // MXFP4 rows of another length, stride or alignment than the kernels read: codes to whole K-steps, scales to words of K-steps
-__global__ __launch_bounds__(256) void copy_mxfp4_kernel(const uint8_t *codes, int64_t codes_stride, const uint8_t *scales, int64_t scales_stride, int bytes,
+__global__ __launch_bounds__(256) void copy_mxfp4_kernel(const uint8_t *codes, int64_t codes_stride, const uint8_t *scales, int64_t scales_stride, int k,
                                                          int blocks, int64_t rows, int steps, uint8_t *to, uint8_t *to_scales) {
     const int64_t pitch = int64_t(steps) * KSTEP, pieces = rows * steps * 4, words = rows * steps;
     for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < pieces + words; i += int64_t(gridDim.x) * 256) {
         if (i < pieces) {
             const int64_t row = i / (steps * 4);
             const int at = int(i - row * (steps * 4)) * 16;
-            v4i v = {0, 0, 0, 0};
-            const uint8_t *const from = codes + row * codes_stride + at;
-            if (at + 16 <= bytes) v = __builtin_bit_cast(v4i, v4u(*reinterpret_cast<const v4u_any *>(from)));
-            else
-                for (int b = 0; b < 16 && at + b < bytes; ++b) v[b / 4] |= int(unsigned(from[b]) << (8 * (b % 4)));
-            *reinterpret_cast<v4i *>(to + row * pitch + at) = v;
+            *reinterpret_cast<v4i *>(to + row * pitch + at) = row_codes(codes + row * codes_stride, at, k);
         } else {
             const int64_t word = i - pieces, step = word / rows, row = word - step * rows;
             unsigned v = 0;
@@ -721,7 +727,7 @@ int tsx_gemm_mxfp4_pack_weights(int32_t k, int32_t n, const uint8_t *codes_dev, 
     const int64_t pieces = tsx::packed_codes(k, n) / 16, words = int64_t(tsx::ksteps_of(k)) * tsx::frags_of(n) * 32;
     const int64_t blocks = std::min<int64_t>(tsx::ceil_div(pieces + words, 256), 1 << 16);
     hipLaunchKernelGGL(tsx::pack_mxfp4_kernel, dim3(unsigned(blocks)), dim3(256), 0, tsx::as_stream(stream), codes_dev, codes_stride, scales_dev, scales_stride,
-                       n, (k + 1) / 2, (k + 31) / 32, tsx::frags_of(n), pieces, words, static_cast<int8_t *>(packed_dev));
+                       n, k, (k + 31) / 32, tsx::frags_of(n), pieces, words, static_cast<int8_t *>(packed_dev));
     TSX_LAUNCH_CHECK("pack_mxfp4_kernel");
     return 0;
 }
@@ -762,7 +768,7 @@ int tsx_gemm_mxfp4(const tsx_mxfp4_gemm *g, void *workspace_dev, size_t workspac
         if (codes) {
             const int64_t units = int64_t(g->m) * steps * 5, blocks = tsx::ceil_div(units, 256);
             hipLaunchKernelGGL(tsx::copy_mxfp4_kernel, dim3(unsigned(std::min<int64_t>(blocks, 1 << 16))), dim3(256), 0, stream, static_cast<const uint8_t *>(g->x_dev),
-                               g->x_stride, g->x_scales_dev, g->x_scales_stride, (g->k + 1) / 2, (g->k + 31) / 32, int64_t(g->m), steps, to, to_scales);
+                               g->x_stride, g->x_scales_dev, g->x_scales_stride, g->k, (g->k + 31) / 32, int64_t(g->m), steps, to, to_scales);
             TSX_LAUNCH_CHECK("copy_mxfp4_kernel");
         } else {
             rc = tsx::quantize_mxfp4_rows(g->m, g->k, steps * tsx::MX_STEP, g->x_dev, g->x_type, g->x_stride,

@@ -356,6 +356,21 @@ def test_product_of_strided_rows(torch, capi):
     assert torch.equal(other.packed, layer.packed)
 
 
+@pytest.mark.parametrize("m", [1, 40, 300])
+@pytest.mark.parametrize("k", [1, 31, 129, 1023])
+def test_codes_behind_odd_rows_are_not_used(torch, capi, m, k):
+    """The upper half of an odd row's last byte may hold anything, in rows and in weights."""
+    rng = np.random.default_rng(k)
+    xc, xs = random_rows(rng, m, k)
+    wc, ws = random_rows(rng, 50, k)
+    (codes, scales), (w_codes, w_scales) = device(torch, xc, xs), device(torch, wc, ws)
+    want = torch.from_numpy(values64(xc, xs) @ values64(wc, ws).T).float()
+    codes[:, -1] |= 0x70
+    w_codes[:, -1] |= 0xF0
+    assert torch.equal(capi.TokenGemmMxfp4(w_codes, w_scales, k=k)(codes, x_scales=scales).cpu(), want)
+    assert torch.equal(capi.dequantize_mxfp4(codes, scales, k=k).cpu(), torch.from_numpy(values64(xc, xs)).float())
+
+
 @pytest.mark.parametrize("kernel,m,n,k", [("3", 1, 40, 5888), ("3", 130, 140, 6016), ("3", 300, 129, 6144), ("4", 3, 300, 4096), ("4", 257, 130, 3584), ("4", 300, 513, 4480),
                                           (None, 2048, 4096, 4352)])
 def test_product_of_long_rows_with_scales_apart(torch, capi, monkeypatch, kernel, m, n, k):
