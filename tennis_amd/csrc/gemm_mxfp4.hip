@@ -618,13 +618,14 @@ int few_tokens(const tsx_mxfp4_gemm *g, const MxGemmParams &q, hipStream_t strea
 // The kernel a call takes, by an estimate of its time in us, fitted to products of 16 .. 8192 rows on 256 .. 8192 columns and K of 256 .. 8192 (bf16).
 // r: workgroups or tiles a CU, ks: K / 1024.  MXFP4 rows: up to 16 the stream over the weights, else tiles.  Those of 64 with K split over two groups of
 // wavefronts take a CU each, so they are for up to 256; those of 64 and 128 share CUs, so that their times go by r once they fill the card and by the length
-// of K before; those of 256 come in whole turns, which a card half full goes through faster.  Measured, in this order (us): 64 x 4096, K = 4096 6.4, 6.8, 11.1,
-// 23.5; 256 x 4096, K = 4096 7.0, 7.1, 11.1, 23.5; 512 x 4096, K = 4096 12.7, 10.4, 12.8, 23.6; 512 x 8192, K = 1024 14, 7.9, 6.7, 11.2; 2048 x 4096, K =
-// 4096 46, 36, 30, 31; 4096^3 91, 70, 48, 42; 4096 x 8192, K = 1024 101, 46, 33, 38; 1024 x 1024, K = 8192 10, 11, 21, 42; 8192^3 588, 530, 326, 267.
+// of K before; those of 256 columns come in whole turns, which a card half full goes through faster.  Measured (us), tiles of 64 by K, of 64, 128, 128 x
+// 256 and 256: 64 x 4096, K = 4096 6.4, 6.8, 11, 16, 24; 256 x 4096, K = 4096 6.9, 6.9, 11, 17, 24; 512 x 4096, K = 4096 13, 10.5, 13, 17, 26; 512 x 8192, K =
+// 1024 14, 8, 6.9, 8, 11; 1024 x 1024, K = 8192 10.4, 11.6, 22, 29, 43; 1024 x 4096, K = 4096 25, 21, 17, 19, 28; 2048 x 4096, K = 4096 46, 36, 28, 25, 30; 4096^3
+// 94, 70, 47, 46, 41; 8192^3 580, 530, 325, 303, 265.
 // Rows of floats: the stream, which quantizes them itself, against tiles behind a launch that does, 3 us and the rows' bytes.  The stream is a workgroup a CU
 // at a time (of up to four rows, several, and always it); the stream and what tiles took with their launch: 64 x 1024, K = 1024 4.3 and 7.4, 128 x 1024 7.0
 // and 7.5; 256 x 256, K = 256 4.0 and 7.2; 128 x 300, K = 4096 5.8 and 9.2; 32 x 4096, K = 300 6.5 and 7.7; 16 x 8192, K = 8192 15.7 and 12.4.
-enum class Kernel { few, tile_64_by_k, tile_64, tile_128, tile_256 };
+enum class Kernel { few, tile_64_by_k, tile_64, tile_128, tile_256, tile_128_256 };
 
 Kernel choose(const tsx_mxfp4_gemm *g) {
     const int m = g->m, n = g->n, k = g->k;
@@ -632,12 +633,13 @@ Kernel choose(const tsx_mxfp4_gemm *g) {
     if (m <= (floats ? 4 : FEW)) return Kernel::few;
     const float ks = float(k) / 1024.f;
     const auto rounds = [&](int rows, int cols) { return float(ceil_div(m, rows) * ceil_div(n, cols)) / 256.f; };
-    const float r16 = rounds(FEW, 16), r64 = rounds(64, 64), r128 = rounds(128, 128), r256 = rounds(256, 256);
+    const float r16 = rounds(FEW, 16), r64 = rounds(64, 64), r128 = rounds(128, 128), r256 = rounds(256, 256), r128_256 = rounds(128, 256);
     const float cost[] = {r64 <= 1.f ? 3.6f + ks * (0.72f + 0.15f * r64) : INFINITY, std::max(3.4f + 0.88f * ks, 2.8f + r64 * (0.42f + 0.97f * ks)),
-                          std::max(3.7f + 1.82f * ks, 3.f + 0.4f * ks + r128 * (0.75f + 2.6f * ks)),
-                          3.f + std::ceil(r256) * (7.7f + 7.65f * ks) * (0.5f + 0.5f * std::min(r256, 1.f))};
+                          std::max(3.7f + 1.82f * ks, 3.f + 0.4f * ks + r128 * (0.75f + 2.75f * ks)),
+                          3.f + std::ceil(r256) * (7.7f + 7.65f * ks) * (0.5f + 0.5f * std::min(r256, 1.f)),
+                          3.f + std::ceil(r128_256) * (3.2f + 4.65f * ks) * (0.54f + 0.46f * std::min(r128_256, 1.f))};
     int best = 0;
-    for (int i = 1; i < 4; ++i)
+    for (int i = 1; i < 5; ++i)
         if (cost[i] < cost[best]) best = i;
     if (floats && m <= FEW_MOST) {
         const float few = 1.2f + std::ceil(r16) * (2.4f + 0.55f * ks);
@@ -653,6 +655,7 @@ int launch(Kernel kernel, const tsx_mxfp4_gemm *g, const MxGemmParams &p, hipStr
         case Kernel::tile_64_by_k: return launch_tile<2, 2, 1, 1, 4, 3, 2, OUT>(p, stream);
         case Kernel::tile_64: return launch_tile<2, 2, 1, 1, 2, 3, 1, OUT>(p, stream);
         case Kernel::tile_128: return launch_tile<2, 2, 2, 2, 1, 3, 1, OUT>(p, stream);
+        case Kernel::tile_128_256: return launch_tile<2, 4, 2, 2, 1, 3, 1, OUT>(p, stream);
         default: return launch_tile<2, 4, 4, 2, 1, 3, 1, OUT>(p, stream);
     }
 }
@@ -688,14 +691,15 @@ struct Plan {
         kernel = choose(g);
         // TSX_MXFP4_KERNEL: that kernel, by its place in the list above, for any call it can take (tests, measurements)
         const char *e = std::getenv("TSX_MXFP4_KERNEL");
-        if (e && e[0] >= (g->m <= FEW_MOST ? '0' : '1') && e[0] <= '4') kernel = Kernel(e[0] - '0');
+        if (e && e[0] >= (g->m <= FEW_MOST ? '0' : '1') && e[0] <= '5') kernel = Kernel(e[0] - '0');
         steps = ceil_div(g->k, MX_STEP);
         copies = g->m > 0 && !reads_in_place(g) && (kernel != Kernel::few || g->x_type == TSX_TYPE_MXFP4);
         // Rows of scales cost a tile a request of 64 cache lines where words of K-steps are four: 0.09 us a K-step in tiles of 128, 0.15 in those of 256.
-        // A launch that turns them is worth 4 us of that (8192^3 291 us without, 2048 x 4096, K = 4096 30).
+        // A launch that turns them is worth 4 us of that (us, without and with: 8192^3 291 and 267, 1024 x 4096, K = 8192 34.5 and 30.5, 2048 17 and 18).
+        // Tiles of 128 x 256 have half the rows to a multiplication, and no second tile beside them that waits too: 34 and 36 at 2048 x 4096, K = 6144.
         const int side = kernel == Kernel::tile_256 ? 256 : 128;
         const float tiles = std::max(1.f, float(ceil_div(g->m, side) * ceil_div(g->n, side)) / 256.f);
-        turns = g->m > 0 && !copies && kernel >= Kernel::tile_128 && float(steps) * tiles * (side == 256 ? 0.15f : 0.09f) > 4.f;
+        turns = g->m > 0 && !copies && (kernel == Kernel::tile_128 || kernel == Kernel::tile_256) && float(steps) * tiles * (side == 256 ? 0.15f : 0.09f) > 4.f;
         code_bytes = copies ? g->m * steps * KSTEP : 0;
         word_bytes = int64_t(g->m) * 4;
     }

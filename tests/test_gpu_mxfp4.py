@@ -188,7 +188,7 @@ def test_dequantize_tokens(torch, capi, name, shape):
 
 # ---------------------------------------------------------------- the product
 
-KERNELS = ["0", "1", "2", "3", "4"]
+KERNELS = ["0", "1", "2", "3", "4", "5"]
 
 
 def act64(y, act, slope=0.1):

@@ -51,7 +51,7 @@ CASES = ([["quantize", rows, cols, kind] for rows in (1, 511, 512, 1 << 20, (1 <
          [["norm", rows, cols, kind] for rows in (1, 511, 512, 1 << 20, (1 << 32) + 1, 1 << 40) for cols in COLS for kind in (0, 1, 2)] +
          [["product", m, n, k, kind, to, kernel] for m in (1, 2, 16, 17, 32, 33, 300, 1 << 14, (1 << 14) + 1, 1 << 20, (1 << 28) - 1)
           for n in (1, 16, 33, 64, 65, 1000, 4096, (1 << 24) - 1) for k, kind in ((1, 2), (64, 4), (1500, 4), (8192, 0), (8192, 4), ((1 << 21) - 1, 1)) for to in (0, 2)
-          for kernel in (None, 0, 1, 2, 3, 4) if m * k <= 1 << 38 and not (kernel == 1 and m * n >= 1 << 34)])      # 1: of few tiles by choice
+          for kernel in (None, 0, 1, 2, 3, 4, 5) if m * k <= 1 << 38 and not (kernel == 1 and m * n >= 1 << 34)])      # 1: of few tiles by choice
 
 
 @pytest.fixture(scope="module")
