@@ -1,9 +1,10 @@
 // Root-mean-square norm of rows, with the residual's addition in front of it; the result in the rows' type, as int8 tokens or as MXFP4.
 //
-//     h = x + residual, rounded to their type;  y = h w r,  r = 1 / sqrt(mean(h^2) + epsilon)
+//     h = x + residual, rounded to their type;  y = h r w,  r = 1 / sqrt(mean(h^2) + epsilon)
 //
-// Bound: HBM, four times the element size a value with a residual: 8192 x 4096 bf16 43 us, 6.3 TB/s (a copy of 1 GiB 5.1); one row of 4096 2.9 us, the launch.
-// A row is read once: T threads share it and hold h and the weight in registers, eight values to a piece, while they find the sum of its squares.  As int8 tokens a row's codes do not know r: with A the largest |h w|, y's largest magnitude is A r, and
+// Bound: HBM, four times the element size a value with a residual: 8192 x 4096 bf16 41 us, 6.6 TB/s (a copy of 1 GiB 5.1); one row of 4096 2.9 us, the launch.
+// A row is read once: T threads share it and hold h and the weight in registers, eight values to a piece, while they find the sum of its squares, and a
+// workgroup requests its next row before it does.  As int8 tokens a row's codes do not know r: with A the largest |h w|, y's largest magnitude is A r, and
 // y 127 / (A r) = h w 127 / A; so the search for A shares the one exchange between the threads with the sum, and only the scale, A r / 127, waits for r.
 #pragma once
 #include "mxfp4.hpp"
@@ -35,7 +36,7 @@ int rms_norm_mxfp4(const RmsNormParams &p, int type, hipStream_t stream);
 constexpr float NORM_LEAST = 0x1p-120f, NORM_DOWN = 0x1p-80f, NORM_UP = 0x1p105f;
 
 template <int TYPE, int TO, int T, int P, bool HELD>
-__global__ __launch_bounds__(T <= 64 ? 256 : T) void rms_norm_kernel(RmsNormParams p) {
+__global__ __launch_bounds__(T <= 64 ? 256 : T, P == 3 && TYPE != TSX_TYPE_F32 ? 4 : 1) void rms_norm_kernel(RmsNormParams p) {
     constexpr int PIECE = 8, THREADS = T <= 64 ? 256 : T, ROWS = THREADS / T, SIZE = TYPE == TSX_TYPE_F32 ? 4 : 2, WAVES = T / 64;
     constexpr int LG = lg_of(T < 64 ? T : 64);
     typedef Run<TYPE, PIECE> Values;
@@ -44,63 +45,88 @@ __global__ __launch_bounds__(T <= 64 ? 256 : T) void rms_norm_kernel(RmsNormPara
     const int tid = threadIdx.x, t = tid % T;
     const int pieces = (p.cols + PIECE - 1) / PIECE, whole = p.cols / PIECE, in_last = p.cols - whole * PIECE;
     const int turns = HELD ? 1 : (pieces + T * P - 1) / (T * P);
+    Values h[P];
+    Weights w[P];
+    // P pieces of a row of values: all requests of a turn first, none behind a branch, where it would be waited for; then what lies behind the row's end
+    // becomes zeros
+    auto load = [&](auto &v, const char *from, int first) __attribute__((always_inline)) {
+        static_for<0, P>([&](auto ic) {
+            constexpr int i = decltype(ic)::value;
+            const int piece = first + t + i * T;
+            if (whole) {       // uniform
+                load_piece(v[i], from, piece * PIECE, p.cols);
+            } else {
+                v[i].clear();
+                if (piece == 0) v[i].load_some(from, p.cols);
+            }
+        });
+    };
+    auto settle = [&](auto &v, int first) __attribute__((always_inline)) {
+        if (whole)
+            static_for<0, P>([&](auto ic) {
+                constexpr int i = decltype(ic)::value;
+                if (first + (i + 1) * T > whole) settle_piece(v[i], (first + t + i * T) * PIECE, p.cols);       // uniform: where the row's end can be
+            });
+    };
+    // HELD: the weights once, and a row's values while the one before is at work
+    Values next_x[P], next_r[P];
+    auto request = [&](int64_t row) __attribute__((always_inline)) {
+        const int64_t at = min(row, p.rows - 1);
+        load(next_x, static_cast<const char *>(p.x) + at * p.x_stride * SIZE, 0);
+        if (p.residual) load(next_r, static_cast<const char *>(p.residual) + at * p.residual_stride * SIZE, 0);
+    };
+    auto weights = [&](int first) __attribute__((always_inline)) {
+        if (p.weight) load(w, reinterpret_cast<const char *>(p.weight), first);
+        else static_for<0, P>([&](auto ic) { static_for<0, PIECE>([&](auto ec) { w[decltype(ic)::value].word[decltype(ec)::value] = 0x3f800000u; }); });
+    };
+    auto add = [&](auto &r) __attribute__((always_inline)) {
+        static_for<0, P>([&](auto ic) {
+            constexpr int i = decltype(ic)::value;
+            float v[PIECE];
+            static_for<0, PIECE>([&](auto ec) { constexpr int e = decltype(ec)::value; v[e] = __fadd_rn(h[i].template get<e>(), r[i].template get<e>()); });
+            h[i].set(v);
+        });
+    };
+    if constexpr (HELD) {
+        request(int64_t(blockIdx.x) * ROWS + tid / T);
+        weights(0);
+        if (p.weight) settle(w, 0);
+    }
     for (int64_t row0 = int64_t(blockIdx.x) * ROWS; row0 < p.rows; row0 += int64_t(gridDim.x) * ROWS) {
         const int64_t row = row0 + tid / T;
         const bool there = row < p.rows;      // a row's threads agree; only T <= 64 has several rows, and some beyond the last one, which are that one again
         const int64_t at = there ? row : p.rows - 1;
-        const char *const x = static_cast<const char *>(p.x) + at * p.x_stride * SIZE;
-        const char *const residual = static_cast<const char *>(p.residual) + at * p.residual_stride * SIZE;
         char *const sum = static_cast<char *>(p.sum) + at * p.sum_stride * SIZE;
-        Values h[P];
-        Weights w[P];
-        // P pieces of a row of values: all requests of a turn first, none behind a branch, where it would be waited for; then what lies behind the row's end
-        // becomes zeros
-        auto load = [&](auto &v, const char *from, int first) __attribute__((always_inline)) {
-            static_for<0, P>([&](auto ic) {
-                constexpr int i = decltype(ic)::value;
-                const int piece = first + t + i * T;
-                if (whole) {       // uniform
-                    load_piece(v[i], from, piece * PIECE, p.cols);
-                } else {
-                    v[i].clear();
-                    if (piece == 0) v[i].load_some(from, p.cols);
-                }
-            });
-        };
-        auto settle = [&](auto &v, int first) __attribute__((always_inline)) {
-            if (whole)
-                static_for<0, P>([&](auto ic) {
-                    constexpr int i = decltype(ic)::value;
-                    if (first + (i + 1) * T > whole) settle_piece(v[i], (first + t + i * T) * PIECE, p.cols);       // uniform: where the row's end can be
-                });
-        };
         auto store = [&](const Values &v, char *to, int piece) __attribute__((always_inline)) {
             if (!there || piece >= pieces) return;
             if (piece < whole) v.store(to + int64_t(piece) * (PIECE * SIZE));
             else v.store_some(to + int64_t(piece) * (PIECE * SIZE), in_last);
         };
-        // h of a turn, and the weights where they are wanted; again: h as it was kept
-        auto fetch = [&](int first, bool again, bool weights) __attribute__((always_inline)) {
+        // h of a row; the next row's values are requested ahead of any store, so that nobody waits for these with them
+        auto take = [&]() __attribute__((always_inline)) {
+            static_for<0, P>([&](auto ic) { h[decltype(ic)::value] = next_x[decltype(ic)::value]; });
+            settle(h, 0);
+            if (p.residual) {
+                settle(next_r, 0);
+                add(next_r);
+            }
+            if (row0 + int64_t(gridDim.x) * ROWS < p.rows) request(row + int64_t(gridDim.x) * ROWS);       // uniform
+            if (p.sum) static_for<0, P>([&](auto ic) { store(h[decltype(ic)::value], sum, t + decltype(ic)::value * T); });
+        };
+        // not HELD: h of a turn, and the weights where they are wanted; again: h as it was kept
+        auto fetch = [&](int first, bool again, bool weighted) __attribute__((always_inline)) {
             const bool adds = p.residual && !(again && p.sum);       // uniform, as all conditions here
             Values r[P];
-            load(h, again && p.sum ? sum : x, first);
-            if (adds) load(r, residual, first);
-            if (weights) {
-                if (p.weight) load(w, reinterpret_cast<const char *>(p.weight), first);
-                else static_for<0, P>([&](auto ic) { static_for<0, PIECE>([&](auto ec) { w[decltype(ic)::value].word[decltype(ec)::value] = 0x3f800000u; }); });
-            }
+            load(h, again && p.sum ? sum : static_cast<const char *>(p.x) + at * p.x_stride * SIZE, first);
+            if (adds) load(r, static_cast<const char *>(p.residual) + at * p.residual_stride * SIZE, first);
+            if (weighted) weights(first);
             settle(h, first);
             if (adds) {
                 settle(r, first);
-                static_for<0, P>([&](auto ic) {
-                    constexpr int i = decltype(ic)::value;
-                    float v[PIECE];
-                    static_for<0, PIECE>([&](auto ec) { constexpr int e = decltype(ec)::value; v[e] = __fadd_rn(h[i].template get<e>(), r[i].template get<e>()); });
-                    h[i].set(v);
-                });
+                add(r);
             }
             if (p.sum && !again) static_for<0, P>([&](auto ic) { store(h[decltype(ic)::value], sum, first + t + decltype(ic)::value * T); });
-            if (weights && p.weight) settle(w, first);
+            if (weighted && p.weight) settle(w, first);
         };
         // the sum of (h lift)^2 and the largest |h lift w| over the row, in all its threads
         float squares, top;
@@ -109,7 +135,8 @@ __global__ __launch_bounds__(T <= 64 ? 256 : T) void rms_norm_kernel(RmsNormPara
             double long_sum = 0;                  // over turns
             unsigned most = 0;                    // magnitudes' bits sort as they do, infinities and NaN last
             for (int turn = 0; turn < turns; ++turn) {
-                if (!HELD || !again) fetch(turn * T * P, again, HELD || TO == NORM_TOKENS);
+                if (!HELD) fetch(turn * T * P, again, TO == NORM_TOKENS);
+                else if (!again) take();
                 float s[2] = {0.f, 0.f};
                 static_for<0, P>([&](auto ic) {
                     constexpr int i = decltype(ic)::value;
@@ -199,16 +226,22 @@ __global__ __launch_bounds__(T <= 64 ? 256 : T) void rms_norm_kernel(RmsNormPara
 template <int TYPE, int TO, int T, int P, bool HELD>
 int launch_rms_norm(const RmsNormParams &p, hipStream_t stream) {
     constexpr int THREADS = T <= 64 ? 256 : T, ROWS = THREADS / T;
-    const int64_t blocks = ceil_div(p.rows, ROWS), most = int64_t(1) << 20;       // beyond that a workgroup takes several rows
-    hipLaunchKernelGGL((rms_norm_kernel<TYPE, TO, T, P, HELD>), dim3(unsigned(blocks < most ? blocks : most)), dim3(THREADS), 0, stream, p);
+    const int64_t blocks = ceil_div(p.rows, ROWS);
+    // A workgroup takes one row after the other, the weights once, where rows are more than twice what the CUs hold at a time: 4096 threads each, 2048 with
+    // the registers of longer rows.  As many rows each, one or all (bf16, us): 400000 x 64 31 and 21, 5000 x 2048 9.4 and 8.3, 20000 x 1000 as int8 22.9 and 22.5;
+    // fewer threads than that: 8192 x 4096 with a residual 43.3 for 40.8.
+    constexpr int AT_ONCE = P == 3 || T * P >= 1024 ? 2048 : 4096;
+    const int64_t slots = 256 * AT_ONCE / THREADS;
+    const int64_t grid = ceil_div(blocks, ceil_div(blocks, slots));
+    hipLaunchKernelGGL((rms_norm_kernel<TYPE, TO, T, P, HELD>), dim3(unsigned(grid)), dim3(THREADS), 0, stream, p);
     TSX_LAUNCH_CHECK("rms_norm_kernel");
     return 0;
 }
 
 template <int TYPE, int TO>
 int rms_norm_type(const RmsNormParams &p, hipStream_t stream) {
-    // One piece of eight values a thread where that makes a workgroup, two or three of a longer row: more of them leave a CU too few threads (bf16 with a
-    // residual, us: 2048 x 2048 256 threads a row 7.5, 128 7.9, 64 8.9; 5000 x 2050 128 threads with three pieces each 16.7, 64 with five 18.4, 256 with two
+    // One piece of eight values a thread where that makes a workgroup, two or three of a longer row: more of them leave a CU too few threads (a row a workgroup, bf16
+    // with a residual, us: 2048 x 2048 256 threads a row 7.5, 128 7.9, 64 8.9; 5000 x 2050 128 threads with three pieces each 16.7, 64 with five 18.4, 256 with two
     // 16.9; 8192 x 4096 256 threads 48, 64 55; 2000 x 8192 512 threads 27, 256 28).  Rows of two pieces a lane stay in a wavefront, with no barrier (8192 x
     // 1000: 11.7, 256 threads 15.9), several short ones to each.  512 threads for rows of up to 4096 while there are few (1 x 4096 3.0, 256 threads 3.2).
     const int64_t pieces = ceil_div(p.cols, 8);

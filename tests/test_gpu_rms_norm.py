@@ -127,6 +127,21 @@ def test_norm(torch, capi, name, m, k):
     check_mxfp4(torch, capi, x, None, None)
 
 
+@pytest.mark.parametrize("m,k,name", [(270001, 20, "bf16"), (66001, 100, "f16"), (16999, 300, "f32"), (17003, 700, "bf16"), (4500, 2000, "f16"), (4501, 2500, "bf16"), (4500, 2200, "f32"),
+                                      (4501, 3500, "bf16"), (1100, 5000, "f16"), (1027, 8000, "f32"), (600, 9001, "bf16"), (530, 17000, "f16")])
+def test_many_rows(torch, capi, m, k, name):
+    """More rows than a launch has workgroups: these take several, one behind the other; a few of them in 2^-70 and 2^70 steps in fp32 and bf16."""
+    rng = np.random.default_rng(k)
+    x, r, w = inputs(torch, rng, m, k, name)
+    if name != "f16":
+        for part in (x, r):
+            part[7::997] *= 2.0 ** 70
+            part[8::991] *= 2.0 ** -70
+    check_rows(torch, capi, x, r, w, name, 0.0)
+    check_tokens(torch, capi, x, r, w, 0.0)
+    check_mxfp4(torch, capi, x, None, w, 0.0)
+
+
 @pytest.mark.parametrize("name", TYPES)
 @pytest.mark.parametrize("k", [5, 100, 1000, 4096, 20000])
 def test_strides(torch, capi, name, k):
