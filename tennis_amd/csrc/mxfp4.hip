@@ -16,14 +16,14 @@ constexpr int PIECE = 8, THREADS = 256;
 struct ToMxParams {
     const void *x;
     MxRows to;
-    Divider pieces;               // of a row, a multiple of 4
+    Divider pieces;               // of a row, a multiple of LANES
     int64_t x_stride;
     unsigned total;               // pieces of all rows
     int cols, cols_out;
 };
 
-// TAILS: rows end inside a piece, or pieces behind their ends are written
-template <int TYPE, bool TAILS>
+// TAILS: rows end inside a piece, or pieces behind their ends are written; LANES: of a block, one where rows are one piece
+template <int TYPE, bool TAILS, int LANES>
 __global__ __launch_bounds__(THREADS) void quantize_mxfp4_kernel(ToMxParams p) {
     constexpr int SIZE = TYPE == TSX_TYPE_F32 ? 4 : 2;
     typedef Run<TYPE, PIECE> Values;
@@ -41,13 +41,13 @@ __global__ __launch_bounds__(THREADS) void quantize_mxfp4_kernel(ToMxParams p) {
         v.clear();
         if (piece == 0) v.load_some(x, p.cols);
     }
-    const unsigned top = over_lanes(v.top(0), 2, [](unsigned a, unsigned b) { return Values::template larger<TYPE>(a, b); });
+    const unsigned top = over_lanes(v.top(0), lg_of(LANES), [](unsigned a, unsigned b) { return Values::template larger<TYPE>(a, b); });
     const unsigned scale = mx_scale(top_value<TYPE>(top)), codes = mx_codes<TYPE>(v, scale);
     if (id >= p.total) return;
     const int left = p.cols_out - piece * PIECE;
     if (!TAILS || left > 0) store_codes(p.to.codes + row * p.to.codes_stride + int64_t(piece) * (PIECE / 2), codes, TAILS ? left : PIECE);
     const int block = piece / 4;
-    if (piece % 4 == 0) p.to.scales[row * p.to.scale_row + (block >> 2) * p.to.scale_group + (block & 3)] = uint8_t(scale);
+    if (piece % LANES == 0) p.to.scales[row * p.to.scale_row + (block >> 2) * p.to.scale_group + (block & 3)] = uint8_t(scale);
 }
 
 struct FromParams {
@@ -113,7 +113,8 @@ int in_runs(int64_t rows, int64_t pieces, F &&launch) {
 
 template <int TYPE>
 int to_mx(int64_t rows, int cols, int cols_out, const void *x, int64_t x_stride, const MxRows &to, hipStream_t stream) {
-    const int64_t pieces = ceil_div(cols_out, MX_BLOCK) * (MX_BLOCK / PIECE);
+    const bool alone = cols_out <= PIECE;      // 16.8 million rows of one bf16 value 85 us, four lanes each 190
+    const int64_t pieces = alone ? 1 : ceil_div(cols_out, MX_BLOCK) * (MX_BLOCK / PIECE);
     return in_runs(rows, pieces, [&](int64_t at, int64_t count) {
         const int64_t total = count * pieces;
         MxRows part = to;
@@ -121,7 +122,7 @@ int to_mx(int64_t rows, int cols, int cols_out, const void *x, int64_t x_stride,
         part.scales += at * to.scale_row;
         const ToMxParams p{static_cast<const char *>(x) + at * x_stride * int64_t(element_bytes(TYPE)), part, Divider(pieces), x_stride, unsigned(total), cols, cols_out};
         const bool tails = cols % MX_BLOCK != 0 || cols_out != cols;
-        hipLaunchKernelGGL((tails ? quantize_mxfp4_kernel<TYPE, true> : quantize_mxfp4_kernel<TYPE, false>), dim3(unsigned(ceil_div(total, THREADS))), dim3(THREADS), 0, stream, p);
+        hipLaunchKernelGGL((alone ? quantize_mxfp4_kernel<TYPE, true, 1> : tails ? quantize_mxfp4_kernel<TYPE, true, 4> : quantize_mxfp4_kernel<TYPE, false, 4>), dim3(unsigned(ceil_div(total, THREADS))), dim3(THREADS), 0, stream, p);
         TSX_LAUNCH_CHECK("quantize_mxfp4_kernel");
         return 0;
     });

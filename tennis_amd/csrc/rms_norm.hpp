@@ -243,10 +243,15 @@ int rms_norm_type(const RmsNormParams &p, hipStream_t stream) {
     // One piece of eight values a thread where that makes a workgroup, two or three of a longer row: more of them leave a CU too few threads (a row a workgroup, bf16
     // with a residual, us: 2048 x 2048 256 threads a row 7.5, 128 7.9, 64 8.9; 5000 x 2050 128 threads with three pieces each 16.7, 64 with five 18.4, 256 with two
     // 16.9; 8192 x 4096 256 threads 48, 64 55; 2000 x 8192 512 threads 27, 256 28).  Rows of two pieces a lane stay in a wavefront, with no barrier (8192 x
-    // 1000: 11.7, 256 threads 15.9), several short ones to each.  512 threads for rows of up to 4096 while there are few (1 x 4096 3.0, 256 threads 3.2).
+    // 1000: 11.7, 256 threads 15.9), several short ones to each, with lanes for their pieces and few more
+    // (16.8 million rows of one value 137 us, four lanes each 389; 2 million of 8 25, 34; 419430 of 40 as int8 on eight lanes 22, on sixteen 34; 83886 of 200 on 32
+    // lanes 20, on 64 31).  512 threads for rows of up to 4096 while there are few (1 x 4096 3.0, 256 threads 3.2).
     const int64_t pieces = ceil_div(p.cols, 8);
+    if (pieces <= 1) return launch_rms_norm<TYPE, TO, 1, 1, true>(p, stream);
     if (pieces <= 4) return launch_rms_norm<TYPE, TO, 4, 1, true>(p, stream);
+    if (pieces <= 8) return launch_rms_norm<TYPE, TO, 8, 1, true>(p, stream);
     if (pieces <= 16) return launch_rms_norm<TYPE, TO, 16, 1, true>(p, stream);
+    if (pieces <= 32) return launch_rms_norm<TYPE, TO, 32, 1, true>(p, stream);
     if (pieces <= 64) return launch_rms_norm<TYPE, TO, 64, 1, true>(p, stream);
     if (pieces <= 128) return launch_rms_norm<TYPE, TO, 64, 2, true>(p, stream);
     if (pieces <= 256) return launch_rms_norm<TYPE, TO, 256, 1, true>(p, stream);
