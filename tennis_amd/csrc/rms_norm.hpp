@@ -33,7 +33,8 @@ int rms_norm_mxfp4(const RmsNormParams &p, int type, hipStream_t stream);
 // A row whose mean square (with epsilon) leaves [2^-120, infinity) in fp32 is taken times a power of two instead; inside, what squares below 2^-126
 // lose is 2^-30 of the mean.  Above: by 2^-80, so that 2^30 squares of the largest number stay below 2^126.  Below: by 2^105; the largest
 // number that can be there, 2^-45 alone among 2^30 columns, becomes 2^60, and the mean with the least one, 2^-149 alone among them, 2^-118.
-constexpr float NORM_LEAST = 0x1p-120f, NORM_DOWN = 0x1p-80f, NORM_UP = 0x1p105f;
+constexpr float NORM_LEAST = 0x1p-120f;
+constexpr int NORM_DOWN = -80, NORM_UP = 105;
 
 template <int TYPE, int TO, int T, int P, bool HELD>
 __global__ __launch_bounds__(T <= 64 ? 256 : T, P == 3 && TYPE != TSX_TYPE_F32 ? 4 : 1) void rms_norm_kernel(RmsNormParams p) {
@@ -128,9 +129,9 @@ __global__ __launch_bounds__(T <= 64 ? 256 : T, P == 3 && TYPE != TSX_TYPE_F32 ?
             if (p.sum && !again) static_for<0, P>([&](auto ic) { store(h[decltype(ic)::value], sum, first + t + decltype(ic)::value * T); });
             if (weighted && p.weight) settle(w, first);
         };
-        // the sum of (h lift)^2 and the largest |h lift w| over the row, in all its threads
+        // the sum of (h 2^up)^2 and the largest |h 2^up w| over the row, in all its threads
         float squares, top;
-        auto statistics = [&](auto lifted, float lift, bool again) __attribute__((always_inline)) {
+        auto statistics = [&](auto lifted, int up, bool again) __attribute__((always_inline)) {
             constexpr bool LIFTED = decltype(lifted)::value;
             double long_sum = 0;                  // over turns
             unsigned most = 0;                    // magnitudes' bits sort as they do, infinities and NaN last
@@ -143,7 +144,7 @@ __global__ __launch_bounds__(T <= 64 ? 256 : T, P == 3 && TYPE != TSX_TYPE_F32 ?
                     static_for<0, PIECE>([&](auto ec) {
                         constexpr int e = decltype(ec)::value;
                         float v = h[i].template get<e>();
-                        if (LIFTED) v = __fmul_rn(v, lift);
+                        if (LIFTED) v = __builtin_ldexpf(v, up);
                         s[e % 2] = __builtin_fmaf(v, v, s[e % 2]);
                         if constexpr (TO == NORM_TOKENS) most = max(most, __builtin_bit_cast(unsigned, __fmul_rn(v, w[i].template get<e>())) & 0x7fffffffu);
                     });
@@ -164,14 +165,23 @@ __global__ __launch_bounds__(T <= 64 ? 256 : T, P == 3 && TYPE != TSX_TYPE_F32 ?
             }
             top = __builtin_bit_cast(float, most);
         };
-        statistics(std::false_type{}, 1.f, false);
-        float mean = __builtin_fmaf(squares, p.inv_cols, p.epsilon), lift = 1.f;
+        statistics(std::false_type{}, 0, false);
+        float mean = __builtin_fmaf(squares, p.inv_cols, p.epsilon);
+        int up = 0;                               // y = (h 2^up) r w
         if (!(mean >= NORM_LEAST && mean < __builtin_inff())) {       // a row's threads agree
-            lift = mean < NORM_LEAST ? NORM_UP : NORM_DOWN;
-            statistics(std::true_type{}, lift, true);
-            mean = __builtin_fmaf(squares, p.inv_cols, __fmul_rn(__fmul_rn(p.epsilon, lift), lift));
+            up = mean < NORM_LEAST ? NORM_UP : NORM_DOWN;
+            statistics(std::true_type{}, up, true);
+            mean = __builtin_fmaf(squares, p.inv_cols, __builtin_ldexpf(p.epsilon, 2 * up));
         }
-        const float r = __builtin_amdgcn_rsqf(mean);
+        float r = __builtin_amdgcn_rsqf(mean);
+        if (TO == NORM_TOKENS && up != 0) {
+            // With r in [1, 2) no |h 2^up w| is more than that |y|: such a row's products stay where y itself stays.
+            const int e = __builtin_amdgcn_frexp_expf(r) - 1;
+            r = __builtin_ldexpf(r, -e);
+            up += e;
+            if (HELD) static_for<0, P>([&](auto ic) { h[decltype(ic)::value].renew_words(); });      // no value of theirs is kept from the passes before: registers
+            statistics(std::true_type{}, up, true);
+        }
         const TokenScale token(top);
         if (TO == NORM_TOKENS && there && t == 0)
             static_cast<float *>(p.scales)[row] = top < __builtin_inff() ? __fdiv_rn(__fmul_rn(top, r), 127.f) : __builtin_nanf("");
@@ -184,7 +194,7 @@ __global__ __launch_bounds__(T <= 64 ? 256 : T, P == 3 && TYPE != TSX_TYPE_F32 ?
                 float y[PIECE];                   // of int8 tokens: y / r
                 static_for<0, PIECE>([&](auto ec) {
                     constexpr int e = decltype(ec)::value;
-                    y[e] = __fmul_rn(h[i].template get<e>(), lift);
+                    y[e] = __builtin_ldexpf(h[i].template get<e>(), up);
                     if constexpr (TO != NORM_TOKENS) y[e] = __fmul_rn(y[e], r);      // ahead of the weight: h w may leave fp32 where y does not
                     y[e] = __fmul_rn(y[e], w[i].template get<e>());
                 });

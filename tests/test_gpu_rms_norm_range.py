@@ -1,0 +1,61 @@
+"""The int8 form of the root-mean-square norm where products of a row's values with the weight leave fp32's normal numbers and y does not.
+
+Codes are the definition's bits of h w rounded to 24 bits, whatever their exponent: a power of two in front of both changes none.  A scale is the
+largest |y| over 127 within R and two more roundings, or a step of the subnormal numbers."""
+import numpy as np
+import pytest
+
+from tests.test_gpu_mxfp4 import U, dtype
+from tests.test_gpu_rms_norm import R, norm64
+from tests.test_gpu_tokens import tokens64
+
+pytestmark = pytest.mark.gpu
+
+COLS = [1, 5, 24, 700, 1030, 5000, 17000]
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch as t
+    assert t.cuda.is_available(), "this test needs the MI355X"
+    return t
+
+
+@pytest.fixture(scope="module")
+def capi():
+    from tennis_amd import capi as c
+    c.lib()
+    return c
+
+
+def products24(h, w):
+    """h w of fp32 numbers rounded to 24 bits, each row times a power of two that makes its largest lie in [1, 2).  The product is exact in 64 bits."""
+    part, e = np.frexp(h * w)
+    top = np.where(part == 0, -10000, e).max(-1, keepdims=True)
+    top = np.where(top == -10000, 0, top)
+    return np.ldexp(np.rint(np.ldexp(part, 24)), e - top + 1 - 24)
+
+
+def rows(rng, m, k):
+    return rng.uniform(0.25, 1.0, (m, k)) * rng.choice([-1.0, 1.0], (m, k))
+
+
+def check_tokens(torch, capi, x, w, epsilon, residual=None):
+    h = x if residual is None else (x.float() + residual.float()).to(x.dtype)
+    q, scales, *total = capi.rms_norm_tokens(x.cuda(), w.cuda(), epsilon, residual=None if residual is None else residual.cuda())
+    assert all(torch.equal(t.cpu(), h) for t in total)
+    assert np.array_equal(q.cpu().numpy(), tokens64(products24(h.double().numpy(), w.double().numpy()))[0])
+    want = np.abs(norm64(h, w, epsilon)).max(-1) / 127.0
+    assert (np.abs(scales.double().cpu().numpy() - want) <= (R + 2 * U) * want + 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("k", COLS)
+def test_products_of_scaled_rows(torch, capi, k, name):
+    """Rows whose mean square is below fp32's normal numbers, and weights that bring h w back into range: what the scaled row times the weight
+    would leave is no matter.  Rows whose mean square is above it, likewise."""
+    rng = np.random.default_rng(k)
+    for sizes, of_weight in (((-70, -80, -100, -62), 100), ((-70, -120), 60), ((-100, -110, -126), 126), ((80, 100, 120), -120), ((70, 126), -20), ((-90, -120), -20)):
+        x = torch.from_numpy(rows(rng, len(sizes), k) * 2.0 ** np.array(sizes)[:, None]).to(dtype(torch, name))
+        w = torch.from_numpy(rng.uniform(0.5, 1.0, k) * 2.0 ** of_weight).float()
+        check_tokens(torch, capi, x, w, 0.0)
