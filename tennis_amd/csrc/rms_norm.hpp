@@ -174,8 +174,10 @@ __global__ __launch_bounds__(T <= 64 ? 256 : T, P == 3 && TYPE != TSX_TYPE_F32 ?
             mean = __builtin_fmaf(squares, p.inv_cols, __builtin_ldexpf(p.epsilon, 2 * up));
         }
         float r = __builtin_amdgcn_rsqf(mean);
-        if (TO == NORM_TOKENS && up != 0) {
-            // With r in [1, 2) no |h 2^up w| is more than that |y|: such a row's products stay where y itself stays.
+        // The least largest |h w| of whose row all products that do not become 0, from 1 / 254 of it on, are normal numbers.
+        constexpr float LEAST_TOP = 0x1p-118f;
+        if (TO == NORM_TOKENS && (up != 0 || top < LEAST_TOP)) {
+            // With r in [1, 2) no |h 2^up w| is more than that |y|, nor less than half of it: such a row's products stay where y itself stays.
             const int e = __builtin_amdgcn_frexp_expf(r) - 1;
             r = __builtin_ldexpf(r, -e);
             up += e;

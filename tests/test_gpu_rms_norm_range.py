@@ -49,6 +49,20 @@ def check_tokens(torch, capi, x, w, epsilon, residual=None):
     assert (np.abs(scales.double().cpu().numpy() - want) <= (R + 2 * U) * want + 2.0 ** -149).all()
 
 
+@pytest.mark.parametrize("name,size,of_weight,epsilon", [("f32", -59, -91, 0.0), ("bf16", -59, -91, 0.0), ("f16", -18, -112, 0.0), ("f32", -20, -114, 0.0),
+                                                         ("f32", -55, -62, 0.0), ("bf16", -25, -100, 1e-6), ("bf16", -30, -95, 1e-6)])
+@pytest.mark.parametrize("k", COLS)
+def test_small_products(torch, capi, k, name, size, of_weight, epsilon):
+    """Rows whose mean square needs no scaling, weights so small that h w is no normal number; the rows beside them are ordinary."""
+    rng = np.random.default_rng(k - size)
+    x = torch.from_numpy(rows(rng, 6, k) * np.array([[2.0 ** size]] * 5 + [[2.0 ** (size + 12)]])).to(dtype(torch, name))
+    w = torch.from_numpy(rng.uniform(0.5, 1.0, k) * 2.0 ** of_weight).float()
+    check_tokens(torch, capi, x, w, epsilon)
+    x[2] = 0.0
+    if epsilon:
+        check_tokens(torch, capi, x, w, epsilon, torch.zeros_like(x))
+
+
 @pytest.mark.parametrize("name", ["f32", "bf16"])
 @pytest.mark.parametrize("k", COLS)
 def test_products_of_scaled_rows(torch, capi, k, name):
