@@ -184,9 +184,10 @@ __global__ __launch_bounds__(T <= 64 ? 256 : T, P == 3 && TYPE != TSX_TYPE_F32 ?
             if (HELD) static_for<0, P>([&](auto ic) { h[decltype(ic)::value].renew_words(); });      // no value of theirs is kept from the passes before: registers
             statistics(std::true_type{}, up, true);
         }
-        const TokenScale token(top);
-        if (TO == NORM_TOKENS && there && t == 0)
-            static_cast<float *>(p.scales)[row] = top < __builtin_inff() ? __fdiv_rn(__fmul_rn(top, r), 127.f) : __builtin_nanf("");
+        const float largest = __fmul_rn(top, r);                      // |y|
+        const bool finite = largest < __builtin_inff();               // false for NaN
+        const TokenScale token(finite ? top : __builtin_inff());      // of y / r: zeros where y leaves fp32
+        if (TO == NORM_TOKENS && there && t == 0) static_cast<float *>(p.scales)[row] = finite ? __fdiv_rn(largest, 127.f) : __builtin_nanf("");
         char *const out = static_cast<char *>(p.out) + at * p.out_stride * (TO == NORM_ROWS ? SIZE : 1);
         for (int turn = 0; turn < turns; ++turn) {
             if (!HELD) fetch(turn * T * P, true, true);

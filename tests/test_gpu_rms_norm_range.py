@@ -1,7 +1,10 @@
-"""The int8 form of the root-mean-square norm where products of a row's values with the weight leave fp32's normal numbers and y does not.
+"""The int8 form of the root-mean-square norm where products of a row's values with the weight leave fp32's normal numbers and y does not, and
+where y leaves fp32.
 
 Codes are the definition's bits of h w rounded to 24 bits, whatever their exponent: a power of two in front of both changes none.  A scale is the
 largest |y| over 127 within R and two more roundings, or a step of the subnormal numbers."""
+import math
+
 import numpy as np
 import pytest
 
@@ -73,3 +76,25 @@ def test_products_of_scaled_rows(torch, capi, k, name):
         x = torch.from_numpy(rows(rng, len(sizes), k) * 2.0 ** np.array(sizes)[:, None]).to(dtype(torch, name))
         w = torch.from_numpy(rng.uniform(0.5, 1.0, k) * 2.0 ** of_weight).float()
         check_tokens(torch, capi, x, w, 0.0)
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("k", [300, 5000, 17000])
+def test_rows_whose_norm_leaves_fp32(torch, capi, k, name):
+    """One value alone in its row: y is the root of the columns' count times the weight.  Where that is beyond fp32 the token has no scale, as a row
+    with an infinity; the rows beside it do not notice."""
+    rng = np.random.default_rng(k)
+    values = rows(rng, 5, k)
+    values[1] = values[3] = 0.0
+    values[1, k // 3], values[3, k - 1] = 0.125, -0.5
+    x = torch.from_numpy(values).to(dtype(torch, name))
+    w = torch.full((k,), 2.0 ** 124)
+    q, scales = capi.rms_norm_tokens(x.cuda(), w.cuda(), 0.0)
+    assert torch.isnan(scales).tolist() == [False, True, False, True, False]
+    q, scales = q.cpu().numpy(), scales.double().cpu().numpy()
+    others = [0, 2, 4]
+    assert not q[[1, 3]].any() and np.array_equal(q[others], tokens64(products24(x.double().numpy(), w.double().numpy()))[0][others])
+    want = np.abs(norm64(x, w, 0.0)).max(-1)[others] / 127.0
+    assert (np.abs(scales[others] - want) <= (R + 2 * U) * want).all()
+    y = capi.rms_norm(x.cuda().float(), w.cuda(), 0.0).cpu()
+    assert math.isinf(y[1, k // 3]) and math.isinf(y[3, k - 1]) and torch.isfinite(y[others]).all()
