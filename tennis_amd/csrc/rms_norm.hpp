@@ -165,73 +165,80 @@ __global__ __launch_bounds__(T <= 64 ? 256 : T, P == 3 && TYPE != TSX_TYPE_F32 ?
             }
             top = __builtin_bit_cast(float, most);
         };
+        char *const out = static_cast<char *>(p.out) + at * p.out_stride * (TO == NORM_ROWS ? SIZE : 1);
+        // the results of a row: y = (h 2^up) r w; up is 0 unless LIFTED
+        auto leave = [&](auto lifted, int up, float r) __attribute__((always_inline)) {
+            constexpr bool LIFTED = decltype(lifted)::value;
+            const float largest = __fmul_rn(top, r);                      // |y|
+            const bool finite = largest < __builtin_inff();               // false for NaN
+            const TokenScale token(finite ? top : __builtin_inff());      // of y / r: zeros where y leaves fp32
+            if (TO == NORM_TOKENS && there && t == 0) static_cast<float *>(p.scales)[row] = finite ? __fdiv_rn(largest, 127.f) : __builtin_nanf("");
+            for (int turn = 0; turn < turns; ++turn) {
+                if (!HELD) fetch(turn * T * P, true, true);
+                static_for<0, P>([&](auto ic) {
+                    constexpr int i = decltype(ic)::value;
+                    const int piece = turn * T * P + t + i * T;
+                    float y[PIECE];                   // of int8 tokens: y / r
+                    static_for<0, PIECE>([&](auto ec) {
+                        constexpr int e = decltype(ec)::value;
+                        y[e] = h[i].template get<e>();
+                        if (LIFTED) y[e] = __builtin_ldexpf(y[e], up);
+                        if constexpr (TO != NORM_TOKENS) y[e] = __fmul_rn(y[e], r);      // ahead of the weight: h w may leave fp32 where y does not
+                        y[e] = __fmul_rn(y[e], w[i].template get<e>());
+                    });
+                    if constexpr (TO == NORM_ROWS) {
+                        Values v;
+                        v.set(y);
+                        store(v, out, piece);
+                    } else if constexpr (TO == NORM_TOKENS) {
+                        if (!there || piece >= pieces) return;
+                        unsigned b[PIECE];
+                        static_for<0, PIECE>([&](auto ec) { constexpr int e = decltype(ec)::value; b[e] = token.bits(__fmul_rn(y[e], token.lift)); });
+                        v2u q = {low_bytes(b[0], b[1], b[2], b[3]), low_bytes(b[4], b[5], b[6], b[7])};
+                        if (token.reciprocal == 0.f) q = v2u{0, 0};
+                        char *const to = out + int64_t(piece) * PIECE;
+                        if (piece < whole) {
+                            *reinterpret_cast<v2u_any *>(to) = q;
+                        } else {
+                            static_for<0, PIECE - 1>([&](auto ec) {
+                                constexpr int e = decltype(ec)::value;
+                                if (e < in_last) to[e] = char(q[e / 4] >> (8 * (e % 4)));
+                            });
+                        }
+                    } else {
+                        Weights v;
+                        v.set(y);
+                        // a block's four lanes: pieces behind the row's end are zeros, but for r: NaN and infinities have to come from the row itself
+                        const unsigned own = piece < pieces ? v.top(0) : 0u;
+                        const unsigned scale = mx_scale(__builtin_bit_cast(float, over_lanes(own, T < 4 ? 0 : 2, [](unsigned a, unsigned b) { return max(a, b); })));
+                        const unsigned codes = mx_codes<TSX_TYPE_F32>(v, scale);
+                        if (!there || piece >= pieces) return;
+                        store_codes(reinterpret_cast<uint8_t *>(out) + int64_t(piece) * (PIECE / 2), codes, piece < whole ? PIECE : in_last);
+                        if (piece % 4 == 0) static_cast<uint8_t *>(p.scales)[at * p.scales_stride + piece / 4] = uint8_t(scale);
+                    }
+                });
+            }
+        };
         statistics(std::false_type{}, 0, false);
         float mean = __builtin_fmaf(squares, p.inv_cols, p.epsilon);
-        int up = 0;                               // y = (h 2^up) r w
+        int up = 0;
         if (!(mean >= NORM_LEAST && mean < __builtin_inff())) {       // a row's threads agree
             up = mean < NORM_LEAST ? NORM_UP : NORM_DOWN;
             statistics(std::true_type{}, up, true);
             mean = __builtin_fmaf(squares, p.inv_cols, __builtin_ldexpf(p.epsilon, 2 * up));
         }
-        float r = __builtin_amdgcn_rsqf(mean);
+        const float r = __builtin_amdgcn_rsqf(mean);
         // The least largest |h w| of whose row all products that do not become 0, from 1 / 254 of it on, are normal numbers.
         constexpr float LEAST_TOP = 0x1p-118f;
+        if (TO == NORM_TOKENS && HELD) static_for<0, P>([&](auto ic) { w[decltype(ic)::value].renew_words(); });      // no product is kept from the search: registers
         if (TO == NORM_TOKENS && (up != 0 || top < LEAST_TOP)) {
             // With r in [1, 2) no |h 2^up w| is more than that |y|, nor less than half of it: such a row's products stay where y itself stays.
+            // It has code of its own: in one path for both, ordinary rows (5000 x 2050) took 5 % longer.
             const int e = __builtin_amdgcn_frexp_expf(r) - 1;
-            r = __builtin_ldexpf(r, -e);
-            up += e;
-            if (HELD) static_for<0, P>([&](auto ic) { h[decltype(ic)::value].renew_words(); });      // no value of theirs is kept from the passes before: registers
-            statistics(std::true_type{}, up, true);
-        }
-        const float largest = __fmul_rn(top, r);                      // |y|
-        const bool finite = largest < __builtin_inff();               // false for NaN
-        const TokenScale token(finite ? top : __builtin_inff());      // of y / r: zeros where y leaves fp32
-        if (TO == NORM_TOKENS && there && t == 0) static_cast<float *>(p.scales)[row] = finite ? __fdiv_rn(largest, 127.f) : __builtin_nanf("");
-        char *const out = static_cast<char *>(p.out) + at * p.out_stride * (TO == NORM_ROWS ? SIZE : 1);
-        for (int turn = 0; turn < turns; ++turn) {
-            if (!HELD) fetch(turn * T * P, true, true);
-            static_for<0, P>([&](auto ic) {
-                constexpr int i = decltype(ic)::value;
-                const int piece = turn * T * P + t + i * T;
-                float y[PIECE];                   // of int8 tokens: y / r
-                static_for<0, PIECE>([&](auto ec) {
-                    constexpr int e = decltype(ec)::value;
-                    y[e] = __builtin_ldexpf(h[i].template get<e>(), up);
-                    if constexpr (TO != NORM_TOKENS) y[e] = __fmul_rn(y[e], r);      // ahead of the weight: h w may leave fp32 where y does not
-                    y[e] = __fmul_rn(y[e], w[i].template get<e>());
-                });
-                if constexpr (TO == NORM_ROWS) {
-                    Values v;
-                    v.set(y);
-                    store(v, out, piece);
-                } else if constexpr (TO == NORM_TOKENS) {
-                    if (!there || piece >= pieces) return;
-                    unsigned b[PIECE];
-                    static_for<0, PIECE>([&](auto ec) { constexpr int e = decltype(ec)::value; b[e] = token.bits(__fmul_rn(y[e], token.lift)); });
-                    v2u q = {low_bytes(b[0], b[1], b[2], b[3]), low_bytes(b[4], b[5], b[6], b[7])};
-                    if (token.reciprocal == 0.f) q = v2u{0, 0};
-                    char *const to = out + int64_t(piece) * PIECE;
-                    if (piece < whole) {
-                        *reinterpret_cast<v2u_any *>(to) = q;
-                    } else {
-                        static_for<0, PIECE - 1>([&](auto ec) {
-                            constexpr int e = decltype(ec)::value;
-                            if (e < in_last) to[e] = char(q[e / 4] >> (8 * (e % 4)));
-                        });
-                    }
-                } else {
-                    Weights v;
-                    v.set(y);
-                    // a block's four lanes: pieces behind the row's end are zeros, but for r: NaN and infinities have to come from the row itself
-                    const unsigned own = piece < pieces ? v.top(0) : 0u;
-                    const unsigned scale = mx_scale(__builtin_bit_cast(float, over_lanes(own, T < 4 ? 0 : 2, [](unsigned a, unsigned b) { return max(a, b); })));
-                    const unsigned codes = mx_codes<TSX_TYPE_F32>(v, scale);
-                    if (!there || piece >= pieces) return;
-                    store_codes(reinterpret_cast<uint8_t *>(out) + int64_t(piece) * (PIECE / 2), codes, piece < whole ? PIECE : in_last);
-                    if (piece % 4 == 0) static_cast<uint8_t *>(p.scales)[at * p.scales_stride + piece / 4] = uint8_t(scale);
-                }
-            });
+            statistics(std::true_type{}, up + e, true);
+            leave(std::true_type{}, up + e, __builtin_ldexpf(r, -e));
+        } else {
+            leave(std::bool_constant<TO != NORM_TOKENS>{}, up, r);
         }
     }
 }
