@@ -454,7 +454,7 @@ int few_tokens(const tsx_token_gemm *g, const TokenGemmParams &q, bool quantizes
 // 131072 x 512, K = 128 58, 29.4, 33.7; 4096^3 107, 77, 62.
 enum class TokenKernel { few_16, few_32, tile_64, tile_128, tile_256 };
 
-constexpr int FEW_MOST = 1 << 14;      // rows of the kernels for few tokens: with more their groups of rows leave a launch's second axis
+constexpr int FEW_MOST = 1 << 14;      // rows up to which the kernels for few tokens are taken (a launch's second axis holds their groups of 16 up to 2^20)
 
 TokenKernel choose(int m, int n, int k) {
     if (m <= 16) return TokenKernel::few_16;

@@ -76,9 +76,10 @@ __device__ __forceinline__ void barrier_but_for() { asm volatile("s_waitcnt vmcn
 // WR x WC wavefronts, each with FR x FC fragments of 32 tokens x 32 columns; S chunks of KS K-steps in LDS, scales behind their codes; KG such groups of
 // wavefronts, each with its part of every chunk's K-steps.
 //
-// Bound: 8192^3 260 us, 4.2 P operations/s, where the matrix cores are busy for 60 % of the cycles at 1.7 GHz, the clock that the card's power leaves
-// (the same instructions on random operands from registers, nothing else: 6.5 P, at 1.55 GHz).  Each multiplication takes 32 cycles of its SIMD; a
-// tile's epilogue and first chunk are 9 us of 67.  4 x 4 fragments on four wavefronts read a third less LDS and take 268 us, one wavefront a SIMD hides less.
+// Bound: 8192^3 260 us (median of calls on codes one behind the other), 4.2 P operations/s: waiting.  The matrix cores are busy for 61 - 65 % of the cycles at
+// 1.7 GHz; the same instructions on random operands from registers, nothing else, make 6.5 P at 1.55 GHz, the clock that the card's power leaves them, so
+// power is 9 % of the difference.  By products of K = 512 .. 8192 a tile takes 6.8 us for 1024 of K (5.0 P) and 9 - 10 of its 65 us for its first chunk and
+// its epilogue, with nothing beside them.  4 x 4 fragments on four wavefronts read a third less LDS and take 268 us, one wavefront a SIMD hides less.
 // Few tiles with a long K wait for one K-step after the other, 0.19 us each in tiles of 64; two groups of wavefronts halve that.
 template <int WR, int WC, int FR, int FC, int KS, int S, int KG, int OUT>
 __global__ __launch_bounds__(WR *WC *KG * 64, WR * FR == 4 && KG == 1 ? 3 : 1) void gemm_mxfp4_kernel(MxGemmParams p) {
@@ -369,7 +370,7 @@ __global__ __launch_bounds__(WR *WC *KG * 64, WR * FR == 4 && KG == 1 ? 3 : 1) v
 // there is no launch ahead of the product and no barrier in it before the partial sums meet.  16x16x128 instruction: accumulator r of lane l is
 // column 4 (l / 16) + r of token l % 16.  4096 columns, K = 4096: one bf16 token 4.1 us, 16 MXFP4 tokens 5.1, of which the weights' bytes are 1.1 and the
 // rest the launch, the first loads' way and the sums through LDS.
-constexpr int FEW = 16, FEW_MOST = 1 << 14;      // more rows would leave a launch's second axis
+constexpr int FEW = 16, FEW_MOST = 1 << 14;      // rows up to which the stream is taken: its estimate is fitted to 8192 (a launch's second axis holds groups of 16 up to 2^20)
 
 struct FewTokens : MxGemmParams {
     const void *values;                // rows of floats
