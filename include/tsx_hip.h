@@ -303,12 +303,14 @@ int tsx_gemm_mxfp4(const tsx_mxfp4_gemm *g, void *workspace_dev, size_t workspac
 /* Root-mean-square norm of rows, with the residual's addition in front of it:
  *   h = x + residual, rounded to their type (h = x without a residual);  y = h / sqrt(mean(h^2) + epsilon) * weight
  * x and residual in one type, each at a stride of its own; where sum_dev is given h is written there (x or residual themselves may be
- * that memory, at the same stride), which a residual needs.  Sums of squares are fp32 or more and do not overflow or vanish: rows whose mean square leaves
- * [2^-120, 3.4e38] are scaled first.  Where epsilon and a row are 0, and where a row has an infinity or NaN, y is what the formula gives:
- * NaN for the zeros, the infinities and every value beside a NaN, 0 for finite values beside infinities.
+ * that memory, at the same stride), which a residual needs.  Sums of squares are fp32 or more and do not overflow or vanish: rows whose
+ * mean square leaves [2^-120, 3.4e38] are scaled first.  Values below 2^-95 of their row's root mean square may lose bits.  Where epsilon
+ * and a row are 0, and where a row has an infinity or NaN, y is what the formula gives: NaN for the zeros, the infinities and every value
+ * beside a NaN, 0 for finite values beside infinities.
  *   rows    y in x's type, at out_stride
- *   tokens  y (as fp32, before any rounding) as int8 tokens, dense, with the rule of tsx_quantize_tokens (a NaN scale where y overflows fp32); of rows that are not scaled first h * weight is
- *           computed on the way: where that overflows fp32 the row gets a NaN scale (where it is too small for fp32 the row is scaled, too)
+ *   tokens  y (as fp32, before any rounding) as int8 tokens, dense, with the rule of tsx_quantize_tokens: a NaN scale where y overflows
+ *           fp32.  Of rows that are not scaled first h * weight is computed on the way; where that overflows fp32 the scale is NaN, too
+ *           (where it is too small for fp32 the row is scaled)
  *   mxfp4   y as MXFP4 rows, with the rule of tsx_quantize_mxfp4, codes [rows][ceil(cols / 2)] and scales [rows][ceil(cols / 32)] dense
  * rows may be 0; cols is at most 2^30. */
 typedef struct tsx_rms_norm {

@@ -2,8 +2,9 @@
 //
 //     h = x + residual, rounded to their type;  y = h r w,  r = 1 / sqrt(mean(h^2) + epsilon)
 //
-// Bound: HBM, four times the element size a value with a residual: 8192 x 4096 bf16 42 us, 6.4 TB/s (a copy of 1 GiB 5.1); one row of 4096 2.5 - 2.9 us, the launch.
-// A row is read once: T threads share it and hold h and the weight in registers, eight values to a piece, while they find the sum of its squares, and a
+// Bound: HBM, four times the element size a value with a residual: 8192 x 4096 bf16 42 us, 6.4 TB/s with half of the input from the
+// caches (a copy of 1 GiB 5.1); one row of 4096 2.5 - 2.9 us, the launch.  A row of up to 16384 values is read once (a longer one again for its results, and
+// for each search on it scaled): T threads share it and hold h and the weight in registers, eight values to a piece, while they find the sum of its squares, and a
 // workgroup requests its next row before it does.  As int8 tokens a row's codes do not know r: with A the largest |h w|, y's largest magnitude is A r, and
 // y 127 / (A r) = h w 127 / A; so the search for A shares the one exchange between the threads with the sum, and only the scale, A r / 127, waits for r.
 #pragma once
