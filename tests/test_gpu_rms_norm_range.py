@@ -98,3 +98,24 @@ def test_rows_whose_norm_leaves_fp32(torch, capi, k, name):
     assert (np.abs(scales[others] - want) <= (R + 2 * U) * want).all()
     y = capi.rms_norm(x.cuda().float(), w.cuda(), 0.0).cpu()
     assert math.isinf(y[1, k // 3]) and math.isinf(y[3, k - 1]) and torch.isfinite(y[others]).all()
+
+
+@pytest.mark.parametrize("m,k,name", [(66001, 100, "bf16"), (17003, 700, "f32"), (4501, 2500, "bf16"), (4500, 2200, "f32"), (1027, 8000, "bf16"), (530, 17000, "f32")])
+def test_scaled_and_ordinary_rows_in_turn(torch, capi, m, k, name):
+    """Workgroups that take several rows: scaled and ordinary ones behind each other, with a residual, so that the sum is written and read again."""
+    rng = np.random.default_rng(m)
+    sizes = 2.0 ** np.array([-59, 20, -75, 3, 0, 70])[np.arange(m) % 6][:, None]
+    x, r = (torch.from_numpy(rows(rng, m, k) * sizes).to(dtype(torch, name)) for _ in range(2))
+    x[5::7], r[5::7] = 0.0, 0.0
+    w = torch.from_numpy(rng.uniform(0.5, 1.0, k) * 2.0 ** -91).float()
+    check_tokens(torch, capi, x, w, 2.0 ** -140, r)
+
+
+@pytest.mark.parametrize("k", [3, 700, 17000])
+def test_weights_of_zeros(torch, capi, k):
+    """y is zeros: codes and scales are, too; without epsilon a row of zeros is NaN."""
+    x = torch.from_numpy(rows(np.random.default_rng(k), 4, k)).bfloat16()
+    x[2] = 0.0
+    for epsilon in (0.0, 1e-6):
+        q, scales = capi.rms_norm_tokens(x.cuda(), torch.zeros(k, device="cuda"), epsilon)
+        assert not q.any() and torch.isnan(scales).tolist() == [False, False, epsilon == 0.0, False] and not scales.nan_to_num(nan=0.0).any()
